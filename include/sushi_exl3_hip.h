@@ -86,7 +86,8 @@ typedef enum {
     EXL3_ERR_RATE_UNSUPPORTED = -13,         /* encoder: RateUnsupported */
     EXL3_ERR_WINDOW_TOO_NARROW = -14,        /* encoder: WindowTooNarrow */
     EXL3_ERR_HESSIAN = -15,                  /* quantizer: HessianNotPositiveDefinite (src/encoder/quantize.zig:351) */
-    EXL3_ERR_GROUP_MISSING = -16             /* Exl3GroupMissing (src/exl3/root.zig:647) */
+    EXL3_ERR_GROUP_MISSING = -16,            /* Exl3GroupMissing (src/exl3/root.zig:647) */
+    EXL3_ERR_ACTIVATION = -17                /* an activation outside exl3_act (an extension's) */
 } exl3_status;
 
 /* One projection's bank (`Proj`, src/exl3/root.zig:28-30). */
@@ -199,6 +200,43 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
                             int32_t out_features, const uint16_t *trellis, int32_t n, const uint16_t *suh,
                             const uint16_t *svh, exl3_decode_t dec, void *y, int32_t y_dtype, void *workspace,
                             size_t workspace_bytes, hipStream_t stream);
+
+/* A linear with an epilogue, and its backward pass: an extension (the reference's linears have no bias, activation or
+ * residual, and no gradients).  The weights stay frozen; bias, inputs and whatever precedes them train.
+ *
+ * Forward: z = linear(x) + bias, y = act(z) + residual, from the f32 sums with one rounding to y's dtype.  bias [out] in
+ * bias_dtype or null; residual [rows][out] in y's dtype or null, not overlapping y; pre [rows][out] in y's dtype receives
+ * z for the backward pass, or is null.  silu is z sigmoid(z), gelu z Phi(z), gelu_tanh its tanh approximation.  Every arm
+ * of exl3_linear finishes this way in its own launch.  x, bias, residual, y, pre and svh 4-byte aligned.
+ *
+ * Backward: from dy [rows][out] (and pre, both in `dtype`, 16-byte aligned; pre unread with EXL3_ACT_NONE)
+ *   dz = dy act'(pre),  dbias [out] = sum over rows of dz (f32; null: not wanted),
+ *   dx [rows][in] = H(f16(s H(dz * svh)) W^T) * suh / s  in dx_dtype,
+ * H the orthonormal Hadamard transform of each 128, W the decoded inner weight and s a power of two per row that brings
+ * the row's largest |dz * svh| to 2^10 .. 2^11 (the prepared gradient is f16 as the prepared input is; gradients lie below
+ * f16's normal range).  residual's gradient is dy itself, x's rounding to f16 is passed through.  Each rounding of pre to
+ * 16 bits moves act' as that of any kept activation does.
+ *
+ * Rows go in chunks of at most 16384, each its own launches. */
+typedef enum {
+    EXL3_ACT_NONE = 0,
+    EXL3_ACT_RELU = 1,
+    EXL3_ACT_SILU = 2,
+    EXL3_ACT_GELU = 3,
+    EXL3_ACT_GELU_TANH = 4
+} exl3_act;
+size_t exl3_linear_epilogue_workspace_size(int32_t rows, int32_t in_features, int32_t out_features, int32_t n);
+int32_t exl3_linear_epilogue(const void *x, int32_t x_dtype, int32_t rows, int32_t in_features, int32_t out_features,
+                             const uint16_t *trellis, int32_t n, const uint16_t *suh, const uint16_t *svh,
+                             exl3_decode_t dec, const void *bias, int32_t bias_dtype, int32_t act, const void *residual,
+                             void *y, int32_t y_dtype, void *pre, void *workspace, size_t workspace_bytes,
+                             hipStream_t stream);
+size_t exl3_linear_epilogue_backward_workspace_size(int32_t rows, int32_t in_features, int32_t out_features);
+int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t rows, int32_t in_features,
+                                      int32_t out_features, const uint16_t *trellis, int32_t n, const uint16_t *suh,
+                                      const uint16_t *svh, exl3_decode_t dec, int32_t act, const void *pre, void *dx,
+                                      int32_t dx_dtype, float *dbias, void *workspace, size_t workspace_bytes,
+                                      hipStream_t stream);
 
 /* `linear.linear` without a workspace, for callers that cannot allocate device memory (code under HIP graph
  * capture, tight serving loops, harnesses that forbid hipMalloc).  No counterpart in the reference, which allocates
@@ -349,6 +387,28 @@ int32_t exl3_moe_tiled_with_shared_bank(const void *x, int32_t x_dtype, int32_t 
  * renormalised over the k picked.  experts <= 1024, k <= 32. */
 int32_t exl3_route_topk(const float *logits, int32_t rows, int32_t experts, int32_t k, uint32_t *inds,
                         float *scores, hipStream_t stream);
+
+/* The router's balance loss with the experts' counts, and the gradient of its logits: an extension beside
+ * exl3_route_topk (the reference serves only).  With p the softmax of logits [rows][experts] (f16, bf16 or f32), T the live
+ * rows (mask [rows] bytes, 0 a padded row; null: all live) and c_e the live rows' slots on expert e,
+ *   weight_e = coef E c_e / (T k) / T,  loss = sum_e weight_e sum_r p_re
+ * (all zero without live rows).  inds [rows][topk]: an id past the experts (-1 too) is a dropped slot and counts nowhere.
+ * A row of -inf logits alone has no probabilities; NaN logits of a live row make the loss NaN, those of a padded row are
+ * never seen.  counts [experts] i32, weight [experts] f32 and loss [1] f32 are written whole.
+ *
+ * exl3_router_backward: dlogits (like logits), zero in padded rows,
+ *   dlogit_re = dloss p_re (weight_e - sum_j weight_j p_rj) + sum over the row's slots i with inds_ri = e of
+ *               s_i (dscores_ri - sum_j s_j dscores_rj),
+ * s the softmax of the logits that the row's slots picked (exl3_route_topk's scores; dropped slots have none).  dloss [1]
+ * is a device scalar.  weight and dloss null: no balance term; dscores null: no routing term.  The counts are constants of
+ * the gradient.  experts <= 1024, topk <= 32. */
+size_t exl3_balance_loss_workspace_size(int32_t rows, int32_t experts);
+int32_t exl3_balance_loss(const void *logits, int32_t dtype, int32_t rows, int32_t experts, const uint32_t *inds,
+                          int32_t topk, const uint8_t *mask, float coef, float *loss, int32_t *counts, float *weight,
+                          void *workspace, size_t workspace_bytes, hipStream_t stream);
+int32_t exl3_router_backward(const void *logits, int32_t dtype, int32_t rows, int32_t experts, const uint32_t *inds,
+                             int32_t topk, const float *dscores, const float *weight, const float *dloss,
+                             const uint8_t *mask, void *dlogits, hipStream_t stream);
 
 /* `layout.tileMajor` / `tileMajorInverse` (src/exl3/layout.zig:139-158): one projection of `experts` experts
  * between the pack order [IT][OT][n] and the pair-major order [OT/2][IT][2][n]. */

@@ -23,6 +23,10 @@ EXPORTS = (
     "exl3_linear_noalloc",
     "exl3_linear_pair_workspace_size",
     "exl3_linear_pair",
+    "exl3_linear_epilogue_workspace_size",
+    "exl3_linear_epilogue",
+    "exl3_linear_epilogue_backward_workspace_size",
+    "exl3_linear_epilogue_backward",
     "exl3_workspace_init",
     "exl3_moe_workspace_size",
     "exl3_moe",
@@ -37,6 +41,9 @@ EXPORTS = (
     "exl3_moe_tiled",
     "exl3_moe_tiled_with_shared_bank",
     "exl3_route_topk",
+    "exl3_balance_loss_workspace_size",
+    "exl3_balance_loss",
+    "exl3_router_backward",
     "exl3_tile_major",
     "exl3_encode_workspace_size",
     "exl3_encode_tiles",
@@ -97,6 +104,14 @@ def load() -> ctypes.CDLL:
     L.exl3_linear_pair_workspace_size.argtypes = [i32, i32, i32, i32, i32]
     L.exl3_linear_pair.argtypes = [vp, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp, DecodeT, vp, i32, vp, vp,
                                    DecodeT, vp, i32, vp, sz, vp]
+    L.exl3_linear_epilogue_workspace_size.restype = sz
+    L.exl3_linear_epilogue_workspace_size.argtypes = [i32, i32, i32, i32]
+    L.exl3_linear_epilogue.argtypes = [vp, i32, i32, i32, i32, vp, i32, vp, vp, DecodeT, vp, i32, i32, vp, vp, i32, vp,
+                                       vp, sz, vp]
+    L.exl3_linear_epilogue_backward_workspace_size.restype = sz
+    L.exl3_linear_epilogue_backward_workspace_size.argtypes = [i32, i32, i32]
+    L.exl3_linear_epilogue_backward.argtypes = [vp, i32, i32, i32, i32, vp, i32, vp, vp, DecodeT, i32, vp, vp, i32, vp,
+                                                vp, sz, vp]
     L.exl3_workspace_init.argtypes = [vp, sz, vp]
     L.exl3_moe_workspace_size.restype = sz
     L.exl3_moe_workspace_size.argtypes = [i32, i32, i32, i32]
@@ -124,6 +139,10 @@ def load() -> ctypes.CDLL:
                                                   ctypes.POINTER(BankT), vp, vp, i32, i32, DecodeT, i32, i32, vp,
                                                   i32, vp, sz, vp]
     L.exl3_route_topk.argtypes = [vp, i32, i32, i32, vp, vp, vp]
+    L.exl3_balance_loss_workspace_size.restype = sz
+    L.exl3_balance_loss_workspace_size.argtypes = [i32, i32]
+    L.exl3_balance_loss.argtypes = [vp, i32, i32, i32, vp, i32, vp, ctypes.c_float, vp, vp, vp, vp, sz, vp]
+    L.exl3_router_backward.argtypes = [vp, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp]
     L.exl3_tile_major.argtypes = [vp, vp, i32, i32, i32, i32, i32, vp]
     L.exl3_encode_workspace_size.restype = sz
     L.exl3_encode_workspace_size.argtypes = [i32, DecodeT, ctypes.c_int64]

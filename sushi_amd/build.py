@@ -23,11 +23,20 @@ SOURCES = [
     "exl3_decode.hip",
     "exl3_moe.hip",
     "exl3_gemm.hip",
+    "exl3_gemm_epilogue.hip",
+    "exl3_moe_gemm.hip",
+    "exl3_gradient.hip",
+    "exl3_router.hip",
     "exl3_gemv_mcg.hip",
     "exl3_gemv_mul1.hip",
     "exl3_gemv_hash.hip",
     "exl3_gemv_pair.hip",
     "exl3_gemv_3inst.hip",
+    "exl3_gemv_epilogue_mcg.hip",
+    "exl3_gemv_epilogue_mul1.hip",
+    "exl3_gemv_epilogue_hash.hip",
+    "exl3_gemv_epilogue_pair.hip",
+    "exl3_gemv_epilogue_3inst.hip",
     "exl3_encode.hip",
     "exl3_quantize.hip",
 ]

@@ -248,7 +248,7 @@ int32_t linear_checks(const void *x, int32_t x_dtype, int32_t groups, int32_t ro
 int32_t linear_impl(const void *x, int32_t x_dtype, int32_t groups, int32_t rows, int32_t in, int32_t out,
                     const uint16_t *trellis, int32_t n, const uint16_t *suh, const uint16_t *svh, exl3_decode_t dec,
                     void *y, int32_t y_dtype, void *ws, size_t ws_bytes, hipStream_t stream, bool split_ok = true,
-                    bool y_rows_major = false) {
+                    bool y_rows_major = false, const EpilogueArgs *epi = nullptr) {
     int fam;
     DecodeK k;
     int32_t rc = linear_checks(x, x_dtype, groups, rows, in, out, trellis, n, suh, svh, dec, y, y_dtype, &fam, &k);
@@ -298,6 +298,7 @@ int32_t linear_impl(const void *x, int32_t x_dtype, int32_t groups, int32_t rows
                      ? reinterpret_cast<unsigned long long *>(w)
                      : nullptr;
         a.fold_arrivals = p.splits;
+        if (epi) return launched(run_gemv_epilogue(fam, a, *epi, stream), "exl3_linear_epilogue (gemv)");
         return launched(run_gemv(fam, PRO_X, a, stream), "exl3_linear (gemv)");
     }
     if (y_rows_major) return fail(EXL3_ERR_BAD_SHAPE, "linear: the row-major grouped output serves up to %d rows", kRowsMax);
@@ -323,7 +324,70 @@ int32_t linear_impl(const void *x, int32_t x_dtype, int32_t groups, int32_t rows
         g.kctr = reinterpret_cast<uint32_t *>(w);
         g.kwait = gemm_split_wait(2L * groups * ((rows + 511) / 512) * (out / 128));
     }
+    if (epi) return launched(run_gemm_epilogue(fam, g, *epi, stream), "exl3_linear_epilogue (gemm)");
     return launched(run_gemm(fam, g, stream), "exl3_linear (gemm)");
+}
+
+// The linear with an epilogue and its backward pass run their rows in chunks of at most this many: the prepared input of a
+// chunk stays within the 32-bit offsets the GEMM reads it with, its scratch within half a GiB at a width of 14336, and a
+// chunk of 64 row tiles of 256 fills the GPU by itself.
+int epilogue_chunk(int width) { return width < 65536 ? 16384 : 1024; }
+
+size_t elem_size(int dt) { return dt == EXL3_DT_F32 ? 4 : 2; }
+const void *at_row(const void *p, size_t row, size_t width, int dt) {
+    return p ? static_cast<const char *>(p) + row * width * elem_size(dt) : nullptr;
+}
+void *at_row(void *p, size_t row, size_t width, int dt) {
+    return p ? static_cast<char *>(p) + row * width * elem_size(dt) : nullptr;
+}
+
+int32_t act_check(int32_t act, const char *what) {
+    if (act < 0 || act >= ACT_COUNT) return fail(EXL3_ERR_ACTIVATION, "%s: unknown activation %d", what, act);
+    return ok();
+}
+
+// The backward pass's launch shape for a chunk of `rows` of `total` rows.
+struct GradPlan {
+    int tile_rows, tiles, chunks, splits;
+    size_t amax, dbias_part, inv, u, part;
+    size_t bytes() const { return kZeroBytes + amax + dbias_part + inv + u + part; }
+};
+
+GradPlan plan_grad(int total, int rows, int in, int out) {
+    GradPlan p;
+    // at most 64 row tiles of at least 64 rows: the partial sums of dbias stay few, and 64 tiles of ceil(out / 512)
+    // workgroups fill the GPU from a width of 2048 on
+    p.tile_rows = std::max(64, (total / 64 + 4) / 4 * 4);
+    p.tiles = (total + p.tile_rows - 1) / p.tile_rows;
+    p.chunks = (out + GRAD_SCAN_COLS - 1) / GRAD_SCAN_COLS;
+    // The contraction is split until the workgroups fill the GPU's 256 CUs (one a CU), each split at least two output
+    // groups.
+    const int tiles = in / 128 * ((rows + 255) / 256), groups = out / 128;
+    p.splits = std::max(1, std::min(256 / std::max(tiles, 1), groups / 2));
+    p.amax = align_up((size_t)total * p.chunks * sizeof(float));
+    p.dbias_part = p.tiles > 1 ? align_up((size_t)p.tiles * out * sizeof(float)) : 0;
+    p.inv = align_up((size_t)rows * sizeof(float));
+    p.u = align_up((size_t)((rows + 15) / 16 * 16) * out * 2);
+    p.part = p.splits > 1 ? align_up((size_t)p.splits * rows * in * sizeof(float)) : 0;
+    return p;
+}
+
+// The largest need over the chunks of a call (the last one may be shorter, and then split further).
+size_t grad_ws(int rows, int in, int out) {
+    if (rows <= 0) return 0;
+    const int chunk = std::min(rows, epilogue_chunk(out)), rest = rows % chunk;
+    const size_t whole = plan_grad(rows, chunk, in, out).bytes();
+    return rest ? std::max(whole, plan_grad(rows, rest, in, out).bytes()) : whole;
+}
+
+int32_t router_checks(const void *logits, int32_t dtype, int32_t rows, int32_t experts, int32_t topk, const char *what) {
+    if (rows < 0 || experts <= 0 || experts > kRouterMaxExperts || topk <= 0 || topk > 32 || topk > experts)
+        return fail(EXL3_ERR_BAD_SHAPE, "%s: rows=%d experts=%d k=%d (experts <= %d, k <= 32)", what, rows, experts, topk,
+                    kRouterMaxExperts);
+    if (!dtype_ok(dtype)) return fail(EXL3_ERR_BAD_DTYPE, "%s: unsupported dtype", what);
+    if (rows && (!logits || reinterpret_cast<uintptr_t>(logits) % elem_size(dtype)))
+        return fail(EXL3_ERR_BAD_SHAPE, "%s: null or unaligned logits", what);
+    return ok();
 }
 
 // Rows above which the routed layer takes the sorted arm (slots grouped into expert windows, each expert's tiles
@@ -1423,6 +1487,191 @@ int32_t exl3_route_topk(const float *logits, int32_t rows, int32_t experts, int3
     if (rows == 0) return ok();
     if (!logits || !inds || !scores) return fail(EXL3_ERR_BAD_SHAPE, "route_topk: null operand");
     return launched(run_route_topk(logits, rows, experts, k, inds, scores, stream), "exl3_route_topk");
+}
+
+size_t exl3_linear_epilogue_workspace_size(int32_t rows, int32_t in_features, int32_t out_features, int32_t n) {
+    if (rows <= 0 || in_features <= 0 || out_features <= 0) return 0;
+    const int chunk = std::min(rows, epilogue_chunk(in_features)), rest = rows % chunk;
+    const size_t whole = linear_ws(1, chunk, in_features, out_features, n);
+    return rest ? std::max(whole, linear_ws(1, rest, in_features, out_features, n)) : whole;
+}
+
+int32_t exl3_linear_epilogue(const void *x, int32_t x_dtype, int32_t rows, int32_t in_features, int32_t out_features,
+                             const uint16_t *trellis, int32_t n, const uint16_t *suh, const uint16_t *svh,
+                             exl3_decode_t dec, const void *bias, int32_t bias_dtype, int32_t act, const void *residual,
+                             void *y, int32_t y_dtype, void *pre, void *workspace, size_t workspace_bytes,
+                             hipStream_t stream) {
+    int fam;
+    DecodeK k;
+    int32_t rc = linear_checks(x, x_dtype, 1, rows, in_features, out_features, trellis, n, suh, svh, dec, y, y_dtype,
+                               &fam, &k);
+    if (rc) return rc;
+    rc = act_check(act, "linear_epilogue");
+    if (rc) return rc;
+    if (bias && !dtype_ok(bias_dtype)) return fail(EXL3_ERR_BAD_DTYPE, "linear_epilogue: unsupported bias dtype");
+    for (const void *p : {bias, residual, (const void *)y, (const void *)pre, (const void *)svh})
+        if (reinterpret_cast<uintptr_t>(p) % 4)
+            return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue: bias, residual, y, pre and svh must be 4-byte aligned");
+    if (rows == 0) return ok();
+    const size_t need = exl3_linear_epilogue_workspace_size(rows, in_features, out_features, n);
+    if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
+        return fail(EXL3_ERR_WORKSPACE, "linear_epilogue: workspace of %zu bytes (256-aligned) needed, got %zu", need,
+                    workspace_bytes);
+    const int chunk = epilogue_chunk(in_features);
+    for (int r = 0; r < rows; r += chunk) {
+        EpilogueArgs e{};
+        e.act = act;
+        e.has_bias = bias != nullptr;
+        e.has_residual = residual != nullptr;
+        // the kernels fetch both words ahead of knowing whether they are used: an absent one's from memory that is there
+        e.bias = bias ? bias : svh;
+        e.bias_dtype = bias ? bias_dtype : EXL3_DT_F16;
+        void *yr = at_row(y, r, out_features, y_dtype);
+        e.residual = residual ? at_row(residual, r, out_features, y_dtype) : yr;
+        e.pre = at_row(pre, r, out_features, y_dtype);
+        rc = linear_impl(at_row(x, r, in_features, x_dtype), x_dtype, 1, std::min(chunk, rows - r), in_features,
+                         out_features, trellis, n, suh, svh, dec, yr, y_dtype, workspace, workspace_bytes, stream, true,
+                         false, &e);
+        if (rc) return rc;
+    }
+    return ok();
+}
+
+size_t exl3_linear_epilogue_backward_workspace_size(int32_t rows, int32_t in_features, int32_t out_features) {
+    if (in_features <= 0 || out_features <= 0) return 0;
+    return grad_ws(rows, in_features, out_features);
+}
+
+int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t rows, int32_t in_features,
+                                      int32_t out_features, const uint16_t *trellis, int32_t n, const uint16_t *suh,
+                                      const uint16_t *svh, exl3_decode_t dec, int32_t act, const void *pre, void *dx,
+                                      int32_t dx_dtype, float *dbias, void *workspace, size_t workspace_bytes,
+                                      hipStream_t stream) {
+    int fam;
+    DecodeK k;
+    int32_t rc = linear_checks(dy, dtype, 1, rows, in_features, out_features, trellis, n, suh, svh, dec, dx, dx_dtype,
+                               &fam, &k);
+    if (rc) return rc;
+    rc = act_check(act, "linear_epilogue_backward");
+    if (rc) return rc;
+    if (in_features / 16 > 0xFFFF || out_features / 16 > 0xFFFF)
+        return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: in=%d out=%d", in_features, out_features);
+    if (rows == 0) {
+        if (dbias) return launched(run_fill_zero(dbias, (size_t)out_features * sizeof(float), stream), "dbias");
+        return ok();
+    }
+    if (act != ACT_NONE && !pre) return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: the activation's pre is missing");
+    if ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(pre)) % 16)
+        return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: dy and pre must be 16-byte aligned");
+    const size_t need = grad_ws(rows, in_features, out_features);
+    if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
+        return fail(EXL3_ERR_WORKSPACE, "linear_epilogue_backward: workspace of %zu bytes (256-aligned) needed, got %zu",
+                    need, workspace_bytes);
+    const int chunk = epilogue_chunk(out_features);
+    GradArgs a{};
+    a.dy = dy;
+    a.pre = act == ACT_NONE ? nullptr : pre;
+    a.dtype = dtype;
+    a.act = act;
+    a.rows = rows;
+    a.in = in_features;
+    a.out = out_features;
+    a.trellis = trellis;
+    a.n = n;
+    a.suh = suh;
+    a.svh = svh;
+    a.k = k;
+    a.dbias = dbias;
+    a.dx_dtype = dx_dtype;
+    const GradPlan p = plan_grad(rows, std::min(rows, chunk), in_features, out_features);
+    char *w = static_cast<char *>(workspace) + kZeroBytes;
+    a.tile_rows = p.tile_rows;
+    a.chunks = p.chunks;
+    a.amax = reinterpret_cast<float *>(w);
+    w += p.amax;
+    a.dbias_part = reinterpret_cast<float *>(w);
+    w += p.dbias_part;
+    a.inv_scale = reinterpret_cast<float *>(w);
+    w += p.inv;
+    hipError_t e = run_grad_scan(a, stream);
+    if (e != hipSuccess) return launched(e, "exl3_linear_epilogue_backward (scan)");
+    for (int r = 0; r < rows; r += chunk) {
+        GradArgs c = a;
+        c.rows = std::min(chunk, rows - r);
+        const GradPlan q = plan_grad(rows, c.rows, in_features, out_features);
+        c.dy = at_row(dy, r, out_features, dtype);
+        c.pre = at_row(a.pre, r, out_features, dtype);
+        c.amax = a.amax + (size_t)r * p.chunks;
+        c.u = reinterpret_cast<uint16_t *>(w);
+        c.part = reinterpret_cast<float *>(w + q.u);
+        c.splits = q.splits;
+        c.dx = at_row(dx, r, in_features, dx_dtype);
+        e = run_grad_gemm(fam, c, stream);
+        if (e != hipSuccess) return launched(e, "exl3_linear_epilogue_backward");
+    }
+    return ok();
+}
+
+size_t exl3_balance_loss_workspace_size(int32_t rows, int32_t experts) {
+    if (rows < 0 || experts <= 0 || experts > kRouterMaxExperts) return 0;
+    const size_t parts = (size_t)balance_parts(rows, experts);
+    return kZeroBytes + (parts > 1 ? 2 * align_up(parts * experts * 4) + align_up(parts * 4) : 0);
+}
+
+int32_t exl3_balance_loss(const void *logits, int32_t dtype, int32_t rows, int32_t experts, const uint32_t *inds,
+                          int32_t topk, const uint8_t *mask, float coef, float *loss, int32_t *counts, float *weight,
+                          void *workspace, size_t workspace_bytes, hipStream_t stream) {
+    int32_t rc = router_checks(logits, dtype, rows, experts, topk, "balance_loss");
+    if (rc) return rc;
+    if ((rows && !inds) || !loss || !counts || !weight) return fail(EXL3_ERR_BAD_SHAPE, "balance_loss: null operand");
+    const size_t need = exl3_balance_loss_workspace_size(rows, experts);
+    if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
+        return fail(EXL3_ERR_WORKSPACE, "balance_loss: workspace of %zu bytes (256-aligned) needed, got %zu", need,
+                    workspace_bytes);
+    const size_t parts = (size_t)balance_parts(rows, experts), plane = align_up(parts * experts * 4);
+    char *w = static_cast<char *>(workspace) + kZeroBytes;
+    BalanceArgs a{};
+    a.logits = logits;
+    a.dtype = dtype;
+    a.rows = rows;
+    a.experts = experts;
+    a.topk = topk;
+    a.inds = inds;
+    a.mask = mask;
+    a.coef = coef;
+    a.loss = loss;
+    a.counts = counts;
+    a.weight = weight;
+    if (parts > 1) {
+        a.part_sum = reinterpret_cast<float *>(w);
+        a.part_count = reinterpret_cast<int *>(w + plane);
+        a.part_live = reinterpret_cast<int *>(w + 2 * plane);
+    }
+    return launched(run_balance_loss(a, stream), "exl3_balance_loss");
+}
+
+int32_t exl3_router_backward(const void *logits, int32_t dtype, int32_t rows, int32_t experts, const uint32_t *inds,
+                             int32_t topk, const float *dscores, const float *weight, const float *dloss,
+                             const uint8_t *mask, void *dlogits, hipStream_t stream) {
+    int32_t rc = router_checks(logits, dtype, rows, experts, topk, "router_backward");
+    if (rc) return rc;
+    if ((weight != nullptr) != (dloss != nullptr))
+        return fail(EXL3_ERR_BAD_SHAPE, "router_backward: the balance term takes both weight and dloss");
+    if (rows == 0) return ok();
+    if (!dlogits || (dscores && !inds)) return fail(EXL3_ERR_BAD_SHAPE, "router_backward: null operand");
+    RouterGradArgs a{};
+    a.logits = logits;
+    a.dtype = dtype;
+    a.rows = rows;
+    a.experts = experts;
+    a.topk = topk;
+    a.inds = inds;
+    a.dscores = dscores;
+    a.weight = weight;
+    a.dloss = dloss;
+    a.mask = mask;
+    a.dlogits = dlogits;
+    return launched(run_router_backward(a, stream), "exl3_router_backward");
 }
 
 int32_t exl3_tile_major(const uint16_t *src, uint16_t *dst, int32_t experts, int32_t it, int32_t ot, int32_t n,

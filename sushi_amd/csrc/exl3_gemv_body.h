@@ -23,6 +23,7 @@
 #include "exl3_kernels.h"
 #include "exl3_tables.h"
 #include "exl3_lane_decode.h"
+#include "exl3_epilogue.h"
 
 namespace exl3 {
 
@@ -98,9 +99,20 @@ struct GemvCtx {
     float sv0, sv1;             // svh of this lane's two outputs, fetched at entry for the finish
 };
 
-// Output FWHT + svh for one row of a 128-output block held as (v0 = col lane, v1 = col lane + 64).
+// Output FWHT + svh for one row of a 128-output block held as (v0 = col lane, v1 = col lane + 64).  EPI: then the
+// epilogue e, its bias and residual words fetched ahead of the transform.
+template <bool EPI>
 __device__ __forceinline__ void finish_block(const GemvArgs &a, const GemvCtx &c, int rho, float v0, float v1,
-                                             int lane) {
+                                             int lane, const EpilogueArgs *e) {
+    if constexpr (EPI) {
+        const size_t col = (size_t)c.og * 128 + lane, i = ((size_t)c.g * a.rows + rho) * a.out + col;
+        const EpilogueWords w = epilogue_fetch(*e, a.y_dtype, col, i);
+        fwht128_wave(v0, v1, lane);
+        store_y(a.y, a.y_dtype, i, epilogue_apply(*e, a.y_dtype, v0 * HAD_SCALE * c.sv0, w.b0, col, w.r0, i));
+        store_y(a.y, a.y_dtype, i + 64,
+                epilogue_apply(*e, a.y_dtype, v1 * HAD_SCALE * c.sv1, w.b1, col + 64, w.r1, i + 64));
+        return;
+    }
     fwht128_wave(v0, v1, lane);
     const size_t yrow = a.y_rows_major ? (size_t)rho * a.groups + c.g : (size_t)c.g * a.rows + rho;
     const size_t yo = yrow * a.out + (size_t)c.og * 128;
@@ -395,9 +407,11 @@ __device__ __forceinline__ float fold_value(unsigned long long t, int S, unsigne
 // and the completing arrival rounds the routed sum to y's dtype before adding the shared expert.  MOE (the down
 // projection's PRO_MID kernels) is a compile-time choice: the dense kernels carry none of the slot, score and
 // shared-expert handling.
-template <int RT, bool WIN, bool MOE, bool SH>
+// EPI: the epilogue runs in the completing arrival, on the whole sum; every arrival fetches the bias and residual words
+// ahead of its adds, so the completing one does not wait for them after its own.
+template <int RT, bool WIN, bool MOE, bool SH, bool EPI>
 __device__ __forceinline__ void fold_finish(const GemvArgs &a, const GemvCtx &c, float (*red)[RT][128], int wave,
-                                            int lane) {
+                                            int lane, const EpilogueArgs *e) {
     for (int r = wave; r < c.rows; r += GEMV_WAVES) {
         float v0 = 0.f, v1 = 0.f;
 #pragma unroll
@@ -428,6 +442,9 @@ __device__ __forceinline__ void fold_finish(const GemvArgs &a, const GemvCtx &c,
         const unsigned long long t0 = fold_term(f0), t1 = fold_term(f1);
         const size_t yo = yrow * a.out + (size_t)c.og * 128;
         unsigned long long *w0 = (shared ? a.sh_fold : a.fold) + yo + lane, *w1 = w0 + 64;
+        const size_t col = (size_t)c.og * 128 + lane;
+        EpilogueWords ew{};
+        if constexpr (EPI) ew = epilogue_fetch(*e, a.y_dtype, col, yo + lane);
         fold_overflow(w0, w1, f0, f1);
         const unsigned long long o0 = __hip_atomic_fetch_add(w0, t0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const unsigned long long o1 = __hip_atomic_fetch_add(w1, t1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -437,13 +454,15 @@ __device__ __forceinline__ void fold_finish(const GemvArgs &a, const GemvCtx &c,
         if constexpr (!MOE) {
             // Both outcomes are settled before either store, so no store waits on the other output's check.
             const bool d0 = (o0 >> FOLD_COUNT_SHIFT) == last, d1 = (o1 >> FOLD_COUNT_SHIFT) == last;
-            const float y0 = d0 ? fold_value(o0 + t0, arrivals, w0) : 0.f;
-            const float y1 = d1 ? fold_value(o1 + t1, arrivals, w1) : 0.f;
+            float y0 = d0 ? fold_value(o0 + t0, arrivals, w0) : 0.f;
+            float y1 = d1 ? fold_value(o1 + t1, arrivals, w1) : 0.f;
             if (d0) {
+                if constexpr (EPI) y0 = epilogue_apply(*e, a.y_dtype, y0, ew.b0, col, ew.r0, yo + lane);
                 store_y(a.y, a.y_dtype, yo + lane, y0);
                 *w0 = 0ull;  // no split of this launch touches it again; the next launch reads it after the boundary
             }
             if (d1) {
+                if constexpr (EPI) y1 = epilogue_apply(*e, a.y_dtype, y1, ew.b1, col + 64, ew.r1, yo + lane + 64);
                 store_y(a.y, a.y_dtype, yo + lane + 64, y1);
                 *w1 = 0ull;
             }
@@ -524,10 +543,11 @@ __device__ __forceinline__ void chain_wait(const GemvArgs &a, const GemvCtx &c, 
 
 // CH: the fused chain's role (0 none; 1 gate/up: planes written through, then the group's arrival counted; 2 down:
 // tile loads, then the wait, then the mid from the planes past the L2).
-template <int FAM, int N, int RT, int PRO, bool WIN, bool SH, bool PIN = false, int CH = 0>
+// EPI: a dense launch with the epilogue e.
+template <int FAM, int N, int RT, int PRO, bool WIN, bool SH, bool PIN = false, int CH = 0, bool EPI = false>
 __device__ __forceinline__ void gemv_body(const GemvArgs &a, GemvCtx &c, const uint16_t *__restrict__ tb,
                                           int n, const DecodeK &k, uint16_t (*xs)[XS_PITCH], float (*red)[RT][128],
-                                          const TiledSrc &ts = TiledSrc{}) {
+                                          const TiledSrc &ts = TiledSrc{}, const EpilogueArgs *e = nullptr) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform: branches on it stay scalar
     const int o = lane >> 3, j = lane & 7;
@@ -649,7 +669,7 @@ __device__ __forceinline__ void gemv_body(const GemvArgs &a, GemvCtx &c, const u
     }
     __syncthreads();
     if (a.fold) {  // the host enables the fold only for split dense launches and the MoE down projection
-        fold_finish<RT, WIN, PRO == PRO_MID, SH>(a, c, red, wave, lane);
+        fold_finish<RT, WIN, PRO == PRO_MID, SH, EPI>(a, c, red, wave, lane, e);
         return;
     }
     const bool direct = c.S == 1 && !a.partial_only;
@@ -662,7 +682,8 @@ __device__ __forceinline__ void gemv_body(const GemvArgs &a, GemvCtx &c, const u
             red[0][r][col] = s * a.out_scale;
         }
         __syncthreads();
-        for (int r = wave; r < c.rows; r += GEMV_WAVES) finish_block(a, c, r, red[0][r][lane], red[0][r][lane + 64], lane);
+        for (int r = wave; r < c.rows; r += GEMV_WAVES)
+            finish_block<EPI>(a, c, r, red[0][r][lane], red[0][r][lane + 64], lane, e);
         return;
     }
 
@@ -713,14 +734,14 @@ __device__ __forceinline__ void gemv_body(const GemvArgs &a, GemvCtx &c, const u
             float v0, v1;
             sum_planes<false>(part + (((size_t)c.g * c.S) * a.rows + r) * a.out + (size_t)c.og * 128,
                               (size_t)a.rows * a.out, c.S, lane, v0, v1);
-            finish_block(a, c, r, v0, v1, lane);
+            finish_block<EPI>(a, c, r, v0, v1, lane, e);
         }
     } else {
         for (int r = 0; r < c.rows; r++) {
             float v0, v1;
             sum_planes<true>(part + (((size_t)c.g * c.S) * a.rows + r) * a.out + (size_t)c.og * 128,
                              (size_t)a.rows * a.out, c.S, lane, v0, v1);
-            finish_block(a, c, r, v0, v1, lane);
+            finish_block<EPI>(a, c, r, v0, v1, lane, e);
         }
     }
     if (lane == 0) *ctr = 0u;  // every split has arrived: the next launch reads it after the kernel boundary
@@ -739,11 +760,12 @@ __device__ __forceinline__ DecodeK rate_constants(const GemvArgs &a, int n) {
 // shared expert).
 // L: the workgroup's index within the group's (output group, split) grid; gy: the group's index in the grid (the
 // fused chain's counters); proj: the projection.  CH: the fused chain's role (gemv_body).
-template <int FAM, int N, int RT, int PRO, bool WIN, bool SH, int CH = 0>
+// EPI: a dense launch with the epilogue e.
+template <int FAM, int N, int RT, int PRO, bool WIN, bool SH, int CH = 0, bool EPI = false>
 __device__ __forceinline__ void gemv_group(int g, const void *x, const uint16_t *tr0, const uint16_t *suh0,
                                            const uint32_t *bank_of, const GemvGeo &geo, int rows, int x_dtype,
                                            const GemvArgs &a, uint16_t (*xs)[XS_PITCH], float (*red)[RT][128], int L,
-                                           int gy, int proj) {
+                                           int gy, int proj, const EpilogueArgs *e = nullptr) {
     GemvCtx c;
     c.x = x;
     c.x_div_m = geo.xdiv_m;
@@ -809,7 +831,8 @@ __device__ __forceinline__ void gemv_group(int g, const void *x, const uint16_t 
     if constexpr (N >= 0) {
         const int n = N ? N : a.n;
         const uint16_t *tb = trellis + (size_t)c.bank * c.IT * c.OT * n;
-        gemv_body<FAM, N, RT, PRO, WIN, SH, (N > 0 && !WIN && !SH && CH == 0), CH>(a, c, tb, n, a.k, xs, red);
+        gemv_body<FAM, N, RT, PRO, WIN, SH, (N > 0 && !WIN && !SH && CH == 0), CH, EPI>(a, c, tb, n, a.k, xs, red,
+                                                                                               TiledSrc{}, e);
     } else if constexpr (N == N_TILED) {
         // Per-tile-rate bank: every tile at TILED_NA or TILED_NB, read through the projection's segment tables (a
         // fused shared expert keeps its own uniform rate, a lane-reader rate the host checked).
@@ -915,6 +938,21 @@ __global__ __launch_bounds__(GEMV_THREADS) void gemv_kernel(const void *x, const
                                             blockIdx.z);
 }
 
+// gemv_kernel for a dense linear with an epilogue: the same preloaded arguments and body.
+template <int FAM, int N, int RT>
+__global__ __launch_bounds__(GEMV_THREADS) void gemv_epilogue_kernel(const void *x, const uint16_t *tr0,
+                                                                     const uint16_t *suh0, const uint32_t *bank_of,
+                                                                     uint32_t tiles, uint32_t sks, uint32_t s_m,
+                                                                     uint32_t xdiv_m, int rows_dt, GemvArgs a,
+                                                                     EpilogueArgs e) {
+    const GemvGeo geo{tiles, sks, s_m, xdiv_m};
+    __shared__ __align__(16) uint16_t xs[RT][XS_PITCH];
+    __shared__ float red[GEMV_WAVES * RT * 128];
+    gemv_group<FAM, N, RT, PRO_X, false, false, 0, true>(blockIdx.y, x, tr0, suh0, bank_of, geo, rows_dt & 0xFFFF,
+                                                         rows_dt >> 16, a, xs, reinterpret_cast<float (*)[RT][128]>(red),
+                                                         blockIdx.x, blockIdx.y, 0, &e);
+}
+
 // The per-slot decode chain in one launch (run_moe_chain): a 1D grid of w1 gate/up workgroups (a1, PRO_X, grid
 // order x = (output group, split), then group, then projection, as gemv_kernel's) and then the down workgroups (a2,
 // PRO_MID).  Workgroups start in index order on each XCD, so when a down workgroup starts every gate/up workgroup
@@ -957,8 +995,8 @@ __global__ __launch_bounds__(GEMV_THREADS) void moe_chain_kernel(GemvArgs a1, Ge
 }
 
 // Separate finish: one wave per (output group, row, group, projection).
-template <int FAM>
-__global__ __launch_bounds__(64) void gemv_finish_kernel(GemvArgs a) {
+template <int FAM, bool EPI>
+__device__ __forceinline__ void gemv_finish(const GemvArgs &a, const EpilogueArgs *e) {
     GemvCtx c;
     c.og = blockIdx.x;
     const int r = blockIdx.y % a.rows;
@@ -976,7 +1014,15 @@ __global__ __launch_bounds__(64) void gemv_finish_kernel(GemvArgs a) {
     float v0, v1;
     sum_planes<false>(part + (((size_t)c.g * a.splits) * a.rows + r) * a.out + (size_t)c.og * 128,
                       (size_t)a.rows * a.out, a.splits, lane, v0, v1);
-    finish_block(a, c, r, v0, v1, lane);
+    finish_block<EPI>(a, c, r, v0, v1, lane, e);
+}
+template <int FAM>
+__global__ __launch_bounds__(64) void gemv_finish_kernel(GemvArgs a) {
+    gemv_finish<FAM, false>(a, nullptr);
+}
+template <int FAM>
+__global__ __launch_bounds__(64) void gemv_finish_epilogue_kernel(GemvArgs a, EpilogueArgs e) {
+    gemv_finish<FAM, true>(a, &e);
 }
 
 template <int FAM, int N, int RT, int PRO, bool WIN, bool SHP = false>
@@ -993,13 +1039,17 @@ static void launch_slot(const GemvArgs &a, dim3 grid, hipStream_t s) {  // one r
     else launch_one<FAM, N, 1, PRO, false, false>(a, grid, s);
 }
 
+// The block-to-tile map's packed fields (gemv_geo) and its divisions' exactness; x rows are found as slot / x_div for up
+// to 2^24 slots.
+static bool gemv_map_ok(const GemvArgs &a) {
+    return a.in / 16 <= 0xFFFF && a.out / 16 <= 0xFFFF && a.splits >= 1 && (a.in / 16) % a.splits == 0 && a.x_div >= 1 &&
+           a.x_div <= 255 && (unsigned long long)(a.out / 128) * a.splits * (unsigned)a.splits < (1ull << 32);
+}
+
 template <int FAM, int N, int PRO>
 static hipError_t launch_gemv_n(const GemvArgs &a, hipStream_t s) {
     const int G = a.out / 128;
-    // the block-to-tile map's packed fields (gemv_geo) and its divisions' exactness
-    if (a.in / 16 > 0xFFFF || a.out / 16 > 0xFFFF || a.splits < 1 || (a.in / 16) % a.splits || a.x_div < 1 ||
-        a.x_div > 255 || (unsigned long long)G * a.splits * (unsigned)a.splits >= (1ull << 32))
-        return hipErrorInvalidValue;  // x rows are found as slot / x_div for up to 2^24 slots
+    if (!gemv_map_ok(a)) return hipErrorInvalidValue;
     dim3 grid((unsigned)(G * a.splits), (unsigned)a.groups, (unsigned)a.nproj);
     if (a.win_count) {  // the sorted MoE arm: expert windows of MOE_WINDOW_ROWS rows, f32 planes or the fold out
         if (a.rows != MOE_WINDOW_ROWS || !(a.partial_only || a.fold)) return hipErrorInvalidValue;
@@ -1098,10 +1148,63 @@ static hipError_t launch_gemv_fam(const GemvArgs &a, hipStream_t s) {
     return launch_gemv_n<FAM, 0, PRO>(a, s);
 }
 
-#ifdef EXL3_GEMV_FAM
-// One translation unit per codebook family (compiled in parallel): exl3_gemv_<family>.hip defines EXL3_GEMV_FAM.
+// A dense linear of up to 16 rows with an epilogue.
+template <int FAM, int N>
+static hipError_t launch_gemv_epilogue_n(const GemvArgs &a, const EpilogueArgs &e, hipStream_t s) {
+    if (!gemv_map_ok(a) || a.rows < 1 || a.rows > 16 || a.nproj != 1 || a.partial_only || a.y_rows_major)
+        return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(a.out / 128 * a.splits), (unsigned)a.groups);
+    const GemvGeo geo = gemv_geo(a);
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, grid, dim3(GEMV_THREADS), 0, s, a.x, a.trellis[0], a.suh[0], a.bank_of, geo.tiles, geo.sks,
+                           geo.s_m, geo.xdiv_m, a.rows | (a.x_dtype << 16), a, e);
+    };
+    if (a.rows <= 1) go(gemv_epilogue_kernel<FAM, N, 1>);
+    else if (a.rows <= 2) go(gemv_epilogue_kernel<FAM, N, 2>);
+    else if (a.rows <= 4) go(gemv_epilogue_kernel<FAM, N, 4>);
+    else if (a.rows <= 8) go(gemv_epilogue_kernel<FAM, N, 8>);
+    else go(gemv_epilogue_kernel<FAM, N, 16>);
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess || a.splits == 1 || a.fused_finish) return err;
+    hipLaunchKernelGGL(gemv_finish_epilogue_kernel<FAM>, dim3((unsigned)(a.out / 128), (unsigned)(a.rows * a.groups)),
+                       dim3(64), 0, s, a, e);
+    return hipGetLastError();
+}
+
+template <int FAM>
+static hipError_t launch_gemv_epilogue_fam(const GemvArgs &a, const EpilogueArgs &e, hipStream_t s) {
+    switch (a.n) {
+    case 16: return launch_gemv_epilogue_n<FAM, 16>(a, e, s);
+    case 24: return launch_gemv_epilogue_n<FAM, 24>(a, e, s);
+    case 32: return launch_gemv_epilogue_n<FAM, 32>(a, e, s);
+    case 40: return launch_gemv_epilogue_n<FAM, 40>(a, e, s);
+    case 48: return launch_gemv_epilogue_n<FAM, 48>(a, e, s);
+    case 64: return launch_gemv_epilogue_n<FAM, 64>(a, e, s);
+    default: break;
+    }
+    if constexpr (FAM != FAM_PAIR) {
+        switch (a.n) {
+        case 80: return launch_gemv_epilogue_n<FAM, 80>(a, e, s);
+        case 96: return launch_gemv_epilogue_n<FAM, 96>(a, e, s);
+        case 112: return launch_gemv_epilogue_n<FAM, 112>(a, e, s);
+        case 128: return launch_gemv_epilogue_n<FAM, 128>(a, e, s);
+        default: break;
+        }
+    }
+    return launch_gemv_epilogue_n<FAM, 0>(a, e, s);
+}
+
 #define EXL3_CAT2(a, b) a##b
 #define EXL3_CAT(a, b) EXL3_CAT2(a, b)
+#ifdef EXL3_GEMV_EPILOGUE_FAM
+// exl3_gemv_epilogue_<family>.hip: the dense launches with an epilogue.
+hipError_t EXL3_CAT(run_gemv_epilogue_, EXL3_GEMV_EPILOGUE_FAM)(const GemvArgs &a, const EpilogueArgs &e, hipStream_t s) {
+    return launch_gemv_epilogue_fam<EXL3_GEMV_EPILOGUE_FAM>(a, e, s);
+}
+#endif
+
+#ifdef EXL3_GEMV_FAM
+// One translation unit per codebook family (compiled in parallel): exl3_gemv_<family>.hip defines EXL3_GEMV_FAM.
 hipError_t EXL3_CAT(run_gemv_fam_, EXL3_GEMV_FAM)(int prologue, const GemvArgs &a, hipStream_t s) {
     return prologue == PRO_MID ? launch_gemv_fam<EXL3_GEMV_FAM, PRO_MID>(a, s)
                                : launch_gemv_fam<EXL3_GEMV_FAM, PRO_X>(a, s);

@@ -19,6 +19,21 @@ hipError_t run_reconstruct_tiled(int fam, const uint16_t *trellis, const uint32_
 
 enum Prologue : int { PRO_X = 0, PRO_MID = 1 };
 
+// What a dense linear does to its finished sums (exl3_epilogue.h): z = sum + bias[col], y = T(act(z) + residual), pre = T(z).
+// bias [out] in bias_dtype; residual and pre [rows][out] in y's dtype, as y is laid out (one bank).  bias and residual are
+// always readable: the host points an absent one at svh / y and clears its flag.  Launches with an epilogue are kernels of
+// their own (the translation units exl3_*_epilogue*.hip): as a run-time choice its code and scalars slowed the plain ones
+// (one row of 4096 x 4096, n = 64: 7.1 -> 7.45 us; 2048 rows of 4096 x 14336 by 0.5%).
+enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_COUNT = 5 };
+struct EpilogueArgs {
+    int act;
+    int has_bias, has_residual;
+    int bias_dtype;
+    const void *bias;
+    const void *residual;
+    void *pre;
+};
+
 // Fused-finish arrival counters sit one per 128-byte line (32 words) in the workspace's counter region.
 constexpr int COUNTER_STRIDE = 32;
 
@@ -163,6 +178,12 @@ constexpr int MOE_WINDOW_ROWS = 4;
 constexpr int SH_ROWS = 4;
 
 hipError_t run_gemv(int fam, int prologue, const GemvArgs &a, hipStream_t s);
+hipError_t run_gemv_epilogue(int fam, const GemvArgs &a, const EpilogueArgs &e, hipStream_t s);  // dense, one bank
+hipError_t run_gemv_epilogue_FAM_MCG(const GemvArgs &a, const EpilogueArgs &e, hipStream_t s);
+hipError_t run_gemv_epilogue_FAM_MUL1(const GemvArgs &a, const EpilogueArgs &e, hipStream_t s);
+hipError_t run_gemv_epilogue_FAM_HASH(const GemvArgs &a, const EpilogueArgs &e, hipStream_t s);
+hipError_t run_gemv_epilogue_FAM_PAIR(const GemvArgs &a, const EpilogueArgs &e, hipStream_t s);
+hipError_t run_gemv_epilogue_FAM_3INST(const GemvArgs &a, const EpilogueArgs &e, hipStream_t s);
 hipError_t run_gemv_fam_FAM_MCG(int prologue, const GemvArgs &a, hipStream_t s);
 hipError_t run_gemv_fam_FAM_MUL1(int prologue, const GemvArgs &a, hipStream_t s);
 hipError_t run_gemv_fam_FAM_HASH(int prologue, const GemvArgs &a, hipStream_t s);
@@ -323,9 +344,69 @@ inline size_t gemm_kpart_bytes(int groups, int rows, int out) {
     return (size_t)groups * ((rows + 511) / 512) * (out / 128) * 2 * 512 * 128 * sizeof(float);
 }
 hipError_t run_gemm(int fam, const GemmArgs &a, hipStream_t s);
+hipError_t run_gemm_epilogue(int fam, const GemmArgs &a, const EpilogueArgs &e, hipStream_t s);  // one bank
+
+// The backward pass of a linear with an epilogue (exl3_gradient.hip).  Rows are a chunk's for run_grad_gemm and all of
+// them for run_grad_scan; amax, inv_scale, dy, pre and dx point at the chunk's first row.
+constexpr int GRAD_SCAN_COLS = 512;  // columns of a scan workgroup (a.chunks = ceil(out / that))
+struct GradArgs {
+    const void *dy;         // [rows][out], 16-byte aligned
+    const void *pre;        // the forward's z, like dy; unread with ACT_NONE
+    int dtype;              // of dy and pre
+    int act;
+    int rows, in, out;
+    const uint16_t *trellis;
+    int n;
+    const uint16_t *suh, *svh;
+    DecodeK k;
+    int tile_rows;          // rows per row tile of the scan
+    int chunks;
+    float *amax;            // [rows][chunks]
+    float *dbias;           // [out] or null
+    float *dbias_part;      // [row tiles][out], with more than one tile
+    float *inv_scale;       // [rows]
+    uint16_t *u;            // prepared gradient, 16-row fragment tiles
+    int splits;             // of the contraction, at most out / 128
+    float *part;            // [splits][rows][in] with more than one split
+    void *dx;
+    int dx_dtype;
+};
+hipError_t run_grad_scan(const GradArgs &a, hipStream_t s);
+hipError_t run_grad_gemm(int fam, const GradArgs &a, hipStream_t s);
 
 hipError_t run_route_topk(const float *logits, int rows, int experts, int k, uint32_t *inds, float *scores,
                           hipStream_t s);
+// The router's balance loss and the gradient of its logits (exl3_router.hip).  mask [rows] bytes (0: a padded row) or null;
+// inds [rows][topk], an id past the experts is a dropped slot; logits [rows][experts] in dtype.
+constexpr int kRouterMaxExperts = 1024;
+constexpr int kBalanceMaxParts = 512;
+struct BalanceArgs {
+    const void *logits;
+    int dtype, rows, experts, topk;
+    const uint32_t *inds;
+    const uint8_t *mask;
+    float coef;
+    float *loss;      // [1]
+    int32_t *counts;  // [experts]
+    float *weight;    // [experts]: the loss's derivative by each expert's sum of probabilities
+    float *part_sum;  // [parts][experts], with more than one part
+    int *part_count;  // [parts][experts]
+    int *part_live;   // [parts]
+};
+struct RouterGradArgs {
+    const void *logits;
+    int dtype, rows, experts, topk;
+    const uint32_t *inds;    // with dscores
+    const float *dscores;    // [rows][topk] or null
+    const float *weight;     // [experts] or null: no balance term
+    const float *dloss;      // [1], with weight
+    const uint8_t *mask;
+    void *dlogits;           // like logits
+};
+int balance_parts(int rows, int experts);
+hipError_t run_balance_loss(const BalanceArgs &a, hipStream_t s);
+hipError_t run_router_backward(const RouterGradArgs &a, hipStream_t s);
+
 hipError_t run_tile_major(const uint16_t *src, uint16_t *dst, int experts, int it, int ot, int n, int inverse,
                           hipStream_t s);
 hipError_t run_fill_zero(void *p, size_t bytes, hipStream_t s);

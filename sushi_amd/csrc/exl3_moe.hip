@@ -10,6 +10,16 @@
 
 namespace exl3 {
 
+hipError_t run_gemv_epilogue(int fam, const GemvArgs &a, const EpilogueArgs &e, hipStream_t s) {
+    switch (fam) {
+    case FAM_MCG: return run_gemv_epilogue_FAM_MCG(a, e, s);
+    case FAM_MUL1: return run_gemv_epilogue_FAM_MUL1(a, e, s);
+    case FAM_HASH: return run_gemv_epilogue_FAM_HASH(a, e, s);
+    case FAM_PAIR: return run_gemv_epilogue_FAM_PAIR(a, e, s);
+    default: return run_gemv_epilogue_FAM_3INST(a, e, s);
+    }
+}
+
 hipError_t run_gemv(int fam, int prologue, const GemvArgs &a, hipStream_t s) {
     switch (fam) {
     case FAM_MCG: return run_gemv_fam_FAM_MCG(prologue, a, s);

@@ -17,7 +17,7 @@ import contextlib
 import ctypes
 import enum
 from dataclasses import dataclass, field
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -94,6 +94,11 @@ class HessianNotPositiveDefinite(Exl3Error):
 
 class Exl3GroupMissing(Exl3Error):
     status = -16
+
+
+class Exl3ActivationUnknown(Exl3Error):
+    """A linear's epilogue takes the activations of ``ACTIVATIONS``."""
+    status = -17
 
 
 _BY_STATUS = {c.status: c for c in Exl3Error.__subclasses__()}
@@ -654,6 +659,99 @@ def linear_pair(x: torch.Tensor, a: Proj, b: Proj, dec_a: Decode, dec_b: Decode)
 
 
 # ---------------------------------------------------------------------------------------------------------------
+# Dense linears with an epilogue, and their gradients over frozen weights (extensions: the reference has neither)
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def _act(act: str) -> int:
+    try:
+        return ACTIVATIONS[act]
+    except (KeyError, TypeError):
+        raise Exl3ActivationUnknown(f"activation {act!r} (one of {', '.join(ACTIVATIONS)})") from None
+
+
+def _one_bank(p: Proj, dec: Decode, what: str) -> None:
+    if p.trellis.dim() != 4 or p.trellis.shape[0] != 1 or tuple(p.suh.shape) != (1, p.in_features) or \
+            tuple(p.svh.shape) != (1, p.out_features):
+        raise BadExl3Shape(f"{what}: trellis {tuple(p.trellis.shape)}, suh {tuple(p.suh.shape)}, svh "
+                           f"{tuple(p.svh.shape)} are not one bank's")
+    dec.require_table()
+    _u16_check(p.trellis, "trellis")
+    _f16_check(p.suh, "suh")
+    _f16_check(p.svh, "svh")
+
+
+def _on_one_device(what: str, *ts: Optional[torch.Tensor]) -> torch.device:
+    """The device of the operands, all of them contiguous tensors of one GPU."""
+    _need_gpu(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise BadExl3Shape(f"{what}: operands on {sorted(str(d) for d in devs)}")
+    return devs.pop()
+
+
+def linear_epilogue(x: torch.Tensor, p: Proj, dec: Decode, bias: Optional[torch.Tensor] = None, act: str = "none",
+                    residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                    with_pre: bool = False):
+    """act(linear(x) + bias) + residual in one pass: x [rows, in] -> y [rows, out] in ``out_dtype`` (x's by default),
+    rounded once.  bias [out] (f16, bf16 or f32), residual [rows, out] in y's dtype; ``act`` is one of ``ACTIVATIONS``.
+    ``with_pre`` returns (y, pre) with pre = linear(x) + bias in y's dtype, which linear_epilogue_backward takes.
+    Not recorded by autograd."""
+    if x.dim() != 2 or p.in_features != x.shape[1]:
+        raise BadExl3Shape(f"linear_epilogue: x {tuple(x.shape)} vs trellis {tuple(p.trellis.shape)}")
+    _one_bank(p, dec, "linear_epilogue")
+    code = _act(act)
+    rows, in_f, out_f = int(x.shape[0]), p.in_features, p.out_features
+    dt = out_dtype or x.dtype
+    if bias is not None and tuple(bias.shape) != (out_f,):
+        raise BadExl3Shape(f"linear_epilogue: bias {tuple(bias.shape)}, expected {(out_f,)}")
+    if residual is not None and (tuple(residual.shape) != (rows, out_f) or residual.dtype != dt):
+        raise BadExl3Shape(f"linear_epilogue: residual {tuple(residual.shape)} {residual.dtype}, expected "
+                           f"{(rows, out_f)} in y's {dt}")
+    dev = _on_one_device("linear_epilogue", x, p.trellis, p.suh, p.svh, bias, residual)
+    with torch.cuda.device(dev):
+        y = torch.empty(rows, out_f, dtype=dt, device=dev)
+        pre = torch.empty_like(y) if with_pre else None
+        L = _lib.load()
+        ws = workspace.get(dev, L.exl3_linear_epilogue_workspace_size(rows, in_f, out_f, p.n))
+        _check(L.exl3_linear_epilogue(x.data_ptr(), _dt(x, "x"), rows, in_f, out_f, p.trellis.data_ptr(), p.n,
+                                      p.suh.data_ptr(), p.svh.data_ptr(), dec.c(), _ptr(bias),
+                                      0 if bias is None else _dt(bias, "bias"), code, _ptr(residual), y.data_ptr(),
+                                      _dt(y, "y"), _ptr(pre), ws.data_ptr(), ws.numel(), _stream(dev)))
+    return (y, pre) if with_pre else y
+
+
+def linear_epilogue_backward(dy: torch.Tensor, p: Proj, dec: Decode, act: str = "none",
+                             pre: Optional[torch.Tensor] = None, with_dbias: bool = False,
+                             dx_dtype: Optional[torch.dtype] = None):
+    """The gradients of linear_epilogue (and, with no activation, of linear) with respect to x and bias, the weights
+    frozen: dy [rows, out] -> (dx [rows, in] in ``dx_dtype``, dy's by default; dbias [out] f32, or None without
+    ``with_dbias``).  ``pre`` is the forward's, in dy's dtype, and needed with an activation.  The residual's gradient is
+    dy itself.  Every sum has a fixed order: equal calls give equal bits."""
+    if dy.dim() != 2 or p.out_features != dy.shape[1]:
+        raise BadExl3Shape(f"linear_epilogue_backward: dy {tuple(dy.shape)} vs trellis {tuple(p.trellis.shape)}")
+    _one_bank(p, dec, "linear_epilogue_backward")
+    code = _act(act)
+    rows, in_f, out_f = int(dy.shape[0]), p.in_features, p.out_features
+    if code == 0:
+        pre = None
+    elif pre is None or pre.shape != dy.shape or pre.dtype != dy.dtype:
+        raise BadExl3Shape(f"linear_epilogue_backward: {act} needs the forward's pre, shaped and typed as dy")
+    dev = _on_one_device("linear_epilogue_backward", dy, p.trellis, p.suh, p.svh, pre)
+    with torch.cuda.device(dev):
+        dx = torch.empty(rows, in_f, dtype=dx_dtype or dy.dtype, device=dev)
+        dbias = torch.empty(out_f, dtype=torch.float32, device=dev) if with_dbias else None
+        L = _lib.load()
+        ws = workspace.get(dev, L.exl3_linear_epilogue_backward_workspace_size(rows, in_f, out_f))
+        _check(L.exl3_linear_epilogue_backward(dy.data_ptr(), _dt(dy, "dy"), rows, in_f, out_f, p.trellis.data_ptr(), p.n,
+                                               p.suh.data_ptr(), p.svh.data_ptr(), dec.c(), code, _ptr(pre),
+                                               dx.data_ptr(), _dt(dx, "dx"), _ptr(dbias), ws.data_ptr(), ws.numel(),
+                                               _stream(dev)))
+    return dx, dbias
+
+
+# ---------------------------------------------------------------------------------------------------------------
 # Routed experts
 
 REDUCE_MAX_TOPK = 32
@@ -993,6 +1091,77 @@ def moe_routing_chain(router_logits: torch.Tensor, k: int):
     _check(_lib.load().exl3_route_topk(lg.data_ptr(), rows, experts, k, inds.data_ptr(), scores.data_ptr(),
                                        _stream(lg.device)))
     return inds, scores
+
+
+class BalanceLoss(NamedTuple):
+    """``loss`` [] f32; ``counts`` [E] i32, the live rows' slots on each expert; ``weight`` [E] f32, the loss's derivative
+    by each expert's sum of probabilities, which moe_router_backward takes."""
+
+    loss: torch.Tensor
+    counts: torch.Tensor
+    weight: torch.Tensor
+
+
+def _router_operands(router_logits, inds, mask, what: str):
+    lg = router_logits
+    if lg.dim() < 2 or inds.dim() != lg.dim() or inds.shape[:-1] != lg.shape[:-1] or \
+            (mask is not None and mask.shape != lg.shape[:-1]):
+        raise BadExl3Shape(f"{what}: logits {tuple(lg.shape)}, inds {tuple(inds.shape)}"
+                           + ("" if mask is None else f", mask {tuple(mask.shape)}"))
+    if inds.dtype not in (torch.int32, getattr(torch, "uint32", torch.int32)):
+        raise BadExl3Dtype(f"{what}: inds dtype {inds.dtype} (u32/i32)")
+    if mask is not None and mask.dtype not in (torch.bool, torch.uint8):
+        raise BadExl3Dtype(f"{what}: mask dtype {mask.dtype} (bool or u8)")
+    rows = 1
+    for v in lg.shape[:-1]:
+        rows *= int(v)
+    return rows, int(lg.shape[-1]), int(inds.shape[-1])
+
+
+def moe_balance_loss(router_logits: torch.Tensor, inds: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                     coef: float = 1.0) -> BalanceLoss:
+    """The load-balance loss of a routing and the experts' counts: router_logits [.., E] (f16, bf16 or f32), inds [.., K]
+    as moe_routing_chain gives them (an id outside 0 .. E - 1 is a dropped slot), mask [..] (False: a padded row).  With T
+    live rows, loss = coef E sum_e (counts_e / (T K)) (mean over live rows of p_e).  An extension: the reference only
+    serves."""
+    rows, experts, topk = _router_operands(router_logits, inds, mask, "moe_balance_loss")
+    dev = _on_one_device("moe_balance_loss", router_logits, inds, mask)
+    with torch.cuda.device(dev):
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty(experts, dtype=torch.int32, device=dev)
+        weight = torch.empty(experts, dtype=torch.float32, device=dev)
+        L = _lib.load()
+        ws = workspace.get(dev, L.exl3_balance_loss_workspace_size(rows, experts))
+        _check(L.exl3_balance_loss(router_logits.data_ptr(), _dt(router_logits, "logits"), rows, experts,
+                                   inds.data_ptr(), topk, _ptr(mask), float(coef), loss.data_ptr(), counts.data_ptr(),
+                                   weight.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)))
+    return BalanceLoss(loss, counts, weight)
+
+
+def moe_router_backward(router_logits: torch.Tensor, inds: torch.Tensor, dscores: Optional[torch.Tensor] = None,
+                        weight: Optional[torch.Tensor] = None, dloss: Optional[torch.Tensor] = None,
+                        mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient of the router's logits, shaped and typed as they are: through moe_routing_chain's scores where dscores
+    [.., K] f32 is given (of the kept slots; see moe_balance_loss for inds and mask), plus ``dloss`` times the balance
+    loss's where ``weight`` (moe_balance_loss's) and ``dloss`` (a f32 tensor of one value) are given.  Padded rows get
+    zeros.  Equal calls give equal bits."""
+    rows, experts, topk = _router_operands(router_logits, inds, mask, "moe_router_backward")
+    if dscores is not None and dscores.shape != inds.shape:
+        raise BadExl3Shape(f"moe_router_backward: dscores {tuple(dscores.shape)} vs inds {tuple(inds.shape)}")
+    if (weight is None) != (dloss is None):
+        raise BadExl3Shape("moe_router_backward: the balance term takes both weight and dloss")
+    if weight is not None and (tuple(weight.shape) != (experts,) or dloss.numel() != 1):
+        raise BadExl3Shape(f"moe_router_backward: weight {tuple(weight.shape)}, dloss {tuple(dloss.shape)}")
+    for t, nm in ((dscores, "dscores"), (weight, "weight"), (dloss, "dloss")):
+        if t is not None and t.dtype != torch.float32:
+            raise BadExl3Dtype(f"moe_router_backward: {nm} dtype {t.dtype} (f32)")
+    dev = _on_one_device("moe_router_backward", router_logits, inds, mask, dscores, weight, dloss)
+    with torch.cuda.device(dev):
+        dlogits = torch.empty_like(router_logits)
+        _check(_lib.load().exl3_router_backward(router_logits.data_ptr(), _dt(router_logits, "logits"), rows, experts,
+                                                inds.data_ptr(), topk, _ptr(dscores), _ptr(weight), _ptr(dloss),
+                                                _ptr(mask), dlogits.data_ptr(), _stream(dev)))
+    return dlogits
 
 
 def tile_major(trellis: torch.Tensor, inverse: bool = False) -> torch.Tensor:
