@@ -207,13 +207,13 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
  * Forward: z = linear(x) + bias, y = act(z) + residual, from the f32 sums with one rounding to y's dtype.  bias [out] in
  * bias_dtype or null; residual [rows][out] in y's dtype or null, not overlapping y; pre [rows][out] in y's dtype receives
  * z for the backward pass, or is null.  silu is z sigmoid(z), gelu z Phi(z), gelu_tanh its tanh approximation.  Every arm
- * of exl3_linear finishes this way in its own launch.  x, bias, residual, y, pre and svh 4-byte aligned.
+ * of exl3_linear finishes this way in its own launch.  x, bias, residual, y and pre 4-byte aligned.
  *
- * Backward: from dy [rows][out] (and pre, both in `dtype`, 16-byte aligned; pre unread with EXL3_ACT_NONE)
+ * Backward: from dy [rows][out] (and pre, both in `dtype`; pre unread with EXL3_ACT_NONE; dy and svh 16-byte aligned, pre 8-byte)
  *   dz = dy act'(pre),  dbias [out] = sum over rows of dz (f32; null: not wanted),
  *   dx [rows][in] = H(f16(s H(dz * svh)) W^T) * suh / s  in dx_dtype,
  * H the orthonormal Hadamard transform of each 128, W the decoded inner weight and s a power of two per row that brings
- * the row's largest |dz * svh| to 2^10 .. 2^11 (the prepared gradient is f16 as the prepared input is; gradients lie below
+ * the row's largest |dy * svh| to 2^10 .. 2^11 (the prepared gradient is f16 as the prepared input is; gradients lie below
  * f16's normal range).  residual's gradient is dy itself, x's rounding to f16 is passed through.  Each rounding of pre to
  * 16 bits moves act' as that of any kept activation does.
  *

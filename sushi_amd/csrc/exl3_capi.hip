@@ -334,6 +334,11 @@ int32_t linear_impl(const void *x, int32_t x_dtype, int32_t groups, int32_t rows
 int epilogue_chunk(int width) { return width < 65536 ? 16384 : 1024; }
 
 size_t elem_size(int dt) { return dt == EXL3_DT_F32 ? 4 : 2; }
+// Width up to which the gradient's prepare finds the largest values of up to 16 rows itself, and rows up to which the last
+// split of a tile to arrive sums the splits.
+constexpr int kGradScanOut = 8192;
+constexpr int kGradFinishRows = 32;
+
 const void *at_row(const void *p, size_t row, size_t width, int dt) {
     return p ? static_cast<const char *>(p) + row * width * elem_size(dt) : nullptr;
 }
@@ -346,28 +351,31 @@ int32_t act_check(int32_t act, const char *what) {
     return ok();
 }
 
-// The backward pass's launch shape for a chunk of `rows` of `total` rows.
+// The backward pass's launch shape for a chunk of rows.
 struct GradPlan {
-    int tile_rows, tiles, chunks, splits;
+    int prep_tiles, tiles, splits;
+    bool scan, finish;  // kernels of their own for the rows' largest values and for the splits' sum
     size_t amax, dbias_part, inv, u, part;
     size_t bytes() const { return kZeroBytes + amax + dbias_part + inv + u + part; }
 };
 
-GradPlan plan_grad(int total, int rows, int in, int out) {
+// `whole`: the chunk is all the rows (its one row tile may then write dbias itself).
+GradPlan plan_grad(int rows, int in, int out, bool whole) {
     GradPlan p;
-    // at most 64 row tiles of at least 64 rows: the partial sums of dbias stay few, and 64 tiles of ceil(out / 512)
-    // workgroups fill the GPU from a width of 2048 on
-    p.tile_rows = std::max(64, (total / 64 + 4) / 4 * 4);
-    p.tiles = (total + p.tile_rows - 1) / p.tile_rows;
-    p.chunks = (out + GRAD_SCAN_COLS - 1) / GRAD_SCAN_COLS;
+    const int rt = (rows + 15) / 16;
+    // 64 rows a prepare workgroup once that leaves eight workgroups a CU: dbias then has a quarter of the partial sums.
+    p.prep_tiles = (long)(rt / 4) * (out / 128) >= 2048 ? 4 : 1;
+    p.tiles = (rt + p.prep_tiles - 1) / p.prep_tiles;
+    p.scan = rows > 16 || out > kGradScanOut;
     // The contraction is split until the workgroups fill the GPU's 256 CUs (one a CU), each split at least two output
     // groups.
     const int tiles = in / 128 * ((rows + 255) / 256), groups = out / 128;
     p.splits = std::max(1, std::min(256 / std::max(tiles, 1), groups / 2));
-    p.amax = align_up((size_t)total * p.chunks * sizeof(float));
-    p.dbias_part = p.tiles > 1 ? align_up((size_t)p.tiles * out * sizeof(float)) : 0;
+    p.finish = rows > kGradFinishRows;
+    p.amax = p.scan ? align_up((size_t)rows * sizeof(float)) : 0;
+    p.dbias_part = p.tiles > 1 || !whole ? align_up((size_t)p.tiles * out * sizeof(float)) : 0;
     p.inv = align_up((size_t)rows * sizeof(float));
-    p.u = align_up((size_t)((rows + 15) / 16 * 16) * out * 2);
+    p.u = align_up((size_t)rt * 16 * out * 2);
     p.part = p.splits > 1 ? align_up((size_t)p.splits * rows * in * sizeof(float)) : 0;
     return p;
 }
@@ -376,8 +384,8 @@ GradPlan plan_grad(int total, int rows, int in, int out) {
 size_t grad_ws(int rows, int in, int out) {
     if (rows <= 0) return 0;
     const int chunk = std::min(rows, epilogue_chunk(out)), rest = rows % chunk;
-    const size_t whole = plan_grad(rows, chunk, in, out).bytes();
-    return rest ? std::max(whole, plan_grad(rows, rest, in, out).bytes()) : whole;
+    const size_t whole = plan_grad(chunk, in, out, chunk == rows).bytes();
+    return rest ? std::max(whole, plan_grad(rest, in, out, false).bytes()) : whole;
 }
 
 int32_t router_checks(const void *logits, int32_t dtype, int32_t rows, int32_t experts, int32_t topk, const char *what) {
@@ -1509,9 +1517,9 @@ int32_t exl3_linear_epilogue(const void *x, int32_t x_dtype, int32_t rows, int32
     rc = act_check(act, "linear_epilogue");
     if (rc) return rc;
     if (bias && !dtype_ok(bias_dtype)) return fail(EXL3_ERR_BAD_DTYPE, "linear_epilogue: unsupported bias dtype");
-    for (const void *p : {bias, residual, (const void *)y, (const void *)pre, (const void *)svh})
+    for (const void *p : {bias, residual, (const void *)y, (const void *)pre})
         if (reinterpret_cast<uintptr_t>(p) % 4)
-            return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue: bias, residual, y, pre and svh must be 4-byte aligned");
+            return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue: bias, residual, y and pre must be 4-byte aligned");
     if (rows == 0) return ok();
     const size_t need = exl3_linear_epilogue_workspace_size(rows, in_features, out_features, n);
     if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
@@ -1521,13 +1529,10 @@ int32_t exl3_linear_epilogue(const void *x, int32_t x_dtype, int32_t rows, int32
     for (int r = 0; r < rows; r += chunk) {
         EpilogueArgs e{};
         e.act = act;
-        e.has_bias = bias != nullptr;
-        e.has_residual = residual != nullptr;
-        // the kernels fetch both words ahead of knowing whether they are used: an absent one's from memory that is there
-        e.bias = bias ? bias : svh;
-        e.bias_dtype = bias ? bias_dtype : EXL3_DT_F16;
+        e.bias = bias;
+        e.bias_dtype = bias_dtype;
         void *yr = at_row(y, r, out_features, y_dtype);
-        e.residual = residual ? at_row(residual, r, out_features, y_dtype) : yr;
+        e.residual = at_row(residual, r, out_features, y_dtype);
         e.pre = at_row(pre, r, out_features, y_dtype);
         rc = linear_impl(at_row(x, r, in_features, x_dtype), x_dtype, 1, std::min(chunk, rows - r), in_features,
                          out_features, trellis, n, suh, svh, dec, yr, y_dtype, workspace, workspace_bytes, stream, true,
@@ -1561,8 +1566,9 @@ int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t row
         return ok();
     }
     if (act != ACT_NONE && !pre) return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: the activation's pre is missing");
-    if ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(pre)) % 16)
-        return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: dy and pre must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(dy) % 16 || reinterpret_cast<uintptr_t>(svh) % 16 ||
+        reinterpret_cast<uintptr_t>(pre) % 8 || reinterpret_cast<uintptr_t>(dx) % elem_size(dx_dtype))
+        return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: dy and svh must be 16-byte aligned, pre 8-byte, dx whole");
     const size_t need = grad_ws(rows, in_features, out_features);
     if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
         return fail(EXL3_ERR_WORKSPACE, "linear_epilogue_backward: workspace of %zu bytes (256-aligned) needed, got %zu",
@@ -1583,30 +1589,29 @@ int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t row
     a.k = k;
     a.dbias = dbias;
     a.dx_dtype = dx_dtype;
-    const GradPlan p = plan_grad(rows, std::min(rows, chunk), in_features, out_features);
-    char *w = static_cast<char *>(workspace) + kZeroBytes;
-    a.tile_rows = p.tile_rows;
-    a.chunks = p.chunks;
-    a.amax = reinterpret_cast<float *>(w);
-    w += p.amax;
-    a.dbias_part = reinterpret_cast<float *>(w);
-    w += p.dbias_part;
-    a.inv_scale = reinterpret_cast<float *>(w);
-    w += p.inv;
-    hipError_t e = run_grad_scan(a, stream);
-    if (e != hipSuccess) return launched(e, "exl3_linear_epilogue_backward (scan)");
     for (int r = 0; r < rows; r += chunk) {
         GradArgs c = a;
         c.rows = std::min(chunk, rows - r);
-        const GradPlan q = plan_grad(rows, c.rows, in_features, out_features);
+        const GradPlan p = plan_grad(c.rows, in_features, out_features, c.rows == rows);
+        char *w = static_cast<char *>(workspace) + kZeroBytes;
+        auto take = [&](size_t bytes) {
+            char *at = w;
+            w += bytes;
+            return bytes ? reinterpret_cast<float *>(at) : nullptr;
+        };
+        c.prep_tiles = p.prep_tiles;
+        c.amax = take(p.amax);
+        c.dbias_part = take(p.dbias_part);
+        c.dbias_adds = r > 0;
+        c.inv_scale = take(p.inv);
+        c.u = reinterpret_cast<uint16_t *>(take(p.u));
+        c.part = take(p.part);
+        c.splits = p.splits;
+        c.counters = p.finish ? nullptr : static_cast<uint32_t *>(workspace);  // at most 256 tiles where splits > 1
         c.dy = at_row(dy, r, out_features, dtype);
         c.pre = at_row(a.pre, r, out_features, dtype);
-        c.amax = a.amax + (size_t)r * p.chunks;
-        c.u = reinterpret_cast<uint16_t *>(w);
-        c.part = reinterpret_cast<float *>(w + q.u);
-        c.splits = q.splits;
         c.dx = at_row(dx, r, in_features, dx_dtype);
-        e = run_grad_gemm(fam, c, stream);
+        const hipError_t e = run_gradient(fam, c, stream);
         if (e != hipSuccess) return launched(e, "exl3_linear_epilogue_backward");
     }
     return ok();
@@ -1614,8 +1619,8 @@ int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t row
 
 size_t exl3_balance_loss_workspace_size(int32_t rows, int32_t experts) {
     if (rows < 0 || experts <= 0 || experts > kRouterMaxExperts) return 0;
-    const size_t parts = (size_t)balance_parts(rows, experts);
-    return kZeroBytes + (parts > 1 ? 2 * align_up(parts * experts * 4) + align_up(parts * 4) : 0);
+    const size_t parts = (size_t)balance_parts(rows, experts), all = parts + balance_joins((int)parts);
+    return kZeroBytes + (parts > 1 ? 2 * align_up(all * experts * 4) + align_up(all * 4) : 0);
 }
 
 int32_t exl3_balance_loss(const void *logits, int32_t dtype, int32_t rows, int32_t experts, const uint32_t *inds,
@@ -1628,7 +1633,8 @@ int32_t exl3_balance_loss(const void *logits, int32_t dtype, int32_t rows, int32
     if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
         return fail(EXL3_ERR_WORKSPACE, "balance_loss: workspace of %zu bytes (256-aligned) needed, got %zu", need,
                     workspace_bytes);
-    const size_t parts = (size_t)balance_parts(rows, experts), plane = align_up(parts * experts * 4);
+    const size_t parts = (size_t)balance_parts(rows, experts);
+    const size_t plane = align_up((parts + balance_joins((int)parts)) * experts * 4);
     char *w = static_cast<char *>(workspace) + kZeroBytes;
     BalanceArgs a{};
     a.logits = logits;
@@ -1646,6 +1652,7 @@ int32_t exl3_balance_loss(const void *logits, int32_t dtype, int32_t rows, int32
         a.part_sum = reinterpret_cast<float *>(w);
         a.part_count = reinterpret_cast<int *>(w + plane);
         a.part_live = reinterpret_cast<int *>(w + 2 * plane);
+        a.counters = static_cast<uint32_t *>(workspace);
     }
     return launched(run_balance_loss(a, stream), "exl3_balance_loss");
 }

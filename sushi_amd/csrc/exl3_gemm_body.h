@@ -278,7 +278,30 @@ __global__ __launch_bounds__(GM_THREADS) void gemm_epilogue_kernel(GemmArgs a, c
     gemm_run<FAM, N, true>(a, wt, &e);
 }
 
-// EPI: with the epilogue e (the residual's words of four rows go out together, ahead of their transforms).
+// Columns i and i + 64 (v[2 r], v[2 r + 1]) of the first `live` of four rows `pitch` elements apart, in dtype dt.
+__device__ __forceinline__ void store_rows4(void *p, int dt, size_t i, size_t pitch, int live, const float (&v)[8]) {
+    if (dt == DT_F32) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (r < live) {
+                store_act<DT_F32>(p, i + r * pitch, v[2 * r]);
+                store_act<DT_F32>(p, i + r * pitch + 64, v[2 * r + 1]);
+            }
+        return;
+    }
+    const uint4 w = pack8(dt == DT_BF16, v);
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    uint16_t *q = static_cast<uint16_t *>(p) + i;
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (r < live) {
+            q[r * pitch] = (uint16_t)ws[r];
+            q[r * pitch + 64] = (uint16_t)(ws[r] >> 16);
+        }
+}
+
+// EPI: with the epilogue e.  The bias words are fetched once; the residual's words of four rows go out together, while the
+// four rows before them are finished.
 template <int FAM, int N, bool EPI>
 __device__ __forceinline__ void gemm4_run(const GemmArgs &a, const EpilogueArgs *e) {
     const int IT = a.in >> 4, OT = a.out >> 4;
@@ -294,41 +317,61 @@ __device__ __forceinline__ void gemm4_run(const GemmArgs &a, const EpilogueArgs 
         mt = L / nog;
     }
     const int g = blockIdx.z;
-    __shared__ __align__(16) uint16_t Bs[2][128 * G4_BP];
+    constexpr int SLABS = 2 * 128 * G4_BP;  // halves
+    __shared__ __align__(16) uint16_t lds[EPI && G4_STAGE_ALL / 2 > SLABS ? G4_STAGE_ALL / 2 : SLABS];
+    uint16_t (*Bs)[128 * G4_BP] = reinterpret_cast<uint16_t (*)[128 * G4_BP]>(lds);
     const int RT = (a.rows + 15) / 16;
     const uint16_t *xfrag0 = a.xp + ((size_t)g * RT + (size_t)mt * (G2_MT / 16)) * (size_t)(a.in / 32) * 512;
     const size_t sv = (size_t)g * a.out + (size_t)og * 128;
     const int lane = threadIdx.x & 63;
     const float s0 = h2f(a.svh[sv + lane]), s1 = h2f(a.svh[sv + lane + 64]);
-    gemm4_tile<FAM, N>(a.in, a.out, og, a.trellis + (size_t)g * IT * OT * N, xfrag0, min(G2_MT, a.rows - mt * G2_MT),
+    const int tile_rows = min(G2_MT, a.rows - mt * G2_MT);
+    uint32_t next0[4] = {}, next1[4] = {};  // EPI: the residual's words of the next four rows
+    bool fetched = false;
+    gemm4_tile<FAM, N, EPI>(a.in, a.out, og, a.trellis + (size_t)g * IT * OT * N, xfrag0, min(G2_MT, a.rows - mt * G2_MT),
                        nullptr, a.k, Bs,
                        [&](int m, int live, float (&v0)[4], float (&v1)[4], int ln, uint32_t)
                            __attribute__((always_inline)) {
                            if constexpr (EPI) {
                                const size_t col = (size_t)og * 128 + ln;
-                               EpilogueWords w[4];
+                               auto fetch = [&](int m4) __attribute__((always_inline)) {
 #pragma unroll
-                               for (int i = 0; i < 4; i++)
-                                   w[i] = epilogue_fetch(*e, a.y_dtype, col,
-                                                         ((size_t)mt * G2_MT + m + min(i, live - 1)) * a.out + col);
-                               fwht128_wave_rows<4>(v0, v1, ln);
-                               // one body for the four rows (the activations are long), the rows shifted through slot 0
-#pragma unroll 1
-                               for (int i = 0; i < live; i++) {
-                                   const size_t yo = ((size_t)mt * G2_MT + m + i) * a.out + col;
-                                   const float z0 = v0[0] * codebook_scale<FAM>() * HAD_SCALE * s0;
-                                   const float z1 = v1[0] * codebook_scale<FAM>() * HAD_SCALE * s1;
-                                   const float y0 = epilogue_apply(*e, a.y_dtype, z0, w[0].b0, col, w[0].r0, yo);
-                                   const float y1 = epilogue_apply(*e, a.y_dtype, z1, w[0].b1, col + 64, w[0].r1,
-                                                                   yo + 64);
-                                   store_y4(a.y, a.y_dtype, yo, y0, y1);
-#pragma unroll
-                                   for (int q = 0; q < 3; q++) {
-                                       v0[q] = v0[q + 1];
-                                       v1[q] = v1[q + 1];
-                                       w[q] = w[q + 1];
+                                   for (int i = 0; i < 4; i++) {
+                                       const size_t o = ((size_t)mt * G2_MT + min(m4 + i, tile_rows - 1)) * a.out + col;
+                                       next0[i] = act_word(e->residual, a.y_dtype, o);
+                                       next1[i] = act_word(e->residual, a.y_dtype, o + 64);
                                    }
+                               };
+                               uint32_t rw[8];  // the rows' words of columns ln and ln + 64
+                               if (e->residual && !fetched) fetch(m);
+                               fetched = true;
+                               float b0 = 0.f, b1 = 0.f;
+                               if (e->bias) {
+                                   b0 = load_any(e->bias, e->bias_dtype, col);
+                                   b1 = load_any(e->bias, e->bias_dtype, col + 64);
                                }
+#pragma unroll
+                               for (int i = 0; i < 4; i++) {
+                                   rw[2 * i] = next0[i];
+                                   rw[2 * i + 1] = next1[i];
+                               }
+                               // a wave's rows are m, m + 4 of each 16
+                               if (e->residual) fetch(m + ((m & 4) ? 12 : 4));
+                               fwht128_wave_rows<4>(v0, v1, ln);
+                               float z[8], y[8];
+#pragma unroll
+                               for (int i = 0; i < 4; i++) {
+                                   z[2 * i] = v0[i] * codebook_scale<FAM>() * HAD_SCALE * s0 + b0;
+                                   z[2 * i + 1] = v1[i] * codebook_scale<FAM>() * HAD_SCALE * s1 + b1;
+                               }
+                               act_eight(e->act, z, y);
+                               if (e->residual) {
+#pragma unroll
+                                   for (int i = 0; i < 8; i++) y[i] += act_from_word(rw[i], a.y_dtype, col);
+                               }
+                               const size_t yo = ((size_t)mt * G2_MT + m) * a.out + col;
+                               store_rows4(a.y, a.y_dtype, yo, a.out, live, y);
+                               if (e->pre) store_rows4(e->pre, a.y_dtype, yo, a.out, live, z);
                                return;
                            }
                            fwht128_wave_rows<4>(v0, v1, ln);
@@ -375,19 +418,6 @@ constexpr int G5_EP = 132;  // its pitch (floats) for the sums of a launch with 
 constexpr int lds_max(int a, int b) { return a > b ? a : b; }
 constexpr int G5_LDS = lds_max(3 * G5_SLAB * 2, G5_WAVES * 16 * G5_SP * 2);
 constexpr int G5_LDS_EPI = lds_max(G5_LDS, G5_WAVES * 16 * G5_EP * 4);
-
-// Eight f32 values rounded to f16 or bf16.
-__device__ __forceinline__ uint4 pack8(bool bf16, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t lo = bf16 ? __bfloat16_as_ushort(__float2bfloat16(v[2 * i])) : __half_as_ushort(__float2half_rn(v[2 * i]));
-        const uint32_t hi = bf16 ? __bfloat16_as_ushort(__float2bfloat16(v[2 * i + 1]))
-                                 : __half_as_ushort(__float2half_rn(v[2 * i + 1]));
-        w[i] = lo | hi << 16;
-    }
-    return uint4{w[0], w[1], w[2], w[3]};
-}
 
 template <int FAM, int N, int MT, int KS, bool EPI>
 __device__ __forceinline__ void gemm5_run(const GemmArgs &a, const EpilogueArgs *e) {
@@ -654,14 +684,14 @@ __device__ __forceinline__ void gemm5_run(const GemmArgs &a, const EpilogueArgs 
     if constexpr (EPI) {
 #pragma unroll
         for (int q = 0; q < 8; q++)
-            ebias[q] = e->has_bias ? load_any(e->bias, e->bias_dtype, ecol + q) : 0.f;
+            ebias[q] = e->bias ? load_any(e->bias, e->bias_dtype, ecol + q) : 0.f;
     }
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
         if (!(rb < RB / 2 ? fin_lo : fin_hi)) continue;
         uint4 res[4] = {};
         if constexpr (EPI) {
-            if (!epi_wide && e->has_residual) {
+            if (!epi_wide && e->residual) {
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const int m = min(m0 + rb * 16 + 4 * q + (lane >> 4), a.rows - 1);
@@ -730,8 +760,9 @@ __device__ __forceinline__ void gemm5_run(const GemmArgs &a, const EpilogueArgs 
                 if (epi_wide) {
 #pragma unroll 1
                     for (int j = 0; j < 8 && live; j++) {
-                        const float y = epilogue_apply(*e, a.y_dtype, er[j], act_word(e->bias, e->bias_dtype, ecol + j),
-                                                       ecol + j, act_word(e->residual, a.y_dtype, yo + j), yo + j);
+                        const float y = epilogue_apply(*e, a.y_dtype, er[j],
+                                                       e->bias ? act_word(e->bias, e->bias_dtype, ecol + j) : 0u,
+                                                       ecol + j, e->residual ? act_word(e->residual, a.y_dtype, yo + j) : 0u, yo + j);
                         store_any(a.y, a.y_dtype, yo + j, y);
                     }
                     continue;
@@ -742,9 +773,14 @@ __device__ __forceinline__ void gemm5_run(const GemmArgs &a, const EpilogueArgs 
                 res[1] = res[2];
                 res[2] = res[3];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    z[j] = er[j] + ebias[j];
-                    y[j] = act_value(e->act, z[j]) + (e->has_residual ? act_from_word(rw[j >> 1], a.y_dtype, j) : 0.f);
+                for (int j = 0; j < 8; j++) z[j] = er[j] + ebias[j];
+                act_eight(e->act, z, y);
+                if (e->residual) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const uint32_t h = j & 1 ? rw[j >> 1] >> 16 : rw[j >> 1] & 0xFFFFu;
+                        y[j] += bf16 ? __uint_as_float(h << 16) : h2f((uint16_t)h);
+                    }
                 }
                 if (live) {
                     *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.y) + yo) = pack8(bf16, y);

@@ -30,6 +30,7 @@ constexpr int G2_BP = 72;    // LDS pitch (halves) of one ping-pong slab column:
 constexpr int G4_BP = 136;   // LDS pitch (halves) of one decode-wave-tile slab column: 128 k + 8 pad
 constexpr int G4_HELP_ROWS = 128;  // live rows up to which MFMA waves 4-7 decode
 constexpr int G2_EP = 129;   // epilogue staging pitch (floats)
+constexpr int G4_STAGE_ALL = G2_MT * G2_EP * 4;  // bytes of a staged 256-row tile
 constexpr int G4_WAVES = 12;
 constexpr int G4_THREADS = 64 * G4_WAVES;
 
@@ -238,7 +239,9 @@ __device__ __forceinline__ void gemm4_decode_waves(R &rd, int nsup, int d, int l
 // wave's row group m0 .. m0 + 63 (loaded before the main loop, so the epilogue finds each row's id with a lane read
 // instead of a memory round trip per row); without, rid is 0.
 // nks: 64-k steps (even), xfrag0 at the first of them; TR as gemm4_mfma_loop.
-template <bool TR = false, class Emit>
+// ALL: every row block is staged before the first is handed on (Bs then holds G4_STAGE_ALL bytes), so emit is one body in a
+// loop: for an epilogue of some length, whose eight copies would not stay in the instruction cache.
+template <bool TR = false, bool ALL = false, class Emit>
 __device__ __forceinline__ void gemm4_mfma_waves(int in, int nks, const uint16_t *__restrict__ xfrag0, int rows,
                                                  const uint32_t *__restrict__ row_ids, uint16_t (*Bs)[128 * G4_BP],
                                                  Emit emit) {
@@ -271,6 +274,29 @@ __device__ __forceinline__ void gemm4_mfma_waves(int in, int nks, const uint16_t
 
     // ---- epilogue (the decode waves have left, so the barriers below join the live MFMA waves): per 16-row block, the
     // two waves of a row group stage their column halves side by side in LDS, then each hands 8 of the rows on.
+    if constexpr (ALL) {
+        float *ep = reinterpret_cast<float *>(&Bs[0][0]) + (wave >> 1) * 64 * G2_EP;
+#pragma unroll
+        for (int rb = 0; rb < 4; rb++)
+#pragma unroll
+            for (int cb = 0; cb < 4; cb++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) ep[(rb * 16 + 4 * h + i) * G2_EP + (cb0 + cb) * 16 + c] = acc[rb][cb][i];
+        __syncthreads();
+#pragma unroll 1
+        for (int q = 0; q < 8; q++) {
+            const int r = (q >> 1) * 16 + (wave & 1) * 8 + (q & 1) * 4, m = m0 + r;
+            if (m >= rows) break;
+            float v0[4], v1[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v0[i] = ep[(r + i) * G2_EP + lane];
+                v1[i] = ep[(r + i) * G2_EP + lane + 64];
+            }
+            emit(m, min(4, rows - m), v0, v1, lane, rid);
+        }
+        return;
+    }
     float *ep = reinterpret_cast<float *>(&Bs[0][0]) + (wave >> 1) * 16 * G2_EP;
 #pragma unroll
     for (int rb = 0; rb < 4; rb++) {
@@ -319,7 +345,7 @@ __device__ __forceinline__ void gemm4_decode_role(bool help, int d, int nsup, in
 // One workgroup's 256-row x 128-column output tile of output group og of a bank at one rate N whose tiles start at
 // `bank` ([in/16][out/16][N]): the decoders (gemm4_decoder) decode, the other waves multiply (gemm4_mfma_waves, whose
 // `emit` receives the raw inner products).
-template <int FAM, int N, class Emit>
+template <int FAM, int N, bool ALL = false, class Emit>
 __device__ __forceinline__ void gemm4_tile(int in, int out, int og, const uint16_t *__restrict__ bank,
                                            const uint16_t *__restrict__ xfrag0, int rows, const uint32_t *row_ids,
                                            const DecodeK &k, uint16_t (*Bs)[128 * G4_BP], Emit emit) {
@@ -332,7 +358,7 @@ __device__ __forceinline__ void gemm4_tile(int in, int out, int og, const uint16
         });
         return;
     }
-    gemm4_mfma_waves(in, in >> 6, xfrag0, rows, row_ids, Bs, emit);  // in is a multiple of 128
+    gemm4_mfma_waves<false, ALL>(in, in >> 6, xfrag0, rows, row_ids, Bs, emit);  // in is a multiple of 128
 }
 
 }  // namespace exl3

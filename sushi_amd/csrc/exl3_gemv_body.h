@@ -407,11 +407,11 @@ __device__ __forceinline__ float fold_value(unsigned long long t, int S, unsigne
 // and the completing arrival rounds the routed sum to y's dtype before adding the shared expert.  MOE (the down
 // projection's PRO_MID kernels) is a compile-time choice: the dense kernels carry none of the slot, score and
 // shared-expert handling.
-// EPI: the epilogue runs in the completing arrival, on the whole sum; every arrival fetches the bias and residual words
-// ahead of its adds, so the completing one does not wait for them after its own.
+// EPI: the epilogue runs in the completing arrival, on the whole sum; every arrival has the bias and residual words of
+// its row at hand (ew: the first row's, the next one's fetched behind each), so the completing one waits for neither.
 template <int RT, bool WIN, bool MOE, bool SH, bool EPI>
 __device__ __forceinline__ void fold_finish(const GemvArgs &a, const GemvCtx &c, float (*red)[RT][128], int wave,
-                                            int lane, const EpilogueArgs *e) {
+                                            int lane, const EpilogueArgs *e, EpilogueWords ew) {
     for (int r = wave; r < c.rows; r += GEMV_WAVES) {
         float v0 = 0.f, v1 = 0.f;
 #pragma unroll
@@ -443,8 +443,6 @@ __device__ __forceinline__ void fold_finish(const GemvArgs &a, const GemvCtx &c,
         const size_t yo = yrow * a.out + (size_t)c.og * 128;
         unsigned long long *w0 = (shared ? a.sh_fold : a.fold) + yo + lane, *w1 = w0 + 64;
         const size_t col = (size_t)c.og * 128 + lane;
-        EpilogueWords ew{};
-        if constexpr (EPI) ew = epilogue_fetch(*e, a.y_dtype, col, yo + lane);
         fold_overflow(w0, w1, f0, f1);
         const unsigned long long o0 = __hip_atomic_fetch_add(w0, t0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const unsigned long long o1 = __hip_atomic_fetch_add(w1, t1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -466,6 +464,8 @@ __device__ __forceinline__ void fold_finish(const GemvArgs &a, const GemvCtx &c,
                 store_y(a.y, a.y_dtype, yo + lane + 64, y1);
                 *w1 = 0ull;
             }
+            if constexpr (EPI)
+                if (r + GEMV_WAVES < c.rows) ew = epilogue_fetch(*e, a.y_dtype, col, yo + lane + (size_t)GEMV_WAVES * a.out);
             continue;
         }
 #pragma unroll
@@ -515,6 +515,13 @@ __device__ __forceinline__ void fetch_svh(GemvCtx &c, int lane) {
     c.sv1 = h2f(c.svh[(size_t)sv + lane + 64]);
 }
 
+// The words of the row that a wave's finish starts with, fetched behind the tile loads.
+__device__ __forceinline__ EpilogueWords epilogue_first(const GemvArgs &a, const GemvCtx &c, int wave, int lane,
+                                                        const EpilogueArgs *e) {
+    const size_t col = (size_t)c.og * 128 + lane, row = (size_t)c.g * a.rows + min(wave, c.rows - 1);
+    return epilogue_fetch(*e, a.y_dtype, col, row * a.out + col);
+}
+
 // A per-tile-rate projection as a workgroup reads it (N == N_TILED): its segment tables and the constants at both
 // rates.
 struct TiledSrc {
@@ -552,6 +559,7 @@ __device__ __forceinline__ void gemv_body(const GemvArgs &a, GemvCtx &c, const u
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform: branches on it stay scalar
     const int o = lane >> 3, j = lane & 7;
     constexpr int RG = RowGroups<RT>::G;
+    EpilogueWords ew{};  // EPI: of the first row this wave finishes
     f4_t accA[RG], accB[RG];
 #pragma unroll
     for (int g = 0; g < RG; g++) accA[g] = accB[g] = f4_t{0.f, 0.f, 0.f, 0.f};
@@ -590,6 +598,7 @@ __device__ __forceinline__ void gemv_body(const GemvArgs &a, GemvCtx &c, const u
         for (int t = 0; t < TPW; t++) load_slot(t, c.kt0 + wave + GEMV_WAVES * min(t, ntiles - 1));
         __builtin_amdgcn_sched_barrier(0);  // svh's address comes from an argument load: its wait stays behind
         fetch_svh<PIN>(c, lane);
+        if constexpr (EPI) ew = epilogue_first(a, c, wave, lane, e);
         if constexpr (CH == 2) chain_wait(a, c, wave);
         prologue<PRO, RT, WIN, SH, CH>(a, c, xs, wave, lane, pr);
         __syncthreads();
@@ -651,6 +660,7 @@ __device__ __forceinline__ void gemv_body(const GemvArgs &a, GemvCtx &c, const u
             }
             mfma_dot<RT>(w, xs, kk, c.rows, accA, accB, lane & 3, read_xfrag(xs, min(lane & 3, RT - 1), kk));
         }
+        if constexpr (EPI) ew = epilogue_first(a, c, wave, lane, e);  // (held through the loop they would spill)
     }
     // the matrix cores take the hash / pair weights as decoded, the codebook's values over 4096 (f16 subnormals
     // among them, which they multiply exactly); out_scale applies the 4096 to every arm alike
@@ -669,7 +679,7 @@ __device__ __forceinline__ void gemv_body(const GemvArgs &a, GemvCtx &c, const u
     }
     __syncthreads();
     if (a.fold) {  // the host enables the fold only for split dense launches and the MoE down projection
-        fold_finish<RT, WIN, PRO == PRO_MID, SH, EPI>(a, c, red, wave, lane, e);
+        fold_finish<RT, WIN, PRO == PRO_MID, SH, EPI>(a, c, red, wave, lane, e, ew);
         return;
     }
     const bool direct = c.S == 1 && !a.partial_only;

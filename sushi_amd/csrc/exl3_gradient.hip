@@ -2,20 +2,22 @@
 // y = act(z) + residual,
 //   dz = dy * act'(z),  dbias = sum over rows of dz,  dx = H(u W^T) * suh,  u = f16(H(dz * svh))
 // (H: the orthonormal Hadamard transform of every 128; residual's gradient is dy itself).  u is rounded to f16 as the
-// forward's prepared input is, under a power of two per row that brings the row's largest |dz * svh| to 2^10 .. 2^11:
+// forward's prepared input is, under a power of two per row that brings the row's largest |dy * svh| to 2^10 .. 2^11:
 // gradients lie far below f16's normal range, and |H v| <= sqrt(128) max |v| keeps the scaled values below 2^15.
 //
-//   grad_scan_kernel     reads dy and pre once: the rows' largest values by column chunk, dbias's partial sums
-//   grad_prepare_kernel  reads them again: u in MFMA A-fragment order, each row's scale
+//   grad_scan_kernel     reads dy: each row's largest |dy * svh| (short calls leave it to the prepare)
+//   grad_prepare_kernel  reads dy and pre: u in MFMA A-fragment order, each row's scale, dbias's sums by row tile
 //   grad_gemm_kernel     u W^T on the decode-wave tile (exl3_gemm_tile.h), the trellis decoded once per 256 rows into the
 //                        same column-major slab as the forward's and read back transposed by the MFMA waves; with few
-//                        row and column tiles the contraction is split and grad_finish_kernel sums the splits in order
+//                        row and column tiles the contraction is split, and the splits' products are summed in order by
+//                        the last of them to arrive (few rows) or by grad_finish_kernel
+// The scale goes by |dy * svh| and not by |dz * svh|, so the activation is evaluated once: every slope is below 1.13, so
+// the bound on the scaled values holds with 13% more, and slopes that are small in a whole row cost it range that f16 has
+// (2^24 between the largest value and where its steps grow).
 #include "exl3_gemm_tile.h"
 #include "exl3_epilogue.h"
 
 namespace exl3 {
-
-constexpr int GS_COLS = GRAD_SCAN_COLS;  // 64 lanes x 8
 
 // Eight consecutive values of a row (16-byte loads; the host checks the alignment).
 template <int DT>
@@ -35,61 +37,54 @@ __device__ __forceinline__ void load8(const void *p, size_t i, float (&v)[8]) {
     }
 }
 
-__device__ __forceinline__ float wave_max_abs(float v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
-    return v;
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, xor_lane_row<1>(v));
+    v = fmaxf(v, xor_lane_row<2>(v));
+    v = fmaxf(v, xor_lane_row<4>(v));
+    v = fmaxf(v, xor_lane_row<8>(v));
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
 }
 
-// Workgroup (column chunk, row tile of a.tile_rows rows): wave w takes the tile's rows w, w + 4, ..., lane l the chunk's
-// columns 8 l .. 8 l + 7.  amax[row][chunk] = max |dz * svh|; dbias_part[tile][col] = sum of dz (one tile: dbias itself).
+// max |dy * svh| over eight columns of a row.
+template <int DT>
+__device__ __forceinline__ float max8(const GradArgs &a, int row, int c) {
+    float d[8], m = 0.f;
+    load8<DT>(a.dy, (size_t)row * a.out + c, d);
+    const uint4 s = *reinterpret_cast<const uint4 *>(a.svh + c);
+    const uint32_t w[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int q = 0; q < 8; q++) m = fmaxf(m, fabsf(d[q] * h2f((uint16_t)(q & 1 ? w[q >> 1] >> 16 : w[q >> 1] & 0xFFFFu))));
+    return m;
+}
+
+// One workgroup a row.
 template <int DT>
 __global__ __launch_bounds__(256) void grad_scan_kernel(GradArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = blockIdx.x * GS_COLS + lane * 8;
-    const bool in = col < a.out;  // out is a multiple of 128, so a lane's eight columns are all in or all out
-    const int c0 = in ? col : 0;
-    float sv[8], sum[8] = {};
-#pragma unroll
-    for (int q = 0; q < 8; q++) sv[q] = in ? h2f(a.svh[c0 + q]) : 0.f;
-    const int r0 = blockIdx.y * a.tile_rows, r1 = min(r0 + a.tile_rows, a.rows);
-    for (int r = r0 + wave; r < r1; r += 4) {
-        float d[8];
-        load8<DT>(a.dy, (size_t)r * a.out + c0, d);
-        if (a.act != ACT_NONE) {
-            float z[8];
-            load8<DT>(a.pre, (size_t)r * a.out + c0, z);
-#pragma unroll
-            for (int q = 0; q < 8; q++) d[q] *= act_slope(a.act, z[q]);
-        }
-        float m = 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; q++) {
-            m = fmaxf(m, fabsf(d[q] * sv[q]));  // columns past the end have sv = 0
-            sum[q] += d[q];
-        }
-        m = wave_max_abs(m);
-        if (lane == 0) a.amax[(size_t)r * a.chunks + blockIdx.x] = m;
-    }
-    if (!a.dbias) return;
-    __shared__ float part[4][GS_COLS];
-#pragma unroll
-    for (int q = 0; q < 8; q++) part[wave][lane * 8 + q] = sum[q];
+    __shared__ float part[4];
+    float m = 0.f;
+#pragma unroll 4
+    for (int c = threadIdx.x * 8; c < a.out; c += 2048) m = fmaxf(m, max8<DT>(a, blockIdx.x, c));
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
     __syncthreads();
-    float *dst = gridDim.y == 1 ? a.dbias : a.dbias_part + (size_t)blockIdx.y * a.out;
-    for (int i = threadIdx.x; i < GS_COLS; i += 256) {
-        const int cc = blockIdx.x * GS_COLS + i;
-        if (cc < a.out) dst[cc] = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
-    }
+    if (threadIdx.x == 0) a.amax[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 }
 
-// dbias from the row tiles' sums, in tile order.
+// dbias from the row tiles' sums, in tile order (four interleaved shares of them, joined in order): 64 columns a
+// workgroup.  A chunk of rows after the first adds to what the ones before it left.
 __global__ __launch_bounds__(256) void grad_dbias_kernel(GradArgs a, int tiles) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= a.out) return;
+    __shared__ float part[4][64];
+    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;  // out is a multiple of 128
     float s = 0.f;
-    for (int t = 0; t < tiles; t++) s += a.dbias_part[(size_t)t * a.out + c];
-    a.dbias[c] = s;
+#pragma unroll 8
+    for (int t = q; t < tiles; t += 4) s += a.dbias_part[(size_t)t * a.out + c];
+    part[q][lane] = s;
+    __syncthreads();
+    if (q == 0) {
+        s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+        a.dbias[c] = a.dbias_adds ? a.dbias[c] + s : s;
+    }
 }
 
 // The power of two that brings m to 2^10 .. 2^11 (1 for zero and non-finite rows), and its inverse, both normal floats.
@@ -100,70 +95,114 @@ __device__ __forceinline__ int grad_exponent(float m) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// u in A-fragment order (gemm_prepare_frag_kernel's), 16 rows x one 128-block of the gradient a workgroup: wave w takes
-// rows 4 w .. 4 w + 3.  Rows past the end are zeros.  inv_scale[row] is written by the workgroups of block 0.
+// Two neighbouring values of a row.
 template <int DT>
+__device__ __forceinline__ void load2(const void *p, size_t i, float &x, float &y) {
+    if constexpr (DT == DT_F32) {
+        const float2 v = *reinterpret_cast<const float2 *>(static_cast<const float *>(p) + i);
+        x = v.x, y = v.y;
+    } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(p) + i);
+        x = DT == DT_F16 ? h2f((uint16_t)w) : __uint_as_float(w << 16);
+        y = DT == DT_F16 ? h2f((uint16_t)(w >> 16)) : __uint_as_float(w & 0xFFFF0000u);
+    }
+}
+
+// u in A-fragment order (gemm_prepare_frag_kernel's): workgroup (128-block b, row tile) takes a.prep_tiles fragment tiles
+// of 16 rows one after another, wave w their rows 4 w .. 4 w + 3, rows past the end as zeros; dbias_part[tile][col] = the
+// tile's sum of dz (one row tile: dbias itself).  inv_scale is written by the workgroups of block 0.
+// A lane holds columns 2 l and 2 l + 1 of a block (one load), which the transform takes as its values l and l + 64: the
+// transform of any order of the index's bits is the same up to that order, so value i is column 2 (i % 64) + i / 64 on both
+// of its sides.
+// SCAN: the rows' largest values are found here, every workgroup reading all of dy (at most 16 rows, every thread a share
+// of each: the second launch costs more than that).
+template <int DT, bool SCAN>
 __global__ __launch_bounds__(256) void grad_prepare_kernel(GradArgs a) {
-    const int b = blockIdx.x, rt = blockIdx.y;
+    const int b = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __shared__ __align__(16) uint16_t t[16][128 + 8];
-    __shared__ int ex[16];
-    const int m0 = rt * 16 + wave * 4;
-    const size_t col = (size_t)b * 128 + lane;
-    float v0[4], v1[4], z0[4], z1[4];
-    const float s0 = h2f(a.svh[col]), s1 = h2f(a.svh[col + 64]);
-#pragma unroll
-    for (int rr = 0; rr < 4; rr++) {
-        const size_t i = (size_t)min(m0 + rr, a.rows - 1) * a.out + col;
-        v0[rr] = load_act<DT>(a.dy, i);
-        v1[rr] = load_act<DT>(a.dy, i + 64);
-    }
-    if (a.act != ACT_NONE) {
+    __shared__ float sums[4][128];
+    __shared__ float tops[4][16];
+    const size_t col = (size_t)b * 128 + 2 * lane;
+    const uint32_t sw = *reinterpret_cast<const uint32_t *>(a.svh + col);
+    const float s0 = h2f((uint16_t)sw), s1 = h2f((uint16_t)(sw >> 16));
+    const float sc = fwht_relaid_sign(lane) * HAD_SCALE;
+    const int i0 = fwht_relaid_col(lane, 0), i1 = fwht_relaid_col(lane, 1);
+    const int c0 = 2 * (i0 & 63) + (i0 >> 6), c1 = 2 * (i1 & 63) + (i1 >> 6);
+    const int RT = (a.rows + 15) / 16, rt0 = blockIdx.y * a.prep_tiles, rt1 = min(rt0 + a.prep_tiles, RT);
+    float b0 = 0.f, b1 = 0.f;
+    for (int rt = rt0; rt < rt1; rt++) {
+        const int m0 = rt * 16 + wave * 4;
+        float v0[4], v1[4], m[4];
 #pragma unroll
         for (int rr = 0; rr < 4; rr++) {
-            const size_t i = (size_t)min(m0 + rr, a.rows - 1) * a.out + col;
-            z0[rr] = load_act<DT>(a.pre, i);
-            z1[rr] = load_act<DT>(a.pre, i + 64);
+            const int row = min(m0 + rr, a.rows - 1);
+            load2<DT>(a.dy, (size_t)row * a.out + col, v0[rr], v1[rr]);
+            if constexpr (!SCAN) m[rr] = a.amax[row];
         }
-    }
-    // the row's largest value over its chunks: 16 lanes a row
-    {
-        const int row = min(rt * 16 + (tid >> 4), a.rows - 1);
-        float m = 0.f;
-        for (int q = tid & 15; q < a.chunks; q += 16) m = fmaxf(m, a.amax[(size_t)row * a.chunks + q]);
-#pragma unroll
-        for (int k = 8; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-        if ((tid & 15) == 0) {
-            const int e = grad_exponent(m);
-            ex[tid >> 4] = e;
-            if (b == 0 && rt * 16 + (tid >> 4) < a.rows) a.inv_scale[rt * 16 + (tid >> 4)] = pow2(-e);
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int rr = 0; rr < 4; rr++) {
         if (a.act != ACT_NONE) {
-            v0[rr] *= act_slope(a.act, z0[rr]);
-            v1[rr] *= act_slope(a.act, z1[rr]);
-        }
-        const bool live = m0 + rr < a.rows;
-        v0[rr] = live ? v0[rr] * s0 : 0.f;
-        v1[rr] = live ? v1[rr] * s1 : 0.f;
-    }
-    fwht128_wave_rows_relaid<4>(v0, v1, lane);
-    const float sc = fwht_relaid_sign(lane) * HAD_SCALE;
-    const int c0 = fwht_relaid_col(lane, 0), c1 = fwht_relaid_col(lane, 1);
+            float z0[4], z1[4];
 #pragma unroll
-    for (int rr = 0; rr < 4; rr++) {
-        const int r = wave * 4 + rr;
-        const float two = pow2(ex[r]);
-        t[r][c0] = __half_as_ushort(__float2half_rn(v0[rr] * sc * two));
-        t[r][c1] = __half_as_ushort(__float2half_rn(v1[rr] * sc * two));
+            for (int rr = 0; rr < 4; rr++) load2<DT>(a.pre, (size_t)min(m0 + rr, a.rows - 1) * a.out + col, z0[rr], z1[rr]);
+            act_slopes<4>(a.act, z0, v0);
+            act_slopes<4>(a.act, z1, v1);
+        }
+        if constexpr (SCAN) {  // one row tile
+            float top[16] = {};
+            for (int c = tid * 8; c < a.out; c += 2048)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    if (r < a.rows) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) top[r + q] = fmaxf(top[r + q], max8<DT>(a, min(r + q, a.rows - 1), c));
+                    }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                top[r] = wave_max(top[r]);
+                if (lane == 0) tops[wave][r] = top[r];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int rr = 0; rr < 4; rr++) {
+                const int r = wave * 4 + rr;
+                m[rr] = fmaxf(fmaxf(tops[0][r], tops[1][r]), fmaxf(tops[2][r], tops[3][r]));
+            }
+        }
+        float two[4];
+#pragma unroll
+        for (int rr = 0; rr < 4; rr++) {
+            const bool live = m0 + rr < a.rows;
+            const int e = grad_exponent(m[rr]);
+            two[rr] = pow2(e);
+            if (b == 0 && lane == 0 && live) a.inv_scale[m0 + rr] = pow2(-e);
+            v0[rr] = live ? v0[rr] : 0.f;
+            v1[rr] = live ? v1[rr] : 0.f;
+            b0 += v0[rr];
+            b1 += v1[rr];
+            v0[rr] *= s0;
+            v1[rr] *= s1;
+        }
+        fwht128_wave_rows_relaid<4>(v0, v1, lane);
+        if (rt > rt0) __syncthreads();  // the tile before has been read
+#pragma unroll
+        for (int rr = 0; rr < 4; rr++) {
+            const int r = wave * 4 + rr;
+            t[r][c0] = __half_as_ushort(__float2half_rn(v0[rr] * sc * two[rr]));
+            t[r][c1] = __half_as_ushort(__float2half_rn(v1[rr] * sc * two[rr]));
+        }
+        __syncthreads();
+        const int c = lane & 15, h = lane >> 4;  // 32-k block `wave` of the 128-block, fragment lane (c, h)
+        const uint4 v = *reinterpret_cast<const uint4 *>(&t[c][wave * 32 + 8 * h]);
+        *reinterpret_cast<uint4 *>(a.u + ((size_t)rt * (a.out / 32) + (size_t)b * 4 + wave) * 512 + (size_t)lane * 8) = v;
     }
+    if (!a.dbias) return;
+    sums[wave][2 * lane] = b0;
+    sums[wave][2 * lane + 1] = b1;
     __syncthreads();
-    const int kq = tid >> 6, c = lane & 15, h = lane >> 4;  // 32-k block kq of the 128-block, fragment lane (c, h)
-    const uint4 v = *reinterpret_cast<const uint4 *>(&t[c][kq * 32 + 8 * h]);
-    *reinterpret_cast<uint4 *>(a.u + ((size_t)rt * (a.out / 32) + (size_t)b * 4 + kq) * 512 + (size_t)lane * 8) = v;
+    if (tid < 128) {
+        float *dst = a.dbias_part ? a.dbias_part + (size_t)blockIdx.y * a.out : a.dbias;
+        dst[b * 128 + tid] = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+    }
 }
 
 // The decoders' reader for the product with the transposed bank: the slab of super-step S is the input block's 8 k-tile
@@ -221,6 +260,19 @@ struct GradReader<FAM, 0> {
     }
 };
 
+// dx of row `row`, input block ib, from the splits' raw products, in split order (one wave).  BYPASS: products of the same
+// launch.
+template <int FAM, bool BYPASS>
+__device__ __forceinline__ void grad_finish_row(const GradArgs &a, int ib, int row, int lane) {
+    const size_t col = (size_t)ib * 128 + lane;
+    const float s0 = h2f(a.suh[col]), s1 = h2f(a.suh[col + 64]), inv = a.inv_scale[row];
+    float v0, v1;
+    sum_planes<BYPASS>(a.part + (size_t)row * a.in + (size_t)ib * 128, (size_t)a.rows * a.in, a.splits, lane, v0, v1);
+    fwht128_wave(v0, v1, lane);
+    const float sc = codebook_scale<FAM>() * HAD_SCALE;
+    store_y4(a.dx, a.dx_dtype, (size_t)row * a.in + col, v0 * (s0 * sc) * inv, v1 * (s1 * sc) * inv);
+}
+
 // Workgroup: a 256-row x 128-column tile of dx (one input block ib) over the output groups of one split.
 template <int FAM, int N>
 __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
@@ -257,8 +309,14 @@ __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (i < live) {
-                        plane[(size_t)i * a.in] = v0[i];
-                        plane[(size_t)i * a.in + 64] = v1[i];
+                        float *p0 = plane + (size_t)i * a.in;
+                        if (a.counters) {  // through to memory: another XCD's workgroup may read them in this launch
+                            __hip_atomic_store(p0, v0[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                            __hip_atomic_store(p0 + 64, v1[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                        } else {
+                            p0[0] = v0[i];
+                            p0[64] = v1[i];
+                        }
                     }
                 return;
             }
@@ -273,32 +331,30 @@ __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
                     store_y4(a.dx, a.dx_dtype, (row + i) * a.in + col, v0[i] * s0 * inv, v1[i] * s1 * inv);
                 }
         });
+    if (a.splits == 1 || !a.counters) return;
+    // The last split of the tile to arrive finishes its rows: the planes are acknowledged before the counter moves and
+    // read past the caches after it, and the counter is left at zero for the next launch.  (Device-wide release and acquire
+    // fences instead write back and drop whole L2s: 5.5 us more for 5 rows of 4096 x 4096.)  The waves here are the ones
+    // with live rows (the others ended before any barrier).
+    if ((wave >> 1) * 64 >= rows) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t *arrived = reinterpret_cast<uint32_t *>(&Bs[0][0]);  // the staging is read: the barrier above
+    uint32_t *ctr = a.counters + (size_t)(mt * nib + ib) * COUNTER_STRIDE;
+    if (wave == 0 && lane == 0)
+        *arrived = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*arrived != (uint32_t)(a.splits - 1)) return;
+    const int waves = 2 * ((rows + 63) / 64);
+    for (int r = wave; r < rows; r += waves) grad_finish_row<FAM, true>(a, ib, mt * G2_MT + r, lane);
+    if (wave == 0 && lane == 0) *ctr = 0u;
 }
 
-// dx from the splits' raw products, in split order: a wave per (input block, row).
+// A wave per (input block, row).
 template <int FAM>
 __global__ __launch_bounds__(256) void grad_finish_kernel(GradArgs a) {
-    const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + (int)(threadIdx.x >> 6);
-    if (row >= a.rows) return;
-    const size_t col = (size_t)blockIdx.x * 128 + lane;
-    const float s0 = h2f(a.suh[col]), s1 = h2f(a.suh[col + 64]), inv = a.inv_scale[row];
-    float v0, v1;
-    sum_planes<false>(a.part + (size_t)row * a.in + (size_t)blockIdx.x * 128, (size_t)a.rows * a.in, a.splits, lane, v0, v1);
-    fwht128_wave(v0, v1, lane);
-    const float sc = codebook_scale<FAM>() * HAD_SCALE;
-    store_y4(a.dx, a.dx_dtype, (size_t)row * a.in + col, v0 * (s0 * sc) * inv, v1 * (s1 * sc) * inv);
-}
-
-hipError_t run_grad_scan(const GradArgs &a, hipStream_t s) {
-    const int tiles = (a.rows + a.tile_rows - 1) / a.tile_rows;
-    const dim3 grid((unsigned)a.chunks, (unsigned)tiles);
-    if (a.dtype == DT_F16) hipLaunchKernelGGL(grad_scan_kernel<DT_F16>, grid, dim3(256), 0, s, a);
-    else if (a.dtype == DT_BF16) hipLaunchKernelGGL(grad_scan_kernel<DT_BF16>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(grad_scan_kernel<DT_F32>, grid, dim3(256), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !a.dbias || tiles == 1) return e;
-    hipLaunchKernelGGL(grad_dbias_kernel, dim3((unsigned)((a.out + 255) / 256)), dim3(256), 0, s, a, tiles);
-    return hipGetLastError();
+    const int row = blockIdx.y * 4 + (int)(threadIdx.x >> 6);
+    if (row < a.rows) grad_finish_row<FAM, false>(a, blockIdx.x, row, threadIdx.x & 63);
 }
 
 template <int FAM, int N>
@@ -306,7 +362,7 @@ static hipError_t launch_grad(const GradArgs &a, hipStream_t s) {
     const unsigned wgs = (unsigned)(a.in / 128) * (unsigned)((a.rows + G2_MT - 1) / G2_MT) * (unsigned)a.splits;
     hipLaunchKernelGGL((grad_gemm_kernel<FAM, N>), dim3(wgs), dim3(G4_THREADS), 0, s, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1) return e;
+    if (e != hipSuccess || a.splits == 1 || a.counters) return e;
     hipLaunchKernelGGL(grad_finish_kernel<FAM>, dim3((unsigned)(a.in / 128), (unsigned)((a.rows + 3) / 4)), dim3(256), 0, s,
                        a);
     return hipGetLastError();
@@ -335,12 +391,28 @@ static hipError_t launch_grad_fam(const GradArgs &a, hipStream_t s) {
     return launch_grad<FAM, 0>(a, s);
 }
 
-hipError_t run_grad_gemm(int fam, const GradArgs &a, hipStream_t s) {
-    const dim3 grid((unsigned)(a.out / 128), (unsigned)((a.rows + 15) / 16));
-    if (a.dtype == DT_F16) hipLaunchKernelGGL(grad_prepare_kernel<DT_F16>, grid, dim3(256), 0, s, a);
-    else if (a.dtype == DT_BF16) hipLaunchKernelGGL(grad_prepare_kernel<DT_BF16>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(grad_prepare_kernel<DT_F32>, grid, dim3(256), 0, s, a);
+template <int DT>
+static hipError_t launch_grad_prepare(const GradArgs &a, hipStream_t s) {
+    const int tiles = ((a.rows + 15) / 16 + a.prep_tiles - 1) / a.prep_tiles;
+    const dim3 grid((unsigned)(a.out / 128), (unsigned)tiles);
+    if (a.amax) {
+        hipLaunchKernelGGL((grad_scan_kernel<DT>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((grad_prepare_kernel<DT, false>), grid, dim3(256), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((grad_prepare_kernel<DT, true>), grid, dim3(256), 0, s, a);
+    }
     const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !a.dbias || !a.dbias_part) return e;
+    hipLaunchKernelGGL(grad_dbias_kernel, dim3((unsigned)(a.out / 64)), dim3(256), 0, s, a, tiles);
+    return hipGetLastError();
+}
+
+hipError_t run_gradient(int fam, const GradArgs &a, hipStream_t s) {
+    const hipError_t e = a.dtype == DT_F16    ? launch_grad_prepare<DT_F16>(a, s)
+                         : a.dtype == DT_BF16 ? launch_grad_prepare<DT_BF16>(a, s)
+                                              : launch_grad_prepare<DT_F32>(a, s);
     if (e != hipSuccess) return e;
     switch (fam) {
     case FAM_MCG: return launch_grad_fam<FAM_MCG>(a, s);

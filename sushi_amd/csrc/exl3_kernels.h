@@ -20,14 +20,12 @@ hipError_t run_reconstruct_tiled(int fam, const uint16_t *trellis, const uint32_
 enum Prologue : int { PRO_X = 0, PRO_MID = 1 };
 
 // What a dense linear does to its finished sums (exl3_epilogue.h): z = sum + bias[col], y = T(act(z) + residual), pre = T(z).
-// bias [out] in bias_dtype; residual and pre [rows][out] in y's dtype, as y is laid out (one bank).  bias and residual are
-// always readable: the host points an absent one at svh / y and clears its flag.  Launches with an epilogue are kernels of
+// bias [out] in bias_dtype; residual and pre [rows][out] in y's dtype, as y is laid out (one bank); each may be null.  Launches with an epilogue are kernels of
 // their own (the translation units exl3_*_epilogue*.hip): as a run-time choice its code and scalars slowed the plain ones
 // (one row of 4096 x 4096, n = 64: 7.1 -> 7.45 us; 2048 rows of 4096 x 14336 by 0.5%).
 enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_COUNT = 5 };
 struct EpilogueArgs {
     int act;
-    int has_bias, has_residual;
     int bias_dtype;
     const void *bias;
     const void *residual;
@@ -346,9 +344,7 @@ inline size_t gemm_kpart_bytes(int groups, int rows, int out) {
 hipError_t run_gemm(int fam, const GemmArgs &a, hipStream_t s);
 hipError_t run_gemm_epilogue(int fam, const GemmArgs &a, const EpilogueArgs &e, hipStream_t s);  // one bank
 
-// The backward pass of a linear with an epilogue (exl3_gradient.hip).  Rows are a chunk's for run_grad_gemm and all of
-// them for run_grad_scan; amax, inv_scale, dy, pre and dx point at the chunk's first row.
-constexpr int GRAD_SCAN_COLS = 512;  // columns of a scan workgroup (a.chunks = ceil(out / that))
+// The backward pass of a linear with an epilogue (exl3_gradient.hip), over one chunk of rows.
 struct GradArgs {
     const void *dy;         // [rows][out], 16-byte aligned
     const void *pre;        // the forward's z, like dy; unread with ACT_NONE
@@ -359,20 +355,20 @@ struct GradArgs {
     int n;
     const uint16_t *suh, *svh;
     DecodeK k;
-    int tile_rows;          // rows per row tile of the scan
-    int chunks;
-    float *amax;            // [rows][chunks]
+    int prep_tiles;         // 16-row tiles a prepare workgroup takes
+    float *amax;            // [rows], or null: the prepare finds the rows' largest values itself
     float *dbias;           // [out] or null
-    float *dbias_part;      // [row tiles][out], with more than one tile
+    int dbias_adds;         // a chunk after the first: dbias holds the ones before it
+    float *dbias_part;      // [row tiles][out]; null where one row tile is all the rows there are
     float *inv_scale;       // [rows]
     uint16_t *u;            // prepared gradient, 16-row fragment tiles
     int splits;             // of the contraction, at most out / 128
     float *part;            // [splits][rows][in] with more than one split
+    uint32_t *counters;     // one a tile of dx, zero between calls: the last split to arrive finishes; or null
     void *dx;
     int dx_dtype;
 };
-hipError_t run_grad_scan(const GradArgs &a, hipStream_t s);
-hipError_t run_grad_gemm(int fam, const GradArgs &a, hipStream_t s);
+hipError_t run_gradient(int fam, const GradArgs &a, hipStream_t s);
 
 hipError_t run_route_topk(const float *logits, int rows, int experts, int k, uint32_t *inds, float *scores,
                           hipStream_t s);
@@ -380,6 +376,7 @@ hipError_t run_route_topk(const float *logits, int rows, int experts, int k, uin
 // inds [rows][topk], an id past the experts is a dropped slot; logits [rows][experts] in dtype.
 constexpr int kRouterMaxExperts = 1024;
 constexpr int kBalanceMaxParts = 512;
+constexpr int kBalanceJoin = 16;  // parts the last workgroup of as many to arrive joins
 struct BalanceArgs {
     const void *logits;
     int dtype, rows, experts, topk;
@@ -389,9 +386,11 @@ struct BalanceArgs {
     float *loss;      // [1]
     int32_t *counts;  // [experts]
     float *weight;    // [experts]: the loss's derivative by each expert's sum of probabilities
-    float *part_sum;  // [parts][experts], with more than one part
-    int *part_count;  // [parts][experts]
-    int *part_live;   // [parts]
+    // with more than one part: the workgroups' and then the joins' (balance_joins of them)
+    float *part_sum;     // [parts + joins][experts]
+    int *part_count;     // [parts + joins][experts]
+    int *part_live;      // [parts + joins]
+    uint32_t *counters;  // 1 + joins of them, COUNTER_STRIDE words apart, zero between calls
 };
 struct RouterGradArgs {
     const void *logits;
@@ -404,6 +403,7 @@ struct RouterGradArgs {
     void *dlogits;           // like logits
 };
 int balance_parts(int rows, int experts);
+inline int balance_joins(int parts) { return (parts + kBalanceJoin - 1) / kBalanceJoin; }
 hipError_t run_balance_loss(const BalanceArgs &a, hipStream_t s);
 hipError_t run_router_backward(const RouterGradArgs &a, hipStream_t s);
 

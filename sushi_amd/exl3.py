@@ -183,7 +183,11 @@ class Decode:
             raise Exl3CodebookTableUnknown(f"{self.codebook.name} decode needs a codebook table")
 
     def c(self) -> _lib.DecodeT:
-        return _lib.DecodeT(int(self.codebook), int(self.window.bits), -1 if self.table is None else int(self.table))
+        c = self.__dict__.get("_c")  # the fields never change, and the library takes the struct by value
+        if c is None:
+            c = _lib.DecodeT(int(self.codebook), int(self.window.bits), -1 if self.table is None else int(self.table))
+            object.__setattr__(self, "_c", c)
+        return c
 
 
 MUL1 = Decode(Codebook.mul1)
@@ -501,8 +505,10 @@ class _Workspace:
         _check(_lib.load().exl3_workspace_init(buf.data_ptr(), buf.numel(), ctypes.c_void_p(handle)))
         return buf
 
-    def get(self, dev: torch.device, nbytes: int) -> torch.Tensor:
-        handle = self._stream_handle(dev)
+    def get(self, dev: torch.device, nbytes: int, handle: Optional[int] = None) -> torch.Tensor:
+        """The buffer of `dev`'s current stream (``handle``, where the caller has it)."""
+        if handle is None:
+            handle = self._stream_handle(dev)
         key = (dev.type, dev.index, handle)
         buf = self._buf.get(key)
         if buf is None or buf.numel() < nbytes:
@@ -671,24 +677,58 @@ def _act(act: str) -> int:
         raise Exl3ActivationUnknown(f"activation {act!r} (one of {', '.join(ACTIVATIONS)})") from None
 
 
-def _one_bank(p: Proj, dec: Decode, what: str) -> None:
-    if p.trellis.dim() != 4 or p.trellis.shape[0] != 1 or tuple(p.suh.shape) != (1, p.in_features) or \
-            tuple(p.svh.shape) != (1, p.out_features):
-        raise BadExl3Shape(f"{what}: trellis {tuple(p.trellis.shape)}, suh {tuple(p.suh.shape)}, svh "
-                           f"{tuple(p.svh.shape)} are not one bank's")
+def _one_bank(p: Proj, dec: Decode, what: str):
+    """(in, out, n) of a one-bank projection, its tensors checked."""
+    t, suh, svh = p.trellis, p.suh, p.svh
+    shape = t.shape
+    if len(shape) != 4 or shape[0] != 1:
+        raise BadExl3Shape(f"{what}: trellis {tuple(shape)} is not one bank's")
+    _, it, ot, n = shape
+    in_f, out_f = it * 16, ot * 16
+    if suh.shape != (1, in_f) or svh.shape != (1, out_f):
+        raise BadExl3Shape(f"{what}: trellis {tuple(shape)}, suh {tuple(suh.shape)}, svh {tuple(svh.shape)} are not one bank's")
     dec.require_table()
-    _u16_check(p.trellis, "trellis")
-    _f16_check(p.suh, "suh")
-    _f16_check(p.svh, "svh")
+    _u16_check(t, "trellis")
+    _f16_check(suh, "suh")
+    _f16_check(svh, "svh")
+    return in_f, out_f, n
 
 
-def _on_one_device(what: str, *ts: Optional[torch.Tensor]) -> torch.device:
-    """The device of the operands, all of them contiguous tensors of one GPU."""
-    _need_gpu(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise BadExl3Shape(f"{what}: operands on {sorted(str(d) for d in devs)}")
-    return devs.pop()
+def _raw_stream_slow(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# A GPU's current stream as the library takes it, without a Stream object (0.1 us against 1.9).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream_slow)
+
+
+class _NoSwitch:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return None
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def _on_one_device(what: str, *ts: Optional[torch.Tensor]):
+    """(device, guard): the one GPU that holds every operand, all of them contiguous, and a context in which it is the
+    current one."""
+    index = -2
+    for t in ts:
+        if t is None:
+            continue
+        i = t.get_device()
+        if i < 0 or not t.is_contiguous():
+            _need_gpu(t)
+        if index != i:
+            if index != -2:
+                raise BadExl3Shape(f"{what}: operands on {sorted({str(t.device) for t in ts if t is not None})}")
+            index = i
+    dev = ts[0].device
+    return dev, _NO_SWITCH if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def linear_epilogue(x: torch.Tensor, p: Proj, dec: Decode, bias: Optional[torch.Tensor] = None, act: str = "none",
@@ -698,27 +738,28 @@ def linear_epilogue(x: torch.Tensor, p: Proj, dec: Decode, bias: Optional[torch.
     rounded once.  bias [out] (f16, bf16 or f32), residual [rows, out] in y's dtype; ``act`` is one of ``ACTIVATIONS``.
     ``with_pre`` returns (y, pre) with pre = linear(x) + bias in y's dtype, which linear_epilogue_backward takes.
     Not recorded by autograd."""
-    if x.dim() != 2 or p.in_features != x.shape[1]:
+    in_f, out_f, n = _one_bank(p, dec, "linear_epilogue")
+    if x.dim() != 2 or x.shape[1] != in_f:
         raise BadExl3Shape(f"linear_epilogue: x {tuple(x.shape)} vs trellis {tuple(p.trellis.shape)}")
-    _one_bank(p, dec, "linear_epilogue")
     code = _act(act)
-    rows, in_f, out_f = int(x.shape[0]), p.in_features, p.out_features
+    rows = x.shape[0]
     dt = out_dtype or x.dtype
-    if bias is not None and tuple(bias.shape) != (out_f,):
+    if bias is not None and bias.shape != (out_f,):
         raise BadExl3Shape(f"linear_epilogue: bias {tuple(bias.shape)}, expected {(out_f,)}")
-    if residual is not None and (tuple(residual.shape) != (rows, out_f) or residual.dtype != dt):
+    if residual is not None and (residual.shape != (rows, out_f) or residual.dtype != dt):
         raise BadExl3Shape(f"linear_epilogue: residual {tuple(residual.shape)} {residual.dtype}, expected "
                            f"{(rows, out_f)} in y's {dt}")
-    dev = _on_one_device("linear_epilogue", x, p.trellis, p.suh, p.svh, bias, residual)
-    with torch.cuda.device(dev):
+    dev, guard = _on_one_device("linear_epilogue", x, p.trellis, p.suh, p.svh, bias, residual)
+    with guard:
         y = torch.empty(rows, out_f, dtype=dt, device=dev)
-        pre = torch.empty_like(y) if with_pre else None
+        pre = torch.empty(rows, out_f, dtype=dt, device=dev) if with_pre else None
         L = _lib.load()
-        ws = workspace.get(dev, L.exl3_linear_epilogue_workspace_size(rows, in_f, out_f, p.n))
-        _check(L.exl3_linear_epilogue(x.data_ptr(), _dt(x, "x"), rows, in_f, out_f, p.trellis.data_ptr(), p.n,
+        stream = _raw_stream(dev.index)
+        ws = workspace.get(dev, L.exl3_linear_epilogue_workspace_size(rows, in_f, out_f, n), stream)
+        _check(L.exl3_linear_epilogue(x.data_ptr(), _dt(x, "x"), rows, in_f, out_f, p.trellis.data_ptr(), n,
                                       p.suh.data_ptr(), p.svh.data_ptr(), dec.c(), _ptr(bias),
                                       0 if bias is None else _dt(bias, "bias"), code, _ptr(residual), y.data_ptr(),
-                                      _dt(y, "y"), _ptr(pre), ws.data_ptr(), ws.numel(), _stream(dev)))
+                                      _dt(y, "y"), _ptr(pre), ws.data_ptr(), ws.numel(), stream))
     return (y, pre) if with_pre else y
 
 
@@ -729,25 +770,26 @@ def linear_epilogue_backward(dy: torch.Tensor, p: Proj, dec: Decode, act: str = 
     frozen: dy [rows, out] -> (dx [rows, in] in ``dx_dtype``, dy's by default; dbias [out] f32, or None without
     ``with_dbias``).  ``pre`` is the forward's, in dy's dtype, and needed with an activation.  The residual's gradient is
     dy itself.  Every sum has a fixed order: equal calls give equal bits."""
-    if dy.dim() != 2 or p.out_features != dy.shape[1]:
+    in_f, out_f, n = _one_bank(p, dec, "linear_epilogue_backward")
+    if dy.dim() != 2 or dy.shape[1] != out_f:
         raise BadExl3Shape(f"linear_epilogue_backward: dy {tuple(dy.shape)} vs trellis {tuple(p.trellis.shape)}")
-    _one_bank(p, dec, "linear_epilogue_backward")
     code = _act(act)
-    rows, in_f, out_f = int(dy.shape[0]), p.in_features, p.out_features
+    rows = dy.shape[0]
     if code == 0:
         pre = None
     elif pre is None or pre.shape != dy.shape or pre.dtype != dy.dtype:
         raise BadExl3Shape(f"linear_epilogue_backward: {act} needs the forward's pre, shaped and typed as dy")
-    dev = _on_one_device("linear_epilogue_backward", dy, p.trellis, p.suh, p.svh, pre)
-    with torch.cuda.device(dev):
+    dev, guard = _on_one_device("linear_epilogue_backward", dy, p.trellis, p.suh, p.svh, pre)
+    with guard:
         dx = torch.empty(rows, in_f, dtype=dx_dtype or dy.dtype, device=dev)
         dbias = torch.empty(out_f, dtype=torch.float32, device=dev) if with_dbias else None
         L = _lib.load()
-        ws = workspace.get(dev, L.exl3_linear_epilogue_backward_workspace_size(rows, in_f, out_f))
-        _check(L.exl3_linear_epilogue_backward(dy.data_ptr(), _dt(dy, "dy"), rows, in_f, out_f, p.trellis.data_ptr(), p.n,
+        stream = _raw_stream(dev.index)
+        ws = workspace.get(dev, L.exl3_linear_epilogue_backward_workspace_size(rows, in_f, out_f), stream)
+        _check(L.exl3_linear_epilogue_backward(dy.data_ptr(), _dt(dy, "dy"), rows, in_f, out_f, p.trellis.data_ptr(), n,
                                                p.suh.data_ptr(), p.svh.data_ptr(), dec.c(), code, _ptr(pre),
                                                dx.data_ptr(), _dt(dx, "dx"), _ptr(dbias), ws.data_ptr(), ws.numel(),
-                                               _stream(dev)))
+                                               stream))
     return dx, dbias
 
 
@@ -1112,10 +1154,8 @@ def _router_operands(router_logits, inds, mask, what: str):
         raise BadExl3Dtype(f"{what}: inds dtype {inds.dtype} (u32/i32)")
     if mask is not None and mask.dtype not in (torch.bool, torch.uint8):
         raise BadExl3Dtype(f"{what}: mask dtype {mask.dtype} (bool or u8)")
-    rows = 1
-    for v in lg.shape[:-1]:
-        rows *= int(v)
-    return rows, int(lg.shape[-1]), int(inds.shape[-1])
+    experts = lg.shape[-1]
+    return (lg.numel() // experts if experts else 0), experts, inds.shape[-1]
 
 
 def moe_balance_loss(router_logits: torch.Tensor, inds: torch.Tensor, mask: Optional[torch.Tensor] = None,
@@ -1125,16 +1165,17 @@ def moe_balance_loss(router_logits: torch.Tensor, inds: torch.Tensor, mask: Opti
     live rows, loss = coef E sum_e (counts_e / (T K)) (mean over live rows of p_e).  An extension: the reference only
     serves."""
     rows, experts, topk = _router_operands(router_logits, inds, mask, "moe_balance_loss")
-    dev = _on_one_device("moe_balance_loss", router_logits, inds, mask)
-    with torch.cuda.device(dev):
+    dev, guard = _on_one_device("moe_balance_loss", router_logits, inds, mask)
+    with guard:
         loss = torch.empty((), dtype=torch.float32, device=dev)
         counts = torch.empty(experts, dtype=torch.int32, device=dev)
         weight = torch.empty(experts, dtype=torch.float32, device=dev)
         L = _lib.load()
-        ws = workspace.get(dev, L.exl3_balance_loss_workspace_size(rows, experts))
+        stream = _raw_stream(dev.index)
+        ws = workspace.get(dev, L.exl3_balance_loss_workspace_size(rows, experts), stream)
         _check(L.exl3_balance_loss(router_logits.data_ptr(), _dt(router_logits, "logits"), rows, experts,
                                    inds.data_ptr(), topk, _ptr(mask), float(coef), loss.data_ptr(), counts.data_ptr(),
-                                   weight.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)))
+                                   weight.data_ptr(), ws.data_ptr(), ws.numel(), stream))
     return BalanceLoss(loss, counts, weight)
 
 
@@ -1150,17 +1191,18 @@ def moe_router_backward(router_logits: torch.Tensor, inds: torch.Tensor, dscores
         raise BadExl3Shape(f"moe_router_backward: dscores {tuple(dscores.shape)} vs inds {tuple(inds.shape)}")
     if (weight is None) != (dloss is None):
         raise BadExl3Shape("moe_router_backward: the balance term takes both weight and dloss")
-    if weight is not None and (tuple(weight.shape) != (experts,) or dloss.numel() != 1):
+    if weight is not None and (weight.shape != (experts,) or dloss.numel() != 1):
         raise BadExl3Shape(f"moe_router_backward: weight {tuple(weight.shape)}, dloss {tuple(dloss.shape)}")
     for t, nm in ((dscores, "dscores"), (weight, "weight"), (dloss, "dloss")):
         if t is not None and t.dtype != torch.float32:
             raise BadExl3Dtype(f"moe_router_backward: {nm} dtype {t.dtype} (f32)")
-    dev = _on_one_device("moe_router_backward", router_logits, inds, mask, dscores, weight, dloss)
-    with torch.cuda.device(dev):
+    dev, guard = _on_one_device("moe_router_backward", router_logits, inds, mask, dscores, weight, dloss)
+    with guard:
         dlogits = torch.empty_like(router_logits)
         _check(_lib.load().exl3_router_backward(router_logits.data_ptr(), _dt(router_logits, "logits"), rows, experts,
                                                 inds.data_ptr(), topk, _ptr(dscores), _ptr(weight), _ptr(dloss),
-                                                _ptr(mask), dlogits.data_ptr(), _stream(dev)))
+                                                _ptr(mask), dlogits.data_ptr(),
+                                                _raw_stream(dev.index)))
     return dlogits
 
 

@@ -137,7 +137,7 @@ def backward(dy, p, odec, act_name="none", pre=None, dx_dtype=None):
     bound = (ddz + dz.shape[0] * 2.0 ** -24 * dz.abs()).sum(0)
     svh = p.svh[0].cpu().double()
     v = dz * svh
-    top = v.abs().amax(1, keepdim=True)
+    top = (g * svh).abs().amax(1, keepdim=True)
     s = torch.where(top > 0, 2.0 ** (10 - torch.floor(torch.log2(top.clamp(min=1e-300)))), torch.ones_like(top))
     u, du = _prepared(v * s, (ddz * svh.abs() + 2.0 ** -24 * v.abs()) * s)
     du = du + 2.0 ** -24  # a row's scale may be the next power of two: f16's subnormal step there

@@ -50,7 +50,7 @@ def test_forward_refusals():
     assert _fwd(xdt=9) == -2 and _fwd(ydt=3) == -2
     assert _fwd(bias=FAKE, bdt=7) == -2
     assert _fwd(bdt=7) == -9  # without a bias its dtype is not looked at
-    for name in ("x", "bias", "res", "y", "pre", "svh"):
+    for name in ("x", "bias", "res", "y", "pre"):
         assert _fwd(**{name: FAKE + 2}) == -1, name
         assert "4-byte" in L.last_error()
 
@@ -59,7 +59,8 @@ def test_backward_refusals():
     assert _bwd(dt=9) == -2
     assert _bwd(act=3) == -1 and "pre" in L.last_error()
     assert _bwd(dy=FAKE + 4) == -1 and "16-byte" in L.last_error()
-    assert _bwd(act=3, pre=FAKE + 8) == -1
+    assert _bwd(act=3, pre=FAKE + 4) == -1 and _bwd(dx=FAKE + 1) == -1 and _bwd(svh=FAKE + 8) == -1
+    assert _bwd(act=3, pre=FAKE + 8) == -9  # pre needs no more than 8 bytes
     assert _bwd(fin=128 * 65536 // 8) == -1
 
 
