@@ -334,11 +334,6 @@ int32_t linear_impl(const void *x, int32_t x_dtype, int32_t groups, int32_t rows
 int epilogue_chunk(int width) { return width < 65536 ? 16384 : 1024; }
 
 size_t elem_size(int dt) { return dt == EXL3_DT_F32 ? 4 : 2; }
-// Width up to which the gradient's prepare finds the largest values of up to 16 rows itself, and rows up to which the last
-// split of a tile to arrive sums the splits.
-constexpr int kGradScanOut = 8192;
-constexpr int kGradFinishRows = 32;
-
 const void *at_row(const void *p, size_t row, size_t width, int dt) {
     return p ? static_cast<const char *>(p) + row * width * elem_size(dt) : nullptr;
 }
@@ -354,7 +349,6 @@ int32_t act_check(int32_t act, const char *what) {
 // The backward pass's launch shape for a chunk of rows.
 struct GradPlan {
     int prep_tiles, tiles, splits;
-    bool scan, finish;  // kernels of their own for the rows' largest values and for the splits' sum
     size_t amax, dbias_part, inv, u, part;
     size_t bytes() const { return kZeroBytes + amax + dbias_part + inv + u + part; }
 };
@@ -366,13 +360,11 @@ GradPlan plan_grad(int rows, int in, int out, bool whole) {
     // 64 rows a prepare workgroup once that leaves eight workgroups a CU: dbias then has a quarter of the partial sums.
     p.prep_tiles = (long)(rt / 4) * (out / 128) >= 2048 ? 4 : 1;
     p.tiles = (rt + p.prep_tiles - 1) / p.prep_tiles;
-    p.scan = rows > 16 || out > kGradScanOut;
     // The contraction is split until the workgroups fill the GPU's 256 CUs (one a CU), each split at least two output
     // groups.
     const int tiles = in / 128 * ((rows + 255) / 256), groups = out / 128;
     p.splits = std::max(1, std::min(256 / std::max(tiles, 1), groups / 2));
-    p.finish = rows > kGradFinishRows;
-    p.amax = p.scan ? align_up((size_t)rows * sizeof(float)) : 0;
+    p.amax = align_up((size_t)rows * sizeof(float));
     p.dbias_part = p.tiles > 1 || !whole ? align_up((size_t)p.tiles * out * sizeof(float)) : 0;
     p.inv = align_up((size_t)rows * sizeof(float));
     p.u = align_up((size_t)rt * 16 * out * 2);
@@ -1607,7 +1599,6 @@ int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t row
         c.u = reinterpret_cast<uint16_t *>(take(p.u));
         c.part = take(p.part);
         c.splits = p.splits;
-        c.counters = p.finish ? nullptr : static_cast<uint32_t *>(workspace);  // at most 256 tiles where splits > 1
         c.dy = at_row(dy, r, out_features, dtype);
         c.pre = at_row(a.pre, r, out_features, dtype);
         c.dx = at_row(dx, r, in_features, dx_dtype);

@@ -5,12 +5,12 @@
 // forward's prepared input is, under a power of two per row that brings the row's largest |dy * svh| to 2^10 .. 2^11:
 // gradients lie far below f16's normal range, and |H v| <= sqrt(128) max |v| keeps the scaled values below 2^15.
 //
-//   grad_scan_kernel     reads dy: each row's largest |dy * svh| (short calls leave it to the prepare)
+//   grad_scan_kernel     reads dy: each row's largest |dy * svh|
 //   grad_prepare_kernel  reads dy and pre: u in MFMA A-fragment order, each row's scale, dbias's sums by row tile
 //   grad_gemm_kernel     u W^T on the decode-wave tile (exl3_gemm_tile.h), the trellis decoded once per 256 rows into the
 //                        same column-major slab as the forward's and read back transposed by the MFMA waves; with few
-//                        row and column tiles the contraction is split, and the splits' products are summed in order by
-//                        the last of them to arrive (few rows) or by grad_finish_kernel
+//                        row and column tiles the contraction is split
+//   grad_finish_kernel   sums the splits' products in their order
 // The scale goes by |dy * svh| and not by |dz * svh|, so the activation is evaluated once: every slope is below 1.13, so
 // the bound on the scaled values holds with 13% more, and slopes that are small in a whole row cost it range that f16 has
 // (2^24 between the largest value and where its steps grow).
@@ -114,15 +114,12 @@ __device__ __forceinline__ void load2(const void *p, size_t i, float &x, float &
 // A lane holds columns 2 l and 2 l + 1 of a block (one load), which the transform takes as its values l and l + 64: the
 // transform of any order of the index's bits is the same up to that order, so value i is column 2 (i % 64) + i / 64 on both
 // of its sides.
-// SCAN: the rows' largest values are found here, every workgroup reading all of dy (at most 16 rows, every thread a share
-// of each: the second launch costs more than that).
-template <int DT, bool SCAN>
+template <int DT>
 __global__ __launch_bounds__(256) void grad_prepare_kernel(GradArgs a) {
     const int b = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __shared__ __align__(16) uint16_t t[16][128 + 8];
     __shared__ float sums[4][128];
-    __shared__ float tops[4][16];
     const size_t col = (size_t)b * 128 + 2 * lane;
     const uint32_t sw = *reinterpret_cast<const uint32_t *>(a.svh + col);
     const float s0 = h2f((uint16_t)sw), s1 = h2f((uint16_t)(sw >> 16));
@@ -138,7 +135,7 @@ __global__ __launch_bounds__(256) void grad_prepare_kernel(GradArgs a) {
         for (int rr = 0; rr < 4; rr++) {
             const int row = min(m0 + rr, a.rows - 1);
             load2<DT>(a.dy, (size_t)row * a.out + col, v0[rr], v1[rr]);
-            if constexpr (!SCAN) m[rr] = a.amax[row];
+            m[rr] = a.amax[row];
         }
         if (a.act != ACT_NONE) {
             float z0[4], z1[4];
@@ -146,27 +143,6 @@ __global__ __launch_bounds__(256) void grad_prepare_kernel(GradArgs a) {
             for (int rr = 0; rr < 4; rr++) load2<DT>(a.pre, (size_t)min(m0 + rr, a.rows - 1) * a.out + col, z0[rr], z1[rr]);
             act_slopes<4>(a.act, z0, v0);
             act_slopes<4>(a.act, z1, v1);
-        }
-        if constexpr (SCAN) {  // one row tile
-            float top[16] = {};
-            for (int c = tid * 8; c < a.out; c += 2048)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    if (r < a.rows) {
-#pragma unroll
-                        for (int q = 0; q < 4; q++) top[r + q] = fmaxf(top[r + q], max8<DT>(a, min(r + q, a.rows - 1), c));
-                    }
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                top[r] = wave_max(top[r]);
-                if (lane == 0) tops[wave][r] = top[r];
-            }
-            __syncthreads();
-#pragma unroll
-            for (int rr = 0; rr < 4; rr++) {
-                const int r = wave * 4 + rr;
-                m[rr] = fmaxf(fmaxf(tops[0][r], tops[1][r]), fmaxf(tops[2][r], tops[3][r]));
-            }
         }
         float two[4];
 #pragma unroll
@@ -260,19 +236,6 @@ struct GradReader<FAM, 0> {
     }
 };
 
-// dx of row `row`, input block ib, from the splits' raw products, in split order (one wave).  BYPASS: products of the same
-// launch.
-template <int FAM, bool BYPASS>
-__device__ __forceinline__ void grad_finish_row(const GradArgs &a, int ib, int row, int lane) {
-    const size_t col = (size_t)ib * 128 + lane;
-    const float s0 = h2f(a.suh[col]), s1 = h2f(a.suh[col + 64]), inv = a.inv_scale[row];
-    float v0, v1;
-    sum_planes<BYPASS>(a.part + (size_t)row * a.in + (size_t)ib * 128, (size_t)a.rows * a.in, a.splits, lane, v0, v1);
-    fwht128_wave(v0, v1, lane);
-    const float sc = codebook_scale<FAM>() * HAD_SCALE;
-    store_y4(a.dx, a.dx_dtype, (size_t)row * a.in + col, v0 * (s0 * sc) * inv, v1 * (s1 * sc) * inv);
-}
-
 // Workgroup: a 256-row x 128-column tile of dx (one input block ib) over the output groups of one split.
 template <int FAM, int N>
 __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
@@ -309,14 +272,8 @@ __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (i < live) {
-                        float *p0 = plane + (size_t)i * a.in;
-                        if (a.counters) {  // through to memory: another XCD's workgroup may read them in this launch
-                            __hip_atomic_store(p0, v0[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                            __hip_atomic_store(p0 + 64, v1[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                        } else {
-                            p0[0] = v0[i];
-                            p0[64] = v1[i];
-                        }
+                        plane[(size_t)i * a.in] = v0[i];
+                        plane[(size_t)i * a.in + 64] = v1[i];
                     }
                 return;
             }
@@ -331,30 +288,22 @@ __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
                     store_y4(a.dx, a.dx_dtype, (row + i) * a.in + col, v0[i] * s0 * inv, v1[i] * s1 * inv);
                 }
         });
-    if (a.splits == 1 || !a.counters) return;
-    // The last split of the tile to arrive finishes its rows: the planes are acknowledged before the counter moves and
-    // read past the caches after it, and the counter is left at zero for the next launch.  (Device-wide release and acquire
-    // fences instead write back and drop whole L2s: 5.5 us more for 5 rows of 4096 x 4096.)  The waves here are the ones
-    // with live rows (the others ended before any barrier).
-    if ((wave >> 1) * 64 >= rows) return;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    uint32_t *arrived = reinterpret_cast<uint32_t *>(&Bs[0][0]);  // the staging is read: the barrier above
-    uint32_t *ctr = a.counters + (size_t)(mt * nib + ib) * COUNTER_STRIDE;
-    if (wave == 0 && lane == 0)
-        *arrived = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (*arrived != (uint32_t)(a.splits - 1)) return;
-    const int waves = 2 * ((rows + 63) / 64);
-    for (int r = wave; r < rows; r += waves) grad_finish_row<FAM, true>(a, ib, mt * G2_MT + r, lane);
-    if (wave == 0 && lane == 0) *ctr = 0u;
 }
 
-// A wave per (input block, row).
+// dx from the splits' raw products, in split order: a wave per (input block, row).  (The last split of a tile to arrive did
+// this for its own rows at first: 0.9 us less for 1 row of 4096 x 4096, a launch being saved, and 0.5 to 1.3 us more for 5
+// and 8 rows, the sums then being a few waves' instead of the whole GPU's.)
 template <int FAM>
 __global__ __launch_bounds__(256) void grad_finish_kernel(GradArgs a) {
-    const int row = blockIdx.y * 4 + (int)(threadIdx.x >> 6);
-    if (row < a.rows) grad_finish_row<FAM, false>(a, blockIdx.x, row, threadIdx.x & 63);
+    const int ib = blockIdx.x, row = blockIdx.y * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= a.rows) return;
+    const size_t col = (size_t)ib * 128 + lane;
+    const float s0 = h2f(a.suh[col]), s1 = h2f(a.suh[col + 64]), inv = a.inv_scale[row];
+    float v0, v1;
+    sum_planes<false>(a.part + (size_t)row * a.in + (size_t)ib * 128, (size_t)a.rows * a.in, a.splits, lane, v0, v1);
+    fwht128_wave(v0, v1, lane);
+    const float sc = codebook_scale<FAM>() * HAD_SCALE;
+    store_y4(a.dx, a.dx_dtype, (size_t)row * a.in + col, v0 * (s0 * sc) * inv, v1 * (s1 * sc) * inv);
 }
 
 template <int FAM, int N>
@@ -362,7 +311,7 @@ static hipError_t launch_grad(const GradArgs &a, hipStream_t s) {
     const unsigned wgs = (unsigned)(a.in / 128) * (unsigned)((a.rows + G2_MT - 1) / G2_MT) * (unsigned)a.splits;
     hipLaunchKernelGGL((grad_gemm_kernel<FAM, N>), dim3(wgs), dim3(G4_THREADS), 0, s, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1 || a.counters) return e;
+    if (e != hipSuccess || a.splits == 1) return e;
     hipLaunchKernelGGL(grad_finish_kernel<FAM>, dim3((unsigned)(a.in / 128), (unsigned)((a.rows + 3) / 4)), dim3(256), 0, s,
                        a);
     return hipGetLastError();
@@ -395,15 +344,11 @@ template <int DT>
 static hipError_t launch_grad_prepare(const GradArgs &a, hipStream_t s) {
     const int tiles = ((a.rows + 15) / 16 + a.prep_tiles - 1) / a.prep_tiles;
     const dim3 grid((unsigned)(a.out / 128), (unsigned)tiles);
-    if (a.amax) {
-        hipLaunchKernelGGL((grad_scan_kernel<DT>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((grad_prepare_kernel<DT, false>), grid, dim3(256), 0, s, a);
-    } else {
-        hipLaunchKernelGGL((grad_prepare_kernel<DT, true>), grid, dim3(256), 0, s, a);
-    }
-    const hipError_t e = hipGetLastError();
+    hipLaunchKernelGGL((grad_scan_kernel<DT>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((grad_prepare_kernel<DT>), grid, dim3(256), 0, s, a);
+    e = hipGetLastError();
     if (e != hipSuccess || !a.dbias || !a.dbias_part) return e;
     hipLaunchKernelGGL(grad_dbias_kernel, dim3((unsigned)(a.out / 64)), dim3(256), 0, s, a, tiles);
     return hipGetLastError();

@@ -356,7 +356,7 @@ struct GradArgs {
     const uint16_t *suh, *svh;
     DecodeK k;
     int prep_tiles;         // 16-row tiles a prepare workgroup takes
-    float *amax;            // [rows], or null: the prepare finds the rows' largest values itself
+    float *amax;            // [rows]: each row's largest |dy * svh|
     float *dbias;           // [out] or null
     int dbias_adds;         // a chunk after the first: dbias holds the ones before it
     float *dbias_part;      // [row tiles][out]; null where one row tile is all the rows there are
@@ -364,7 +364,6 @@ struct GradArgs {
     uint16_t *u;            // prepared gradient, 16-row fragment tiles
     int splits;             // of the contraction, at most out / 128
     float *part;            // [splits][rows][in] with more than one split
-    uint32_t *counters;     // one a tile of dx, zero between calls: the last split to arrive finishes; or null
     void *dx;
     int dx_dtype;
 };
