@@ -1611,7 +1611,7 @@ int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t row
 size_t exl3_balance_loss_workspace_size(int32_t rows, int32_t experts) {
     if (rows < 0 || experts <= 0 || experts > kRouterMaxExperts) return 0;
     const size_t parts = (size_t)balance_parts(rows, experts), all = parts + balance_joins((int)parts);
-    return kZeroBytes + (parts > 1 ? 2 * align_up(all * experts * 4) + align_up(all * 4) : 0);
+    return kZeroBytes + (parts > 1 ? align_up(all * experts * 8) + align_up(all * 4) : 0);
 }
 
 int32_t exl3_balance_loss(const void *logits, int32_t dtype, int32_t rows, int32_t experts, const uint32_t *inds,
@@ -1625,7 +1625,7 @@ int32_t exl3_balance_loss(const void *logits, int32_t dtype, int32_t rows, int32
         return fail(EXL3_ERR_WORKSPACE, "balance_loss: workspace of %zu bytes (256-aligned) needed, got %zu", need,
                     workspace_bytes);
     const size_t parts = (size_t)balance_parts(rows, experts);
-    const size_t plane = align_up((parts + balance_joins((int)parts)) * experts * 4);
+    const size_t words = align_up((parts + balance_joins((int)parts)) * experts * 8);
     char *w = static_cast<char *>(workspace) + kZeroBytes;
     BalanceArgs a{};
     a.logits = logits;
@@ -1640,9 +1640,8 @@ int32_t exl3_balance_loss(const void *logits, int32_t dtype, int32_t rows, int32
     a.counts = counts;
     a.weight = weight;
     if (parts > 1) {
-        a.part_sum = reinterpret_cast<float *>(w);
-        a.part_count = reinterpret_cast<int *>(w + plane);
-        a.part_live = reinterpret_cast<int *>(w + 2 * plane);
+        a.parts = reinterpret_cast<uint64_t *>(w);
+        a.part_live = reinterpret_cast<int *>(w + words);
         a.counters = static_cast<uint32_t *>(workspace);
     }
     return launched(run_balance_loss(a, stream), "exl3_balance_loss");

@@ -386,8 +386,7 @@ struct BalanceArgs {
     int32_t *counts;  // [experts]
     float *weight;    // [experts]: the loss's derivative by each expert's sum of probabilities
     // with more than one part: the workgroups' and then the joins' (balance_joins of them)
-    float *part_sum;     // [parts + joins][experts]
-    int *part_count;     // [parts + joins][experts]
+    uint64_t *parts;     // [parts + joins][experts]: sum (high half) and count
     int *part_live;      // [parts + joins]
     uint32_t *counters;  // 1 + joins of them, COUNTER_STRIDE words apart, zero between calls
 };
