@@ -348,7 +348,7 @@ int32_t act_check(int32_t act, const char *what) {
 
 // The backward pass's launch shape for a chunk of rows.
 struct GradPlan {
-    int prep_tiles, tiles, splits;
+    int prep_tiles, tiles, tile_rows, splits;
     size_t amax, dbias_part, inv, u, part;
     size_t bytes() const { return kZeroBytes + amax + dbias_part + inv + u + part; }
 };
@@ -360,9 +360,13 @@ GradPlan plan_grad(int rows, int in, int out, bool whole) {
     // 64 rows a prepare workgroup once that leaves eight workgroups a CU: dbias then has a quarter of the partial sums.
     p.prep_tiles = (long)(rt / 4) * (out / 128) >= 2048 ? 4 : 1;
     p.tiles = (rt + p.prep_tiles - 1) / p.prep_tiles;
+    // Tiles of dx: as few row tiles of up to 256 as hold the rows, even in steps of 64 (a tile's waves hold 64 rows each; the
+    // longest tile of a launch sets its time).
+    const int row_tiles = (rows + 255) / 256;
+    p.tile_rows = 64 * ((rows + 64 * row_tiles - 1) / (64 * row_tiles));
     // The contraction is split until the workgroups fill the GPU's 256 CUs (one a CU), each split at least two output
     // groups.
-    const int tiles = in / 128 * ((rows + 255) / 256), groups = out / 128;
+    const int tiles = in / 128 * row_tiles, groups = out / 128;
     p.splits = std::max(1, std::min(256 / std::max(tiles, 1), groups / 2));
     p.amax = align_up((size_t)rows * sizeof(float));
     p.dbias_part = p.tiles > 1 || !whole ? align_up((size_t)p.tiles * out * sizeof(float)) : 0;
@@ -1598,6 +1602,7 @@ int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t row
         c.inv_scale = take(p.inv);
         c.u = reinterpret_cast<uint16_t *>(take(p.u));
         c.part = take(p.part);
+        c.tile_rows = p.tile_rows;
         c.splits = p.splits;
         c.dy = at_row(dy, r, out_features, dtype);
         c.pre = at_row(a.pre, r, out_features, dtype);

@@ -236,10 +236,11 @@ struct GradReader<FAM, 0> {
     }
 };
 
-// Workgroup: a 256-row x 128-column tile of dx (one input block ib) over the output groups of one split.
+// Workgroup: a tile of dx of a.tile_rows rows (up to 256) x 128 columns (one input block ib) over the output groups of one
+// split.
 template <int FAM, int N>
 __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
-    const int nib = a.in / 128, nm = (a.rows + G2_MT - 1) / G2_MT, nog = a.out / 128;
+    const int nib = a.in / 128, nm = (a.rows + a.tile_rows - 1) / a.tile_rows, nog = a.out / 128;
     const int sp = (int)blockIdx.x / (nib * nm), L = (int)blockIdx.x - sp * nib * nm;
     int ib, mt;
     if (nm <= 8 && 8 % nm == 0 && nib % (8 / nm) == 0) {  // a row tile's workgroups share an XCD (its u in one L2)
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
     }
     const int g0 = (int)((long)nog * sp / a.splits), nsup = (int)((long)nog * (sp + 1) / a.splits) - g0;  // >= 1 each
     __shared__ __align__(16) uint16_t Bs[2][128 * G4_BP];
-    const int rows = min(G2_MT, a.rows - mt * G2_MT);
+    const int rows = min(a.tile_rows, a.rows - mt * a.tile_rows);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int d = gemm4_decoder(wave, rows);
@@ -262,11 +263,11 @@ __global__ __launch_bounds__(G4_THREADS) void grad_gemm_kernel(GradArgs a) {
         });
         return;
     }
-    const uint16_t *u0 = a.u + (size_t)mt * (G2_MT / 16) * (size_t)(a.out / 32) * 512 + (size_t)g0 * 4 * 512;
+    const uint16_t *u0 = a.u + (size_t)mt * (a.tile_rows / 16) * (size_t)(a.out / 32) * 512 + (size_t)g0 * 4 * 512;
     gemm4_mfma_waves<true>(
         a.out, 2 * nsup, u0, rows, nullptr, Bs,
         [&](int m, int live, float (&v0)[4], float (&v1)[4], int ln, uint32_t) __attribute__((always_inline)) {
-            const size_t row = (size_t)mt * G2_MT + m, col = (size_t)ib * 128 + ln;
+            const size_t row = (size_t)mt * a.tile_rows + m, col = (size_t)ib * 128 + ln;
             if (a.splits > 1) {  // the raw products, for grad_finish_kernel
                 float *plane = a.part + ((size_t)sp * a.rows + row) * a.in + col;
 #pragma unroll
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(256) void grad_finish_kernel(GradArgs a) {
 
 template <int FAM, int N>
 static hipError_t launch_grad(const GradArgs &a, hipStream_t s) {
-    const unsigned wgs = (unsigned)(a.in / 128) * (unsigned)((a.rows + G2_MT - 1) / G2_MT) * (unsigned)a.splits;
+    const unsigned wgs = (unsigned)(a.in / 128) * (unsigned)((a.rows + a.tile_rows - 1) / a.tile_rows) * (unsigned)a.splits;
     hipLaunchKernelGGL((grad_gemm_kernel<FAM, N>), dim3(wgs), dim3(G4_THREADS), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;

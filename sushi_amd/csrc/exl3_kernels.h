@@ -362,6 +362,7 @@ struct GradArgs {
     float *dbias_part;      // [row tiles][out]; null where one row tile is all the rows there are
     float *inv_scale;       // [rows]
     uint16_t *u;            // prepared gradient, 16-row fragment tiles
+    int tile_rows;          // of a tile of dx: a multiple of 64 up to 256
     int splits;             // of the contraction, at most out / 128
     float *part;            // [splits][rows][in] with more than one split
     void *dx;

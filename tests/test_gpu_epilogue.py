@@ -207,6 +207,22 @@ def test_gradients_against_f64(dev, case):
         assert dbias is None
 
 
+@pytest.mark.parametrize("rows,in_f,out_f", [(256, 128, 256), (320, 256, 384), (384, 128, 256), (385, 128, 256),
+                                             (512, 256, 128), (513, 128, 256), (576, 384, 256), (577, 128, 256),
+                                             (2089, 128, 8192)])
+def test_gradients_at_the_ends_of_row_tiles(dev, rows, in_f, out_f):
+    """Row tiles of 192 and 256 rows, full and with a rest, and the prepare that takes four row tiles a workgroup."""
+    dec, odec = E.DECODES["mcg"]
+    p = _proj(rows, in_f, out_f, 48, dev)
+    dy = _normal(rows, "dy", (rows, out_f), BF16, dev)
+    pre = _normal(rows, "pre", (rows, out_f), BF16, dev, 1.5)
+    dx, dbias = exl3.linear_epilogue_backward(dy, p, dec, act="silu", pre=pre, with_dbias=True)
+    torch.cuda.synchronize()
+    wx, bx, wb, bb = E.backward(dy, p, odec, "silu", pre, None)
+    _held(dx, wx, bx, "dx")
+    _held(dbias, wb, bb, "dbias")
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-7, 1e4, 1e30])
 def test_gradients_of_any_scale(dev, scale):
     """f16's range bounds neither small nor large gradients: every row's prepared values are rescaled."""
