@@ -209,7 +209,8 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
  * z for the backward pass, or is null.  silu is z sigmoid(z), gelu z Phi(z), gelu_tanh its tanh approximation.  Every arm
  * of exl3_linear finishes this way in its own launch.  x, bias, residual, y and pre 4-byte aligned.
  *
- * Backward: from dy [rows][out] (and pre, both in `dtype`; pre unread with EXL3_ACT_NONE; dy and svh 16-byte aligned, pre 8-byte)
+ * Backward: from dy [rows][out] (and pre, both in `dtype`; pre unread with EXL3_ACT_NONE; dy and svh 16-byte aligned,
+ * pre 8-byte)
  *   dz = dy act'(pre),  dbias [out] = sum over rows of dz (f32; null: not wanted),
  *   dx [rows][in] = H(f16(s H(dz * svh)) W^T) * suh / s  in dx_dtype,
  * H the orthonormal Hadamard transform of each 128, W the decoded inner weight and s a power of two per row that brings

@@ -1,5 +1,6 @@
 // The decode-wave GEMM tile: decode waves fill an LDS slab with a bank's weights while MFMA waves multiply it.  Shared by
-// the dense and routed prefill GEMMs (exl3_gemm.hip) and the product with the transposed bank (exl3_gradient.hip).
+// the dense and routed prefill GEMMs (exl3_gemm_body.h, exl3_moe_gemm.hip) and the product with the transposed
+// bank (exl3_gradient.hip).
 #pragma once
 #include "exl3_kernels.h"
 #include "exl3_lane_decode.h"

@@ -20,9 +20,10 @@ hipError_t run_reconstruct_tiled(int fam, const uint16_t *trellis, const uint32_
 enum Prologue : int { PRO_X = 0, PRO_MID = 1 };
 
 // What a dense linear does to its finished sums (exl3_epilogue.h): z = sum + bias[col], y = T(act(z) + residual), pre = T(z).
-// bias [out] in bias_dtype; residual and pre [rows][out] in y's dtype, as y is laid out (one bank); each may be null.  Launches with an epilogue are kernels of
-// their own (the translation units exl3_*_epilogue*.hip): as a run-time choice its code and scalars slowed the plain ones
-// (one row of 4096 x 4096, n = 64: 7.1 -> 7.45 us; 2048 rows of 4096 x 14336 by 0.5%).
+// bias [out] in bias_dtype; residual and pre [rows][out] in y's dtype, as y is laid out (one bank); each may be null.
+// Launches with an epilogue are kernels of their own (the translation units exl3_*_epilogue*.hip): as a run-time choice
+// its code and scalars slowed the plain ones (one row of 4096 x 4096, n = 64: 7.1 -> 7.45 us; 2048 rows of 4096 x 14336
+// by 0.5%).
 enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_COUNT = 5 };
 struct EpilogueArgs {
     int act;
