@@ -206,8 +206,9 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
  *
  * Forward: z = linear(x) + bias, y = act(z) + residual, from the f32 sums with one rounding to y's dtype.  bias [out] in
  * bias_dtype or null; residual [rows][out] in y's dtype or null, not overlapping y; pre [rows][out] in y's dtype receives
- * z for the backward pass, or is null.  silu is z sigmoid(z), gelu z Phi(z), gelu_tanh its tanh approximation.  Every arm
- * of exl3_linear finishes this way in its own launch.  x, bias, residual, y and pre 4-byte aligned.
+ * z for the backward pass, or is null.  silu is z sigmoid(z), gelu z Phi(z), gelu_tanh its tanh approximation.  Up to 16 rows
+ * the sums are exl3_linear's bit for bit; past them, where exl3_linear's tiles would leave CUs idle, the contraction is
+ * split over workgroups and its parts added in a fixed order.  x, bias, residual, y and pre 4-byte aligned.
  *
  * Backward: from dy [rows][out] (and pre, both in `dtype`; pre unread with EXL3_ACT_NONE; dy and svh 16-byte aligned,
  * pre 8-byte)
@@ -218,7 +219,8 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
  * f16's normal range).  residual's gradient is dy itself, x's rounding to f16 is passed through.  Each rounding of pre to
  * 16 bits moves act' as that of any kept activation does.
  *
- * Rows go in chunks of at most 16384, each its own launches. */
+ * Rows go in chunks of at most 16384, each its own launches.  A workspace size holds for its rows; a caller of several row
+ * counts takes the largest of theirs. */
 typedef enum {
     EXL3_ACT_NONE = 0,
     EXL3_ACT_RELU = 1,

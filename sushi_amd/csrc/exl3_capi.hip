@@ -243,6 +243,38 @@ int32_t linear_checks(const void *x, int32_t x_dtype, int32_t groups, int32_t ro
     return ok();
 }
 
+// How the decode-wave tile covers a product of `rows` rows, n columns and contraction k where the contraction may be split
+// over workgroups (launches with an epilogue, gradients).  As few row tiles of up to 256 as hold the rows, even in steps of
+// 64 (a tile's waves hold 64 rows each; the longest tile of a launch sets its time); splits until the workgroups fill the
+// 256 CUs (one a CU), each at least 256 long.
+struct TileSplit {
+    int tile_rows, splits;
+};
+TileSplit tile_split(int rows, int n, int k) {
+    const int row_tiles = (rows + 255) / 256, tiles = n / 128 * row_tiles;
+    return {64 * ((rows + 64 * row_tiles - 1) / (64 * row_tiles)), std::max(1, std::min(256 / std::max(tiles, 1), k / 256))};
+}
+
+// The decode-wave tile's k split in a linear with an epilogue: past the GEMV's rows, at a rate with a lane reader, no arm
+// pinned.  Its sums go through f32 planes to a finish kernel over the whole GPU, which also pays for one split while the
+// planes are small: in the tile the epilogue is the work of the waves that hold rows alone (MCG, gelu and residual, us in the
+// tile against planes: 64 x 256 x 8192 21.1 / 13.2, 64 x 4096 x 24576 50.9 / 46.9, 300 x 8192 x 10112 126 / 120.5, and past the
+// limit 128 x 4096 x 28672 56.6 / 57.0, 200 x 4096 x 32768 78.3 / 86.6).  splits 0: the tile finishes.  Split against the plain
+// linear in one split: 57 x 8960 x 3968 79.7 -> 24.6 us, 300 x 4096 x 4096 65.3 -> 32.3, 777 x 14336 x 4096 186 -> 119.
+constexpr size_t kPlanesAlone = 3u << 20;
+GemmSplit epilogue_split(int rows, int in, int out, int n) {
+    if (rows <= kRowsMax || !dense_lane_rate(n) || knob(EXL3_KNOB_GEMM_ARM, 0)) return {0, 256, nullptr};
+    const TileSplit t = tile_split(rows, out, in);
+    if (t.splits == 1 && (size_t)rows * out > kPlanesAlone) return {0, 256, nullptr};
+    return {t.splits, t.tile_rows, nullptr};
+}
+size_t planes_bytes(const GemmSplit &s, int rows, int out) {
+    return s.splits > 0 ? align_up((size_t)s.splits * rows * out * sizeof(float)) : 0;
+}
+size_t epilogue_ws(int rows, int in, int out, int n) {
+    return linear_ws(1, rows, in, out, n) + planes_bytes(epilogue_split(rows, in, out, n), rows, out);
+}
+
 // y_rows_major (decode-GEMV row counts only): group g's row r lands in output row r * groups + g, so y is
 // [rows][groups * out] (linearGroupedRows's layout, src/exl3/linear.zig:97-117) instead of [groups][rows][out].
 int32_t linear_impl(const void *x, int32_t x_dtype, int32_t groups, int32_t rows, int32_t in, int32_t out,
@@ -324,7 +356,13 @@ int32_t linear_impl(const void *x, int32_t x_dtype, int32_t groups, int32_t rows
         g.kctr = reinterpret_cast<uint32_t *>(w);
         g.kwait = gemm_split_wait(2L * groups * ((rows + 511) / 512) * (out / 128));
     }
-    if (epi) return launched(run_gemm_epilogue(fam, g, *epi, stream), "exl3_linear_epilogue (gemm)");
+    if (epi) {
+        GemmSplit split = epilogue_split(rows, in, out, n);
+        if (ws_bytes < need + planes_bytes(split, rows, out))  // (an arm unpinned since the caller's check)
+            return fail(EXL3_ERR_WORKSPACE, "linear_epilogue: workspace of %zu bytes needed", need + planes_bytes(split, rows, out));
+        if (split.splits > 0) split.part = reinterpret_cast<float *>(w + need);
+        return launched(run_gemm_epilogue(fam, g, *epi, split, stream), "exl3_linear_epilogue (gemm)");
+    }
     return launched(run_gemm(fam, g, stream), "exl3_linear (gemm)");
 }
 
@@ -360,14 +398,9 @@ GradPlan plan_grad(int rows, int in, int out, bool whole) {
     // 64 rows a prepare workgroup once that leaves eight workgroups a CU: dbias then has a quarter of the partial sums.
     p.prep_tiles = (long)(rt / 4) * (out / 128) >= 2048 ? 4 : 1;
     p.tiles = (rt + p.prep_tiles - 1) / p.prep_tiles;
-    // Tiles of dx: as few row tiles of up to 256 as hold the rows, even in steps of 64 (a tile's waves hold 64 rows each; the
-    // longest tile of a launch sets its time).
-    const int row_tiles = (rows + 255) / 256;
-    p.tile_rows = 64 * ((rows + 64 * row_tiles - 1) / (64 * row_tiles));
-    // The contraction is split until the workgroups fill the GPU's 256 CUs (one a CU), each split at least two output
-    // groups.
-    const int tiles = in / 128 * row_tiles, groups = out / 128;
-    p.splits = std::max(1, std::min(256 / std::max(tiles, 1), groups / 2));
+    const TileSplit t = tile_split(rows, in, out);
+    p.tile_rows = t.tile_rows;
+    p.splits = t.splits;
     p.amax = align_up((size_t)rows * sizeof(float));
     p.dbias_part = p.tiles > 1 || !whole ? align_up((size_t)p.tiles * out * sizeof(float)) : 0;
     p.inv = align_up((size_t)rows * sizeof(float));
@@ -1496,8 +1529,8 @@ int32_t exl3_route_topk(const float *logits, int32_t rows, int32_t experts, int3
 size_t exl3_linear_epilogue_workspace_size(int32_t rows, int32_t in_features, int32_t out_features, int32_t n) {
     if (rows <= 0 || in_features <= 0 || out_features <= 0) return 0;
     const int chunk = std::min(rows, epilogue_chunk(in_features)), rest = rows % chunk;
-    const size_t whole = linear_ws(1, chunk, in_features, out_features, n);
-    return rest ? std::max(whole, linear_ws(1, rest, in_features, out_features, n)) : whole;
+    const size_t whole = epilogue_ws(chunk, in_features, out_features, n);
+    return rest ? std::max(whole, epilogue_ws(rest, in_features, out_features, n)) : whole;
 }
 
 int32_t exl3_linear_epilogue(const void *x, int32_t x_dtype, int32_t rows, int32_t in_features, int32_t out_features,

@@ -138,6 +138,15 @@ __device__ __forceinline__ void act_slopes(int act, const float (&z)[N], float (
 #undef EXL3_ACT_SLOPES
 }
 
+// Two f32 values rounded to f16 or bf16 (gfx950 converts to both to nearest even).
+__device__ __forceinline__ uint32_t pack2(bool bf16, float x, float y) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+    return bf16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{x, y}), bf2_t))
+                : __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{x, y}), h2_t));
+}
+
 // Eight f32 values rounded to f16 or bf16, two at a time (gfx950 converts to both to nearest even).
 __device__ __forceinline__ uint4 pack8(bool bf16, const float (&v)[8]) {
     typedef float f2_t __attribute__((ext_vector_type(2)));

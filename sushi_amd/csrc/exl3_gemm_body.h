@@ -391,6 +391,118 @@ __global__ __launch_bounds__(G4_THREADS) void gemm4_epilogue_kernel(GemmArgs a, 
     gemm4_run<FAM, N, true>(a, &e);
 }
 
+// A tile of sp.tile_rows rows x 128 columns over one split's k: the raw products to its plane.
+template <int FAM, int N>
+__global__ __launch_bounds__(G4_THREADS) void gemm4_split_kernel(GemmArgs a, GemmSplit sp) {
+    const int OT = a.out >> 4, nog = a.out / 128, nm = (a.rows + sp.tile_rows - 1) / sp.tile_rows, nk = a.in / 128;
+    const int s = (int)blockIdx.x / (nog * nm), L = (int)blockIdx.x - s * nog * nm;
+    const int og = L % nog, mt = L / nog;
+    const int k0 = (int)((long)nk * s / sp.splits), nsup = (int)((long)nk * (s + 1) / sp.splits) - k0;  // >= 1 each
+    __shared__ __align__(16) uint16_t Bs[2][128 * G4_BP];
+    const int rows = min(sp.tile_rows, a.rows - mt * sp.tile_rows);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int d = gemm4_decoder(wave, rows);
+    if (d >= 0) {
+        gemm4_decode_role<FAM>(rows <= G4_HELP_ROWS, d, nsup, lane, Bs, [&](int r, int rs, int loads) {
+            return RateReader<FAM, N>(a.trellis + (size_t)k0 * 8 * OT * N, r, rs, OT, og, loads, lane, a.k);
+        });
+        return;
+    }
+    const uint16_t *xfrag0 =
+        a.xp + (size_t)mt * (sp.tile_rows / 16) * (size_t)(a.in / 32) * 512 + (size_t)k0 * 4 * 512;
+    float *plane = sp.part + ((size_t)s * a.rows + (size_t)mt * sp.tile_rows) * a.out + (size_t)og * 128;
+    gemm4_mfma_waves<false>(
+        a.in, 2 * nsup, xfrag0, rows, nullptr, Bs,
+        [&](int m, int live, float (&v0)[4], float (&v1)[4], int ln, uint32_t) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i < live) {
+                    float *p = plane + (size_t)(m + i) * a.out + ln;
+                    p[0] = v0[i];
+                    p[64] = v1[i];
+                }
+        });
+}
+
+// Columns i and i + 1 (i even) of a row in dtype dt, 4-byte aligned.
+__device__ __forceinline__ void load_pair(const void *p, int dt, size_t i, float &x, float &y) {
+    if (dt == DT_F32) {
+        x = static_cast<const float *>(p)[i];
+        y = static_cast<const float *>(p)[i + 1];
+        return;
+    }
+    const uint32_t w = act_word(p, dt, i);
+    x = act_from_word(w, dt, 0);
+    y = act_from_word(w, dt, 1);
+}
+__device__ __forceinline__ void store_pair(void *p, int dt, size_t i, float x, float y) {
+    if (dt == DT_F32) {
+        static_cast<float *>(p)[i] = x;
+        static_cast<float *>(p)[i + 1] = y;
+        return;
+    }
+    *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p) + i) = pack2(dt == DT_BF16, x, y);
+}
+
+// The outputs from the splits' planes, summed in split order: a wave takes R rows of an output block.  A lane holds columns
+// 2 l and 2 l + 1 (the transform of any order of the index's bits is the same up to that order), so every access but the
+// f32 rows' is one word or two of a lane.
+template <int FAM, int R>
+__global__ __launch_bounds__(256) void gemm_split_finish_kernel(GemmArgs a, GemmSplit sp, EpilogueArgs e) {
+    const int og = blockIdx.x, row0 = (blockIdx.y * 4 + (int)(threadIdx.x >> 6)) * R, lane = threadIdx.x & 63;
+    if (row0 >= a.rows) return;
+    const int live = min(R, a.rows - row0);
+    const size_t col = (size_t)og * 128 + 2 * lane;
+    float r0[R] = {}, r1[R] = {}, b0 = 0.f, b1 = 0.f;
+    if (e.residual) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            load_pair(e.residual, a.y_dtype, (size_t)(row0 + min(r, live - 1)) * a.out + col, r0[r], r1[r]);
+    }
+    if (e.bias) {
+        b0 = load_any(e.bias, e.bias_dtype, col);
+        b1 = load_any(e.bias, e.bias_dtype, col + 1);
+    }
+    constexpr float SC = codebook_scale<FAM>() * HAD_SCALE;
+    const float s0 = h2f(a.svh[col]) * SC, s1 = h2f(a.svh[col + 1]) * SC;
+    constexpr int CH = R == 1 ? 8 : 4;  // splits' loads in flight
+    const size_t stride = (size_t)a.rows * a.out;
+    float v0[R] = {}, v1[R] = {};
+    for (int q0 = 0; q0 < sp.splits; q0 += CH) {
+        float2 t[CH][R];
+#pragma unroll
+        for (int q = 0; q < CH; q++)
+#pragma unroll
+            for (int r = 0; r < R; r++)
+                t[q][r] = *reinterpret_cast<const float2 *>(sp.part + (size_t)min(q0 + q, sp.splits - 1) * stride +
+                                                            (size_t)(row0 + min(r, live - 1)) * a.out + col);
+#pragma unroll
+        for (int q = 0; q < CH; q++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                v0[r] += q0 + q < sp.splits ? t[q][r].x : 0.f;
+                v1[r] += q0 + q < sp.splits ? t[q][r].y : 0.f;
+            }
+    }
+    float z[8] = {}, y[8];
+    if constexpr (R == 1) fwht128_wave(v0[0], v1[0], lane);
+    else fwht128_wave_rows<R>(v0, v1, lane);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        z[2 * r] = v0[r] * s0 + b0;
+        z[2 * r + 1] = v1[r] * s1 + b1;
+    }
+    act_eight(e.act, z, y);
+#pragma unroll
+    for (int r = 0; r < R; r++)
+        if (r < live) {
+            const size_t i = (size_t)(row0 + r) * a.out + col;
+            store_pair(a.y, a.y_dtype, i, y[2 * r] + r0[r], y[2 * r + 1] + r1[r]);
+            if (e.pre) store_pair(e.pre, a.y_dtype, i, z[2 * r], z[2 * r + 1]);
+        }
+}
+
 // ---- the ping-pong GEMM (hash-product families at the lane-reader rates)
 //
 // A workgroup of 8 waves owns an MT-row x 128-column output tile (MT = 256 or 512; one Hadamard block wide, so the
@@ -810,14 +922,18 @@ __global__ __launch_bounds__(G5_THREADS, 1) void gemm5_epilogue_kernel(GemmArgs 
 
 // The launchers, for plain linears (EPI = false, e null) and those with an epilogue: exl3_gemm.hip builds the former,
 // exl3_gemm_epilogue.hip the latter.
+struct GemmEpilogue {
+    EpilogueArgs args;
+    GemmSplit split;
+};
 template <int FAM, int N, int MT, int KS, bool EPI>
-static void launch_gemm5(const GemmArgs &a, const EpilogueArgs *e, dim3 grid, hipStream_t s) {
-    if constexpr (EPI) hipLaunchKernelGGL((gemm5_epilogue_kernel<FAM, N, MT, KS>), grid, dim3(G5_THREADS), 0, s, a, *e);
+static void launch_gemm5(const GemmArgs &a, const GemmEpilogue *e, dim3 grid, hipStream_t s) {
+    if constexpr (EPI) hipLaunchKernelGGL((gemm5_epilogue_kernel<FAM, N, MT, KS>), grid, dim3(G5_THREADS), 0, s, a, e->args);
     else hipLaunchKernelGGL((gemm5_kernel<FAM, N, MT, KS>), grid, dim3(G5_THREADS), 0, s, a);
 }
 
 template <int FAM, int N, bool EPI>
-static hipError_t launch_gemm_lane_n(const GemmArgs &a, const EpilogueArgs *e, hipStream_t s) {
+static hipError_t launch_gemm_lane_n(const GemmArgs &a, const GemmEpilogue *e, hipStream_t s) {
     if (a.x_dtype == DT_F16) launch_gemm_prepare_frag<DT_F16>(a, s);
     else if (a.x_dtype == DT_BF16) launch_gemm_prepare_frag<DT_BF16>(a, s);
     else launch_gemm_prepare_frag<DT_F32>(a, s);
@@ -846,22 +962,38 @@ static hipError_t launch_gemm_lane_n(const GemmArgs &a, const EpilogueArgs *e, h
             return hipGetLastError();
         }
     }
+    if constexpr (EPI) {
+        if (e->split.part) {
+            const GemmSplit &sp = e->split;
+            const int tiles = (a.out / 128) * ((a.rows + sp.tile_rows - 1) / sp.tile_rows);
+            hipLaunchKernelGGL((gemm4_split_kernel<FAM, N>), dim3((unsigned)(tiles * sp.splits)), dim3(G4_THREADS), 0, s, a, sp);
+            const hipError_t launched = hipGetLastError();
+            if (launched != hipSuccess) return launched;
+            // four rows a wave once that leaves four waves a SIMD (200 rows of 2560 x 16384, two splits, gelu: 12.2 -> 9.5 us;
+            // 600 rows of 2048 x 2048, 9600 rows of a block, 1 us more)
+            const bool four = (long)a.rows * (a.out / 128) >= 16384;
+            const dim3 fg((unsigned)(a.out / 128), (unsigned)((a.rows + (four ? 15 : 3)) / (four ? 16 : 4)));
+            if (four) hipLaunchKernelGGL((gemm_split_finish_kernel<FAM, 4>), fg, dim3(256), 0, s, a, sp, e->args);
+            else hipLaunchKernelGGL((gemm_split_finish_kernel<FAM, 1>), fg, dim3(256), 0, s, a, sp, e->args);
+            return hipGetLastError();
+        }
+    }
     dim3 grid((unsigned)((a.out / 128) * ((a.rows + G2_MT - 1) / G2_MT)), 1, (unsigned)a.groups);
-    if constexpr (EPI) hipLaunchKernelGGL((gemm4_epilogue_kernel<FAM, N>), grid, dim3(G4_THREADS), 0, s, a, *e);
+    if constexpr (EPI) hipLaunchKernelGGL((gemm4_epilogue_kernel<FAM, N>), grid, dim3(G4_THREADS), 0, s, a, e->args);
     else hipLaunchKernelGGL((gemm4_kernel<FAM, N>), grid, dim3(G4_THREADS), 0, s, a);
     return hipGetLastError();
 }
 
 template <int FAM, int N, bool EPI>
-static hipError_t launch_gemm_n(const GemmArgs &a, const uint16_t *wt, const EpilogueArgs *e, hipStream_t s) {
+static hipError_t launch_gemm_n(const GemmArgs &a, const uint16_t *wt, const GemmEpilogue *e, hipStream_t s) {
     dim3 grid((unsigned)(a.out / 128), (unsigned)((a.rows + GM_MT - 1) / GM_MT), (unsigned)a.groups);
-    if constexpr (EPI) hipLaunchKernelGGL((gemm_epilogue_kernel<FAM, N>), grid, dim3(GM_THREADS), 0, s, a, wt, *e);
+    if constexpr (EPI) hipLaunchKernelGGL((gemm_epilogue_kernel<FAM, N>), grid, dim3(GM_THREADS), 0, s, a, wt, e->args);
     else hipLaunchKernelGGL((gemm_kernel<FAM, N>), grid, dim3(GM_THREADS), 0, s, a, wt);
     return hipGetLastError();
 }
 
 template <int FAM, bool EPI>
-static hipError_t launch_gemm_fam(const GemmArgs &a, const EpilogueArgs *e, hipStream_t s) {
+static hipError_t launch_gemm_fam(const GemmArgs &a, const GemmEpilogue *e, hipStream_t s) {
     switch (a.n) {
     case 16: return launch_gemm_lane_n<FAM, 16, EPI>(a, e, s);
     case 24: return launch_gemm_lane_n<FAM, 24, EPI>(a, e, s);
@@ -898,7 +1030,7 @@ static hipError_t launch_gemm_fam(const GemmArgs &a, const EpilogueArgs *e, hipS
 }
 
 template <bool EPI>
-static hipError_t launch_gemm(int fam, const GemmArgs &a, const EpilogueArgs *e, hipStream_t s) {
+static hipError_t launch_gemm(int fam, const GemmArgs &a, const GemmEpilogue *e, hipStream_t s) {
     switch (fam) {
     case FAM_MCG: return launch_gemm_fam<FAM_MCG, EPI>(a, e, s);
     case FAM_MUL1: return launch_gemm_fam<FAM_MUL1, EPI>(a, e, s);

@@ -343,7 +343,15 @@ inline size_t gemm_kpart_bytes(int groups, int rows, int out) {
     return (size_t)groups * ((rows + 511) / 512) * (out / 128) * 2 * 512 * 128 * sizeof(float);
 }
 hipError_t run_gemm(int fam, const GemmArgs &a, hipStream_t s);
-hipError_t run_gemm_epilogue(int fam, const GemmArgs &a, const EpilogueArgs &e, hipStream_t s);  // one bank
+// k split over workgroups on the decode-wave tile (launches with an epilogue): part [splits][rows][out] f32, or null where
+// the tile finishes its rows itself.
+struct GemmSplit {
+    int splits;
+    int tile_rows;  // rows a tile holds: a multiple of 64 up to 256
+    float *part;
+};
+hipError_t run_gemm_epilogue(int fam, const GemmArgs &a, const EpilogueArgs &e, const GemmSplit &split,
+                             hipStream_t s);  // one bank
 
 // The backward pass of a linear with an epilogue (exl3_gradient.hip), over one chunk of rows.
 struct GradArgs {

@@ -102,9 +102,34 @@ def test_epilogue_on_every_gemv_finish(dev, knobs):
 @pytest.mark.parametrize("rows", [1, 4, 11, 16, 31, 300, 700])
 @pytest.mark.parametrize("n", [48, 96, 18])
 def test_an_empty_epilogue_is_linear_bit_for_bit(dev, rows, n, dtype):
+    """On one arm: unpinned, wider calls split k where exl3_linear does not."""
     p = _proj(3, 512, 384, n, dev)
     x = _normal(4, "x", (rows, 512), dtype, dev)
-    assert torch.equal(exl3.linear_epilogue(x, p, exl3.MCG), exl3.linear(x, p, exl3.MCG))
+    with exl3.arm_overrides(gemm_arm=4):
+        assert torch.equal(exl3.linear_epilogue(x, p, exl3.MCG), exl3.linear(x, p, exl3.MCG))
+    if rows <= 16 or n == 18:
+        assert torch.equal(exl3.linear_epilogue(x, p, exl3.MCG), exl3.linear(x, p, exl3.MCG))
+
+
+# rows, in, out: one split through the planes, two and more with uneven parts, row tiles of 64, 128, 192 and 256 rows with
+# and without a rest, row counts whose plain linear takes another tile
+SPLIT = [(17, 128, 128), (17, 640, 128), (64, 256, 384), (65, 1152, 256), (128, 512, 128), (129, 896, 128),
+         (256, 768, 256), (257, 640, 128), (320, 1408, 128), (384, 512, 256), (385, 512, 128), (513, 768, 256),
+         (577, 512, 128)]
+
+
+@pytest.mark.parametrize("n,cb,dtype", [(48, "3inst", BF16), (24, "pair1", F16), (128, "mul1", F32), (40, "spec1", BF16)])
+@pytest.mark.parametrize("rows,in_f,out_f", SPLIT)
+def test_epilogue_with_k_in_splits(dev, rows, in_f, out_f, n, cb, dtype):
+    _forward_case(dev, rows, in_f, out_f, n, cb, dtype, "gelu", dtype, True, True)
+
+
+def test_row_splits_past_the_halves_tile(dev):
+    """Rows and widths where the plain linear takes k in halves or the 512-row tile keep those."""
+    for rows, out_f in ((300, 10240), (520, 12288)):
+        p = _proj(31, 256, out_f, 48, dev)
+        x = _normal(31, "x", (rows, 256), F16, dev)
+        assert torch.equal(exl3.linear_epilogue(x, p, exl3.MCG), exl3.linear(x, p, exl3.MCG))
 
 
 def test_epilogue_of_unaligned_and_small_operands(dev):
