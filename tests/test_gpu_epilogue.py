@@ -374,3 +374,32 @@ def test_streams_have_their_own_scratch(dev):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(got[i], want[i])
+
+
+def test_operators_share_a_workspace_and_streams_do_not(dev):
+    """The fold's words, the joins' counters and the splits' planes on one buffer, call after call in any order, and on two
+    streams at once: every result as when it ran alone."""
+    p = _proj(41, 1024, 512, 48, dev)
+    one, many = _normal(42, "a", (3, 1024), F16, dev), _normal(42, "b", (77, 1024), F16, dev)
+    dy = _normal(42, "d", (77, 512), F16, dev)
+    logits = _normal(42, "l", (9000, 64), BF16, dev)
+    inds = torch.randint(0, 64, (9000, 4), dtype=torch.int32, device=dev, generator=torch.Generator(dev).manual_seed(7))
+    calls = [lambda: exl3.moe_balance_loss(logits, inds), lambda: (exl3.linear(one, p, exl3.MCG),),
+             lambda: (exl3.linear_epilogue(many, p, exl3.MCG, act="silu"),),
+             lambda: exl3.linear_epilogue_backward(dy, p, exl3.MCG, with_dbias=True),
+             lambda: (exl3.linear_epilogue(one, p, exl3.MCG, act="gelu", residual=dy[:3]),)]
+    want = []
+    for call in calls:
+        want.append(call())
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = []
+    for step in range(3):
+        for i, s in enumerate(streams):
+            s.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(s):
+                got += [(k, calls[k]()) for k in ((step + 2 * i + j) % 5 for j in range(5))]
+    torch.cuda.synchronize()
+    for k, outs in got:
+        for a, b in zip(outs, want[k]):
+            assert torch.equal(a, b), k
