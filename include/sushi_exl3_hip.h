@@ -215,7 +215,7 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
  *   dz = dy act'(pre),  dbias [out] = sum over rows of dz (f32; null: not wanted),
  *   dx [rows][in] = H(f16(s H(dz * svh)) W^T) * suh / s  in dx_dtype,
  * H the orthonormal Hadamard transform of each 128, W the decoded inner weight and s a power of two per row that brings
- * the row's largest |dy * svh| to 2^10 .. 2^11 (the prepared gradient is f16 as the prepared input is; gradients lie below
+ * the row's largest |dz * svh| to 2^10 .. 2^11 (the prepared gradient is f16 as the prepared input is; gradients lie below
  * f16's normal range).  residual's gradient is dy itself, x's rounding to f16 is passed through.  Each rounding of pre to
  * 16 bits moves act' as that of any kept activation does.
  *

@@ -2,38 +2,40 @@
 // y = act(z) + residual,
 //   dz = dy * act'(z),  dbias = sum over rows of dz,  dx = H(u W^T) * suh,  u = f16(H(dz * svh))
 // (H: the orthonormal Hadamard transform of every 128; residual's gradient is dy itself).  u is rounded to f16 as the
-// forward's prepared input is, under a power of two per row that brings the row's largest |dy * svh| to 2^10 .. 2^11:
-// gradients lie far below f16's normal range, and |H v| <= sqrt(128) max |v| keeps the scaled values below 2^15.
+// forward's prepared input is, under a power of two per row that brings the row's largest |dz * svh| to 2^10 .. 2^11:
+// gradients lie far below f16's normal range, and |H v| <= sqrt(128) max |v| keeps the scaled values below 2^15.  (The largest
+// |dy * svh| would spare the scan pre and the slopes, but a row whose activations are all saturated, or one large gradient on
+// a dead unit, would then leave u in f16's subnormals: at pre = -7 +- 0.2 with gelu dx was off by 28 to 43% of its row's
+// largest value, at -9, with gelu_tanh at -6.5 or silu at -30 all of it.)
 //
-//   grad_scan_kernel     reads dy: each row's largest |dy * svh|
+//   grad_scan_kernel     reads dy and pre: each row's largest |dz * svh|
 //   grad_prepare_kernel  reads dy and pre: u in MFMA A-fragment order, each row's scale, dbias's sums by row tile
 //   grad_gemm_kernel     u W^T on the decode-wave tile (exl3_gemm_tile.h), the trellis decoded once per 256 rows into the
 //                        same column-major slab as the forward's and read back transposed by the MFMA waves; with few
 //                        row and column tiles the contraction is split
 //   grad_finish_kernel   sums the splits' products in their order
 // What bounds it and what it took (MI355X, medians of traced launches): 2048 rows of 4096 x 14336, n = 48, bf16,
-// gelu_tanh: scan 12 us (59 MB, 4.8 TB/s), prepare 42 to 47 (176 MB, 3.7 to 4.2 TB/s), dbias 5, product 235 to 266 (240
-// GFLOP, 0.90 to 1.02 PFLOP/s against 1.09 of a library product of f16 matrices, by the card's clock); 333 rows of 2560
-// x 16384, n = 96: 6 + 11 + 5, product 50 (its decode: 240 workgroups, every weight decoded by each of two row tiles),
-// finish 5; 5 rows of 4096 x 4096: 2.4 + 3.1 + 9.0 + 2.6 (each launch's floor about 2).
-//
-// The scale goes by |dy * svh| and not by |dz * svh|, so the activation is evaluated once: every slope is below 1.13, so
-// the bound on the scaled values holds with 13% more, and slopes that are small in a whole row cost it range that f16 has
-// (2^24 between the largest value and where its steps grow).
+// gelu_tanh: scan 28 us (117 MB and every slope; 12 us without an activation, dy alone at 4.8 TB/s), prepare 39 to 46 (176
+// MB, 3.8 to 4.5 TB/s), dbias 5, product 241 to 269 (240 GFLOP, 0.89 to 1.00 PFLOP/s against 1.09 of a library product of
+// f16 matrices, by the card's clock); 333 rows of 2560 x 16384, n = 96, gelu: 10 + 11 + 5, product 50 (its decode: 240
+// workgroups, every weight decoded by each of two row tiles), finish 5; 5 rows of 4096 x 4096: 2.4 + 3.1 + 8.6 + 2.2 (each
+// launch's floor about 2).
 #include "exl3_gemm_tile.h"
 #include "exl3_epilogue.h"
 
 namespace exl3 {
 
-// Eight consecutive values of a row (16-byte loads; the host checks the alignment).
+// Eight consecutive values of a row, 8-byte aligned (the host checks; the 16-byte loads need 4).
 template <int DT>
 __device__ __forceinline__ void load8(const void *p, size_t i, float (&v)[8]) {
     if constexpr (DT == DT_F32) {
-        const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-        const float4 b = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + 4);
+        typedef float f4a __attribute__((ext_vector_type(4), aligned(8)));
+        const f4a a = *reinterpret_cast<const f4a *>(static_cast<const float *>(p) + i);
+        const f4a b = *reinterpret_cast<const f4a *>(static_cast<const float *>(p) + i + 4);
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+        typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(8)));
+        const u4a a = *reinterpret_cast<const u4a *>(static_cast<const uint16_t *>(p) + i);
         const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
         for (int q = 0; q < 8; q++) {
@@ -52,25 +54,31 @@ __device__ __forceinline__ float wave_max(float v) {
     return fmaxf(v, __shfl_xor(v, 32));
 }
 
-// max |dy * svh| over eight columns of a row.
-template <int DT>
+// max |dz * svh| over eight columns of a row.  ACT: through an activation.
+template <int DT, bool ACT>
 __device__ __forceinline__ float max8(const GradArgs &a, int row, int c) {
     float d[8], m = 0.f;
     load8<DT>(a.dy, (size_t)row * a.out + c, d);
     const uint4 s = *reinterpret_cast<const uint4 *>(a.svh + c);
+    if constexpr (ACT) {
+        float z[8];
+        load8<DT>(a.pre, (size_t)row * a.out + c, z);
+        act_slopes<8>(a.act, z, d);
+    }
     const uint32_t w[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
     for (int q = 0; q < 8; q++) m = fmaxf(m, fabsf(d[q] * h2f((uint16_t)(q & 1 ? w[q >> 1] >> 16 : w[q >> 1] & 0xFFFFu))));
     return m;
 }
 
-// One workgroup a row.
-template <int DT>
+// One workgroup a row.  Through an activation its slopes are the time: they are evaluated here and again in the prepare (kept
+// between them, dz would be four bytes an element to write and read in place of pre's two).
+template <int DT, bool ACT>
 __global__ __launch_bounds__(256) void grad_scan_kernel(GradArgs a) {
     __shared__ float part[4];
     float m = 0.f;
-#pragma unroll 4
-    for (int c = threadIdx.x * 8; c < a.out; c += 2048) m = fmaxf(m, max8<DT>(a, blockIdx.x, c));
+#pragma unroll ACT ? 1 : 4
+    for (int c = threadIdx.x * 8; c < a.out; c += 2048) m = fmaxf(m, max8<DT, ACT>(a, blockIdx.x, c));
     m = wave_max(m);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
     __syncthreads();
@@ -351,7 +359,8 @@ template <int DT>
 static hipError_t launch_grad_prepare(const GradArgs &a, hipStream_t s) {
     const int tiles = ((a.rows + 15) / 16 + a.prep_tiles - 1) / a.prep_tiles;
     const dim3 grid((unsigned)(a.out / 128), (unsigned)tiles);
-    hipLaunchKernelGGL((grad_scan_kernel<DT>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    if (a.act == ACT_NONE) hipLaunchKernelGGL((grad_scan_kernel<DT, false>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((grad_scan_kernel<DT, true>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((grad_prepare_kernel<DT>), grid, dim3(256), 0, s, a);

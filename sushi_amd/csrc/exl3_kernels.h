@@ -365,7 +365,7 @@ struct GradArgs {
     const uint16_t *suh, *svh;
     DecodeK k;
     int prep_tiles;         // 16-row tiles a prepare workgroup takes
-    float *amax;            // [rows]: each row's largest |dy * svh|
+    float *amax;            // [rows]: each row's largest |dz * svh|
     float *dbias;           // [out] or null
     int dbias_adds;         // a chunk after the first: dbias holds the ones before it
     float *dbias_part;      // [row tiles][out]; null where one row tile is all the rows there are
