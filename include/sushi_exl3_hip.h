@@ -206,7 +206,8 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
  *
  * Forward: z = linear(x) + bias, y = act(z) + residual, from the f32 sums with one rounding to y's dtype.  bias [out] in
  * bias_dtype or null; residual [rows][out] in y's dtype or null, not overlapping y; pre [rows][out] in y's dtype receives
- * z for the backward pass, or is null.  silu is z sigmoid(z), gelu z Phi(z), gelu_tanh its tanh approximation.  Up to 16 rows
+ * z for the backward pass, or is null.  silu is z sigmoid(z), gelu z Phi(z), gelu_tanh its tanh approximation, each within
+ * 2e-5 of its own value down to z = -12 (3e-6 down to -5), so small values keep their precision too.  Up to 16 rows
  * the sums are exl3_linear's bit for bit; past them, where exl3_linear's tiles would leave CUs idle, the contraction is
  * split over workgroups and its parts added in a fixed order.  x, bias, residual, y and pre 4-byte aligned.
  *

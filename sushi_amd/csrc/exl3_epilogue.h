@@ -7,10 +7,13 @@
 namespace exl3 {
 
 // The activations run on the hardware's exp2 and reciprocal (an ulp each).  A row block's epilogue holds no other work, so
-// their instructions are its time: with the library's erfc and f32 divisions 200 rows of 2560 x 16384 with gelu, finished
-// in the tile, took 67 us, now 51.9, against 48.1 without an activation (2048 rows of 4096 x 14336: 238.5 against 223.1, silu 229.8).
-// gelu's normal CDF: Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, erfc(x) = P(t) exp(-x^2) with
-// t = 1 / (1 + p x) for x >= 0, within 1.5e-7; its exp is also the density of the slope.
+// their instructions are its time: 200 rows of 2560 x 16384, finished in the tile, take 48.3 us without an activation, 49.4
+// with silu, 50.4 with gelu_tanh, 52.7 with gelu (67 with the library's erfc and f32 divisions); 2048 rows of 4096 x 14336
+// 230.4, 237.3, 240.0 and 245.9.
+// gelu's normal CDF: its lower tail is Phi(-x) = t P(t) exp(-x^2 / 2) for x >= 0 with t = 1 / (1 + 0.21 x), P the polynomial of
+// degree 8 with the least relative error (1.9e-8) up to x = 14.5, past which an f32 exp vanishes.  So the tail keeps its
+// relative precision: within 5e-7 from -1 on, 1.5e-6 down to -5, 8e-6 at -12, there the exp's argument's rounding.  The exp
+// is also the density of the slope.
 __device__ __forceinline__ float rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 constexpr float GELU_A = 0.7978845608028654f;   // sqrt(2 / pi)
 constexpr float GELU_B = 0.044715f;
@@ -18,10 +21,18 @@ constexpr float INV_SQRT_2PI = 0.3989422804014327f;
 
 // Phi(z), and exp(-z^2 / 2) in `ex`.
 __device__ __forceinline__ float normal_cdf(float z, float &ex) {
-    const float x = fabsf(z) * 0.7071067811865476f, t = rcp(1.f + 0.3275911f * x);
-    const float poly = ((((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f) * t;
-    ex = __expf(-x * x);
-    const float q = 0.5f * poly * ex;
+    const float t = rcp(1.f + 0.21f * fabsf(z));
+    float poly = -0.0712944642f;
+    poly = poly * t + 0.281802952f;
+    poly = poly * t - 0.326489985f;
+    poly = poly * t + 0.344983011f;
+    poly = poly * t - 0.0907701403f;
+    poly = poly * t + 0.123471074f;
+    poly = poly * t + 0.0695700124f;
+    poly = poly * t + 0.0850124061f;
+    poly = poly * t + 0.0837151557f;
+    ex = __builtin_amdgcn_exp2f(z * z * -0.72134752f);  // -log2(e) / 2
+    const float q = poly * t * ex;
     return z >= 0.f ? 1.f - q : q;
 }
 
@@ -37,8 +48,8 @@ __device__ __forceinline__ float act_value(int act, float z) {
     return z * rcp(1.f + __expf(-u));
 }
 
-// act'(z).  Past |z| = 100 every slope is its limit to the last bit of an f32, and the formulas' products of an overflowed
-// and a vanished factor are never formed; NaN fails the comparisons and stays NaN.
+// act'(z).  Past |z| = 100 every slope is its limit to the last bit of an f32, and is taken as that: the formulas' products of
+// an overflowed and a vanished factor (inf * 0) are formed there and dropped.  NaN fails the comparisons and stays NaN.
 __device__ __forceinline__ float act_slope(int act, float z) {
     if (act == ACT_NONE) return 1.f;
     if (act == ACT_RELU) return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
