@@ -205,11 +205,12 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
  * residual, and no gradients).  The weights stay frozen; bias, inputs and whatever precedes them train.
  *
  * Forward: z = linear(x) + bias, y = act(z) + residual, from the f32 sums with one rounding to y's dtype.  bias [out] in
- * bias_dtype or null; residual [rows][out] in y's dtype or null, not overlapping y; pre [rows][out] in y's dtype receives
- * z for the backward pass, or is null.  silu is z sigmoid(z), gelu z Phi(z), gelu_tanh its tanh approximation, each within
- * 2e-5 of its own value down to z = -12 (3e-6 down to -5), so small values keep their precision too.  Up to 16 rows
- * the sums are exl3_linear's bit for bit; past them, where exl3_linear's tiles would leave CUs idle, the contraction is
- * split over workgroups and its parts added in a fixed order.  x, bias, residual, y and pre 4-byte aligned.
+ * bias_dtype or null; residual [rows][out] in y's dtype or null; pre [rows][out] in y's dtype receives z for the backward
+ * pass, or is null.  y and pre share no memory with x, bias, residual or each other (refused).  silu is z sigmoid(z), gelu
+ * z Phi(z), gelu_tanh its tanh approximation, each within 2e-5 of its own value down to z = -12 (3e-6 down to -5), so small
+ * values keep their precision too.  Up to 16 rows the sums are exl3_linear's bit for bit; past them, where exl3_linear's
+ * tiles would leave CUs idle, the contraction is split over workgroups and its parts added in a fixed order.  x, bias,
+ * residual, y and pre 4-byte aligned.
  *
  * Backward: from dy [rows][out] (and pre, both in `dtype`; pre unread with EXL3_ACT_NONE; dy and svh 16-byte aligned,
  * pre 8-byte)
@@ -219,6 +220,9 @@ int32_t exl3_linear_grouped(const void *x, int32_t x_dtype, int32_t groups, int3
  * the row's largest |dz * svh| to 2^10 .. 2^11 (the prepared gradient is f16 as the prepared input is; gradients lie below
  * f16's normal range).  residual's gradient is dy itself, x's rounding to f16 is passed through.  Each rounding of pre to
  * 16 bits moves act' as that of any kept activation does.
+ *
+ * dbias shares no memory with dy, pre or dx (refused); dx may take the place of dy or pre row for row, and within one chunk
+ * of rows overlap them in any way.
  *
  * Rows go in chunks of at most 16384, each its own launches.  A workspace size holds for its rows; a caller of several row
  * counts takes the largest of theirs. */

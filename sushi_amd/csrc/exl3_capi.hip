@@ -379,6 +379,12 @@ void *at_row(void *p, size_t row, size_t width, int dt) {
     return p ? static_cast<char *>(p) + row * width * elem_size(dt) : nullptr;
 }
 
+// Whether two buffers of a and b bytes share memory (a null one shares none).
+bool overlap(const void *p, size_t a, const void *q, size_t b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+    return p && q && x < y + b && y < x + a;
+}
+
 int32_t act_check(int32_t act, const char *what) {
     if (act < 0 || act >= ACT_COUNT) return fail(EXL3_ERR_ACTIVATION, "%s: unknown activation %d", what, act);
     return ok();
@@ -1554,6 +1560,13 @@ int32_t exl3_linear_epilogue(const void *x, int32_t x_dtype, int32_t rows, int32
     if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
         return fail(EXL3_ERR_WORKSPACE, "linear_epilogue: workspace of %zu bytes (256-aligned) needed, got %zu", need,
                     workspace_bytes);
+    // workgroups read all of x, bias and residual while others write
+    const size_t x_bytes = (size_t)rows * in_features * elem_size(x_dtype), y_bytes = (size_t)rows * out_features * elem_size(y_dtype);
+    const size_t bias_bytes = (size_t)out_features * elem_size(bias_dtype);
+    for (const void *w : {(const void *)y, (const void *)pre})
+        if (overlap(w, y_bytes, x, x_bytes) || overlap(w, y_bytes, residual, y_bytes) || overlap(w, y_bytes, bias, bias_bytes))
+            return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue: y and pre must not overlap x, bias or residual");
+    if (overlap(y, y_bytes, pre, y_bytes)) return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue: y and pre must not overlap");
     const int chunk = epilogue_chunk(in_features);
     for (int r = 0; r < rows; r += chunk) {
         EpilogueArgs e{};
@@ -1603,6 +1616,17 @@ int32_t exl3_linear_epilogue_backward(const void *dy, int32_t dtype, int32_t row
         return fail(EXL3_ERR_WORKSPACE, "linear_epilogue_backward: workspace of %zu bytes (256-aligned) needed, got %zu",
                     need, workspace_bytes);
     const int chunk = epilogue_chunk(out_features);
+    const size_t dy_bytes = (size_t)rows * out_features * elem_size(dtype), dx_bytes = (size_t)rows * in_features * elem_size(dx_dtype);
+    const void *read[2] = {dy, act == ACT_NONE ? nullptr : pre};
+    for (const void *p : read) {
+        if (overlap(dbias, (size_t)out_features * sizeof(float), p, dy_bytes))
+            return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: dbias must not overlap dy or pre");
+        // a chunk's rows are read before its dx is written, the chunks after it are not
+        if (rows > chunk && !(dx == p && dx_bytes == dy_bytes) && overlap(dx, dx_bytes, p, dy_bytes))
+            return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: dx overlaps rows of dy or pre still to be read");
+    }
+    if (overlap(dbias, (size_t)out_features * sizeof(float), dx, dx_bytes))
+        return fail(EXL3_ERR_BAD_SHAPE, "linear_epilogue_backward: dbias must not overlap dx");
     GradArgs a{};
     a.dy = dy;
     a.pre = act == ACT_NONE ? nullptr : pre;
