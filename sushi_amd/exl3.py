@@ -1146,7 +1146,7 @@ class BalanceLoss(NamedTuple):
 
 def _router_operands(router_logits, inds, mask, what: str):
     lg = router_logits
-    if lg.dim() < 2 or inds.dim() != lg.dim() or inds.shape[:-1] != lg.shape[:-1] or \
+    if lg.dim() < 1 or inds.dim() != lg.dim() or inds.shape[:-1] != lg.shape[:-1] or \
             (mask is not None and mask.shape != lg.shape[:-1]):
         raise BadExl3Shape(f"{what}: logits {tuple(lg.shape)}, inds {tuple(inds.shape)}"
                            + ("" if mask is None else f", mask {tuple(mask.shape)}"))
