@@ -499,12 +499,15 @@ static int lanes_of(int experts) {
     return experts <= 64 ? 8 : experts <= 128 ? 16 : experts <= 256 ? 32 : 64;
 }
 
-// Workgroups of the balance loss: one while a single pass or two of it hold the rows (the join costs more), else one for
-// each set of rows it holds at once, at most two a CU.
+// Workgroups of the balance loss: one for up to eight sets of the rows it holds at once (the join costs more), else one for
+// each set, at most two a CU.  One workgroup against one for each set, us in a graph, top-8: 64 rows of 128 experts (two sets)
+// 3.9 and 7.8, 128 rows (four) 4.8 and 7.9, 256 (eight) 7.0 and 7.7; eight sets of 64, 256 and 512 experts 7.0 and 7.8, 7.5 and
+// 8.4, 7.5 and 8.7; from there on a set costs half a microsecond.
+constexpr long kBalanceAlone = 8;
 int balance_parts(int rows, int experts) {
     const int at_once = BL_THREADS / lanes_of(experts);
     const long sets = ((long)rows + at_once - 1) / at_once;
-    return (int)(sets <= 2 ? 1 : sets < kBalanceMaxParts ? sets : kBalanceMaxParts);
+    return (int)(sets <= kBalanceAlone ? 1 : sets < kBalanceMaxParts ? sets : kBalanceMaxParts);
 }
 
 template <int PER, int DT>

@@ -65,7 +65,13 @@ def test_router_gradient_past_one_pass(dev, case, parts):
     assert torch.equal(got, exl3.moe_router_backward(logits, inds, dscores=ds, weight=w, dloss=dl, mask=mask))
 
 
-@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(v).replace("torch.", "") for v in c))
+# the loss's last rows of one workgroup and the first of several: eight sets of 512 / L rows and nine
+SETS = [(512, 64, 4, BF16, True, True), (513, 64, 4, BF16, True, True), (256, 128, 6, F32, False, True),
+        (257, 100, 6, F16, True, False), (128, 256, 8, F32, True, True), (129, 256, 8, F32, True, True),
+        (64, 512, 8, BF16, False, False), (65, 1000, 8, F32, True, True)]
+
+
+@pytest.mark.parametrize("case", CASES + SETS, ids=lambda c: "-".join(str(v).replace("torch.", "") for v in c))
 def test_balance_loss_past_one_pass(dev, case):
     rows = case[0]
     print(f"[balance] {case}", flush=True)
