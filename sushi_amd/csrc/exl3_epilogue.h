@@ -158,22 +158,9 @@ __device__ __forceinline__ uint32_t pack2(bool bf16, float x, float y) {
                 : __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{x, y}), h2_t));
 }
 
-// Eight f32 values rounded to f16 or bf16, two at a time (gfx950 converts to both to nearest even).
+// Eight of them.
 __device__ __forceinline__ uint4 pack8(bool bf16, const float (&v)[8]) {
-    typedef float f2_t __attribute__((ext_vector_type(2)));
-    typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
-    typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-    uint32_t w[4];
-    if (bf16) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{v[2 * i], v[2 * i + 1]}), bf2_t));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{v[2 * i], v[2 * i + 1]}), h2_t));
-    }
-    return uint4{w[0], w[1], w[2], w[3]};
+    return uint4{pack2(bf16, v[0], v[1]), pack2(bf16, v[2], v[3]), pack2(bf16, v[4], v[5]), pack2(bf16, v[6], v[7])};
 }
 
 }  // namespace exl3
