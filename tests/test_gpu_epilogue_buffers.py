@@ -1,4 +1,5 @@
-"""dx in the place of dy: the C entry reads a chunk's dy whole before it writes the chunk's dx."""
+"""The gradient with dx in the place of dy (the C entry reads a chunk's dy whole before it writes the chunk's dx), and with
+pre at the least alignment that is documented."""
 import pytest
 import torch
 
@@ -25,3 +26,18 @@ def test_dx_in_place_of_dy(dev, rows, width, act):
     assert rc == 0, L.last_error()
     torch.cuda.synchronize()
     assert torch.equal(dy, want) and torch.equal(got, db)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_pre_at_eight_bytes(dev, dtype):
+    """pre needs no more than 8-byte alignment, also where a row is read 16 bytes at a time."""
+    p = _proj(83, 256, 640, 32, dev)
+    dy, pre = (_normal(84, n, (70, 640), dtype, dev) for n in ("dy", "pre"))
+    skip = 8 // pre.element_size()
+    odd = torch.empty(70 * 640 + skip, dtype=dtype, device=dev)[skip:].view(70, 640)
+    odd.copy_(pre)
+    assert odd.data_ptr() % 16 == 8
+    for act in ("relu", "silu", "gelu", "gelu_tanh"):
+        a = exl3.linear_epilogue_backward(dy, p, exl3.MCG, act=act, pre=pre, with_dbias=True)
+        b = exl3.linear_epilogue_backward(dy, p, exl3.MCG, act=act, pre=odd, with_dbias=True)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
