@@ -418,6 +418,72 @@ int32_t exl3_router_backward(const void *logits, int32_t dtype, int32_t rows, in
                              int32_t topk, const float *dscores, const float *weight, const float *dloss,
                              const uint8_t *mask, void *dlogits, hipStream_t stream);
 
+/* The choice of experts, beside exl3_route_topk: an extension (the reference's router is that chain).  With x a row of
+ * logits [rows][experts] (f16, bf16 or f32) and p = softmax(x) or sigmoid(x) by `score`:
+ *   c = p + bias (bias [experts] f32 or null; it moves the choice alone),
+ *   of `groups` groups of experts / groups neighbours the topk_groups with the largest value, the sum of a group's group_top
+ *   (1 or 2) largest c; of their experts the topk with the largest c,
+ *   score_i = scale p_i / (renormalize ? sum over the picks of p : 1).
+ * Picks are listed in falling c, equal ones (and equal groups) by their number; the order is that of the values in 64 bits
+ * (without bias, and with one group or group_top 1, of the logits themselves), whatever the f32 roundings of another batch.
+ * An expert is out of the choice by a logit of -inf or NaN (under softmax +inf too) or a bias of -inf or NaN; a row with a
+ * NaN logit (under softmax +inf too) has NaN scores.  A slot that no expert is left for, and every slot of a row that mask
+ * [rows] (bytes, or null) leaves out, holds id 0xFFFFFFFF and score 0, whatever the row's logits: a dropped slot for
+ * exl3_balance_loss and the gradients (exl3_moe clamps it to the last expert, times 0).  inds [rows][topk], scores f32
+ * [rows][topk]; they overlap no input and not each other (refused).  experts <= 1024, topk <= 32, groups <= 64 and a divisor of
+ * experts, topk_groups groups hold at least topk experts.
+ *
+ * exl3_route_backward: dlogits (like logits; it overlaps no input) from dscores f32 [rows][topk], the choice held fixed.  With
+ * r the scores over scale and ds = scale dscores, the row's slots i on expert e add up (a dropped slot has none):
+ *   softmax, renormalised  r_i (ds_i - sum_j r_j ds_j);     sigmoid, renormalised  the same times 1 - p_i;
+ *   softmax                p_i ds_i, and each expert - p_e sum_j p_j ds_j;     sigmoid  p_i (1 - p_i) ds_i.
+ * Padded rows get zeros.  The balance loss's gradient is exl3_router_backward's and adds to it.  Equal calls give equal bits. */
+typedef enum { EXL3_SCORE_SOFTMAX = 0, EXL3_SCORE_SIGMOID = 1 } exl3_score;
+int32_t exl3_route(const void *logits, int32_t dtype, int32_t rows, int32_t experts, int32_t topk, const float *bias,
+                   int32_t score, int32_t groups, int32_t topk_groups, int32_t group_top, int32_t renormalize, float scale,
+                   const uint8_t *mask, uint32_t *inds, float *scores, hipStream_t stream);
+int32_t exl3_route_backward(const void *logits, int32_t dtype, int32_t rows, int32_t experts, const uint32_t *inds,
+                            int32_t topk, const float *dscores, int32_t score, int32_t renormalize, float scale,
+                            const uint8_t *mask, void *dlogits, hipStream_t stream);
+
+/* The norms after a block and before the next one, with the block's gate and the residual stream between: an extension (the
+ * reference's trunk norms through MLX).  With rms(v) = v / sqrt(mean v^2 + eps) over the row:
+ *   n = post ? rms(y) (weight_offset + post) : y,
+ *   h_out = residual_scale h + block_scale gate n,      x_out = rms(h_out) (weight_offset + pre).
+ * y and x_out [rows][width] in dtype, h (or null: 0) and h_out in h_dtype, which is dtype or f32; post and pre [width] in
+ * f16, bf16 or f32 each, or null (without pre there is no x_out); gate by gate_kind: none, [width] or [rows] in gate_dtype, or
+ * [rows][width] in dtype.  x_out comes of the h_out that is not rounded yet; each output is rounded once.  h_out may be h and
+ * x_out may be y; other overlaps of an output are refused.  eps > 0, width <= 16384.
+ *
+ * Backward, from dh (like h_out, or null: 0), dx (like x_out, with pre), y and h (h_out as the forward wrote it, with pre):
+ * dy (like y), dresidual (like h, or null: not wanted), dpost and dpre f32 [width] (with post, pre), dgate as gate was broadcast:
+ * f32 [width] or [rows], or [rows][width] in dtype (null without a gate).  dy may be y or dx, dresidual may be dh or h;
+ * other overlaps are refused.  Equal calls give equal bits. */
+typedef enum { EXL3_GATE_NONE = 0, EXL3_GATE_CHANNEL = 1, EXL3_GATE_ROW = 2, EXL3_GATE_FULL = 3 } exl3_gate;
+int32_t exl3_block_norm(const void *y, int32_t dtype, const void *h, int32_t h_dtype, int32_t rows, int32_t width,
+                        const void *post, int32_t post_dtype, const void *gate, int32_t gate_dtype, int32_t gate_kind,
+                        const void *pre, int32_t pre_dtype, float eps, float weight_offset, float residual_scale,
+                        float block_scale, void *h_out, void *x_out, hipStream_t stream);
+size_t exl3_block_norm_backward_workspace_size(int32_t rows, int32_t width);
+int32_t exl3_block_norm_backward(const void *dh, const void *dx, const void *y, int32_t dtype, const void *h, int32_t h_dtype,
+                                 int32_t rows, int32_t width, const void *post, int32_t post_dtype, const void *gate,
+                                 int32_t gate_dtype, int32_t gate_kind, const void *pre, int32_t pre_dtype, float eps,
+                                 float weight_offset, float residual_scale, float block_scale, void *dy, void *dresidual,
+                                 float *dpost, float *dpre, void *dgate, void *workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
+
+/* The clip of many gradients by their global norm: an extension.  norm = sqrt(sum over `count` tensors of g^2), scale =
+ * norm <= max_norm ? 1 : max_norm / norm, out = g scale; result f32 [2] on the device receives norm and scale.  grads, numel,
+ * dtypes, out and out_dtypes are host arrays, read before the call returns (a captured graph keeps the addresses that they held).  A
+ * tensor of numel values lies contiguous in f16, bf16 or f32; out null: in place, with nothing written where scale is 1;
+ * else each out[i] holds numel[i] values of its type and overlaps no other tensor (it may be grads[i] in the same type).
+ * Squares add in 64 bits.  A norm of inf makes scale 0 (and inf * 0 NaN), of NaN NaN.  max_norm >= 0, inf for the norm alone.
+ * Equal calls give equal bits. */
+size_t exl3_clip_grad_norm_workspace_size(int32_t count);
+int32_t exl3_clip_grad_norm(int32_t count, const void *const *grads, const int64_t *numel, const int32_t *dtypes,
+                            void *const *out, const int32_t *out_dtypes, float max_norm, float *result, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+
 /* `layout.tileMajor` / `tileMajorInverse` (src/exl3/layout.zig:139-158): one projection of `experts` experts
  * between the pack order [IT][OT][n] and the pair-major order [OT/2][IT][2][n]. */
 int32_t exl3_tile_major(const uint16_t *src, uint16_t *dst, int32_t experts, int32_t it, int32_t ot, int32_t n,

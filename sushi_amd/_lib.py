@@ -44,6 +44,13 @@ EXPORTS = (
     "exl3_balance_loss_workspace_size",
     "exl3_balance_loss",
     "exl3_router_backward",
+    "exl3_route",
+    "exl3_route_backward",
+    "exl3_block_norm",
+    "exl3_block_norm_backward_workspace_size",
+    "exl3_block_norm_backward",
+    "exl3_clip_grad_norm_workspace_size",
+    "exl3_clip_grad_norm",
     "exl3_tile_major",
     "exl3_encode_workspace_size",
     "exl3_encode_tiles",
@@ -143,6 +150,17 @@ def load() -> ctypes.CDLL:
     L.exl3_balance_loss_workspace_size.argtypes = [i32, i32]
     L.exl3_balance_loss.argtypes = [vp, i32, i32, i32, vp, i32, vp, ctypes.c_float, vp, vp, vp, vp, sz, vp]
     L.exl3_router_backward.argtypes = [vp, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp]
+    f32 = ctypes.c_float
+    L.exl3_route.argtypes = [vp, i32, i32, i32, i32, vp, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp]
+    L.exl3_route_backward.argtypes = [vp, i32, i32, i32, vp, i32, vp, i32, i32, f32, vp, vp, vp]
+    L.exl3_block_norm.argtypes = [vp, i32, vp, i32, i32, i32, vp, i32, vp, i32, i32, vp, i32, f32, f32, f32, f32, vp, vp, vp]
+    L.exl3_block_norm_backward_workspace_size.restype = sz
+    L.exl3_block_norm_backward_workspace_size.argtypes = [i32, i32]
+    L.exl3_block_norm_backward.argtypes = [vp, vp, vp, i32, vp, i32, i32, i32, vp, i32, vp, i32, i32, vp, i32, f32, f32, f32,
+                                           f32, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.exl3_clip_grad_norm_workspace_size.restype = sz
+    L.exl3_clip_grad_norm_workspace_size.argtypes = [i32]
+    L.exl3_clip_grad_norm.argtypes = [i32, vp, vp, vp, vp, vp, f32, vp, vp, sz, vp]
     L.exl3_tile_major.argtypes = [vp, vp, i32, i32, i32, i32, i32, vp]
     L.exl3_encode_workspace_size.restype = sz
     L.exl3_encode_workspace_size.argtypes = [i32, DecodeT, ctypes.c_int64]

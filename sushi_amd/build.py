@@ -27,6 +27,9 @@ SOURCES = [
     "exl3_moe_gemm.hip",
     "exl3_gradient.hip",
     "exl3_router.hip",
+    "exl3_route.hip",
+    "exl3_norm.hip",
+    "exl3_clip.hip",
     "exl3_gemv_mcg.hip",
     "exl3_gemv_mul1.hip",
     "exl3_gemv_hash.hip",

@@ -8,10 +8,14 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
+#include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
+#include <new>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "sushi_exl3_hip.h"
 #include "exl3_kernels.h"
@@ -1731,6 +1735,327 @@ int32_t exl3_router_backward(const void *logits, int32_t dtype, int32_t rows, in
     a.mask = mask;
     a.dlogits = dlogits;
     return launched(run_router_backward(a, stream), "exl3_router_backward");
+}
+
+// Whether a written buffer shares memory with a read one that it does not replace in whole, or with another written one.
+namespace {
+struct Span {
+    const void *p;
+    size_t bytes;
+};
+bool spans_clash(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (auto w = written.begin(); w != written.end(); ++w) {
+        for (const Span &r : read)
+            if (overlap(w->p, w->bytes, r.p, r.bytes)) return true;
+        for (auto v = written.begin(); v != w; ++v)
+            if (overlap(w->p, w->bytes, v->p, v->bytes)) return true;
+    }
+    return false;
+}
+}  // namespace
+
+int32_t exl3_route(const void *logits, int32_t dtype, int32_t rows, int32_t experts, int32_t topk, const float *bias,
+                   int32_t score, int32_t groups, int32_t topk_groups, int32_t group_top, int32_t renormalize, float scale,
+                   const uint8_t *mask, uint32_t *inds, float *scores, hipStream_t stream) {
+    int32_t rc = router_checks(logits, dtype, rows, experts, topk, "route");
+    if (rc) return rc;
+    if (score != EXL3_SCORE_SOFTMAX && score != EXL3_SCORE_SIGMOID) return fail(EXL3_ERR_ACTIVATION, "route: unknown score %d", score);
+    if (groups <= 0 || groups > kRouteMaxGroups || experts % groups || topk_groups <= 0 || topk_groups > groups || group_top < 1 ||
+        group_top > 2 || group_top > experts / groups || topk > topk_groups * (experts / groups))
+        return fail(EXL3_ERR_BAD_SHAPE, "route: %d of %d groups of %d experts by their %d largest for k=%d (groups <= %d)", topk_groups,
+                    groups, experts, group_top, topk, kRouteMaxGroups);
+    if (rows == 0) return ok();
+    if (!inds || !scores) return fail(EXL3_ERR_BAD_SHAPE, "route: null operand");
+    for (const void *p : {(const void *)bias, (const void *)inds, (const void *)scores})
+        if (reinterpret_cast<uintptr_t>(p) % 4) return fail(EXL3_ERR_BAD_SHAPE, "route: bias, inds and scores must be 4-byte aligned");
+    const size_t slots = (size_t)rows * topk * 4;
+    if (spans_clash({{inds, slots}, {scores, slots}}, {{logits, (size_t)rows * experts * elem_size(dtype)},
+                                                       {bias, (size_t)experts * 4}, {mask, (size_t)rows}}))
+        return fail(EXL3_ERR_BAD_SHAPE, "route: inds and scores must not overlap the inputs or each other");
+    RouteArgs a{};
+    a.logits = logits;
+    a.dtype = dtype;
+    a.rows = rows;
+    a.experts = experts;
+    a.topk = topk;
+    a.bias = bias;
+    a.sigmoid = score == EXL3_SCORE_SIGMOID;
+    a.groups = groups;
+    a.taken = topk_groups;
+    a.group_top = group_top;
+    a.renorm = renormalize != 0;
+    a.scale = scale;
+    a.mask = mask;
+    a.inds = inds;
+    a.scores = scores;
+    return launched(run_route(a, stream), "exl3_route");
+}
+
+int32_t exl3_route_backward(const void *logits, int32_t dtype, int32_t rows, int32_t experts, const uint32_t *inds,
+                            int32_t topk, const float *dscores, int32_t score, int32_t renormalize, float scale,
+                            const uint8_t *mask, void *dlogits, hipStream_t stream) {
+    int32_t rc = router_checks(logits, dtype, rows, experts, topk, "route_backward");
+    if (rc) return rc;
+    if (score != EXL3_SCORE_SOFTMAX && score != EXL3_SCORE_SIGMOID)
+        return fail(EXL3_ERR_ACTIVATION, "route_backward: unknown score %d", score);
+    if (rows == 0) return ok();
+    if (!inds || !dscores || !dlogits) return fail(EXL3_ERR_BAD_SHAPE, "route_backward: null operand");
+    if (reinterpret_cast<uintptr_t>(inds) % 4 || reinterpret_cast<uintptr_t>(dscores) % 4 ||
+        reinterpret_cast<uintptr_t>(dlogits) % elem_size(dtype))
+        return fail(EXL3_ERR_BAD_SHAPE, "route_backward: unaligned operand");
+    const size_t slots = (size_t)rows * topk * 4, row_bytes = (size_t)rows * experts * elem_size(dtype);
+    if (spans_clash({{dlogits, row_bytes}}, {{logits, row_bytes}, {inds, slots}, {dscores, slots}, {mask, (size_t)rows}}))
+        return fail(EXL3_ERR_BAD_SHAPE, "route_backward: dlogits must not overlap the inputs");
+    RouteGradArgs a{};
+    a.logits = logits;
+    a.dtype = dtype;
+    a.rows = rows;
+    a.experts = experts;
+    a.topk = topk;
+    a.inds = inds;
+    a.dscores = dscores;
+    a.sigmoid = score == EXL3_SCORE_SIGMOID;
+    a.renorm = renormalize != 0;
+    a.scale = scale;
+    a.mask = mask;
+    a.dlogits = dlogits;
+    return launched(run_route_backward(a, stream), "exl3_route_backward");
+}
+
+namespace {
+
+// What both directions of the block's norms check; the bytes of a gate in *gate_bytes.
+int32_t block_norm_checks(const char *what, int32_t dtype, int32_t h_dtype, int32_t rows, int32_t width, const void *post,
+                          int32_t post_dtype, const void *gate, int32_t gate_dtype, int32_t gate_kind, const void *pre,
+                          int32_t pre_dtype, float eps, size_t *gate_bytes) {
+    if (rows < 0 || width <= 0 || width > kNormMaxWidth)
+        return fail(EXL3_ERR_BAD_SHAPE, "%s: rows=%d width=%d (width <= %d)", what, rows, width, kNormMaxWidth);
+    if (!dtype_ok(dtype) || (h_dtype != dtype && h_dtype != EXL3_DT_F32))
+        return fail(EXL3_ERR_BAD_DTYPE, "%s: y's type must be f16, bf16 or f32 and the residual's that or f32", what);
+    if ((post && !dtype_ok(post_dtype)) || (pre && !dtype_ok(pre_dtype)) || (gate_kind != GATE_NONE && !dtype_ok(gate_dtype)))
+        return fail(EXL3_ERR_BAD_DTYPE, "%s: unsupported weight or gate dtype", what);
+    // (a gate of no rows may have no address)
+    if (gate_kind < GATE_NONE || gate_kind > GATE_FULL || (rows > 0 && (gate_kind != GATE_NONE) != (gate != nullptr)))
+        return fail(EXL3_ERR_BAD_SHAPE, "%s: gate kind %d and its operand do not agree", what, gate_kind);
+    if (gate_kind == GATE_FULL && gate_dtype != dtype) return fail(EXL3_ERR_BAD_DTYPE, "%s: a full gate is in y's type", what);
+    if (!(eps > 0.f)) return fail(EXL3_ERR_BAD_SHAPE, "%s: eps must be positive", what);
+    *gate_bytes = gate_kind == GATE_NONE ? 0
+                                         : (gate_kind == GATE_CHANNEL ? 1 : (size_t)rows) * (gate_kind == GATE_ROW ? 1 : (size_t)width) *
+                                               elem_size(gate_dtype);
+    return ok();
+}
+
+bool unaligned(const void *p, int dt) { return reinterpret_cast<uintptr_t>(p) % elem_size(dt) != 0; }
+
+}  // namespace
+
+int32_t exl3_block_norm(const void *y, int32_t dtype, const void *h, int32_t h_dtype, int32_t rows, int32_t width,
+                        const void *post, int32_t post_dtype, const void *gate, int32_t gate_dtype, int32_t gate_kind,
+                        const void *pre, int32_t pre_dtype, float eps, float weight_offset, float residual_scale,
+                        float block_scale, void *h_out, void *x_out, hipStream_t stream) {
+    size_t gate_bytes;
+    int32_t rc = block_norm_checks("block_norm", dtype, h_dtype, rows, width, post, post_dtype, gate, gate_dtype, gate_kind, pre,
+                                   pre_dtype, eps, &gate_bytes);
+    if (rc) return rc;
+    if (rows == 0) return ok();
+    if (!y || !h_out || (pre != nullptr) != (x_out != nullptr))
+        return fail(EXL3_ERR_BAD_SHAPE, "block_norm: null operand (x_out goes with pre)");
+    if (unaligned(y, dtype) || unaligned(x_out, dtype) || unaligned(h, h_dtype) || unaligned(h_out, h_dtype) ||
+        unaligned(post, post_dtype) || unaligned(pre, pre_dtype) || unaligned(gate, gate_dtype))
+        return fail(EXL3_ERR_BAD_SHAPE, "block_norm: unaligned operand");
+    const size_t yb = (size_t)rows * width * elem_size(dtype), hb = (size_t)rows * width * elem_size(h_dtype);
+    // (a row's values are all read before the first is written)
+    const Span ys{y, x_out == y ? 0 : yb}, hs{h, h_out == h ? 0 : hb};
+    const Span post_s{post, (size_t)width * elem_size(post_dtype)}, pre_s{pre, (size_t)width * elem_size(pre_dtype)}, gate_s{gate, gate_bytes};
+    if (spans_clash({{h_out, hb}}, {{y, yb}, hs, post_s, pre_s, gate_s}) || spans_clash({{x_out, yb}}, {ys, {h, hb}, post_s, pre_s, gate_s}) ||
+        overlap(x_out, yb, h_out, hb))
+        return fail(EXL3_ERR_BAD_SHAPE, "block_norm: h_out may be h and x_out may be y, other overlaps may not be");
+    NormArgs a{};
+    a.y = y;
+    a.dtype = dtype;
+    a.hdtype = h_dtype;
+    a.rows = rows;
+    a.width = width;
+    a.h = h;
+    a.post = post;
+    a.pre = pre;
+    a.gate = gate;
+    a.post_dtype = post_dtype;
+    a.pre_dtype = pre_dtype;
+    a.gate_dtype = gate_dtype;
+    a.gate_kind = gate_kind;
+    a.eps = eps;
+    a.offset = weight_offset;
+    a.residual_scale = residual_scale;
+    a.block_scale = block_scale;
+    a.h_out = h_out;
+    a.x_out = x_out;
+    return launched(run_norm(a, stream), "exl3_block_norm");
+}
+
+size_t exl3_block_norm_backward_workspace_size(int32_t rows, int32_t width) {
+    if (rows < 0 || width <= 0 || width > kNormMaxWidth) return 0;
+    return kZeroBytes + align_up((size_t)norm_backward_parts(rows, width) * 3 * width * sizeof(float));
+}
+
+int32_t exl3_block_norm_backward(const void *dh, const void *dx, const void *y, int32_t dtype, const void *h, int32_t h_dtype,
+                                 int32_t rows, int32_t width, const void *post, int32_t post_dtype, const void *gate,
+                                 int32_t gate_dtype, int32_t gate_kind, const void *pre, int32_t pre_dtype, float eps,
+                                 float weight_offset, float residual_scale, float block_scale, void *dy, void *dresidual,
+                                 float *dpost, float *dpre, void *dgate, void *workspace, size_t workspace_bytes,
+                                 hipStream_t stream) {
+    size_t gate_bytes;
+    int32_t rc = block_norm_checks("block_norm_backward", dtype, h_dtype, rows, width, post, post_dtype, gate, gate_dtype, gate_kind,
+                                   pre, pre_dtype, eps, &gate_bytes);
+    if (rc) return rc;
+    if ((post != nullptr) != (dpost != nullptr) || (pre != nullptr) != (dpre != nullptr) ||
+        (gate_kind == GATE_CHANNEL && !dgate) || (rows && (gate_kind != GATE_NONE) != (dgate != nullptr)))
+        return fail(EXL3_ERR_BAD_SHAPE, "block_norm_backward: dpost, dpre and dgate go with post, pre and gate");
+    if (rows == 0) {
+        for (void *p : {(void *)dpost, (void *)dpre, gate_kind == GATE_CHANNEL ? dgate : nullptr}) {
+            if (!p) continue;
+            rc = launched(run_fill_zero(p, (size_t)width * sizeof(float), stream), "exl3_block_norm_backward");
+            if (rc) return rc;
+        }
+        return ok();
+    }
+    if (!y || !dy || (pre != nullptr) != (dx != nullptr) || (pre && !h) || (!pre && !dh))
+        return fail(EXL3_ERR_BAD_SHAPE, "block_norm_backward: null operand (dx and h go with pre; without it there is dh)");
+    const int dgate_dtype = gate_kind == GATE_FULL ? dtype : EXL3_DT_F32;
+    if (unaligned(y, dtype) || unaligned(dx, dtype) || unaligned(dy, dtype) || unaligned(h, h_dtype) || unaligned(dh, h_dtype) ||
+        unaligned(dresidual, h_dtype) || unaligned(post, post_dtype) || unaligned(pre, pre_dtype) || unaligned(gate, gate_dtype) ||
+        unaligned(dpost, EXL3_DT_F32) || unaligned(dpre, EXL3_DT_F32) || unaligned(dgate, dgate_dtype))
+        return fail(EXL3_ERR_BAD_SHAPE, "block_norm_backward: unaligned operand");
+    const size_t need = exl3_block_norm_backward_workspace_size(rows, width);
+    if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
+        return fail(EXL3_ERR_WORKSPACE, "block_norm_backward: workspace of %zu bytes (256-aligned) needed, got %zu", need, workspace_bytes);
+    const size_t yb = (size_t)rows * width * elem_size(dtype), hb = (size_t)rows * width * elem_size(h_dtype);
+    const size_t wb = (size_t)width * sizeof(float);
+    const size_t dgb = gate_kind == GATE_CHANNEL ? wb : gate_kind == GATE_ROW ? (size_t)rows * sizeof(float) : gate_kind == GATE_FULL ? yb : 0;
+    if (!pre) dx = h = nullptr;  // not read
+    const Span post_s{post, (size_t)width * elem_size(post_dtype)}, pre_s{pre, (size_t)width * elem_size(pre_dtype)}, gate_s{gate, gate_bytes};
+    const Span y_s{y, yb}, dx_s{dx, yb}, h_s{h, hb}, dh_s{dh, hb};
+    auto but = [](const Span &s, const void *p) { return Span{s.p, s.p == p ? 0 : s.bytes}; };
+    if (spans_clash({{dpost, wb}, {dpre, wb}, {dgate, dgb}}, {y_s, dx_s, h_s, dh_s, post_s, pre_s, gate_s, {dy, yb}, {dresidual, hb}}) ||
+        spans_clash({{dy, yb}}, {but(y_s, dy), but(dx_s, dy), h_s, dh_s, post_s, pre_s, gate_s, {dresidual, hb}}) ||
+        spans_clash({{dresidual, hb}}, {but(h_s, dresidual), but(dh_s, dresidual), y_s, dx_s, post_s, pre_s, gate_s}))
+        return fail(EXL3_ERR_BAD_SHAPE, "block_norm_backward: dy may be y or dx, dresidual dh or h, other overlaps may not be");
+    NormGradArgs a{};
+    a.dh = dh;
+    a.dx = dx;
+    a.y = y;
+    a.h = h;
+    a.dtype = dtype;
+    a.hdtype = h_dtype;
+    a.rows = rows;
+    a.width = width;
+    a.post = post;
+    a.pre = pre;
+    a.gate = gate;
+    a.post_dtype = post_dtype;
+    a.pre_dtype = pre_dtype;
+    a.gate_dtype = gate_dtype;
+    a.gate_kind = gate_kind;
+    a.eps = eps;
+    a.offset = weight_offset;
+    a.residual_scale = residual_scale;
+    a.block_scale = block_scale;
+    a.dy = dy;
+    a.dres = dresidual;
+    a.dpost = dpost;
+    a.dpre = dpre;
+    a.dgate = dgate;
+    a.parts = norm_backward_parts(rows, width);
+    a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kZeroBytes);
+    return launched(run_norm_backward(a, stream), "exl3_block_norm_backward");
+}
+
+size_t exl3_clip_grad_norm_workspace_size(int32_t count) {
+    if (count <= 0) return 0;
+    const size_t launches = ((size_t)count + kClipTensors - 1) / kClipTensors;
+    return kZeroBytes + kAlign + align_up(launches * kClipParts * sizeof(double));
+}
+
+int32_t exl3_clip_grad_norm(int32_t count, const void *const *grads, const int64_t *numel, const int32_t *dtypes,
+                            void *const *out, const int32_t *out_dtypes, float max_norm, float *result, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream) try {
+    if (count <= 0 || !grads || !numel || !dtypes || (out != nullptr) != (out_dtypes != nullptr) || !result ||
+        reinterpret_cast<uintptr_t>(result) % 4)
+        return fail(EXL3_ERR_BAD_SHAPE, "clip_grad_norm: no tensors, or a null operand");
+    if (!(max_norm >= 0.f)) return fail(EXL3_ERR_BAD_SHAPE, "clip_grad_norm: max_norm must not be negative or NaN");
+    struct Range {
+        uintptr_t begin, end;
+        bool written;
+    };
+    std::vector<Range> ranges;
+    ranges.reserve(2 * (size_t)count + 1);
+    const bool scales = out || max_norm < INFINITY;
+    for (int i = 0; i < count; i++) {
+        if (numel[i] < 0 || numel[i] > kClipMaxElements) return fail(EXL3_ERR_BAD_SHAPE, "clip_grad_norm: tensor %d of %lld values", i, (long long)numel[i]);
+        if (!dtype_ok(dtypes[i]) || (out && !dtype_ok(out_dtypes[i]))) return fail(EXL3_ERR_BAD_DTYPE, "clip_grad_norm: unsupported dtype of tensor %d", i);
+        if (numel[i] == 0) continue;
+        const uintptr_t g = reinterpret_cast<uintptr_t>(grads[i]), o = out ? reinterpret_cast<uintptr_t>(out[i]) : g;
+        const int odt = out ? out_dtypes[i] : dtypes[i];
+        if (!g || !o || g % elem_size(dtypes[i]) || o % elem_size(odt))
+            return fail(EXL3_ERR_BAD_SHAPE, "clip_grad_norm: null or unaligned tensor %d", i);
+        if (o == g && odt != dtypes[i]) return fail(EXL3_ERR_BAD_DTYPE, "clip_grad_norm: tensor %d in place in another type", i);
+        if (o != g || !scales) ranges.push_back({g, g + (size_t)numel[i] * elem_size(dtypes[i]), false});
+        if (scales) ranges.push_back({o, o + (size_t)numel[i] * elem_size(odt), true});
+    }
+    const uintptr_t res = reinterpret_cast<uintptr_t>(result);
+    ranges.push_back({res, res + 2 * sizeof(float), true});
+    std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.begin < b.begin; });
+    uintptr_t read_end = 0, write_end = 0;
+    for (const Range &r : ranges) {
+        if (r.begin < write_end || (r.written && r.begin < read_end))
+            return fail(EXL3_ERR_BAD_SHAPE, "clip_grad_norm: a written tensor overlaps another tensor");
+        (r.written ? write_end : read_end) = std::max(r.written ? write_end : read_end, r.end);
+    }
+    const size_t need = exl3_clip_grad_norm_workspace_size(count);
+    if (workspace_bytes < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % kAlign)
+        return fail(EXL3_ERR_WORKSPACE, "clip_grad_norm: workspace of %zu bytes (256-aligned) needed, got %zu", need, workspace_bytes);
+    // the tensors of one launch from `next` on, those without values left out
+    auto fill = [&](int &next, ClipTensors &t) {
+        t.count = t.chunks = 0;
+        for (; next < count && t.count < kClipTensors; next++) {
+            if (!numel[next]) continue;
+            const int k = t.count++;
+            t.g[k] = grads[next];
+            t.out[k] = out ? out[next] : const_cast<void *>(grads[next]);
+            t.n[k] = numel[next];
+            t.first[k] = t.chunks;
+            t.dtype[k] = (uint8_t)dtypes[next];
+            t.out_dtype[k] = (uint8_t)(out ? out_dtypes[next] : dtypes[next]);
+            t.chunks += (int32_t)((numel[next] + kClipChunk - 1) / kClipChunk);
+        }
+    };
+    ClipTensors t{};
+    ClipArgs a{};
+    a.factors = reinterpret_cast<float *>(static_cast<char *>(workspace) + kZeroBytes);
+    a.parts = reinterpret_cast<double *>(static_cast<char *>(workspace) + kZeroBytes + kAlign);
+    a.counter = static_cast<uint32_t *>(workspace);
+    a.max_norm = max_norm;
+    a.result = result;
+    int next = 0;
+    do {
+        fill(next, t);
+        const int parts = t.chunks ? clip_parts(t.chunks) : 1;
+        a.first_part = a.all_parts;
+        a.all_parts += parts;
+        const hipError_t e = run_clip_norm(t, a, next == count, stream);
+        if (e != hipSuccess) return launched(e, "exl3_clip_grad_norm");
+    } while (next < count);
+    if (!scales) return ok();
+    next = 0;
+    do {
+        fill(next, t);
+        if (!t.chunks) continue;
+        const hipError_t e = run_clip_scale(t, a.factors, stream);
+        if (e != hipSuccess) return launched(e, "exl3_clip_grad_norm (scale)");
+    } while (next < count);
+    return ok();
+} catch (const std::bad_alloc &) {
+    return fail(EXL3_ERR_LAUNCH, "clip_grad_norm: out of host memory");
 }
 
 int32_t exl3_tile_major(const uint16_t *src, uint16_t *dst, int32_t experts, int32_t it, int32_t ot, int32_t n,

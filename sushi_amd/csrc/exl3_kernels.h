@@ -415,6 +415,92 @@ inline int balance_joins(int parts) { return (parts + kBalanceJoin - 1) / kBalan
 hipError_t run_balance_loss(const BalanceArgs &a, hipStream_t s);
 hipError_t run_router_backward(const RouterGradArgs &a, hipStream_t s);
 
+// The choice of experts (exl3_route.hip): logits [rows][experts] in dtype, bias [experts] or null, mask as above.
+constexpr int kRouteMaxGroups = 64;
+struct RouteArgs {
+    const void *logits;
+    int dtype, rows, experts, topk;
+    const float *bias;
+    int sigmoid;                  // p: sigmoid (1) or softmax (0)
+    int groups, taken, group_top;
+    int renorm;
+    float scale;
+    const uint8_t *mask;
+    uint32_t *inds;               // [rows][topk]
+    float *scores;
+};
+struct RouteGradArgs {
+    const void *logits;
+    int dtype, rows, experts, topk;
+    const uint32_t *inds;
+    const float *dscores;  // [rows][topk]
+    int sigmoid, renorm;
+    float scale;
+    const uint8_t *mask;
+    void *dlogits;         // like logits
+};
+hipError_t run_route(const RouteArgs &a, hipStream_t s);
+hipError_t run_route_backward(const RouteGradArgs &a, hipStream_t s);
+
+// The norms before and after a block (exl3_norm.hip), rms(v) = v / sqrt(mean v^2 + eps):
+//   n = post ? rms(y) (offset + post) : y,   h' = residual_scale h + block_scale gate n,   x' = rms(h') (offset + pre).
+// y, x' and a full gate [rows][width] in dtype; h, h' in hdtype; the weights and a gate [width] or [rows] in wdtype each.
+enum Gate : int { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_ROW = 2, GATE_FULL = 3 };
+constexpr int kNormMaxWidth = 16384;
+struct NormArgs {
+    const void *y;
+    int dtype, hdtype, rows, width;
+    const void *h;               // or null
+    const void *post, *pre, *gate;
+    int post_dtype, pre_dtype, gate_dtype, gate_kind;
+    float eps, offset, residual_scale, block_scale;
+    void *h_out;
+    void *x_out;                 // with pre
+};
+// Its gradient, from dh (like h', or null), dx (like x', with pre), y and h' (with pre).
+struct NormGradArgs {
+    const void *dh, *dx, *y, *h;
+    int dtype, hdtype, rows, width;
+    const void *post, *pre, *gate;
+    int post_dtype, pre_dtype, gate_dtype, gate_kind;
+    float eps, offset, residual_scale, block_scale;
+    void *dy;        // like y
+    void *dres;      // like h, or null
+    float *dpost, *dpre;  // [width], with post / pre
+    void *dgate;     // f32 [width] or [rows], or like y
+    int parts;       // workgroups
+    float *part;     // [parts][sums][width]: dpre, dpost and dgate [width], those that there are
+};
+int norm_backward_parts(int rows, int width);
+hipError_t run_norm(const NormArgs &a, hipStream_t s);
+hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s);
+
+// The clip of many gradients by their global norm (exl3_clip.hip): the tensors of one launch as arguments.
+constexpr int kClipTensors = 128;    // a launch's (its arguments stay within 4 KiB)
+constexpr int kClipChunk = 8192;     // elements a workgroup takes at once
+constexpr int kClipParts = 1024;     // workgroups a launch
+constexpr int64_t kClipMaxElements = int64_t(1) << 36;  // of a tensor: a launch's chunks are numbered in 32 bits
+struct ClipTensors {
+    const void *g[kClipTensors];
+    void *out[kClipTensors];
+    int64_t n[kClipTensors];
+    int32_t first[kClipTensors];     // its first chunk in the launch
+    uint8_t dtype[kClipTensors], out_dtype[kClipTensors];
+    int32_t count, chunks;
+};
+struct ClipArgs {
+    double *parts;      // of every launch's workgroups
+    int first_part;     // this launch's first
+    int all_parts;      // the last launch's last workgroup sums them all
+    uint32_t *counter;  // zero between calls
+    float max_norm;
+    float *result;      // [2]: norm, scale
+    float *factors;     // [2]: whose product is the scale that the second pass multiplies by
+};
+inline int clip_parts(int chunks) { return chunks < kClipParts ? chunks : kClipParts; }
+hipError_t run_clip_norm(const ClipTensors &t, const ClipArgs &a, bool last, hipStream_t s);
+hipError_t run_clip_scale(const ClipTensors &t, const float *factors, hipStream_t s);
+
 hipError_t run_tile_major(const uint16_t *src, uint16_t *dst, int experts, int it, int ot, int n, int inverse,
                           hipStream_t s);
 hipError_t run_fill_zero(void *p, size_t bytes, hipStream_t s);

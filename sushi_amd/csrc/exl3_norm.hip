@@ -1,0 +1,426 @@
+// The norms before and after a block with its gate and residual, and their gradient.  With rms(v) = v / sqrt(mean v^2 + eps):
+//   n = post ? rms(y) (o + post) : y,   h' = a h + b g n,   x' = rms(h') (o + pre)
+// and backwards, from dh and dx, with r and q the factors of rms(h') and rms(y):
+//   u = dx (o + pre),  H = dh + r (u - h' r^2 mean(u h')),  dpre = sum over rows of dx h' r,  dh_in = a H
+//   dg = b H n (summed as the gate was broadcast),  z = b H g,  dpost = sum over rows of z y q,
+//   v = post ? z (o + post) : z,   dy = post ? q (v - y q^2 mean(v y)) : z.
+// Everything is f32 up to the one rounding of each output; x' comes of the h' that is not yet rounded, the gradient's r of
+// the h' that was kept.  Both passes are bound by the rows' bytes.
+#include "exl3_kernels.h"
+#include "exl3_epilogue.h"
+
+#include <initializer_list>
+#include <type_traits>
+
+namespace exl3 {
+
+// A thread's values of a row are NV vectors of 8, the i-th from 8 (i TPR + t) on.  Rows of odd widths begin anywhere, so a
+// vector is a load of 16 bytes at its elements' alignment (global memory takes any), and the one that passes the row's end
+// goes by elements.
+using Words4 = uint32_t __attribute__((ext_vector_type(4)));
+using Words4At2 = Words4 __attribute__((aligned(2)));
+using Words4At4 = Words4 __attribute__((aligned(4)));
+
+// Element c of an array at the wave's address p: a byte offset of 32 bits, so that the address stays in scalar registers.
+template <int DT>
+__device__ __forceinline__ const char *elem(const void *p, uint32_t c) {
+    return static_cast<const char *>(p) + c * (DT == DT_F32 ? 4u : 2u);
+}
+template <int DT>
+__device__ __forceinline__ char *elem(void *p, uint32_t c) {
+    return static_cast<char *>(p) + c * (DT == DT_F32 ? 4u : 2u);
+}
+
+// Values c .. c + 7 of an array from p on; zeros from `width` on.
+template <int DT>
+__device__ __forceinline__ void load8(const void *p, uint32_t c, uint32_t width, float (&v)[8]) {
+    if (c + 8 <= width) {
+        if constexpr (DT == DT_F32) {
+            const Words4At4 *s = reinterpret_cast<const Words4At4 *>(elem<DT>(p, c));
+            const Words4 lo = s[0], hi = s[1];
+#pragma unroll
+            for (int q = 0; q < 4; q++) v[q] = __uint_as_float(lo[q]), v[4 + q] = __uint_as_float(hi[q]);
+        } else {
+            const Words4 w = *reinterpret_cast<const Words4At2 *>(elem<DT>(p, c));
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if constexpr (DT == DT_F16) v[2 * q] = h2f((uint16_t)w[q]), v[2 * q + 1] = h2f((uint16_t)(w[q] >> 16));
+                else v[2 * q] = __uint_as_float(w[q] << 16), v[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; q++) v[q] = c + q < width ? load_act<DT>(elem<DT>(p, c), q) : 0.f;
+    }
+}
+__device__ __forceinline__ void load8_any(const void *p, int dt, uint32_t c, uint32_t width, float (&v)[8]) {
+    if (dt == DT_F16) load8<DT_F16>(p, c, width, v);
+    else if (dt == DT_BF16) load8<DT_BF16>(p, c, width, v);
+    else load8<DT_F32>(p, c, width, v);
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(void *p, uint32_t c, uint32_t width, const float (&v)[8]) {
+    if (c + 8 <= width) {
+        if constexpr (DT == DT_F32) {
+            Words4At4 *s = reinterpret_cast<Words4At4 *>(elem<DT>(p, c));
+            Words4 lo, hi;
+#pragma unroll
+            for (int q = 0; q < 4; q++) lo[q] = __float_as_uint(v[q]), hi[q] = __float_as_uint(v[4 + q]);
+            s[0] = lo;
+            s[1] = hi;
+        } else {
+            Words4 w;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if constexpr (DT == DT_F16)
+                    w[q] = __half_as_ushort(__float2half_rn(v[2 * q])) | (uint32_t)__half_as_ushort(__float2half_rn(v[2 * q + 1])) << 16;
+                else
+                    w[q] = __bfloat16_as_ushort(__float2bfloat16(v[2 * q])) |
+                           (uint32_t)__bfloat16_as_ushort(__float2bfloat16(v[2 * q + 1])) << 16;
+            }
+            *reinterpret_cast<Words4At2 *>(elem<DT>(p, c)) = w;
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; q++)
+            if (c + q < width) store_act<DT>(elem<DT>(p, c), q, v[q]);
+    }
+}
+
+// The row's sum of N values a thread: over a wave, then over the row's waves by way of LDS (in wave order; `red` is the
+// reduction's own, so one barrier does).
+template <int TPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        v[k] += xor_lane_row<1>(v[k]);
+        v[k] += xor_lane_row<2>(v[k]);
+        v[k] += xor_lane_row<4>(v[k]);
+        v[k] += xor_lane_row<8>(v[k]);
+        v[k] += __shfl_xor(v[k], 16);
+        v[k] += __shfl_xor(v[k], 32);
+    }
+    if constexpr (TPR > 64) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < N; k++) red[wave][k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            float s = red[0][k];
+#pragma unroll
+            for (int w = 1; w < TPR / 64; w++) s += red[w][k];
+            v[k] = s;
+        }
+    }
+}
+
+__device__ __forceinline__ const void *row_at(const void *p, size_t row, int width, int dt) {
+    return p ? static_cast<const char *>(p) + row * width * (dt == DT_F32 ? 4 : 2) : nullptr;
+}
+__device__ __forceinline__ void *row_at(void *p, size_t row, int width, int dt) {
+    return p ? static_cast<char *>(p) + row * width * (dt == DT_F32 ? 4 : 2) : nullptr;
+}
+
+// A row's gate: 8 values of a thread.
+template <int DT>
+__device__ __forceinline__ void gate8(const void *gate, int kind, int gate_dtype, size_t row, uint32_t c, uint32_t width, float (&g)[8]) {
+    if (kind == GATE_CHANNEL) load8_any(gate, gate_dtype, c, width, g);
+    else if (kind == GATE_FULL) load8<DT>(row_at(gate, row, width, DT), c, width, g);
+    else {
+        const float v = kind == GATE_ROW ? load_any(gate, gate_dtype, row) : 1.f;
+#pragma unroll
+        for (int q = 0; q < 8; q++) g[q] = v;
+    }
+}
+
+constexpr int norm_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// A row by TPR threads (a wave's, or a workgroup's), each NV vectors of 8.
+template <int DT, int HT, int TPR, int NV>
+__global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
+    constexpr int ROWS = norm_threads(TPR) / TPR;
+    const int t = threadIdx.x & (TPR - 1);
+    const size_t row = (size_t)blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+    __shared__ float red[2][TPR / 64][1];
+    if (TPR == 64 && row >= (size_t)a.rows) return;  // a wave's row; else the grid is the rows
+    const void *y = row_at(a.y, row, a.width, DT), *h = row_at(a.h, row, a.width, HT);
+    float n[NV][8], s[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        load8<DT>(y, (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
+        if (h) load8<HT>(h, (uint32_t)(i * TPR + t) * 8, a.width, s[i]);
+    }
+    float f = 1.f;
+    if (a.post) {
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int q = 0; q < 8; q++) sum[0] += n[i][q] * n[i][q];
+        row_sum<TPR, 1>(sum, red[0]);
+        f = 1.f / sqrtf(sum[0] / (float)a.width + a.eps);
+    }
+    float sum[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        float w[8];
+        if (a.post) {
+            load8_any(a.post, a.post_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+#pragma unroll
+            for (int q = 0; q < 8; q++) n[i][q] *= f * (a.offset + w[q]);
+        }
+        if (a.gate_kind != GATE_NONE) {
+            gate8<DT>(a.gate, a.gate_kind, a.gate_dtype, row, (uint32_t)(i * TPR + t) * 8, a.width, w);
+#pragma unroll
+            for (int q = 0; q < 8; q++) n[i][q] *= w[q];
+        }
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            n[i][q] *= a.block_scale;
+            if (h) n[i][q] += a.residual_scale * s[i][q];
+            sum[0] += n[i][q] * n[i][q];
+        }
+        store8<HT>(row_at(a.h_out, row, a.width, HT), (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
+    }
+    if (!a.pre) return;
+    row_sum<TPR, 1>(sum, red[1]);
+    f = 1.f / sqrtf(sum[0] / (float)a.width + a.eps);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        float w[8];
+        load8_any(a.pre, a.pre_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+#pragma unroll
+        for (int q = 0; q < 8; q++) n[i][q] *= f * (a.offset + w[q]);
+        store8<DT>(row_at(a.x_out, row, a.width, DT), (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
+    }
+}
+
+// The gradient.  A workgroup takes rows blockIdx.x, + gridDim.x, ..., keeps its columns' sums (dpre, dpost, a channel gate's)
+// in registers (up to 16 a thread) or in its part, and leaves them there for the join.
+template <int DT, int HT, int TPR, int NV>
+__global__ __launch_bounds__(TPR) void norm_backward_kernel(NormGradArgs a) {
+    const int t = threadIdx.x;
+    __shared__ float red[2][TPR / 64][3], red2[2][TPR / 64][2];
+    const float inv_width = 1.f / (float)a.width;
+    const bool channel = a.gate_kind == GATE_CHANNEL;
+    // this workgroup's sums, one after another as they are wanted
+    const int sums = (a.pre != nullptr) + (a.post != nullptr) + channel;
+    float *part = a.part + (size_t)blockIdx.x * sums * a.width;
+    float *part_post = part + (a.pre ? a.width : 0), *part_gate = part_post + (a.post ? a.width : 0);
+    constexpr bool REGS = NV <= 2;
+    using Acc = float[REGS ? NV : 1][8];
+    Acc acc_pre = {}, acc_post = {}, acc_gate = {};
+    bool first = true;
+    int flip = 0;
+    auto add = [&](Acc &acc, float *at, int i, const float (&v)[8]) {
+        if constexpr (REGS) {
+#pragma unroll
+            for (int q = 0; q < 8; q++) acc[i][q] += v[q];
+        } else {
+            float o[8];
+            if (first) {
+                store8<DT_F32>(at, (uint32_t)(i * TPR + t) * 8, a.width, v);
+                return;
+            }
+            load8<DT_F32>(at, (uint32_t)(i * TPR + t) * 8, a.width, o);
+#pragma unroll
+            for (int q = 0; q < 8; q++) o[q] += v[q];
+            store8<DT_F32>(at, (uint32_t)(i * TPR + t) * 8, a.width, o);
+        }
+    };
+    for (size_t row = blockIdx.x; row < (size_t)a.rows; row += gridDim.x, first = false, flip ^= 1) {
+        const void *py = row_at(a.y, row, a.width, DT), *ph = row_at(a.h, row, a.width, HT);
+        const void *pdh = row_at(a.dh, row, a.width, HT), *pdx = row_at(a.dx, row, a.width, DT);
+        float y[NV][8], H[NV][8], h[REGS ? NV : 1][8], dx[REGS ? NV : 1][8];  // (past 16 values a thread h and dx are read twice)
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            load8<DT>(py, (uint32_t)(i * TPR + t) * 8, a.width, y[i]);
+            if (pdh) load8<HT>(pdh, (uint32_t)(i * TPR + t) * 8, a.width, H[i]);
+            else
+#pragma unroll
+                for (int q = 0; q < 8; q++) H[i][q] = 0.f;
+            if (REGS && a.pre) {
+                load8<HT>(ph, (uint32_t)(i * TPR + t) * 8, a.width, h[i % (REGS ? NV : 1)]);
+                load8<DT>(pdx, (uint32_t)(i * TPR + t) * 8, a.width, dx[i % (REGS ? NV : 1)]);
+            }
+        }
+        auto again = [&](int i) -> int {  // where vector i of h and dx is
+            if constexpr (REGS) return i;
+            load8<HT>(ph, (uint32_t)(i * TPR + t) * 8, a.width, h[0]);
+            load8<DT>(pdx, (uint32_t)(i * TPR + t) * 8, a.width, dx[0]);
+            return 0;
+        };
+        float s[3] = {0.f, 0.f, 0.f};  // of h'^2, u h', y^2
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if (a.pre) {
+                float w[8];
+                const int k = again(i);
+                load8_any(a.pre, a.pre_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    s[0] += h[k][q] * h[k][q];
+                    s[1] += dx[k][q] * (a.offset + w[q]) * h[k][q];
+                }
+            }
+            if (a.post)
+#pragma unroll
+                for (int q = 0; q < 8; q++) s[2] += y[i][q] * y[i][q];
+        }
+        if (a.pre || a.post) row_sum<TPR, 3>(s, red[flip]);
+        const float r = a.pre ? 1.f / sqrtf(s[0] * inv_width + a.eps) : 0.f;
+        const float along = r * r * (s[1] * inv_width);
+        const float qf = a.post ? 1.f / sqrtf(s[2] * inv_width + a.eps) : 1.f;
+        float s2[2] = {0.f, 0.f};  // of v y, b H n
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            float w[8], d[8];
+            if (a.pre) {
+                const int k = again(i);
+                load8_any(a.pre, a.pre_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    H[i][q] += r * (dx[k][q] * (a.offset + w[q]) - h[k][q] * along);
+                    d[q] = dx[k][q] * (h[k][q] * r);
+                }
+                add(acc_pre, part, i, d);
+            }
+            if (a.dres) {
+#pragma unroll
+                for (int q = 0; q < 8; q++) d[q] = a.residual_scale * H[i][q];
+                store8<HT>(row_at(a.dres, row, a.width, HT), (uint32_t)(i * TPR + t) * 8, a.width, d);
+            }
+            if (a.post) {
+                load8_any(a.post, a.post_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+#pragma unroll
+                for (int q = 0; q < 8; q++) w[q] += a.offset;
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; q++) w[q] = 1.f;
+            }
+#pragma unroll
+            for (int q = 0; q < 8; q++) H[i][q] *= a.block_scale;
+            float g[8];
+            gate8<DT>(a.gate, a.gate_kind, a.gate_dtype, row, (uint32_t)(i * TPR + t) * 8, a.width, g);
+            if (a.gate_kind != GATE_NONE) {
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    d[q] = H[i][q] * (y[i][q] * qf * w[q]);
+                    s2[1] += d[q];
+                }
+                if (channel) add(acc_gate, part_gate, i, d);
+                if (a.gate_kind == GATE_FULL) store8<DT>(row_at(a.dgate, row, a.width, DT), (uint32_t)(i * TPR + t) * 8, a.width, d);
+            }
+            if (a.post) {
+#pragma unroll
+                for (int q = 0; q < 8; q++) d[q] = H[i][q] * g[q] * (y[i][q] * qf);
+                add(acc_post, part_post, i, d);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                H[i][q] *= g[q] * w[q];  // v
+                s2[0] += H[i][q] * y[i][q];
+            }
+        }
+        if (a.post || a.gate_kind == GATE_ROW) row_sum<TPR, 2>(s2, red2[flip]);
+        if (a.gate_kind == GATE_ROW && t == 0) static_cast<float *>(a.dgate)[row] = s2[1];
+        const float along_y = qf * qf * (s2[0] * inv_width);
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if (a.post)
+#pragma unroll
+                for (int q = 0; q < 8; q++) H[i][q] = qf * (H[i][q] - y[i][q] * along_y);
+            store8<DT>(row_at(a.dy, row, a.width, DT), (uint32_t)(i * TPR + t) * 8, a.width, H[i]);
+        }
+    }
+    if constexpr (REGS) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if (a.pre) store8<DT_F32>(part, (uint32_t)(i * TPR + t) * 8, a.width, acc_pre[i]);
+            if (a.post) store8<DT_F32>(part_post, (uint32_t)(i * TPR + t) * 8, a.width, acc_post[i]);
+            if (channel) store8<DT_F32>(part_gate, (uint32_t)(i * TPR + t) * 8, a.width, acc_gate[i]);
+        }
+    }
+}
+
+// A column's sum over the parts: the lanes of a wave hold 64 columns, the workgroup's waves a share of the parts each, in
+// order; the shares add in wave order.
+constexpr int NJ_WAVES = 16;
+__global__ __launch_bounds__(64 * NJ_WAVES) void norm_join_kernel(const float *part, int parts, int sums, int width, float *d0, float *d1,
+                                                                  float *d2) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, total = sums * width, c = blockIdx.x * 64 + lane;
+    __shared__ float share[NJ_WAVES][64];
+    float s = 0.f;
+    if (c < total)
+        for (int p = wave; p < parts; p += NJ_WAVES) s += part[(size_t)p * total + c];
+    share[wave][lane] = s;
+    __syncthreads();
+    if (wave || c >= total) return;
+    for (int w = 1; w < NJ_WAVES; w++) s += share[w][lane];
+    const int k = c / width;
+    (k == 0 ? d0 : k == 1 ? d1 : d2)[c - k * width] = s;
+}
+
+int norm_backward_parts(int rows, int width) { return rows < 512 ? rows : 512; }
+
+template <class F>
+static hipError_t with_types(int dt, int ht, F f) {
+    using std::integral_constant;
+    if (dt == DT_F32) return f(integral_constant<int, DT_F32>{}, integral_constant<int, DT_F32>{});
+    if (dt == DT_F16)
+        return ht == DT_F32 ? f(integral_constant<int, DT_F16>{}, integral_constant<int, DT_F32>{})
+                            : f(integral_constant<int, DT_F16>{}, integral_constant<int, DT_F16>{});
+    return ht == DT_F32 ? f(integral_constant<int, DT_BF16>{}, integral_constant<int, DT_F32>{})
+                        : f(integral_constant<int, DT_BF16>{}, integral_constant<int, DT_BF16>{});
+}
+
+hipError_t run_norm(const NormArgs &a, hipStream_t s) {
+    return with_types(a.dtype, a.hdtype, [&](auto DT, auto HT) {
+        constexpr int dt = decltype(DT)::value, ht = decltype(HT)::value;
+        auto go = [&](auto TPR, auto NV) {
+            constexpr int tpr = decltype(TPR)::value, nv = decltype(NV)::value, rows = norm_threads(tpr) / tpr;
+            const dim3 grid((unsigned)(((long)a.rows + rows - 1) / rows)), block(norm_threads(tpr));
+            hipLaunchKernelGGL((norm_kernel<dt, ht, tpr, nv>), grid, block, 0, s, a);
+            return hipGetLastError();
+        };
+        using std::integral_constant;
+        if (a.width <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+        if (a.width <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+        if (a.width <= 4096) return go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+        if (a.width <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+        return go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    });
+}
+
+hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
+    hipError_t e = with_types(a.dtype, a.hdtype, [&](auto DT, auto HT) {
+        constexpr int dt = decltype(DT)::value, ht = decltype(HT)::value;
+        auto go = [&](auto TPR, auto NV) {
+            constexpr int tpr = decltype(TPR)::value, nv = decltype(NV)::value;
+            hipLaunchKernelGGL((norm_backward_kernel<dt, ht, tpr, nv>), dim3(a.parts), dim3(tpr), 0, s, a);
+            return hipGetLastError();
+        };
+        using std::integral_constant;
+        if (a.width <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+        if (a.width <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+        if (a.width <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+        if (a.width <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+        return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+    });
+    if (e != hipSuccess) return e;
+    float *to[3], **next = to;
+    if (a.pre) *next++ = a.dpre;
+    if (a.post) *next++ = a.dpost;
+    if (a.gate_kind == GATE_CHANNEL) *next++ = static_cast<float *>(a.dgate);
+    const int sums = (int)(next - to);
+    if (!sums) return hipSuccess;
+    for (int k = sums; k < 3; k++) to[k] = to[0];
+    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)((sums * a.width + 63) / 64)), dim3(64 * NJ_WAVES), 0, s, a.part, a.parts, sums,
+                       a.width, to[0], to[1], to[2]);
+    return hipGetLastError();
+}
+
+}  // namespace exl3

@@ -1206,6 +1206,217 @@ def moe_router_backward(router_logits: torch.Tensor, inds: torch.Tensor, dscores
     return dlogits
 
 
+# ---------------------------------------------------------------------------------------------------------------
+# Between routed layers (extensions: the reference's router is moe_routing_chain, and it only serves)
+
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _score(score: str) -> int:
+    try:
+        return SCORES[score]
+    except (KeyError, TypeError):
+        raise Exl3ActivationUnknown(f"score {score!r} (one of {', '.join(SCORES)})") from None
+
+
+def moe_route(router_logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, score: str = "softmax",
+              groups: int = 1, topk_groups: int = 1, group_top: int = 1, renormalize: bool = True, scale: float = 1.0,
+              mask: Optional[torch.Tensor] = None):
+    """The choice of experts, for routers that moe_routing_chain does not cover: router_logits [.., E] (f16, bf16 or f32) ->
+    (inds [.., k] i32, scores [.., k] f32).  With p the logits' softmax or sigmoid (``score``) and c = p + bias ([E] f32, for the
+    choice alone): of ``groups`` groups of neighbouring experts the ``topk_groups`` with the largest sum of their ``group_top`` (1
+    or 2) largest c, of their experts the k largest c in falling order, equal ones by their number; the scores are scale p, over
+    the sum of the picks' p with ``renormalize``.  A logit or bias of -inf takes its expert out.  Slots that no expert is left for
+    and rows that mask [..] leaves out hold -1 and 0.  The choice is that of 64-bit values: it does not change with the batch."""
+    lg = router_logits
+    if lg.dim() < 1 or (mask is not None and mask.shape != lg.shape[:-1]):
+        raise BadExl3Shape(f"moe_route: logits {tuple(lg.shape)}" + ("" if mask is None else f", mask {tuple(mask.shape)}"))
+    if mask is not None and mask.dtype not in (torch.bool, torch.uint8):
+        raise BadExl3Dtype(f"moe_route: mask dtype {mask.dtype} (bool or u8)")
+    experts = lg.shape[-1]
+    if bias is not None and (bias.shape != (experts,) or bias.dtype != torch.float32):
+        raise BadExl3Shape(f"moe_route: bias {tuple(bias.shape)} {bias.dtype}, expected {(experts,)} in float32")
+    code, dt = _score(score), _dt(lg, "logits")
+    rows = lg.numel() // experts if experts else 0
+    dev, guard = _on_one_device("moe_route", lg, bias, mask)
+    with guard:
+        shape = (*lg.shape[:-1], max(k, 0))
+        inds = torch.empty(shape, dtype=torch.int32, device=dev)
+        scores = torch.empty(shape, dtype=torch.float32, device=dev)
+        _check(_lib.load().exl3_route(lg.data_ptr(), dt, rows, experts, k, _ptr(bias), code, groups, topk_groups, group_top,
+                                      bool(renormalize), float(scale), _ptr(mask), inds.data_ptr(), scores.data_ptr(),
+                                      _raw_stream(dev.index)))
+    return inds, scores
+
+
+def moe_route_backward(router_logits: torch.Tensor, inds: torch.Tensor, dscores: torch.Tensor, score: str = "softmax",
+                       renormalize: bool = True, scale: float = 1.0, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient of moe_route's logits through its scores, the choice held fixed: dscores [.., K] f32 -> like router_logits.
+    ``score``, ``renormalize``, ``scale`` and ``mask`` as in the forward; an id outside 0 .. E - 1 is a dropped slot, without a
+    score.  The balance loss's gradient is moe_router_backward's (with ``weight`` and ``dloss`` alone) and adds to it.  Equal
+    calls give equal bits."""
+    rows, experts, topk = _router_operands(router_logits, inds, mask, "moe_route_backward")
+    if dscores.shape != inds.shape:
+        raise BadExl3Shape(f"moe_route_backward: dscores {tuple(dscores.shape)} vs inds {tuple(inds.shape)}")
+    if dscores.dtype != torch.float32:
+        raise BadExl3Dtype(f"moe_route_backward: dscores dtype {dscores.dtype} (f32)")
+    code, dt = _score(score), _dt(router_logits, "logits")
+    dev, guard = _on_one_device("moe_route_backward", router_logits, inds, mask, dscores)
+    with guard:
+        dlogits = torch.empty_like(router_logits)
+        _check(_lib.load().exl3_route_backward(router_logits.data_ptr(), dt, rows, experts, inds.data_ptr(), topk,
+                                               dscores.data_ptr(), code, bool(renormalize), float(scale), _ptr(mask),
+                                               dlogits.data_ptr(), _raw_stream(dev.index)))
+    return dlogits
+
+
+class BlockNorm(NamedTuple):
+    """``h`` the new residual stream, ``x`` the next block's input (None without a pre norm)."""
+
+    h: torch.Tensor
+    x: Optional[torch.Tensor]
+
+
+class BlockNormGrads(NamedTuple):
+    """The gradients of block_norm's y (in y's dtype), h (``dresidual``, in h's), weights (f32) and gate (f32; in y's dtype
+    where the gate has a value for each of y's); None for what there was not."""
+
+    dy: torch.Tensor
+    dresidual: Optional[torch.Tensor]
+    dpost_weight: Optional[torch.Tensor]
+    dpre_weight: Optional[torch.Tensor]
+    dgate: Optional[torch.Tensor]
+
+
+_GATE_NONE, _GATE_CHANNEL, _GATE_ROW, _GATE_FULL = range(4)
+
+
+def _block_norm_operands(what: str, y, hs, post_weight, pre_weight, gate):
+    """(rows, width, gate kind), the operands' shapes and types checked; hs: what is shaped as y."""
+    if y.dim() < 1:
+        raise BadExl3Shape(f"{what}: y has no width")
+    shape, width = y.shape, y.shape[-1]
+    for t in hs:
+        if t is not None and t.shape != shape:
+            raise BadExl3Shape(f"{what}: {tuple(t.shape)} beside y {tuple(shape)}")
+    for w in (post_weight, pre_weight):
+        if w is not None and w.shape != (width,):
+            raise BadExl3Shape(f"{what}: weight {tuple(w.shape)}, expected {(width,)}")
+    kind = _GATE_NONE
+    if gate is not None:
+        if gate.shape == (width,):
+            kind = _GATE_CHANNEL
+        elif gate.shape == (*shape[:-1], 1):
+            kind = _GATE_ROW
+        elif gate.shape == shape:
+            kind = _GATE_FULL
+        else:
+            raise BadExl3Shape(f"{what}: gate {tuple(gate.shape)} for y {tuple(shape)}: one value a channel, a row or each")
+    return (y.numel() // width if width else 0), width, kind
+
+
+def _dt_or(t: Optional[torch.Tensor], what: str, default: int = 0) -> int:
+    return default if t is None else _dt(t, what)
+
+
+def block_norm(y: torch.Tensor, h: Optional[torch.Tensor] = None, post_weight: Optional[torch.Tensor] = None,
+               pre_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               weight_offset: float = 0.0, residual_scale: float = 1.0, block_scale: float = 1.0) -> BlockNorm:
+    """From a block's output y [.., D] and the residual stream h [.., D] to the next block's input, in one pass:
+
+        h_new = residual_scale h + block_scale gate n,   n = rms(y) (weight_offset + post_weight), or y without a post norm
+        x = rms(h_new) (weight_offset + pre_weight),     rms(v) = v / sqrt(mean v^2 + eps)
+
+    y and x share a dtype (f16, bf16 or f32); h and h_new are in that or f32 (without h, h_new is in y's).  post_weight and
+    pre_weight [D] f16, bf16 or f32 each; gate [D] or [.., 1] in any of them, or like y.  x comes of h_new before its rounding.
+    Not recorded by autograd."""
+    rows, width, kind = _block_norm_operands("block_norm", y, (h,), post_weight, pre_weight, gate)
+    dt = _dt(y, "y")
+    hdt = _dt_or(h, "h", dt)
+    dev, guard = _on_one_device("block_norm", y, h, post_weight, pre_weight, gate)
+    with guard:
+        h_new = torch.empty_like(y if h is None else h)
+        x = None if pre_weight is None else torch.empty_like(y)
+        _check(_lib.load().exl3_block_norm(y.data_ptr(), dt, _ptr(h), hdt, rows, width, _ptr(post_weight),
+                                           _dt_or(post_weight, "post_weight"), _ptr(gate), _dt_or(gate, "gate"), kind,
+                                           _ptr(pre_weight), _dt_or(pre_weight, "pre_weight"), eps, weight_offset,
+                                           residual_scale, block_scale, h_new.data_ptr(), _ptr(x), _raw_stream(dev.index)))
+    return BlockNorm(h_new, x)
+
+
+def block_norm_backward(dh: Optional[torch.Tensor], dx: Optional[torch.Tensor], y: torch.Tensor, h: Optional[torch.Tensor],
+                        post_weight: Optional[torch.Tensor] = None, pre_weight: Optional[torch.Tensor] = None,
+                        gate: Optional[torch.Tensor] = None, eps: float = 1e-6, weight_offset: float = 0.0,
+                        residual_scale: float = 1.0, block_scale: float = 1.0, with_dresidual: bool = True) -> BlockNormGrads:
+    """block_norm's gradient from dh (of its h; None: zero) and dx (of its x, with pre_weight), with y as it went in and h as
+    it came out (needed with pre_weight); the rest as in the forward.  Every sum has a fixed order: equal calls give equal
+    bits."""
+    what = "block_norm_backward"
+    rows, width, kind = _block_norm_operands(what, y, (dh, dx, h), post_weight, pre_weight, gate)
+    if pre_weight is None:
+        dx = h = None
+    if (pre_weight is not None and (dx is None or h is None)) or (pre_weight is None and dh is None):
+        raise BadExl3Shape(f"{what}: a pre norm needs dx and h, and without one dh is needed")
+    if dx is not None and dx.dtype != y.dtype:
+        raise BadExl3Dtype(f"{what}: dx {dx.dtype}, y {y.dtype}")
+    if dh is not None and h is not None and dh.dtype != h.dtype:
+        raise BadExl3Dtype(f"{what}: dh {dh.dtype}, h {h.dtype}")
+    stream_like = h if dh is None else dh
+    dt, hdt = _dt(y, "y"), _dt(stream_like, "dh")
+    dev, guard = _on_one_device(what, y, dh, dx, h, post_weight, pre_weight, gate)
+    with guard:
+        dy = torch.empty_like(y)
+        dres = torch.empty_like(stream_like) if with_dresidual else None
+        dpost = None if post_weight is None else torch.empty(width, dtype=torch.float32, device=dev)
+        dpre = None if pre_weight is None else torch.empty(width, dtype=torch.float32, device=dev)
+        dgate = None
+        if gate is not None:
+            dgate = torch.empty(gate.shape, dtype=gate.dtype if kind == _GATE_FULL else torch.float32, device=dev)
+        L = _lib.load()
+        stream = _raw_stream(dev.index)
+        ws = workspace.get(dev, L.exl3_block_norm_backward_workspace_size(rows, width), stream)
+        _check(L.exl3_block_norm_backward(_ptr(dh), _ptr(dx), y.data_ptr(), dt, _ptr(h), hdt, rows, width, _ptr(post_weight),
+                                          _dt_or(post_weight, "post_weight"), _ptr(gate), _dt_or(gate, "gate"), kind,
+                                          _ptr(pre_weight), _dt_or(pre_weight, "pre_weight"), eps, weight_offset,
+                                          residual_scale, block_scale, dy.data_ptr(), _ptr(dres), _ptr(dpost), _ptr(dpre),
+                                          _ptr(dgate), ws.data_ptr(), ws.numel(), stream))
+    return BlockNormGrads(dy, dres, dpost, dpre, dgate)
+
+
+class GradNorm(NamedTuple):
+    """``norm`` [] f32 of all the gradients, ``scale`` [] f32 that they were multiplied by."""
+
+    norm: torch.Tensor
+    scale: torch.Tensor
+
+
+def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> GradNorm:
+    """Clips gradients (f16, bf16 or f32 each, of any shapes) by their global norm, on the device: norm = sqrt(sum of all g^2),
+    scale = min(1, max_norm / norm), g *= scale in place, or g scale into ``out`` (a tensor for each gradient, of any of these
+    dtypes and the same shape).  ``max_norm`` inf with no ``out`` only measures.  A norm of inf or NaN comes out as that, with a
+    scale of 0 or NaN.  Squares add in 64 bits and in a fixed order: equal calls give equal bits."""
+    grads = list(grads)
+    if not grads:
+        raise BadExl3Shape("clip_grad_norm: no gradients")
+    outs = None if out is None else list(out)
+    if outs is not None and [t.shape for t in outs] != [t.shape for t in grads]:
+        raise BadExl3Shape("clip_grad_norm: out must hold a tensor of each gradient's shape")
+    n = len(grads)
+    dev, guard = _on_one_device("clip_grad_norm", *grads, *(outs or ()))
+    with guard:
+        result = torch.empty(2, dtype=torch.float32, device=dev)
+        L = _lib.load()
+        stream = _raw_stream(dev.index)
+        ws = workspace.get(dev, L.exl3_clip_grad_norm_workspace_size(n), stream)
+        ptrs, i32s = ctypes.c_void_p * n, ctypes.c_int32 * n
+        _check(L.exl3_clip_grad_norm(n, ptrs(*[t.data_ptr() for t in grads]),
+                                     (ctypes.c_int64 * n)(*[t.numel() for t in grads]), i32s(*[_dt(t, "gradient") for t in grads]),
+                                     None if outs is None else ptrs(*[t.data_ptr() for t in outs]),
+                                     None if outs is None else i32s(*[_dt(t, "out") for t in outs]), float(max_norm),
+                                     result.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+    return GradNorm(*result.unbind())
+
+
 def tile_major(trellis: torch.Tensor, inverse: bool = False) -> torch.Tensor:
     """`layout.tileMajor` (layout.zig:139-158) over [E, IT, OT, n]; ``inverse`` undoes it."""
     _need_gpu(trellis)
