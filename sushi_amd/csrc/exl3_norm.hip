@@ -6,87 +6,13 @@
 //   v = post ? z (o + post) : z,   dy = post ? q (v - y q^2 mean(v y)) : z.
 // Everything is f32 up to the one rounding of each output; x' comes of the h' that is not yet rounded, the gradient's r of
 // the h' that was kept.  Both passes are bound by the rows' bytes.
-#include "exl3_kernels.h"
+#include "exl3_vec.h"
 #include "exl3_epilogue.h"
 
 #include <initializer_list>
 #include <type_traits>
 
 namespace exl3 {
-
-// A thread's values of a row are NV vectors of 8, the i-th from 8 (i TPR + t) on.  Rows of odd widths begin anywhere, so a
-// vector is a load of 16 bytes at its elements' alignment (global memory takes any), and the one that passes the row's end
-// goes by elements.
-using Words4 = uint32_t __attribute__((ext_vector_type(4)));
-using Words4At2 = Words4 __attribute__((aligned(2)));
-using Words4At4 = Words4 __attribute__((aligned(4)));
-
-// Element c of an array at the wave's address p: a byte offset of 32 bits, so that the address stays in scalar registers.
-template <int DT>
-__device__ __forceinline__ const char *elem(const void *p, uint32_t c) {
-    return static_cast<const char *>(p) + c * (DT == DT_F32 ? 4u : 2u);
-}
-template <int DT>
-__device__ __forceinline__ char *elem(void *p, uint32_t c) {
-    return static_cast<char *>(p) + c * (DT == DT_F32 ? 4u : 2u);
-}
-
-// Values c .. c + 7 of an array from p on; zeros from `width` on.
-template <int DT>
-__device__ __forceinline__ void load8(const void *p, uint32_t c, uint32_t width, float (&v)[8]) {
-    if (c + 8 <= width) {
-        if constexpr (DT == DT_F32) {
-            const Words4At4 *s = reinterpret_cast<const Words4At4 *>(elem<DT>(p, c));
-            const Words4 lo = s[0], hi = s[1];
-#pragma unroll
-            for (int q = 0; q < 4; q++) v[q] = __uint_as_float(lo[q]), v[4 + q] = __uint_as_float(hi[q]);
-        } else {
-            const Words4 w = *reinterpret_cast<const Words4At2 *>(elem<DT>(p, c));
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if constexpr (DT == DT_F16) v[2 * q] = h2f((uint16_t)w[q]), v[2 * q + 1] = h2f((uint16_t)(w[q] >> 16));
-                else v[2 * q] = __uint_as_float(w[q] << 16), v[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int q = 0; q < 8; q++) v[q] = c + q < width ? load_act<DT>(elem<DT>(p, c), q) : 0.f;
-    }
-}
-__device__ __forceinline__ void load8_any(const void *p, int dt, uint32_t c, uint32_t width, float (&v)[8]) {
-    if (dt == DT_F16) load8<DT_F16>(p, c, width, v);
-    else if (dt == DT_BF16) load8<DT_BF16>(p, c, width, v);
-    else load8<DT_F32>(p, c, width, v);
-}
-
-template <int DT>
-__device__ __forceinline__ void store8(void *p, uint32_t c, uint32_t width, const float (&v)[8]) {
-    if (c + 8 <= width) {
-        if constexpr (DT == DT_F32) {
-            Words4At4 *s = reinterpret_cast<Words4At4 *>(elem<DT>(p, c));
-            Words4 lo, hi;
-#pragma unroll
-            for (int q = 0; q < 4; q++) lo[q] = __float_as_uint(v[q]), hi[q] = __float_as_uint(v[4 + q]);
-            s[0] = lo;
-            s[1] = hi;
-        } else {
-            Words4 w;
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if constexpr (DT == DT_F16)
-                    w[q] = __half_as_ushort(__float2half_rn(v[2 * q])) | (uint32_t)__half_as_ushort(__float2half_rn(v[2 * q + 1])) << 16;
-                else
-                    w[q] = __bfloat16_as_ushort(__float2bfloat16(v[2 * q])) |
-                           (uint32_t)__bfloat16_as_ushort(__float2bfloat16(v[2 * q + 1])) << 16;
-            }
-            *reinterpret_cast<Words4At2 *>(elem<DT>(p, c)) = w;
-        }
-    } else {
-#pragma unroll
-        for (int q = 0; q < 8; q++)
-            if (c + q < width) store_act<DT>(elem<DT>(p, c), q, v[q]);
-    }
-}
 
 // The row's sum of N values a thread: over a wave, then over the row's waves by way of LDS (in wave order; `red` is the
 // reduction's own, so one barrier does).
