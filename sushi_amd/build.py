@@ -28,6 +28,9 @@ SOURCES = [
     "exl3_gradient.hip",
     "exl3_router.hip",
     "exl3_route.hip",
+    "exl3_route_f16.hip",
+    "exl3_route_bf16.hip",
+    "exl3_route_f32.hip",
     "exl3_norm.hip",
     "exl3_clip.hip",
     "exl3_gemv_mcg.hip",

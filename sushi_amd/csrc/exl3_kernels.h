@@ -440,6 +440,9 @@ struct RouteGradArgs {
     void *dlogits;         // like logits
 };
 hipError_t run_route(const RouteArgs &a, hipStream_t s);
+hipError_t run_route_f16(const RouteArgs &a, hipStream_t s);
+hipError_t run_route_bf16(const RouteArgs &a, hipStream_t s);
+hipError_t run_route_f32(const RouteArgs &a, hipStream_t s);
 hipError_t run_route_backward(const RouteGradArgs &a, hipStream_t s);
 
 // The norms before and after a block (exl3_norm.hip), rms(v) = v / sqrt(mean v^2 + eps):

@@ -48,6 +48,16 @@ struct Raw8 {
             else w[q / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(at)[q] << (16 * (q & 1));
         }
     }
+    // -inf in place of all but the first n.
+    __device__ __forceinline__ void keep(int n) {
+        constexpr uint32_t LOW = DT == DT_F32 ? 0xFF800000u : DT == DT_F16 ? 0xFC00u : 0xFF80u;
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            if constexpr (DT == DT_F32) w[q] = q < n ? w[q] : LOW;
+            else if (q & 1) w[q / 2] = q < n ? w[q / 2] : (w[q / 2] & 0xFFFFu) | LOW << 16;
+            else w[q / 2] = q < n ? w[q / 2] : (w[q / 2] & 0xFFFF0000u) | LOW;
+        }
+    }
     __device__ __forceinline__ float get(int q) const {
         if constexpr (DT == DT_F32) return __uint_as_float(w[q]);
         else if constexpr (DT == DT_F16) return h2f((uint16_t)(q & 1 ? w[q / 2] >> 16 : w[q / 2]));
