@@ -14,6 +14,7 @@ namespace exl3 {
 
 constexpr int RT_THREADS = 256;
 constexpr int RT_WAVES = RT_THREADS / 64;
+constexpr int kListUnits = 128;  // units of eight experts that the lists serve
 constexpr int NO_EXPERT = 0x7FFFFFFF;
 
 // The value of lane (lane ^ H) where the lanes that differ below bit H hold the same: the mirror of 8 or 16 lanes then serves
@@ -56,57 +57,49 @@ __device__ __forceinline__ float pick_weight(const RouteArgs &a, float x, float 
     return (x >= 0.f ? 1.f : e) / (1.f + e);
 }
 
-// A row by one wave, lane l holding experts l, l + 64, ...; everything that decides in 64 bits.  buf: 64 PER values of the
-// wave's, with groups.
-template <int PER, int DT>
+// A row by one wave, lane l taking experts l, l + 64, ...; everything that decides in 64 bits, held in `buf` (a value an expert,
+// the wave's).  Rolled loops: a wave that takes a row here has this code to fetch, and it is most of its time.
+template <int DT>
 __device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int lane, double *buf) {
     const size_t at = row * a.experts;
-    float x[PER];
-    double c[PER];
-    uint32_t out = 0;  // bit i: expert lane + 64 i is out of the choice
+    const bool by_logit = !a.bias && (a.groups == 1 || a.group_top == 1);
+    const bool whole = !a.sigmoid && !(by_logit && a.renorm);
     bool bad = false;
     float mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = lane + 64 * i;
-        x[i] = load_act<DT>(a.logits, at + min(e, a.experts - 1));
-        const bool nan = x[i] != x[i] || (!a.sigmoid && x[i] == INFINITY);
-        bad |= nan && e < a.experts;
-        const float b = a.bias && e < a.experts ? a.bias[e] : 0.f;
-        const bool off = e >= a.experts || nan || x[i] == -INFINITY || !(b > -INFINITY);
-        out |= off ? 1u << i : 0u;
-        // (an expert that its bias takes out still has its share of the softmax)
-        if (e < a.experts && !nan) mx = fmaxf(mx, x[i]);
+    for (int e = lane; e < a.experts; e += 64) {
+        const float x = load_act<DT>(a.logits, at + e);
+        const bool nan = x != x || (!a.sigmoid && x == INFINITY);
+        bad |= nan;
+        mx = fmaxf(mx, nan ? -INFINITY : x);
+        buf[e] = nan ? -INFINITY : (double)x;
     }
     bad = __any(bad);
     mx = group_max<64>(mx);
-    const bool by_logit = !a.bias && (a.groups == 1 || a.group_top == 1);
-    double den = 1.;
-    if (!a.sigmoid && !(by_logit && a.renorm)) {
-        den = 0.;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const bool in = lane + 64 * i < a.experts && x[i] > -INFINITY && x[i] < INFINITY;
-            c[i] = in ? exp((double)x[i] - (double)mx) : 0.;
-            den += c[i];
+    double den = 0.;
+    if (!by_logit || whole) {
+        const double from = a.sigmoid || mx == -INFINITY ? 0. : (double)mx;
+        for (int e = lane; e < a.experts; e += 64) {
+            const double x = buf[e], y = exp(a.sigmoid ? -x : x - from);
+            den += y;
+            if (!by_logit) buf[e] = x == -INFINITY ? x : a.sigmoid ? 1. / (1. + y) : y;
         }
+    }
+    if (whole) {
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) den += __shfl_xor(den, m);
     }
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = lane + 64 * i;
-        if (by_logit) c[i] = (double)x[i];
-        else {
-            const double p = a.sigmoid ? 1. / (1. + exp(-(double)x[i])) : c[i] / den;
-            c[i] = p + (a.bias && e < a.experts ? (double)a.bias[e] : 0.);
+    if (!by_logit) {
+        for (int e = lane; e < a.experts; e += 64) {
+            double c = buf[e];
+            const float b = a.bias ? a.bias[e] : 0.f;
+            // (an expert that its bias takes out still has its share of the softmax)
+            const bool off = c == -INFINITY || !(b > -INFINITY);
+            buf[e] = off ? -INFINITY : (whole ? c / den : c) + (double)b;
         }
     }
     if (a.groups > 1) {
         // a lane a group
         const int size = a.experts / a.groups;
-#pragma unroll
-        for (int i = 0; i < PER; i++) buf[lane + 64 * i] = (out >> i) & 1u ? -INFINITY : c[i];
         wave_order();
         double c1 = -INFINITY, c2 = -INFINITY;
         const int g0 = min(lane, a.groups - 1) * size;
@@ -123,26 +116,22 @@ __device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int la
             ahead += better(w, g, worth, lane) ? 1 : 0;
         }
         const uint64_t open = __ballot(ahead < a.taken && worth > -INFINITY);
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int g = min(lane + 64 * i, a.experts - 1) / size;
-            out |= (open >> g) & 1 ? 0u : 1u << i;
-        }
+        for (int e = lane; e < a.experts; e += 64)
+            if (!((open >> (e / size)) & 1)) buf[e] = -INFINITY;
     }
     int mine = NO_EXPERT;
     for (int j = 0; j < a.topk; j++) {
         double bc = -INFINITY;
         int bi = NO_EXPERT;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int e = lane + 64 * i;
-            const bool take = !((out >> i) & 1u) && better(c[i], e, bc, bi);
-            bc = take ? c[i] : bc;
+        for (int e = lane; e < a.experts; e += 64) {
+            const double c = buf[e];
+            const bool take = c > bc;  // (of a lane's equal ones the first)
+            bc = take ? c : bc;
             bi = take ? e : bi;
         }
         wave_best(bc, bi);
         if (bi == NO_EXPERT) break;
-        out |= (bi & 63) == lane ? 1u << (bi >> 6) : 0u;
+        if ((bi & 63) == lane) buf[bi] = -INFINITY;
         mine = lane == j ? bi : mine;
     }
     const bool has = mine != NO_EXPERT;
@@ -160,9 +149,9 @@ __device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int la
 }
 
 // More than eight picks (or more units than the lists hold): a wave a row.
-template <int PER, int DT>
+template <int DT>
 __global__ __launch_bounds__(RT_THREADS) void route_kernel(RouteArgs a) {
-    __shared__ double buf[RT_WAVES][64 * PER];
+    extern __shared__ double row_buf[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const size_t row = (size_t)blockIdx.x * RT_WAVES + wave;
     if (row >= (size_t)a.rows) return;
@@ -173,21 +162,25 @@ __global__ __launch_bounds__(RT_THREADS) void route_kernel(RouteArgs a) {
         }
         return;
     }
-    route_row<PER, DT>(a, row, lane, buf[wave]);
+    route_row<DT>(a, row, lane, row_buf + wave * a.experts);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // Up to eight picks, several rows a wave.  A row is held by L lanes in units of eight experts, unit u = i L + l the i-th of lane l;
 // a unit's experts are one group's (a group's last unit may be short).  Each lane sorts its units' keys and merges them into
-// its best T, then log2(L) merges with other lanes leave the row's best T in every lane.
+// its best T, then log2(L) merges with other lanes leave the row's best T in every lane, and the best of the others beside them.
 //
-// A key is 32 bits: a value and, in the low bits, the complement of its expert's number, so a comparator of a sorting network
+// A key is 32 bits: a value and, in the low bits, the complement of its expert's place, so a comparator of a sorting network
 // is one maximum and one minimum of integers.  (A whole f32 above a number, as an f64, costs four times as much a comparator:
-// 65521 rows of 256 bf16 logits 23.6 us.)
-//   EXACT: the choice is by 16-bit logits, whose f32 bits leave the low ones free; the keys' order is the choice's.
-//   Otherwise a key holds M - v, M the row's largest value, as a float of 5 exponent bits (2^-20 .. 2^12) and what mantissa is
-//   left (18 bits for 256 experts).  Where two values that decide lie closer than that or than v's own f32 error tells, the
-//   wave takes the row again in 64 bits.
+// 65521 rows of 256 bf16 logits 23.6 us.)  The value is
+//   a 16-bit logit, whose f32 bits leave the low ones free (EXACT: the keys' order is the choice's),
+//   an f32 logit's distance from the row's largest, as a float of 5 exponent bits (2^-20 .. 2^12) and what mantissa is left,
+//   or c in steps of the range that p and the bias span.
+// Where two values of the last two kinds decide and lie closer than their key or c's own f32 error tells, the wave takes the
+// row again in 64 bits.
+//
+// The loops over a lane's units stay rolled: the kernel is short, so a call of few rows fetches less of it, and few registers
+// leave room for more waves.
 __device__ __forceinline__ void comparator(int &a, int &b) {
     const int hi = max(a, b), lo = min(a, b);
     a = hi;
@@ -208,11 +201,14 @@ __device__ __forceinline__ void sort_keys(int (&k)[4]) {
     comparator(k[1], k[2]);
 }
 // The T largest of two falling lists, falling: the maxima of one list and the other backwards rise and then fall or the other
-// way round, which log2(T) steps sort.
+// way round, which log2(T) steps sort.  The largest of those left out goes into `next`.
 template <int T>
-__device__ __forceinline__ void merge_keys(int (&k)[T], const int (&o)[T]) {
+__device__ __forceinline__ void merge_keys(int (&k)[T], const int (&o)[T], int &next) {
 #pragma unroll
-    for (int i = 0; i < T; i++) k[i] = max(k[i], o[T - 1 - i]);
+    for (int i = 0; i < T; i++) {
+        next = max(next, min(k[i], o[T - 1 - i]));
+        k[i] = max(k[i], o[T - 1 - i]);
+    }
 #pragma unroll
     for (int d = T / 2; d > 0; d /= 2)
 #pragma unroll
@@ -220,11 +216,12 @@ __device__ __forceinline__ void merge_keys(int (&k)[T], const int (&o)[T]) {
             if (!(i & d)) comparator(k[i], k[i | d]);
 }
 template <int H, int T>
-__device__ __forceinline__ void merge_lanes(int (&k)[T]) {
+__device__ __forceinline__ void merge_lanes(int (&k)[T], int &next) {
     int o[T];
 #pragma unroll
     for (int i = 0; i < T; i++) o[i] = xor_lane_int<H>(k[i]);
-    merge_keys(k, o);
+    next = max(next, xor_lane_int<H>(next));
+    merge_keys(k, o, next);
 }
 
 // Whether any of a row's L lanes holds true.
@@ -245,44 +242,49 @@ __device__ __forceinline__ float near_of(const RouteArgs &a, float inv_den, floa
 
 // M - v as 31 bits, and back (to its truncation): 0 below 2^-20, 0x7FFFFFFF for an expert that is out.
 constexpr uint32_t kDistBase = 107u << 23, kDistOut = (1u << 28) - 1;
-template <int ID_BITS>  // (of which a key keeps 28 - (ID_BITS - 3))
-__device__ __forceinline__ uint32_t dist_bits(float d) {
-    return min(__builtin_elementwise_sub_sat(__float_as_uint(d), kDistBase), kDistOut - (1u << (ID_BITS - 3)));
-}
+__device__ __forceinline__ uint32_t dist_bits(float d) { return __builtin_elementwise_sub_sat(__float_as_uint(d), kDistBase); }
 __device__ __forceinline__ float bits_dist(uint32_t b) { return b == 0 ? 0.f : __uint_as_float(b + kDistBase); }
 
-template <int L, int NU, int T, int DT, bool BY_LOGIT, bool GROUPED>
-__global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a) {
-    constexpr int ROWS = 64 / L, PER = (L * NU * 8 + 63) / 64;
+template <int L, int T, int DT, bool BY_LOGIT, bool GROUPED>
+__global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, int nu, int id_bits, int wave_lds) {
+    constexpr int ROWS = 64 / L;
     constexpr bool EXACT = BY_LOGIT && DT != DT_F32;
-    constexpr int ID_BITS = L * NU * 8 <= 64 ? 6 : L * NU * 8 <= 128 ? 7 : L * NU * 8 <= 256 ? 8 : L * NU * 8 <= 512 ? 9 : 10;
-    constexpr int ID = (1 << ID_BITS) - 1;  // numbers are units' places, 8 u + q
     constexpr float LOG2E = 1.4426950408889634f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (L - 1), grp = lane / L;
-    __shared__ __align__(16) float bias_lds[BY_LOGIT ? 4 : L * NU * 8];
-    __shared__ float2 unit_top[GROUPED ? RT_WAVES : 1][GROUPED ? ROWS : 1][GROUPED ? L * NU + 1 : 1];
-    __shared__ float worth_lds[GROUPED ? RT_WAVES : 1][GROUPED ? ROWS : 1][GROUPED ? kRouteMaxGroups + 1 : 1];
-    __shared__ double buf[GROUPED && !EXACT ? RT_WAVES : 1][GROUPED && !EXACT ? 64 * PER : 1];
+    extern __shared__ __align__(16) double row_buf[];  // wave_lds bytes a wave
+    char *const mem = reinterpret_cast<char *>(row_buf) + wave * wave_lds;
+    __shared__ __align__(16) float bias_lds[BY_LOGIT ? 4 : 8 * kListUnits];
+    __shared__ float range[RT_WAVES][2];
     const int size = a.experts / a.groups, units = (size + 7) / 8;
-    auto first_of = [&](int u) { return GROUPED ? u / units * size + u % units * 8 : u * 8; };
+    const uint32_t over = (65536 + units - 1) / units;  // u / units = u over >> 16 for the units here
+    auto first_of = [&](int u) { return GROUPED ? (int)(u * over >> 16) * (size - units * 8) + u * 8 : u * 8; };
     auto count_of = [&](int u) {
-        const int left = GROUPED ? (u < a.groups * units ? size - u % units * 8 : 0) : size - u * 8;
-        return max(0, min(8, left));
+        const int g = GROUPED ? (int)(u * over >> 16) : 0;
+        return g < a.groups ? max(0, min(8, size - (u - g * units) * 8)) : 0;
     };
-    int first[NU], n[NU];  // a unit's first expert and how many it holds
-#pragma unroll
-    for (int i = 0; i < NU; i++) {
-        first[i] = first_of(i * L + l);
-        n[i] = count_of(i * L + l);
-    }
+    const int id_mask = EXACT ? 1023 : (1 << id_bits) - 1;  // a key's low bits: the complement of the expert's place, 8 u + q
+    float lo = 0.f, steps = 0.f, largest = 0.f;             // c's steps: (c - lo) steps + 1; no |c| is above `largest`
     if constexpr (!BY_LOGIT) {
-        for (int s = threadIdx.x; s < L * NU * 8; s += RT_THREADS) {
+        float least = INFINITY, most = -INFINITY;
+        for (int s = threadIdx.x; s < L * nu * 8; s += RT_THREADS) {
             const bool is = (s & 7) < count_of(s / 8);
-            const float b = is && a.bias ? a.bias[first_of(s / 8) + (s & 7)] : 0.f;
+            float b = is ? a.bias ? a.bias[first_of(s / 8) + (s & 7)] : 0.f : -INFINITY;
             // (NaN is out of the choice; what passes 2^125 goes by 64 bits where it decides, and adds up in f32)
-            bias_lds[s] = b > -INFINITY ? fminf(fmaxf(b, -0x1p125f), 0x1p125f) : -INFINITY;
+            b = b > -INFINITY ? fminf(fmaxf(b, -0x1p125f), 0x1p125f) : -INFINITY;
+            bias_lds[s] = b;
+            least = fminf(least, b > -INFINITY ? b : INFINITY);
+            most = fmaxf(most, b);
         }
+        least = -group_max<64>(-least);
+        most = group_max<64>(most);
+        range[wave][0] = least;
+        range[wave][1] = most;
         __syncthreads();
+#pragma unroll
+        for (int w = 0; w < RT_WAVES; w++) least = fminf(least, range[w][0]), most = fmaxf(most, range[w][1]);
+        lo = least;
+        largest = fmaxf(fabsf(least), fabsf(most) + 1.f);
+        steps = most >= least ? (float)((1u << (31 - id_bits)) - 16) / (1.0625f + (most - least)) : 0.f;
     }
     const int bad_class = a.sigmoid ? 0x003 : 0x203;  // NaN; under softmax +inf too
     const size_t rows = (size_t)a.rows, step = (size_t)gridDim.x * RT_WAVES * ROWS;
@@ -290,101 +292,104 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a) {
         const size_t r = r0 + grp;
         const bool in = r < rows, live = in && (!a.mask || a.mask[in ? r : 0] != 0);
         const char *row = static_cast<const char *>(a.logits) + (in ? r : r0) * a.experts * (DT == DT_F32 ? 4 : 2);
-        Raw8<DT> raw[NU];
-#pragma unroll
-        for (int i = 0; i < NU; i++) {
-            if (n[i] > 0 && first[i] + 8 <= a.experts) raw[i].load(elem<DT>(row, first[i]));
-            else raw[i].load_some(elem<DT>(row, first[i]), n[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NU; i++)
-            if (n[i] < 8) raw[i].keep(n[i]);  // -inf past a unit's experts
-        // the values that the choice goes by, -inf for an expert that is out of it
-        float v[NU][8], mx = -INFINITY;
         bool bad = false;
-#pragma unroll
-        for (int i = 0; i < NU; i++)
+        // A unit's logits, -inf for experts that are out by them and past the unit's own.
+        auto load = [&](int u, float (&v)[8]) {
+            Raw8<DT> raw;
+            const int first = first_of(u), n = count_of(u);
+            if (n > 0 && first + 8 <= a.experts) raw.load(elem<DT>(row, first));
+            else raw.load_some(elem<DT>(row, first), n);
+            if (n < 8) raw.keep(n);
 #pragma unroll
             for (int q = 0; q < 8; q++) {
-                const float x = raw[i].get(q);
+                const float x = raw.get(q);
                 const bool nan = __builtin_amdgcn_classf(x, bad_class);
                 bad |= nan;
-                v[i][q] = nan ? -INFINITY : x;
-                mx = fmaxf(mx, v[i][q]);
+                v[q] = nan ? -INFINITY : x;
             }
-        bad = group_any<L>(bad);
-        float inv = 1.f;
+        };
         const bool whole = !a.sigmoid && !(BY_LOGIT && a.renorm);  // the softmax over the row
-        if (whole || !EXACT) {
+        float mx = -INFINITY, inv = 1.f;
+        if (whole || (BY_LOGIT && !EXACT)) {
+#pragma unroll 1
+            for (int i = 0; i < nu; i++) {
+                float v[8];
+                load(i * L + l, v);
+#pragma unroll
+                for (int q = 0; q < 8; q++) mx = fmaxf(mx, v[q]);
+            }
             mx = group_max<L>(mx);
             mx = mx == -INFINITY ? 0.f : mx;
         }
-        float top_v = mx;  // the largest value
-        if (whole || !BY_LOGIT) {
+        if (whole) {
             float den = 0.f;
-            if (!BY_LOGIT) top_v = -INFINITY;
-            const float by = a.sigmoid ? -LOG2E : LOG2E, from = a.sigmoid ? 0.f : mx;
+#pragma unroll 1
+            for (int i = 0; i < nu; i++) {
+                float v[8];
+                load(i * L + l, v);
 #pragma unroll
-            for (int i = 0; i < NU; i++)
+                for (int q = 0; q < 8; q++) den += __builtin_amdgcn_exp2f(LOG2E * (v[q] - mx));
+            }
+            inv = rcp(group_sum<L>(den));
+        }
+        // The values that the choice goes by, -inf for an expert that is out of it.
+        auto values = [&](int u, float (&v)[8]) {
+            load(u, v);
+            if constexpr (!BY_LOGIT) {
+                const float4 *b = reinterpret_cast<const float4 *>(bias_lds + u * 8);
+                const float4 b0 = b[0], b1 = b[1];
+                const float bias[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
-                    const float x = v[i][q], e = __builtin_amdgcn_exp2f(by * (x - from));
-                    den += e;
-                    if constexpr (!BY_LOGIT) v[i][q] = x == -INFINITY ? x : a.sigmoid ? rcp(1.f + e) : e;
+                    const float x = v[q];
+                    const float e = __builtin_amdgcn_exp2f(a.sigmoid ? -LOG2E * x : LOG2E * (x - mx));
+                    const float p = a.sigmoid ? rcp(1.f + e) : e * inv;
+                    v[q] = x == -INFINITY ? x : p + bias[q];
                 }
-            if (whole) {
-                den = group_sum<L>(den);
-                inv = rcp(den);
             }
-            if constexpr (!BY_LOGIT) {
-                const float p = a.sigmoid ? 1.f : inv;
-#pragma unroll
-                for (int i = 0; i < NU; i++) {
-                    const float4 *b = reinterpret_cast<const float4 *>(bias_lds + (i * L + l) * 8);
-                    const float4 lo = b[0], hi = b[1];
-                    const float bias[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-                    for (int q = 0; q < 8; q++) {
-                        v[i][q] = v[i][q] * p + bias[q];
-                        top_v = fmaxf(top_v, v[i][q]);
-                    }
-                }
-                top_v = group_max<L>(top_v);
-                top_v = top_v == -INFINITY ? 0.f : top_v;
-            }
-        }
+        };
         bool near = false;
+        uint64_t open = ~uint64_t(0);
+        float *const vals = reinterpret_cast<float *>(mem) + grp * (L * nu * 8);
         if constexpr (GROUPED) {
             // each unit's two largest, each group's, its place among the groups
-#pragma unroll
-            for (int i = 0; i < NU; i++) {
-                float m1 = v[i][0], m2 = -INFINITY;
+            float2 *const unit_top = reinterpret_cast<float2 *>(mem + 2048 * nu) + grp * (L * nu);
+            float *const worth = reinterpret_cast<float *>(mem + 2560 * nu) + grp * a.groups;
+#pragma unroll 1
+            for (int i = 0; i < nu; i++) {
+                float v[8];
+                const int u = i * L + l;
+                values(u, v);
+                float m1 = v[0], m2 = -INFINITY;
 #pragma unroll
                 for (int q = 1; q < 8; q++) {
-                    m2 = __builtin_amdgcn_fmed3f(m1, m2, v[i][q]);
-                    m1 = fmaxf(m1, v[i][q]);
+                    m2 = __builtin_amdgcn_fmed3f(m1, m2, v[q]);
+                    m1 = fmaxf(m1, v[q]);
                 }
-                unit_top[wave][grp][i * L + l] = float2{m1, m2};
+                float4 *o = reinterpret_cast<float4 *>(vals + u * 8);
+                o[0] = float4{v[0], v[1], v[2], v[3]};
+                o[1] = float4{v[4], v[5], v[6], v[7]};
+                unit_top[u] = float2{m1, m2};
             }
             wave_order();
             for (int g = l; g < a.groups; g += L) {
                 float m1 = -INFINITY, m2 = -INFINITY;
                 for (int u = g * units; u < (g + 1) * units; u++) {
-                    const float2 o = unit_top[wave][grp][u];
+                    const float2 o = unit_top[u];
                     m2 = fmaxf(fmaxf(m2, o.y), fminf(m1, o.x));
                     m1 = fmaxf(m1, o.x);
                 }
-                worth_lds[wave][grp][g] = a.group_top == 2 && m2 > -INFINITY ? m1 + m2 : m1;
+                worth[g] = a.group_top == 2 && m2 > -INFINITY ? m1 + m2 : m1;
             }
             wave_order();
-            uint64_t open = 0;
+            open = 0;
             for (int g0 = 0; g0 < a.groups; g0 += L) {
                 const int g = g0 + l;
-                const float w = g < a.groups ? worth_lds[wave][grp][g] : -INFINITY;
-                const float tol = BY_LOGIT ? 0.f : near_of(a, inv, fabsf(w)) * 2.f;
+                const float w = g < a.groups ? worth[g] : -INFINITY;
+                const float tol = BY_LOGIT ? 0.f : near_of(a, inv, largest) * 2.f;
                 int ahead = 0, surely = 0, maybe = 0;
                 for (int o = 0; o < a.groups; o++) {
-                    const float x = worth_lds[wave][grp][o];
+                    const float x = worth[o];
                     ahead += x > w || (x == w && o < g) ? 1 : 0;
                     if constexpr (!BY_LOGIT) {
                         surely += x > w + tol ? 1 : 0;
@@ -397,75 +402,82 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a) {
                 open |= ((b >> (lane & ~(L - 1))) & (L == 64 ? ~uint64_t(0) : (uint64_t(1) << (L & 63)) - 1)) << g0;
             }
             wave_order();
-#pragma unroll
-            for (int i = 0; i < NU; i++) {
-                const bool is = n[i] > 0 && (open >> min((i * L + l) / units, 63)) & 1;
-#pragma unroll
-                for (int q = 0; q < 8; q++) v[i][q] = is ? v[i][q] : -INFINITY;
-            }
         }
-        int best[T];
+        int best[T], next = INT32_MIN;
+#pragma unroll 1
+        for (int i = 0; i < nu; i++) {
+            const int u = i * L + l;
+            float v[8];
+            if constexpr (GROUPED) {
+                const float4 *o = reinterpret_cast<const float4 *>(vals + u * 8);
+                const float4 v0 = o[0], v1 = o[1];
+                const bool is = (open >> min((int)(u * over >> 16), 63)) & 1;
+                const float w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-        for (int i = 0; i < NU; i++) {
-            int k[T];
+                for (int q = 0; q < 8; q++) v[q] = is ? w[q] : -INFINITY;
+            } else {
+                values(u, v);
+            }
+            const int not_id = ~(u * 8) & id_mask;  // of the unit's first: q less for its q-th
 #pragma unroll
             for (int part = 0; part < 8 / T; part++) {
+                int k[T];
 #pragma unroll
-                for (int q = 0; q < T; q++) {
-                    const int not_id = ~((i * L + l) * 8 + part * T + q) & ID;
-                    const float x = v[i][part * T + q];
+                for (int j = 0; j < T; j++) {
+                    const int q = part * T + j;
+                    const float x = v[q];
                     if constexpr (EXACT) {
                         const int b = __float_as_int(x + 0.f);  // (-0 is 0)
-                        k[q] = b ^ (((b >> 31) & (0x7FFFFFFF & ~ID)) | not_id);
+                        k[j] = b ^ (((b >> 31) & (0x7FFFFFFF & ~1023)) | (not_id - q));
+                    } else if constexpr (BY_LOGIT) {
+                        const uint32_t d = x == -INFINITY ? kDistOut : min(dist_bits(mx - x), kDistOut - (1u << (id_bits - 3)));
+                        k[j] = (int)(((~d << 3) & (uint32_t)(0x7FFFFFFF & ~id_mask)) | (uint32_t)(not_id - q));
                     } else {
-                        const uint32_t d = x == -INFINITY ? kDistOut : dist_bits<ID_BITS>(top_v - x);
-                        k[q] = (int)(((~d << 3) & (0x7FFFFFFF & ~ID)) | not_id);
+                        const uint32_t c = x == -INFINITY ? 0u : (uint32_t)((x - lo) * steps) + 1u;
+                        k[j] = (int)(c << id_bits | (uint32_t)(not_id - q));
                     }
                 }
                 sort_keys(k);
-                if (i == 0 && part == 0) {
+                if (part == 0 && i == 0) {
 #pragma unroll
                     for (int q = 0; q < T; q++) best[q] = k[q];
                 } else {
-                    merge_keys(best, k);
+                    merge_keys(best, k, next);
                 }
             }
         }
-        merge_lanes<1>(best);
-        merge_lanes<2>(best);
-        merge_lanes<4>(best);
-        if constexpr (L > 8) merge_lanes<8>(best);
-        if constexpr (L > 16) merge_lanes<16>(best);
-        if constexpr (L > 32) merge_lanes<32>(best);
-        // keys of experts that are out: what -inf, or kDistOut, makes
-        constexpr int OUT = EXACT ? (int)(0xFF800000u ^ (0x7FFFFFFFu & ~ID)) | ID : ID;
+        merge_lanes<1>(best, next);
+        merge_lanes<2>(best, next);
+        merge_lanes<4>(best, next);
+        if constexpr (L > 8) merge_lanes<8>(best, next);
+        if constexpr (L > 16) merge_lanes<16>(best, next);
+        if constexpr (L > 32) merge_lanes<32>(best, next);
+        bad = group_any<L>(bad);
+        // keys of experts that are out: what -inf, kDistOut or no step makes
+        const int out = EXACT ? (int)(0xFF800000u ^ (0x7FFFFFFFu & ~1023u)) | 1023 : id_mask;
         if constexpr (!EXACT) {
             // Two values that decide and lie close: the row goes by 64 bits.
-            auto dist = [](int key) { return bits_dist((~(uint32_t)key & (0x7FFFFFFFu & ~ID)) >> 3); };
-            constexpr float STEP = 1.f / (float)(1 << (26 - ID_BITS));  // two truncations, relative
-            const float tol = BY_LOGIT ? 0x1p-22f * fabsf(top_v) : near_of(a, inv, fabsf(top_v));
-            float last = 0.f, bound = 0.f;
+            int last = 0;
+            if constexpr (BY_LOGIT) {
+                const float tol = 0x1p-22f * fabsf(mx), part = 1.f - 2.f / (float)(1 << (26 - id_bits));  // two truncations
+                auto dist = [&](int key) { return bits_dist((~(uint32_t)key & (uint32_t)(0x7FFFFFFF & ~id_mask)) >> 3); };
 #pragma unroll
-            for (int i = 0; i < T; i++) {
-                if (i > a.topk) continue;
-                const float d = dist(best[i]);
-                const bool is = best[i] > OUT;
-                if (i > 0) near |= is && d * (1.f - STEP) - last <= tol + (d < 0x1p-19f ? 0x1p-20f : 0.f);
-                if (i < a.topk) {
-                    near |= is && d >= 0x1p11f;  // at the end of the distances
-                    last = d;
-                    bound = is ? d : -1.f;
+                for (int i = 0; i <= T; i++) {
+                    const int key = i < T ? best[i < T ? i : 0] : next;
+                    const float d = dist(key);
+                    // (at the end of the distances too)
+                    if (i <= a.topk && key > out)
+                        near |= (i > 0 && d * part - dist(last) <= tol + (d < 0x1p-19f ? 0x1p-20f : 0.f)) || (i < a.topk && d >= 0x1p11f);
+                    last = key;
                 }
-            }
-            if (a.topk == T) {
-                const float edge = top_v - (bound * (1.f + STEP) + tol + 0x1p-20f);
-                int above = 0;
+            } else {
+                const int tol = (int)fminf(near_of(a, inv, largest) * steps, 0x1p30f) + 3;
 #pragma unroll
-                for (int i = 0; i < NU; i++)
-#pragma unroll
-                    for (int q = 0; q < 8; q++) above += v[i][q] >= edge ? 1 : 0;
-                above = (int)group_sum<L>((float)above);
-                near |= above > T && bound >= 0.f;
+                for (int i = 0; i <= T; i++) {
+                    const int key = (i < T ? best[i < T ? i : 0] : next) >> id_bits;
+                    if (i > 0 && i <= a.topk && key > 0) near |= last - key <= tol;
+                    last = key;
+                }
             }
             near = group_any<L>(near) && live;
         }
@@ -473,12 +485,12 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a) {
         int key = best[0];
 #pragma unroll
         for (int i = 1; i < T; i++) key = (l & (T - 1)) == i ? best[i] : key;
-        const bool has = l < T && l < a.topk && key > OUT;
-        const int place = ~key & ID, e = GROUPED ? first_of(place >> 3) + (place & 7) : place;
+        const bool has = l < T && l < a.topk && key > out;
+        const int place = ~key & id_mask, e = GROUPED ? first_of(place >> 3) + (place & 7) : place;
         float px;
         if constexpr (EXACT) {
-            const int b = (key & ~ID);
-            px = __int_as_float(b ^ ((b >> 31) & (0x7FFFFFFF & ~ID)));
+            const int b = key & ~1023;
+            px = __int_as_float(b ^ ((b >> 31) & (0x7FFFFFFF & ~1023)));
         } else {
             px = load_act<DT>(elem<DT>(row, has ? e : 0), 0);
         }
@@ -495,49 +507,52 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a) {
         }
         if constexpr (!EXACT) {
             uint64_t again = __ballot(near && l == 0);
+#pragma unroll 1
             while (again) {
                 const int at = __ffsll((unsigned long long)again) - 1;
                 again &= again - 1;
-                route_row<PER, DT>(a, r0 + at / L, lane, buf[GROUPED ? wave : 0]);
+                wave_order();
+                route_row<DT>(a, r0 + at / L, lane, reinterpret_cast<double *>(mem));
+                wave_order();
             }
         }
     }
 }
 
-template <int L, int NU, int T, int DT>
-static hipError_t launch_lists(const RouteArgs &a, hipStream_t s) {
+// Lanes a row: so many that a lane has at most four units, and with few rows one each.
+template <int L, int T, int DT>
+static hipError_t launch_lists(const RouteArgs &a, int units, hipStream_t s) {
     constexpr int at_once = RT_THREADS / L;
     const long wgs = ((long)a.rows + at_once - 1) / at_once;
     const dim3 grid((unsigned)(wgs < 2048 ? wgs : 2048));
     const bool grouped = a.groups > 1, by_logit = !a.bias && (!grouped || a.group_top == 1);
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(RT_THREADS), 0, s, a); };
-    if (by_logit) grouped ? go(route_lists_kernel<L, NU, T, DT, true, true>) : go(route_lists_kernel<L, NU, T, DT, true, false>);
-    else grouped ? go(route_lists_kernel<L, NU, T, DT, false, true>) : go(route_lists_kernel<L, NU, T, DT, false, false>);
+    const int nu = (units + L - 1) / L;
+    int id_bits = 6;
+    while ((1 << id_bits) < L * nu * 8) id_bits++;
+    // the values, the units' two largest and the groups' worths of a wave's rows; a row's values in 64 bits
+    const int lists = grouped ? nu * 2560 + (64 / L * a.groups * 4 + 15) / 16 * 16 : 0, row = (a.experts * 8 + 15) / 16 * 16;
+    const int lds = lists > row ? lists : row;
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(RT_THREADS), RT_WAVES * lds, s, a, nu, id_bits, lds); };
+    if (by_logit) grouped ? go(route_lists_kernel<L, T, DT, true, true>) : go(route_lists_kernel<L, T, DT, true, false>);
+    else grouped ? go(route_lists_kernel<L, T, DT, false, true>) : go(route_lists_kernel<L, T, DT, false, false>);
     return hipGetLastError();
 }
 
 template <int T, int DT>
-static hipError_t with_units(const RouteArgs &a, int units, hipStream_t s) {
-    if (units <= 8) return launch_lists<8, 1, T, DT>(a, s);
-    if (units <= 16) return launch_lists<8, 2, T, DT>(a, s);
-    if (units <= 32) return launch_lists<8, 4, T, DT>(a, s);
-    if (units <= 64) return launch_lists<16, 4, T, DT>(a, s);
-    return launch_lists<32, 4, T, DT>(a, s);
+static hipError_t with_lanes(const RouteArgs &a, int units, hipStream_t s) {
+    const bool few = a.rows <= 2048;
+    if (units <= 8 || (!few && units <= 32)) return launch_lists<8, T, DT>(a, units, s);
+    if (units <= 16 || (!few && units <= 64)) return launch_lists<16, T, DT>(a, units, s);
+    if (units <= 32 || !few) return launch_lists<32, T, DT>(a, units, s);
+    return launch_lists<64, T, DT>(a, units, s);
 }
-
-constexpr int kListUnits = 128;
 
 template <int DT>
 static hipError_t route_of_type(const RouteArgs &a, hipStream_t s) {
     const int units = a.groups * ((a.experts / a.groups + 7) / 8);
-    if (a.topk <= 8 && units <= kListUnits) return a.topk <= 4 ? with_units<4, DT>(a, units, s) : with_units<8, DT>(a, units, s);
-    const unsigned grid = (unsigned)(((long)a.rows + RT_WAVES - 1) / RT_WAVES);
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(grid), dim3(RT_THREADS), 0, s, a); };
-    if (a.experts <= 64) go(route_kernel<1, DT>);
-    else if (a.experts <= 128) go(route_kernel<2, DT>);
-    else if (a.experts <= 256) go(route_kernel<4, DT>);
-    else if (a.experts <= 512) go(route_kernel<8, DT>);
-    else go(route_kernel<16, DT>);
+    if (a.topk <= 8 && units <= kListUnits) return a.topk <= 4 ? with_lanes<4, DT>(a, units, s) : with_lanes<8, DT>(a, units, s);
+    const dim3 grid((unsigned)(((long)a.rows + RT_WAVES - 1) / RT_WAVES));
+    hipLaunchKernelGGL(route_kernel<DT>, grid, dim3(RT_THREADS), RT_WAVES * a.experts * sizeof(double), s, a);
     return hipGetLastError();
 }
 

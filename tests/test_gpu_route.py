@@ -119,7 +119,10 @@ def test_experts_out_of_the_choice_and_odd_logits(dev, k, score, grouped):
     bias = _bias(3, 32)
     out = bias.clone()
     out[8:16], out[17] = -math.inf, math.nan
-    for b in (None, bias, out, bias * 1000):
+    far = bias.clone()
+    far[4], far[6], far[25] = math.inf, 3e38, -3e38
+    none = torch.full((32,), -math.inf)
+    for b in (None, bias, out, bias * 1000, far, none):
         for renorm in (True, False):
             for dtype in (F32, BF16):
                 _check(lg.to(dtype).to(dev), k, bias=None if b is None else b.to(dev), score=score, renormalize=renorm, **kw)
