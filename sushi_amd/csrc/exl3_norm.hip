@@ -14,19 +14,23 @@
 
 namespace exl3 {
 
+// A wave's sum, in every lane: pairs, quads, 8 and 16 lanes by exchanges, then each row of 16 adds what the rows before it hold.
+__device__ __forceinline__ float wave_total(float v) {
+    v += xor_lane_row<1>(v);
+    v += xor_lane_row<2>(v);
+    v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, false));  // (quads hold one value)
+    v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, false));
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x142, 0xA, 0xF, false));  // row_bcast:15
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x143, 0xC, 0xF, false));  // row_bcast:31
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
 // The row's sum of N values a thread: over a wave, then over the row's waves by way of LDS (in wave order; `red` is the
 // reduction's own, so one barrier does).
 template <int TPR, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[N]) {
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-        v[k] += xor_lane_row<1>(v[k]);
-        v[k] += xor_lane_row<2>(v[k]);
-        v[k] += xor_lane_row<4>(v[k]);
-        v[k] += xor_lane_row<8>(v[k]);
-        v[k] += __shfl_xor(v[k], 16);
-        v[k] += __shfl_xor(v[k], 32);
-    }
+    for (int k = 0; k < N; k++) v[k] = wave_total(v[k]);
     if constexpr (TPR > 64) {
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0)
@@ -51,10 +55,10 @@ __device__ __forceinline__ void *row_at(void *p, size_t row, int width, int dt) 
 }
 
 // A row's gate: 8 values of a thread.
-template <int DT>
+template <int DT, bool WHOLE>
 __device__ __forceinline__ void gate8(const void *gate, int kind, int gate_dtype, size_t row, uint32_t c, uint32_t width, float (&g)[8]) {
-    if (kind == GATE_CHANNEL) load8_any(gate, gate_dtype, c, width, g);
-    else if (kind == GATE_FULL) load8<DT>(row_at(gate, row, width, DT), c, width, g);
+    if (kind == GATE_CHANNEL) load8_any<WHOLE>(gate, gate_dtype, c, width, g);
+    else if (kind == GATE_FULL) load8<DT, WHOLE>(row_at(gate, row, width, DT), c, width, g);
     else {
         const float v = kind == GATE_ROW ? load_any(gate, gate_dtype, row) : 1.f;
 #pragma unroll
@@ -65,7 +69,7 @@ __device__ __forceinline__ void gate8(const void *gate, int kind, int gate_dtype
 constexpr int norm_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 // A row by TPR threads (a wave's, or a workgroup's), each NV vectors of 8.
-template <int DT, int HT, int TPR, int NV>
+template <int DT, int HT, int TPR, int NV, bool WHOLE>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
     constexpr int ROWS = norm_threads(TPR) / TPR;
     const int t = threadIdx.x & (TPR - 1);
@@ -76,9 +80,10 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
     float n[NV][8], s[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        load8<DT>(y, (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
-        if (h) load8<HT>(h, (uint32_t)(i * TPR + t) * 8, a.width, s[i]);
+        load8<DT, WHOLE>(y, (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
+        if (h) load8<HT, WHOLE>(h, (uint32_t)(i * TPR + t) * 8, a.width, s[i]);
     }
+    const float inv_width = 1.f / (float)a.width;
     float f = 1.f;
     if (a.post) {
         float sum[1] = {0.f};
@@ -87,19 +92,19 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
 #pragma unroll
             for (int q = 0; q < 8; q++) sum[0] += n[i][q] * n[i][q];
         row_sum<TPR, 1>(sum, red[0]);
-        f = 1.f / sqrtf(sum[0] / (float)a.width + a.eps);
+        f = __builtin_amdgcn_rsqf(sum[0] * inv_width + a.eps);
     }
     float sum[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         float w[8];
         if (a.post) {
-            load8_any(a.post, a.post_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+            load8_any<WHOLE>(a.post, a.post_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
 #pragma unroll
             for (int q = 0; q < 8; q++) n[i][q] *= f * (a.offset + w[q]);
         }
         if (a.gate_kind != GATE_NONE) {
-            gate8<DT>(a.gate, a.gate_kind, a.gate_dtype, row, (uint32_t)(i * TPR + t) * 8, a.width, w);
+            gate8<DT, WHOLE>(a.gate, a.gate_kind, a.gate_dtype, row, (uint32_t)(i * TPR + t) * 8, a.width, w);
 #pragma unroll
             for (int q = 0; q < 8; q++) n[i][q] *= w[q];
         }
@@ -109,38 +114,39 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
             if (h) n[i][q] += a.residual_scale * s[i][q];
             sum[0] += n[i][q] * n[i][q];
         }
-        store8<HT>(row_at(a.h_out, row, a.width, HT), (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
+        store8<HT, WHOLE>(row_at(a.h_out, row, a.width, HT), (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
     }
     if (!a.pre) return;
     row_sum<TPR, 1>(sum, red[1]);
-    f = 1.f / sqrtf(sum[0] / (float)a.width + a.eps);
+    f = __builtin_amdgcn_rsqf(sum[0] * inv_width + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         float w[8];
-        load8_any(a.pre, a.pre_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+        load8_any<WHOLE>(a.pre, a.pre_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
 #pragma unroll
         for (int q = 0; q < 8; q++) n[i][q] *= f * (a.offset + w[q]);
-        store8<DT>(row_at(a.x_out, row, a.width, DT), (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
+        store8<DT, WHOLE>(row_at(a.x_out, row, a.width, DT), (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
     }
 }
 
-// The gradient.  A workgroup takes rows blockIdx.x, + gridDim.x, ..., keeps its columns' sums (dpre, dpost, a channel gate's)
-// in registers (up to 16 a thread) or in its part, and leaves them there for the join.
-template <int DT, int HT, int TPR, int NV>
-__global__ __launch_bounds__(TPR) void norm_backward_kernel(NormGradArgs a) {
+// The gradient.  A workgroup takes rows blockIdx.x, + gridDim.x, ..., with the next row's values in flight, and keeps its columns'
+// sums (dpre, dpost, a channel gate's) in registers, up to 16 a thread, or in its part, and leaves them there for the join.
+template <int DT, int HT, int TPR, int NV, bool WHOLE, bool CHANNEL>
+__global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && (WHOLE || !CHANNEL) ? 4 : 2) void norm_backward_kernel(NormGradArgs a) {
+    constexpr bool REGS = NV <= 2, AHEAD = NV == 1;
     const int t = threadIdx.x;
-    __shared__ float red[2][TPR / 64][3], red2[2][TPR / 64][2];
+    __shared__ float red[2][TPR / 64][3], red2[2][TPR / 64][1];
     const float inv_width = 1.f / (float)a.width;
-    const bool channel = a.gate_kind == GATE_CHANNEL;
+    const int gate_kind = CHANNEL ? GATE_CHANNEL : a.gate_kind;
     // this workgroup's sums, one after another as they are wanted
-    const int sums = (a.pre != nullptr) + (a.post != nullptr) + channel;
+    const int sums = (a.pre != nullptr) + (a.post != nullptr) + CHANNEL;
     float *part = a.part + (size_t)blockIdx.x * sums * a.width;
     float *part_post = part + (a.pre ? a.width : 0), *part_gate = part_post + (a.post ? a.width : 0);
-    constexpr bool REGS = NV <= 2;
     using Acc = float[REGS ? NV : 1][8];
     Acc acc_pre = {}, acc_post = {}, acc_gate = {};
     bool first = true;
     int flip = 0;
+    auto col = [&](int i) { return (uint32_t)(i * TPR + t) * 8; };
     auto add = [&](Acc &acc, float *at, int i, const float (&v)[8]) {
         if constexpr (REGS) {
 #pragma unroll
@@ -148,126 +154,163 @@ __global__ __launch_bounds__(TPR) void norm_backward_kernel(NormGradArgs a) {
         } else {
             float o[8];
             if (first) {
-                store8<DT_F32>(at, (uint32_t)(i * TPR + t) * 8, a.width, v);
+                store8<DT_F32, WHOLE>(at, col(i), a.width, v);
                 return;
             }
-            load8<DT_F32>(at, (uint32_t)(i * TPR + t) * 8, a.width, o);
+            load8<DT_F32, WHOLE>(at, col(i), a.width, o);
 #pragma unroll
             for (int q = 0; q < 8; q++) o[q] += v[q];
-            store8<DT_F32>(at, (uint32_t)(i * TPR + t) * 8, a.width, o);
+            store8<DT_F32, WHOLE>(at, col(i), a.width, o);
         }
     };
-    for (size_t row = blockIdx.x; row < (size_t)a.rows; row += gridDim.x, first = false, flip ^= 1) {
-        const void *py = row_at(a.y, row, a.width, DT), *ph = row_at(a.h, row, a.width, HT);
-        const void *pdh = row_at(a.dh, row, a.width, HT), *pdx = row_at(a.dx, row, a.width, DT);
-        float y[NV][8], H[NV][8], h[REGS ? NV : 1][8], dx[REGS ? NV : 1][8];  // (past 16 values a thread h and dx are read twice)
+    // the weights with their offset, kept where a thread has eight columns
+    float wpre[8], wpost[8], wgate[8];
+    auto pre_of = [&](int i, bool now) {
+        if (AHEAD != now) return;
+        load8_any<WHOLE>(a.pre, a.pre_dtype, col(i), a.width, wpre);
+#pragma unroll
+        for (int q = 0; q < 8; q++) wpre[q] += a.offset;
+    };
+    auto post_of = [&](int i, bool now) {
+        if (AHEAD != now) return;
+        if (a.post) load8_any<WHOLE>(a.post, a.post_dtype, col(i), a.width, wpost);
+#pragma unroll
+        for (int q = 0; q < 8; q++) wpost[q] = a.post ? wpost[q] + a.offset : 1.f;
+    };
+    if constexpr (AHEAD) {
+        if (a.pre) pre_of(0, true);
+        post_of(0, true);
+        if (CHANNEL) load8_any<WHOLE>(a.gate, a.gate_dtype, col(0), a.width, wgate);
+    }
+    struct Row {
+        Raw8<DT> y[NV], dx[REGS ? NV : 1];
+        Raw8<HT> dh[1], h[REGS ? NV : 1];
+    };
+    auto fetch = [&](size_t row, Row &r) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            load8<DT>(py, (uint32_t)(i * TPR + t) * 8, a.width, y[i]);
-            if (pdh) load8<HT>(pdh, (uint32_t)(i * TPR + t) * 8, a.width, H[i]);
-            else
-#pragma unroll
-                for (int q = 0; q < 8; q++) H[i][q] = 0.f;
+            load_raw<DT, WHOLE>(row_at(a.y, row, a.width, DT), col(i), a.width, r.y[i]);
+            if (AHEAD && a.dh) load_raw<HT, WHOLE>(row_at(a.dh, row, a.width, HT), col(i), a.width, r.dh[0]);
             if (REGS && a.pre) {
-                load8<HT>(ph, (uint32_t)(i * TPR + t) * 8, a.width, h[i % (REGS ? NV : 1)]);
-                load8<DT>(pdx, (uint32_t)(i * TPR + t) * 8, a.width, dx[i % (REGS ? NV : 1)]);
+                load_raw<HT, WHOLE>(row_at(a.h, row, a.width, HT), col(i), a.width, r.h[i % (REGS ? NV : 1)]);
+                load_raw<DT, WHOLE>(row_at(a.dx, row, a.width, DT), col(i), a.width, r.dx[i % (REGS ? NV : 1)]);
             }
         }
+    };
+    Row now;
+    if constexpr (AHEAD) fetch(blockIdx.x, now);
+    for (size_t row = blockIdx.x; row < (size_t)a.rows; row += gridDim.x, first = false, flip ^= 1) {
         auto again = [&](int i) -> int {  // where vector i of h and dx is
             if constexpr (REGS) return i;
-            load8<HT>(ph, (uint32_t)(i * TPR + t) * 8, a.width, h[0]);
-            load8<DT>(pdx, (uint32_t)(i * TPR + t) * 8, a.width, dx[0]);
+            load_raw<HT, WHOLE>(row_at(a.h, row, a.width, HT), col(i), a.width, now.h[0]);
+            load_raw<DT, WHOLE>(row_at(a.dx, row, a.width, DT), col(i), a.width, now.dx[0]);
             return 0;
         };
+        if constexpr (!AHEAD) fetch(row, now);
+        const float row_gate = gate_kind == GATE_ROW ? load_any(a.gate, a.gate_dtype, row) : 1.f;
+        Raw8<DT> y[NV];
+        float H[NV][8];
+        auto now_y = [&](int i, int q) { return y[i].get(q); };
         float s[3] = {0.f, 0.f, 0.f};  // of h'^2, u h', y^2
 #pragma unroll
         for (int i = 0; i < NV; i++) {
+#pragma unroll
+            for (int q = 0; q < 8; q++) H[i][q] = AHEAD && a.dh ? now.dh[0].get(q) : 0.f;
+            if (!AHEAD && a.dh) load8<HT, WHOLE>(row_at(a.dh, row, a.width, HT), col(i), a.width, H[i]);
+            y[i] = now.y[i];
             if (a.pre) {
-                float w[8];
                 const int k = again(i);
-                load8_any(a.pre, a.pre_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+                pre_of(i, false);
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
-                    s[0] += h[k][q] * h[k][q];
-                    s[1] += dx[k][q] * (a.offset + w[q]) * h[k][q];
+                    const float h = now.h[k].get(q);
+                    s[0] += h * h;
+                    s[1] += now.dx[k].get(q) * wpre[q] * h;
                 }
             }
             if (a.post)
 #pragma unroll
-                for (int q = 0; q < 8; q++) s[2] += y[i][q] * y[i][q];
+                for (int q = 0; q < 8; q++) s[2] += now_y(i, q) * now_y(i, q);
+        }
+        // (a row's h and dx leave for good below where they are kept, so that the next row's may come)
+        Raw8<HT> h1 = now.h[0];
+        Raw8<DT> dx1 = now.dx[0];
+        if constexpr (AHEAD) {
+            if (row + gridDim.x < (size_t)a.rows) fetch(row + gridDim.x, now);
         }
         if (a.pre || a.post) row_sum<TPR, 3>(s, red[flip]);
-        const float r = a.pre ? 1.f / sqrtf(s[0] * inv_width + a.eps) : 0.f;
+        const float r = a.pre ? __builtin_amdgcn_rsqf(s[0] * inv_width + a.eps) : 0.f;
         const float along = r * r * (s[1] * inv_width);
-        const float qf = a.post ? 1.f / sqrtf(s[2] * inv_width + a.eps) : 1.f;
-        float s2[2] = {0.f, 0.f};  // of v y, b H n
+        const float qf = a.post ? __builtin_amdgcn_rsqf(s[2] * inv_width + a.eps) : 1.f;
+        float s2[1] = {0.f};  // of v y
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            float w[8], d[8];
+            float d[8];
             if (a.pre) {
-                const int k = again(i);
-                load8_any(a.pre, a.pre_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
+                const int k = AHEAD ? 0 : again(i);
+                pre_of(i, false);
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
-                    H[i][q] += r * (dx[k][q] * (a.offset + w[q]) - h[k][q] * along);
-                    d[q] = dx[k][q] * (h[k][q] * r);
+                    const float h = AHEAD ? h1.get(q) : now.h[k].get(q), dx = AHEAD ? dx1.get(q) : now.dx[k].get(q);
+                    H[i][q] += r * (dx * wpre[q] - h * along);
+                    d[q] = dx * (h * r);
                 }
                 add(acc_pre, part, i, d);
             }
             if (a.dres) {
 #pragma unroll
                 for (int q = 0; q < 8; q++) d[q] = a.residual_scale * H[i][q];
-                store8<HT>(row_at(a.dres, row, a.width, HT), (uint32_t)(i * TPR + t) * 8, a.width, d);
+                store8<HT, WHOLE>(row_at(a.dres, row, a.width, HT), col(i), a.width, d);
             }
-            if (a.post) {
-                load8_any(a.post, a.post_dtype, (uint32_t)(i * TPR + t) * 8, a.width, w);
-#pragma unroll
-                for (int q = 0; q < 8; q++) w[q] += a.offset;
-            } else {
-#pragma unroll
-                for (int q = 0; q < 8; q++) w[q] = 1.f;
-            }
+            post_of(i, false);
 #pragma unroll
             for (int q = 0; q < 8; q++) H[i][q] *= a.block_scale;
-            float g[8];
-            gate8<DT>(a.gate, a.gate_kind, a.gate_dtype, row, (uint32_t)(i * TPR + t) * 8, a.width, g);
-            if (a.gate_kind != GATE_NONE) {
+            if (CHANNEL || gate_kind == GATE_FULL) {
+                float g[8];
+                if constexpr (CHANNEL && AHEAD) {
+#pragma unroll
+                    for (int q = 0; q < 8; q++) g[q] = wgate[q];
+                } else {
+                    gate8<DT, WHOLE>(a.gate, gate_kind, a.gate_dtype, row, col(i), a.width, g);
+                }
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
-                    d[q] = H[i][q] * (y[i][q] * qf * w[q]);
-                    s2[1] += d[q];
+                    d[q] = H[i][q] * (now_y(i, q) * qf * wpost[q]);
+                    H[i][q] *= g[q];
                 }
-                if (channel) add(acc_gate, part_gate, i, d);
-                if (a.gate_kind == GATE_FULL) store8<DT>(row_at(a.dgate, row, a.width, DT), (uint32_t)(i * TPR + t) * 8, a.width, d);
+                if (CHANNEL) add(acc_gate, part_gate, i, d);
+                else store8<DT, WHOLE>(row_at(a.dgate, row, a.width, DT), col(i), a.width, d);
             }
             if (a.post) {
 #pragma unroll
-                for (int q = 0; q < 8; q++) d[q] = H[i][q] * g[q] * (y[i][q] * qf);
+                for (int q = 0; q < 8; q++) {
+                    d[q] = H[i][q] * (now_y(i, q) * (qf * row_gate));
+                    H[i][q] *= wpost[q];  // v, but for the row's gate
+                    s2[0] += H[i][q] * now_y(i, q);
+                }
                 add(acc_post, part_post, i, d);
-            }
+            } else if (gate_kind == GATE_ROW) {
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-                H[i][q] *= g[q] * w[q];  // v
-                s2[0] += H[i][q] * y[i][q];
+                for (int q = 0; q < 8; q++) s2[0] += H[i][q] * now_y(i, q);
             }
         }
-        if (a.post || a.gate_kind == GATE_ROW) row_sum<TPR, 2>(s2, red2[flip]);
-        if (a.gate_kind == GATE_ROW && t == 0) static_cast<float *>(a.dgate)[row] = s2[1];
-        const float along_y = qf * qf * (s2[0] * inv_width);
+        if (a.post || gate_kind == GATE_ROW) row_sum<TPR, 1>(s2, red2[flip]);
+        // (a row's gate is a factor of the whole row: its gradient and the mean come of one sum)
+        if (gate_kind == GATE_ROW && t == 0) static_cast<float *>(a.dgate)[row] = s2[0] * qf;
+        const float along_y = qf * qf * (s2[0] * inv_width), out = qf * row_gate;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            if (a.post)
 #pragma unroll
-                for (int q = 0; q < 8; q++) H[i][q] = qf * (H[i][q] - y[i][q] * along_y);
-            store8<DT>(row_at(a.dy, row, a.width, DT), (uint32_t)(i * TPR + t) * 8, a.width, H[i]);
+            for (int q = 0; q < 8; q++) H[i][q] = out * (a.post ? H[i][q] - now_y(i, q) * along_y : H[i][q]);
+            store8<DT, WHOLE>(row_at(a.dy, row, a.width, DT), col(i), a.width, H[i]);
         }
     }
     if constexpr (REGS) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            if (a.pre) store8<DT_F32>(part, (uint32_t)(i * TPR + t) * 8, a.width, acc_pre[i]);
-            if (a.post) store8<DT_F32>(part_post, (uint32_t)(i * TPR + t) * 8, a.width, acc_post[i]);
-            if (channel) store8<DT_F32>(part_gate, (uint32_t)(i * TPR + t) * 8, a.width, acc_gate[i]);
+            if (a.pre) store8<DT_F32, WHOLE>(part, col(i), a.width, acc_pre[i]);
+            if (a.post) store8<DT_F32, WHOLE>(part_post, col(i), a.width, acc_post[i]);
+            if (CHANNEL) store8<DT_F32, WHOLE>(part_gate, col(i), a.width, acc_gate[i]);
         }
     }
 }
@@ -280,8 +323,10 @@ __global__ __launch_bounds__(64 * NJ_WAVES) void norm_join_kernel(const float *p
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, total = sums * width, c = blockIdx.x * 64 + lane;
     __shared__ float share[NJ_WAVES][64];
     float s = 0.f;
-    if (c < total)
+    if (c < total) {
+#pragma unroll 8
         for (int p = wave; p < parts; p += NJ_WAVES) s += part[(size_t)p * total + c];
+    }
     share[wave][lane] = s;
     __syncthreads();
     if (wave || c >= total) return;
@@ -309,7 +354,8 @@ hipError_t run_norm(const NormArgs &a, hipStream_t s) {
         auto go = [&](auto TPR, auto NV) {
             constexpr int tpr = decltype(TPR)::value, nv = decltype(NV)::value, rows = norm_threads(tpr) / tpr;
             const dim3 grid((unsigned)(((long)a.rows + rows - 1) / rows)), block(norm_threads(tpr));
-            hipLaunchKernelGGL((norm_kernel<dt, ht, tpr, nv>), grid, block, 0, s, a);
+            if (a.width % 8 == 0) hipLaunchKernelGGL((norm_kernel<dt, ht, tpr, nv, true>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((norm_kernel<dt, ht, tpr, nv, false>), grid, block, 0, s, a);
             return hipGetLastError();
         };
         using std::integral_constant;
@@ -326,8 +372,15 @@ hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
         constexpr int dt = decltype(DT)::value, ht = decltype(HT)::value;
         auto go = [&](auto TPR, auto NV) {
             constexpr int tpr = decltype(TPR)::value, nv = decltype(NV)::value;
-            hipLaunchKernelGGL((norm_backward_kernel<dt, ht, tpr, nv>), dim3(a.parts), dim3(tpr), 0, s, a);
-            return hipGetLastError();
+            auto kernel = [&](auto WHOLE, auto CHANNEL) {
+                hipLaunchKernelGGL((norm_backward_kernel<dt, ht, tpr, nv, decltype(WHOLE)::value, decltype(CHANNEL)::value>), dim3(a.parts),
+                                   dim3(tpr), 0, s, a);
+                return hipGetLastError();
+            };
+            const bool whole = a.width % 8 == 0;
+            using std::true_type, std::false_type;
+            if (a.gate_kind == GATE_CHANNEL) return whole ? kernel(true_type{}, true_type{}) : kernel(false_type{}, true_type{});
+            return whole ? kernel(true_type{}, false_type{}) : kernel(false_type{}, false_type{});
         };
         using std::integral_constant;
         if (a.width <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});

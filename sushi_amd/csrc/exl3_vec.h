@@ -91,35 +91,46 @@ struct Raw8 {
     }
 };
 
-// Values c .. c + 7 of an array from p on; zeros from `width` on.
-template <int DT>
-__device__ __forceinline__ void load8(const void *p, uint32_t c, uint32_t width, float (&v)[8]) {
-    if (c + 8 <= width) {
-        Raw8<DT> r;
-        r.load(elem<DT>(p, c));
-#pragma unroll
-        for (int q = 0; q < 8; q++) v[q] = r.get(q);
-    } else {
-#pragma unroll
-        for (int q = 0; q < 8; q++) v[q] = c + q < width ? load_act<DT>(elem<DT>(p, c), q) : 0.f;
-    }
-}
-__device__ __forceinline__ void load8_any(const void *p, int dt, uint32_t c, uint32_t width, float (&v)[8]) {
-    if (dt == DT_F16) load8<DT_F16>(p, c, width, v);
-    else if (dt == DT_BF16) load8<DT_BF16>(p, c, width, v);
-    else load8<DT_F32>(p, c, width, v);
+// How many of the eight values from c on lie before `width`, counted where it is asked for: in a loop over rows the masks of
+// a row's last vector would otherwise be kept in scalar registers that the loop needs.
+__device__ __forceinline__ int left_of(uint32_t c, uint32_t width) {
+    int n = max(0, (int)(width - c));
+    asm volatile("" : "+v"(n));
+    return n;
 }
 
-template <int DT>
+// Values c .. c + 7 of an array from p on; zeros from `width` on.  WHOLE: the width is a multiple of eight, so a vector lies
+// inside or outside.
+template <int DT, bool WHOLE>
+__device__ __forceinline__ void load_raw(const void *p, uint32_t c, uint32_t width, Raw8<DT> &r) {
+    if (WHOLE ? c < width : c + 8 <= width) r.load(elem<DT>(p, c));
+    else r.load_some(elem<DT>(p, c), WHOLE ? 0 : left_of(c, width));
+}
+template <int DT, bool WHOLE = false>
+__device__ __forceinline__ void load8(const void *p, uint32_t c, uint32_t width, float (&v)[8]) {
+    Raw8<DT> r;
+    load_raw<DT, WHOLE>(p, c, width, r);
+#pragma unroll
+    for (int q = 0; q < 8; q++) v[q] = r.get(q);
+}
+template <bool WHOLE = false>
+__device__ __forceinline__ void load8_any(const void *p, int dt, uint32_t c, uint32_t width, float (&v)[8]) {
+    if (dt == DT_F16) load8<DT_F16, WHOLE>(p, c, width, v);
+    else if (dt == DT_BF16) load8<DT_BF16, WHOLE>(p, c, width, v);
+    else load8<DT_F32, WHOLE>(p, c, width, v);
+}
+
+template <int DT, bool WHOLE = false>
 __device__ __forceinline__ void store8(void *p, uint32_t c, uint32_t width, const float (&v)[8]) {
-    if (c + 8 <= width) {
+    if (WHOLE ? c < width : c + 8 <= width) {
         Raw8<DT> r;
         r.set(v);
         r.store(elem<DT>(p, c));
-    } else {
+    } else if (!WHOLE) {
+        const int n = left_of(c, width);
 #pragma unroll
         for (int q = 0; q < 8; q++)
-            if (c + q < width) store_act<DT>(elem<DT>(p, c), q, v[q]);
+            if (q < n) store_act<DT>(elem<DT>(p, c), q, v[q]);
     }
 }
 
