@@ -2020,12 +2020,8 @@ int32_t exl3_clip_grad_norm(int32_t count, const void *const *grads, const int64
         for (; next < count && t.count < kClipTensors; next++) {
             if (!numel[next]) continue;
             const int k = t.count++;
-            t.g[k] = grads[next];
-            t.out[k] = out ? out[next] : const_cast<void *>(grads[next]);
-            t.n[k] = numel[next];
-            t.first[k] = t.chunks;
-            t.dtype[k] = (uint8_t)dtypes[next];
-            t.out_dtype[k] = (uint8_t)(out ? out_dtypes[next] : dtypes[next]);
+            t.e[k] = {grads[next], out ? out[next] : const_cast<void *>(grads[next]), numel[next], t.chunks, (uint8_t)dtypes[next],
+                      (uint8_t)(out ? out_dtypes[next] : dtypes[next])};
             t.chunks += (int32_t)((numel[next] + kClipChunk - 1) / kClipChunk);
         }
     };

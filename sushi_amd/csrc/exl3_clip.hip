@@ -1,66 +1,69 @@
 // The clip of many gradients by their global norm: norm = sqrt(sum of all g^2), scale = norm <= max_norm ? 1 : max_norm / norm,
 // out = g scale.  Two passes over the gradients, as the scale needs every one of them; each is bound by its bytes.
 //
-// The tensors of a launch come as arguments.  They are cut into chunks of kClipChunk elements, numbered over the launch, and
-// workgroup b takes chunks b, b + gridDim.x, ...  Squares are summed in 64 bits (an f32's square passes f32's range at 2e19),
-// a workgroup's in a fixed order into its part, and the last workgroup to arrive in the last launch sums the parts in theirs.
-#include "exl3_kernels.h"
+// The tensors of a launch come as arguments.  They are cut into chunks of kClipChunk elements, numbered over the launch, and a
+// workgroup takes a run of them, so that it looks for its tensor once for each that it touches.  Squares are summed in 64 bits
+// (an f32's square passes f32's range at 2e19), a workgroup's in a fixed order into its part, and the last workgroup to arrive
+// in the last launch sums the parts in theirs.
+#include "exl3_vec.h"
 
 namespace exl3 {
 
 constexpr int CL_THREADS = 256;
+constexpr int CL_AHEAD = 4;  // vectors of eight that a thread has in flight
+constexpr int CL_STEP = CL_THREADS * 8 * CL_AHEAD;
 
-// The tensor of chunk c: the last whose first chunk is not past it (tensors without elements have no chunks).
+// The tensor of chunk c: the last whose first chunk is not past it (tensors without elements are left out).
 __device__ __forceinline__ int tensor_of(const ClipTensors &t, int c) {
     const int lane = threadIdx.x & 63;
     int before = 0;
 #pragma unroll
-    for (int i = 0; i < kClipTensors; i += 64) before += __popcll(__ballot(i + lane < t.count && t.first[min(i + lane, kClipTensors - 1)] <= c));
+    for (int i = 0; i < kClipTensors; i += 64)
+        before += __popcll(__ballot(i + lane < t.count && t.e[min(i + lane, kClipTensors - 1)].first <= c));
     return __builtin_amdgcn_readfirstlane(before - 1);
 }
 
-template <int DT>
-struct Vec {
-    static constexpr int N = DT == DT_F32 ? 4 : 8;  // elements of a 16-byte load
-    static __device__ __forceinline__ void load(const void *p, int64_t i, float (&v)[N]) {
-        if constexpr (DT == DT_F32) {
-            const float4 u = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-            v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if constexpr (DT == DT_F16) v[2 * q] = h2f((uint16_t)w[q]), v[2 * q + 1] = h2f((uint16_t)(w[q] >> 16));
-                else v[2 * q] = __uint_as_float(w[q] << 16), v[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
-            }
-        }
+// Calls f(entry, from, end) for the elements of each tensor in this workgroup's run of chunks.
+template <class F>
+__device__ __forceinline__ void for_run(const ClipTensors &t, F f) {
+    const int per = (t.chunks + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int last = min(t.chunks, ((int)blockIdx.x + 1) * per);
+    for (int c = (int)blockIdx.x * per; c < last;) {
+        const ClipEntry e = t.e[tensor_of(t, c)];
+        const int64_t from = (int64_t)(c - e.first) * kClipChunk, end = min(from + (int64_t)(last - c) * kClipChunk, e.n);
+        f(e, from, end);
+        c += (int)((end - from + kClipChunk - 1) / kClipChunk);
     }
-};
+}
 
 template <int DT>
-__device__ __forceinline__ double chunk_squares(const void *g, int64_t from, int64_t end) {
-    constexpr int N = Vec<DT>::N;
-    double s = 0.;
-    if (reinterpret_cast<uintptr_t>(g) % 16 == 0) {
-        int64_t i = from + (int64_t)threadIdx.x * N;
-        for (; i + N <= end; i += CL_THREADS * N) {
-            float v[N];
-            Vec<DT>::load(g, i, v);
+__device__ __forceinline__ double squares(const char *g, int64_t count) {
+    constexpr int SIZE = DT == DT_F32 ? 4 : 2;
+    double s[2] = {0., 0.};
+    int64_t i = (int64_t)threadIdx.x * 8;
+    for (; i - (int64_t)threadIdx.x * 8 + CL_STEP <= count; i += CL_STEP) {
+        Raw8<DT> r[CL_AHEAD];
 #pragma unroll
-            for (int q = 0; q < N; q++) s += (double)v[q] * (double)v[q];
-        }
-        for (; i < end; i++) {  // one thread's, the last few
-            const double v = load_act<DT>(g, i);
-            s += v * v;
-        }
-    } else {
-        for (int64_t i = from + threadIdx.x; i < end; i += CL_THREADS) {
-            const double v = load_act<DT>(g, i);
-            s += v * v;
+        for (int k = 0; k < CL_AHEAD; k++) r[k].load(g + (i + k * CL_THREADS * 8) * SIZE);
+#pragma unroll
+        for (int k = 0; k < CL_AHEAD; k++)
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const double v = r[k].get(q);
+                s[q & 1] = fma(v, v, s[q & 1]);
+            }
+    }
+    for (; i < count; i += CL_THREADS * 8) {
+        Raw8<DT> r;
+        if (i + 8 <= count) r.load(g + i * SIZE);
+        else r.load_some(g + i * SIZE, (int)(count - i));
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            const double v = r.get(q);
+            s[q & 1] = fma(v, v, s[q & 1]);
         }
     }
-    return s;
+    return s[0] + s[1];
 }
 
 __device__ __forceinline__ double workgroup_sum(double s, double *red) {
@@ -80,21 +83,18 @@ __global__ __launch_bounds__(CL_THREADS) void clip_norm_kernel(ClipTensors t, Cl
     __shared__ double red[CL_THREADS / 64];
     __shared__ int flag;
     double s = 0.;
-    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int k = tensor_of(t, c);
-        const int64_t from = (int64_t)(c - t.first[k]) * kClipChunk, end = min(from + kClipChunk, t.n[k]);
-        const int dt = t.dtype[k];
-        if (dt == DT_F16) s += chunk_squares<DT_F16>(t.g[k], from, end);
-        else if (dt == DT_BF16) s += chunk_squares<DT_BF16>(t.g[k], from, end);
-        else s += chunk_squares<DT_F32>(t.g[k], from, end);
-    }
+    for_run(t, [&](const ClipEntry &e, int64_t from, int64_t end) {
+        const char *g = static_cast<const char *>(e.g) + from * (e.dtype == DT_F32 ? 4 : 2);
+        s += e.dtype == DT_F16    ? squares<DT_F16>(g, end - from)
+             : e.dtype == DT_BF16 ? squares<DT_BF16>(g, end - from)
+                                  : squares<DT_F32>(g, end - from);
+    });
     s = workgroup_sum(s, red);
     // A part is written through to memory and read past the caches, and counted once its store is acknowledged.
     if (threadIdx.x == 0) __hip_atomic_store(a.parts + a.first_part + blockIdx.x, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     if constexpr (LAST) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
         if (threadIdx.x == 0) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             const uint32_t old = __hip_atomic_fetch_add(a.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             flag = old == gridDim.x - 1;
             if (flag) __hip_atomic_store(a.counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -102,8 +102,14 @@ __global__ __launch_bounds__(CL_THREADS) void clip_norm_kernel(ClipTensors t, Cl
         __syncthreads();
         if (!flag) return;
         s = 0.;
-        for (int p = threadIdx.x; p < a.all_parts; p += CL_THREADS)
-            s += __hip_atomic_load(a.parts + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        for (int p0 = threadIdx.x; p0 < a.all_parts; p0 += 4 * CL_THREADS) {
+            double v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                v[i] = __hip_atomic_load(a.parts + min(p0 + i * CL_THREADS, a.all_parts - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+#pragma unroll
+            for (int i = 0; i < 4; i++) s += p0 + i * CL_THREADS < a.all_parts ? v[i] : 0.;
+        }
         s = workgroup_sum(s, red);
         if (threadIdx.x == 0) {
             const double norm = sqrt(s);
@@ -118,29 +124,58 @@ __global__ __launch_bounds__(CL_THREADS) void clip_norm_kernel(ClipTensors t, Cl
     }
 }
 
+// Each vector is read by the thread that writes it, in place too.
 template <int DT, int OT>
-__device__ __forceinline__ void chunk_scale(const void *g, void *out, int64_t from, int64_t end, float scale, float rest) {
-    for (int64_t i = from + threadIdx.x; i < end; i += CL_THREADS) store_act<OT>(out, i, load_act<DT>(g, i) * scale * rest);
+__device__ __forceinline__ void scaled(const char *g, char *out, int64_t count, float scale, float rest) {
+    constexpr int SIZE = DT == DT_F32 ? 4 : 2, OSIZE = OT == DT_F32 ? 4 : 2;
+    auto times = [&](const Raw8<DT> &r, Raw8<OT> &o) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) v[q] = r.get(q) * scale * rest;
+        o.set(v);
+    };
+    int64_t i = (int64_t)threadIdx.x * 8;
+    for (; i - (int64_t)threadIdx.x * 8 + CL_STEP <= count; i += CL_STEP) {
+        Raw8<DT> r[CL_AHEAD];
+#pragma unroll
+        for (int k = 0; k < CL_AHEAD; k++) r[k].load(g + (i + k * CL_THREADS * 8) * SIZE);
+#pragma unroll
+        for (int k = 0; k < CL_AHEAD; k++) {
+            Raw8<OT> o;
+            times(r[k], o);
+            o.store(out + (i + k * CL_THREADS * 8) * OSIZE);
+        }
+    }
+    for (; i < count; i += CL_THREADS * 8) {
+        Raw8<DT> r;
+        if (i + 8 <= count) {
+            Raw8<OT> o;
+            r.load(g + i * SIZE);
+            times(r, o);
+            o.store(out + i * OSIZE);
+        } else {
+            for (int64_t j = i; j < count; j++) store_act<OT>(out, j, load_act<DT>(g, j) * scale * rest);
+        }
+    }
 }
 
 template <int DT>
-__device__ __forceinline__ void chunk_scale_to(const void *g, void *out, int ot, int64_t from, int64_t end, float scale, float rest) {
-    if (ot == DT_F16) chunk_scale<DT, DT_F16>(g, out, from, end, scale, rest);
-    else if (ot == DT_BF16) chunk_scale<DT, DT_BF16>(g, out, from, end, scale, rest);
-    else chunk_scale<DT, DT_F32>(g, out, from, end, scale, rest);
+__device__ __forceinline__ void scaled_to(const char *g, char *out, int ot, int64_t count, float scale, float rest) {
+    if (ot == DT_F16) scaled<DT, DT_F16>(g, out, count, scale, rest);
+    else if (ot == DT_BF16) scaled<DT, DT_BF16>(g, out, count, scale, rest);
+    else scaled<DT, DT_F32>(g, out, count, scale, rest);
 }
 
 __global__ __launch_bounds__(CL_THREADS) void clip_scale_kernel(ClipTensors t, const float *factors) {
     const float scale = factors[0], rest = factors[1];
-    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int k = tensor_of(t, c);
-        if (scale == 1.f && t.g[k] == t.out[k]) continue;  // in place there is nothing to do
-        const int64_t from = (int64_t)(c - t.first[k]) * kClipChunk, end = min(from + kClipChunk, t.n[k]);
-        const int dt = t.dtype[k];
-        if (dt == DT_F16) chunk_scale_to<DT_F16>(t.g[k], t.out[k], t.out_dtype[k], from, end, scale, rest);
-        else if (dt == DT_BF16) chunk_scale_to<DT_BF16>(t.g[k], t.out[k], t.out_dtype[k], from, end, scale, rest);
-        else chunk_scale_to<DT_F32>(t.g[k], t.out[k], t.out_dtype[k], from, end, scale, rest);
-    }
+    for_run(t, [&](const ClipEntry &e, int64_t from, int64_t end) {
+        if (scale == 1.f && e.g == e.out) return;  // in place there is nothing to do
+        const char *g = static_cast<const char *>(e.g) + from * (e.dtype == DT_F32 ? 4 : 2);
+        char *out = static_cast<char *>(e.out) + from * (e.out_dtype == DT_F32 ? 4 : 2);
+        if (e.dtype == DT_F16) scaled_to<DT_F16>(g, out, e.out_dtype, end - from, scale, rest);
+        else if (e.dtype == DT_BF16) scaled_to<DT_BF16>(g, out, e.out_dtype, end - from, scale, rest);
+        else scaled_to<DT_F32>(g, out, e.out_dtype, end - from, scale, rest);
+    });
 }
 
 hipError_t run_clip_norm(const ClipTensors &t, const ClipArgs &a, bool last, hipStream_t s) {
@@ -151,7 +186,7 @@ hipError_t run_clip_norm(const ClipTensors &t, const ClipArgs &a, bool last, hip
 }
 
 hipError_t run_clip_scale(const ClipTensors &t, const float *factors, hipStream_t s) {
-    hipLaunchKernelGGL(clip_scale_kernel, dim3((unsigned)(t.chunks < 4096 ? t.chunks : 4096)), dim3(CL_THREADS), 0, s, t, factors);
+    hipLaunchKernelGGL(clip_scale_kernel, dim3((unsigned)clip_parts(t.chunks)), dim3(CL_THREADS), 0, s, t, factors);
     return hipGetLastError();
 }
 

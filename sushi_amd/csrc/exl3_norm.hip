@@ -132,7 +132,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
 // The gradient.  A workgroup takes rows blockIdx.x, + gridDim.x, ..., with the next row's values in flight, and keeps its columns'
 // sums (dpre, dpost, a channel gate's) in registers, up to 16 a thread, or in its part, and leaves them there for the join.
 template <int DT, int HT, int TPR, int NV, bool WHOLE, bool CHANNEL>
-__global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && (WHOLE || !CHANNEL) ? 4 : 2) void norm_backward_kernel(NormGradArgs a) {
+__global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && !CHANNEL ? 4 : 2) void norm_backward_kernel(NormGradArgs a) {
     constexpr bool REGS = NV <= 2, AHEAD = NV == 1;
     const int t = threadIdx.x;
     __shared__ float red[2][TPR / 64][3], red2[2][TPR / 64][1];
@@ -163,25 +163,20 @@ __global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && (WHOLE || !CHANNEL)
             store8<DT_F32, WHOLE>(at, col(i), a.width, o);
         }
     };
-    // the weights with their offset, kept where a thread has eight columns
+    // the weights with their offset, kept where a thread has eight columns (their loads follow the first row's)
     float wpre[8], wpost[8], wgate[8];
-    auto pre_of = [&](int i, bool now) {
-        if (AHEAD != now) return;
+    auto pre_of = [&](int i) {
+        if constexpr (AHEAD) return;
         load8_any<WHOLE>(a.pre, a.pre_dtype, col(i), a.width, wpre);
 #pragma unroll
         for (int q = 0; q < 8; q++) wpre[q] += a.offset;
     };
-    auto post_of = [&](int i, bool now) {
-        if (AHEAD != now) return;
+    auto post_of = [&](int i) {
+        if constexpr (AHEAD) return;
         if (a.post) load8_any<WHOLE>(a.post, a.post_dtype, col(i), a.width, wpost);
 #pragma unroll
         for (int q = 0; q < 8; q++) wpost[q] = a.post ? wpost[q] + a.offset : 1.f;
     };
-    if constexpr (AHEAD) {
-        if (a.pre) pre_of(0, true);
-        post_of(0, true);
-        if (CHANNEL) load8_any<WHOLE>(a.gate, a.gate_dtype, col(0), a.width, wgate);
-    }
     struct Row {
         Raw8<DT> y[NV], dx[REGS ? NV : 1];
         Raw8<HT> dh[1], h[REGS ? NV : 1];
@@ -198,7 +193,19 @@ __global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && (WHOLE || !CHANNEL)
         }
     };
     Row now;
-    if constexpr (AHEAD) fetch(blockIdx.x, now);
+    if constexpr (AHEAD) {
+        fetch(blockIdx.x, now);
+        RawAny pre, post, gate;
+        if (a.pre) pre.load<WHOLE>(a.pre, a.pre_dtype, col(0), a.width);
+        if (a.post) post.load<WHOLE>(a.post, a.post_dtype, col(0), a.width);
+        if (CHANNEL) gate.load<WHOLE>(a.gate, a.gate_dtype, col(0), a.width);
+        if (a.pre) pre.get(a.pre_dtype, a.offset, wpre);
+        if (a.post) post.get(a.post_dtype, a.offset, wpost);
+        else
+#pragma unroll
+            for (int q = 0; q < 8; q++) wpost[q] = 1.f;
+        if (CHANNEL) gate.get(a.gate_dtype, 0.f, wgate);
+    }
     for (size_t row = blockIdx.x; row < (size_t)a.rows; row += gridDim.x, first = false, flip ^= 1) {
         auto again = [&](int i) -> int {  // where vector i of h and dx is
             if constexpr (REGS) return i;
@@ -220,7 +227,7 @@ __global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && (WHOLE || !CHANNEL)
             y[i] = now.y[i];
             if (a.pre) {
                 const int k = again(i);
-                pre_of(i, false);
+                pre_of(i);
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
                     const float h = now.h[k].get(q);
@@ -248,7 +255,7 @@ __global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && (WHOLE || !CHANNEL)
             float d[8];
             if (a.pre) {
                 const int k = AHEAD ? 0 : again(i);
-                pre_of(i, false);
+                pre_of(i);
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
                     const float h = AHEAD ? h1.get(q) : now.h[k].get(q), dx = AHEAD ? dx1.get(q) : now.dx[k].get(q);
@@ -262,7 +269,7 @@ __global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && (WHOLE || !CHANNEL)
                 for (int q = 0; q < 8; q++) d[q] = a.residual_scale * H[i][q];
                 store8<HT, WHOLE>(row_at(a.dres, row, a.width, HT), col(i), a.width, d);
             }
-            post_of(i, false);
+            post_of(i);
 #pragma unroll
             for (int q = 0; q < 8; q++) H[i][q] *= a.block_scale;
             if (CHANNEL || gate_kind == GATE_FULL) {
@@ -316,16 +323,20 @@ __global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && (WHOLE || !CHANNEL)
 }
 
 // A column's sum over the parts: the lanes of a wave hold 64 columns, the workgroup's waves a share of the parts each, in
-// order; the shares add in wave order.
-constexpr int NJ_WAVES = 16;
+// order, NJ_AHEAD loads at a time; the shares add in wave order.
+constexpr int NJ_WAVES = 16, NJ_AHEAD = 16;
 __global__ __launch_bounds__(64 * NJ_WAVES) void norm_join_kernel(const float *part, int parts, int sums, int width, float *d0, float *d1,
                                                                   float *d2) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, total = sums * width, c = blockIdx.x * 64 + lane;
     __shared__ float share[NJ_WAVES][64];
+    const float *at = part + min(c, total - 1);
     float s = 0.f;
-    if (c < total) {
-#pragma unroll 8
-        for (int p = wave; p < parts; p += NJ_WAVES) s += part[(size_t)p * total + c];
+    for (int p0 = wave; p0 < parts; p0 += NJ_WAVES * NJ_AHEAD) {
+        float v[NJ_AHEAD];
+#pragma unroll
+        for (int i = 0; i < NJ_AHEAD; i++) v[i] = at[(size_t)min(p0 + i * NJ_WAVES, parts - 1) * total];
+#pragma unroll
+        for (int i = 0; i < NJ_AHEAD; i++) s += p0 + i * NJ_WAVES < parts ? v[i] : 0.f;
     }
     share[wave][lane] = s;
     __syncthreads();
