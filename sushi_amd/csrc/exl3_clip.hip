@@ -23,16 +23,18 @@ __device__ __forceinline__ int tensor_of(const ClipTensors &t, int c) {
     return __builtin_amdgcn_readfirstlane(before - 1);
 }
 
-// Calls f(entry, from, end) for the elements of each tensor in this workgroup's run of chunks.
-template <class F>
+// Calls f(entry, from, end) for the elements of each tensor in this workgroup's run of chunks, the last tensor first if BACK.
+template <bool BACK, class F>
 __device__ __forceinline__ void for_run(const ClipTensors &t, F f) {
     const int per = (t.chunks + (int)gridDim.x - 1) / (int)gridDim.x;
-    const int last = min(t.chunks, ((int)blockIdx.x + 1) * per);
-    for (int c = (int)blockIdx.x * per; c < last;) {
-        const ClipEntry e = t.e[tensor_of(t, c)];
+    int first = min(t.chunks, (int)blockIdx.x * per), last = min(t.chunks, first + per);
+    while (first < last) {
+        const ClipEntry e = t.e[tensor_of(t, BACK ? last - 1 : first)];
+        const int c = BACK ? max(first, e.first) : first;
         const int64_t from = (int64_t)(c - e.first) * kClipChunk, end = min(from + (int64_t)(last - c) * kClipChunk, e.n);
         f(e, from, end);
-        c += (int)((end - from + kClipChunk - 1) / kClipChunk);
+        if (BACK) last = c;
+        else first += (int)((end - from + kClipChunk - 1) / kClipChunk);
     }
 }
 
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(CL_THREADS) void clip_norm_kernel(ClipTensors t, Cl
     __shared__ double red[CL_THREADS / 64];
     __shared__ int flag;
     double s = 0.;
-    for_run(t, [&](const ClipEntry &e, int64_t from, int64_t end) {
+    for_run<false>(t, [&](const ClipEntry &e, int64_t from, int64_t end) {
         const char *g = static_cast<const char *>(e.g) + from * (e.dtype == DT_F32 ? 4 : 2);
         s += e.dtype == DT_F16    ? squares<DT_F16>(g, end - from)
              : e.dtype == DT_BF16 ? squares<DT_BF16>(g, end - from)
@@ -124,7 +126,8 @@ __global__ __launch_bounds__(CL_THREADS) void clip_norm_kernel(ClipTensors t, Cl
     }
 }
 
-// Each vector is read by the thread that writes it, in place too.
+// Each vector is read by the thread that writes it, in place too.  From the end to the beginning, as the first pass read the end
+// last: what of it the memory-side cache still holds is not read from memory again.
 template <int DT, int OT>
 __device__ __forceinline__ void scaled(const char *g, char *out, int64_t count, float scale, float rest) {
     constexpr int SIZE = DT == DT_F32 ? 4 : 2, OSIZE = OT == DT_F32 ? 4 : 2;
@@ -134,8 +137,19 @@ __device__ __forceinline__ void scaled(const char *g, char *out, int64_t count, 
         for (int q = 0; q < 8; q++) v[q] = r.get(q) * scale * rest;
         o.set(v);
     };
-    int64_t i = (int64_t)threadIdx.x * 8;
-    for (; i - (int64_t)threadIdx.x * 8 + CL_STEP <= count; i += CL_STEP) {
+    const int64_t whole = count / CL_STEP * CL_STEP;
+    for (int64_t i = whole + (int64_t)threadIdx.x * 8; i < count; i += CL_THREADS * 8) {
+        if (i + 8 <= count) {
+            Raw8<DT> r;
+            Raw8<OT> o;
+            r.load(g + i * SIZE);
+            times(r, o);
+            o.store(out + i * OSIZE);
+        } else {
+            for (int64_t j = i; j < count; j++) store_act<OT>(out, j, load_act<DT>(g, j) * scale * rest);
+        }
+    }
+    for (int64_t i = whole - CL_STEP + (int64_t)threadIdx.x * 8; i >= 0; i -= CL_STEP) {
         Raw8<DT> r[CL_AHEAD];
 #pragma unroll
         for (int k = 0; k < CL_AHEAD; k++) r[k].load(g + (i + k * CL_THREADS * 8) * SIZE);
@@ -144,17 +158,6 @@ __device__ __forceinline__ void scaled(const char *g, char *out, int64_t count, 
             Raw8<OT> o;
             times(r[k], o);
             o.store(out + (i + k * CL_THREADS * 8) * OSIZE);
-        }
-    }
-    for (; i < count; i += CL_THREADS * 8) {
-        Raw8<DT> r;
-        if (i + 8 <= count) {
-            Raw8<OT> o;
-            r.load(g + i * SIZE);
-            times(r, o);
-            o.store(out + i * OSIZE);
-        } else {
-            for (int64_t j = i; j < count; j++) store_act<OT>(out, j, load_act<DT>(g, j) * scale * rest);
         }
     }
 }
@@ -168,7 +171,7 @@ __device__ __forceinline__ void scaled_to(const char *g, char *out, int ot, int6
 
 __global__ __launch_bounds__(CL_THREADS) void clip_scale_kernel(ClipTensors t, const float *factors) {
     const float scale = factors[0], rest = factors[1];
-    for_run(t, [&](const ClipEntry &e, int64_t from, int64_t end) {
+    for_run<true>(t, [&](const ClipEntry &e, int64_t from, int64_t end) {
         if (scale == 1.f && e.g == e.out) return;  // in place there is nothing to do
         const char *g = static_cast<const char *>(e.g) + from * (e.dtype == DT_F32 ? 4 : 2);
         char *out = static_cast<char *>(e.out) + from * (e.out_dtype == DT_F32 ? 4 : 2);
