@@ -26,12 +26,12 @@ __device__ __forceinline__ float wave_total(float v) {
 }
 
 // The row's sum of N values a thread: over a wave, then over the row's waves by way of LDS (in wave order; `red` is the
-// reduction's own, so one barrier does).
-template <int TPR, int N>
+// reduction's own, so one barrier does; what of it stands for waves that the workgroup has not is zero).
+template <int MAXT, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[N]) {
 #pragma unroll
     for (int k = 0; k < N; k++) v[k] = wave_total(v[k]);
-    if constexpr (TPR > 64) {
+    if constexpr (MAXT > 64) {
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
@@ -41,7 +41,7 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[N]) {
         for (int k = 0; k < N; k++) {
             float s = red[0][k];
 #pragma unroll
-            for (int w = 1; w < TPR / 64; w++) s += red[w][k];
+            for (int w = 1; w < MAXT / 64; w++) s += red[w][k];
             v[k] = s;
         }
     }
@@ -66,16 +66,17 @@ __device__ __forceinline__ void gate8(const void *gate, int kind, int gate_dtype
     }
 }
 
-constexpr int norm_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
-
-// A row by TPR threads (a wave's, or a workgroup's), each NV vectors of 8.
-template <int DT, int HT, int TPR, int NV, bool WHOLE>
-__global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
-    constexpr int ROWS = norm_threads(TPR) / TPR;
-    const int t = threadIdx.x & (TPR - 1);
-    const size_t row = (size_t)blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
-    __shared__ float red[2][TPR / 64][1];
-    if (TPR == 64 && row >= (size_t)a.rows) return;  // a wave's row; else the grid is the rows
+// A row by TPR threads (a wave, or a workgroup of up to MAXT), each NV vectors of 8.
+template <int DT, int HT, int MAXT, int NV, bool WHOLE>
+__global__ __launch_bounds__(MAXT == 64 ? 256 : MAXT) void norm_kernel(NormArgs a) {
+    const int TPR = MAXT == 64 ? 64 : blockDim.x, t = MAXT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const size_t row = MAXT == 64 ? (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+    __shared__ float red[2][MAXT / 64][1];
+    if (MAXT == 64 && row >= (size_t)a.rows) return;  // a wave's row; else the grid is the rows
+    if (MAXT > 64) {
+        if (threadIdx.x < 2 * MAXT / 64) (&red[0][0][0])[threadIdx.x] = 0.f;
+        __syncthreads();
+    }
     const void *y = row_at(a.y, row, a.width, DT), *h = row_at(a.h, row, a.width, HT);
     float n[NV][8], s[NV][8];
 #pragma unroll
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
         for (int i = 0; i < NV; i++)
 #pragma unroll
             for (int q = 0; q < 8; q++) sum[0] += n[i][q] * n[i][q];
-        row_sum<TPR, 1>(sum, red[0]);
+        row_sum<MAXT, 1>(sum, red[0]);
         f = __builtin_amdgcn_rsqf(sum[0] * inv_width + a.eps);
     }
     float sum[1] = {0.f};
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
         store8<HT, WHOLE>(row_at(a.h_out, row, a.width, HT), (uint32_t)(i * TPR + t) * 8, a.width, n[i]);
     }
     if (!a.pre) return;
-    row_sum<TPR, 1>(sum, red[1]);
+    row_sum<MAXT, 1>(sum, red[1]);
     f = __builtin_amdgcn_rsqf(sum[0] * inv_width + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; i++) {
@@ -131,11 +132,16 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(NormArgs a) {
 
 // The gradient.  A workgroup takes rows blockIdx.x, + gridDim.x, ..., with the next row's values in flight, and keeps its columns'
 // sums (dpre, dpost, a channel gate's) in registers, up to 16 a thread, or in its part, and leaves them there for the join.
-template <int DT, int HT, int TPR, int NV, bool WHOLE, bool CHANNEL>
-__global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && !CHANNEL ? 4 : 2) void norm_backward_kernel(NormGradArgs a) {
+template <int DT, int HT, int MAXT, int NV, bool WHOLE, bool CHANNEL>
+__global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CHANNEL ? 4 : 2) void norm_backward_kernel(NormGradArgs a) {
     constexpr bool REGS = NV <= 2, AHEAD = NV == 1;
-    const int t = threadIdx.x;
-    __shared__ float red[2][TPR / 64][3], red2[2][TPR / 64][1];
+    const int t = threadIdx.x, TPR = blockDim.x;
+    __shared__ float red[2][MAXT / 64][3], red2[2][MAXT / 64][1];
+    if (MAXT > 64) {
+        for (int i = t; i < 6 * MAXT / 64; i += TPR) (&red[0][0][0])[i] = 0.f;
+        if (t < 2 * MAXT / 64) (&red2[0][0][0])[t] = 0.f;
+        __syncthreads();
+    }
     const float inv_width = 1.f / (float)a.width;
     const int gate_kind = CHANNEL ? GATE_CHANNEL : a.gate_kind;
     // this workgroup's sums, one after another as they are wanted
@@ -245,7 +251,7 @@ __global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && !CHANNEL ? 4 : 2) v
         if constexpr (AHEAD) {
             if (row + gridDim.x < (size_t)a.rows) fetch(row + gridDim.x, now);
         }
-        if (a.pre || a.post) row_sum<TPR, 3>(s, red[flip]);
+        if (a.pre || a.post) row_sum<MAXT, 3>(s, red[flip]);
         const float r = a.pre ? __builtin_amdgcn_rsqf(s[0] * inv_width + a.eps) : 0.f;
         const float along = r * r * (s[1] * inv_width);
         const float qf = a.post ? __builtin_amdgcn_rsqf(s[2] * inv_width + a.eps) : 1.f;
@@ -301,7 +307,7 @@ __global__ __launch_bounds__(TPR, NV == 1 && HT != DT_F32 && !CHANNEL ? 4 : 2) v
                 for (int q = 0; q < 8; q++) s2[0] += H[i][q] * now_y(i, q);
             }
         }
-        if (a.post || gate_kind == GATE_ROW) row_sum<TPR, 1>(s2, red2[flip]);
+        if (a.post || gate_kind == GATE_ROW) row_sum<MAXT, 1>(s2, red2[flip]);
         // (a row's gate is a factor of the whole row: its gradient and the mean come of one sum)
         if (gate_kind == GATE_ROW && t == 0) static_cast<float *>(a.dgate)[row] = s2[0] * qf;
         const float along_y = qf * qf * (s2[0] * inv_width), out = qf * row_gate;
@@ -346,8 +352,6 @@ __global__ __launch_bounds__(64 * NJ_WAVES) void norm_join_kernel(const float *p
     (k == 0 ? d0 : k == 1 ? d1 : d2)[c - k * width] = s;
 }
 
-int norm_backward_parts(int rows, int width) { return rows < 512 ? rows : 512; }
-
 template <class F>
 static hipError_t with_types(int dt, int ht, F f) {
     using std::integral_constant;
@@ -359,33 +363,46 @@ static hipError_t with_types(int dt, int ht, F f) {
                         : f(integral_constant<int, DT_BF16>{}, integral_constant<int, DT_BF16>{});
 }
 
+// The threads of a row of `width` values at nv vectors each, in whole waves.
+static int row_threads(int width, int nv) { return (width + 512 * nv - 1) / (512 * nv) * 64; }
+
 hipError_t run_norm(const NormArgs &a, hipStream_t s) {
     return with_types(a.dtype, a.hdtype, [&](auto DT, auto HT) {
         constexpr int dt = decltype(DT)::value, ht = decltype(HT)::value;
-        auto go = [&](auto TPR, auto NV) {
-            constexpr int tpr = decltype(TPR)::value, nv = decltype(NV)::value, rows = norm_threads(tpr) / tpr;
-            const dim3 grid((unsigned)(((long)a.rows + rows - 1) / rows)), block(norm_threads(tpr));
-            if (a.width % 8 == 0) hipLaunchKernelGGL((norm_kernel<dt, ht, tpr, nv, true>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((norm_kernel<dt, ht, tpr, nv, false>), grid, block, 0, s, a);
+        auto go = [&](auto MAXT, auto NV) {
+            constexpr int maxt = decltype(MAXT)::value, nv = decltype(NV)::value;
+            const dim3 grid((unsigned)(maxt == 64 ? ((long)a.rows + 3) / 4 : a.rows)), block(maxt == 64 ? 256 : row_threads(a.width, nv));
+            if (a.width % 8 == 0) hipLaunchKernelGGL((norm_kernel<dt, ht, maxt, nv, true>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((norm_kernel<dt, ht, maxt, nv, false>), grid, block, 0, s, a);
             return hipGetLastError();
         };
         using std::integral_constant;
         if (a.width <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
         if (a.width <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-        if (a.width <= 4096) return go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
         if (a.width <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
         return go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
     });
 }
 
+// A thread has one vector of the row up to 6144 values (12 waves: 168 registers), then two and four.
+static int backward_vectors(int width) { return width <= 6144 ? 1 : width <= 8192 ? 2 : 4; }
+
+// Workgroups of the gradient: what the CUs hold at once at a width, two workgroups of up to 8 waves each or one, and no more
+// than the rows.
+int norm_backward_parts(int rows, int width) {
+    const int waves = row_threads(width, backward_vectors(width)) / 64;
+    const int most = 256 * (waves <= 2 ? 8 : waves <= 4 ? 4 : waves <= 8 ? 2 : 1);
+    return rows < most ? rows : most;
+}
+
 hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
     hipError_t e = with_types(a.dtype, a.hdtype, [&](auto DT, auto HT) {
         constexpr int dt = decltype(DT)::value, ht = decltype(HT)::value;
-        auto go = [&](auto TPR, auto NV) {
-            constexpr int tpr = decltype(TPR)::value, nv = decltype(NV)::value;
+        auto go = [&](auto MAXT, auto NV) {
+            constexpr int maxt = decltype(MAXT)::value, nv = decltype(NV)::value;
             auto kernel = [&](auto WHOLE, auto CHANNEL) {
-                hipLaunchKernelGGL((norm_backward_kernel<dt, ht, tpr, nv, decltype(WHOLE)::value, decltype(CHANNEL)::value>), dim3(a.parts),
-                                   dim3(tpr), 0, s, a);
+                hipLaunchKernelGGL((norm_backward_kernel<dt, ht, maxt, nv, decltype(WHOLE)::value, decltype(CHANNEL)::value>), dim3(a.parts),
+                                   dim3(row_threads(a.width, nv)), 0, s, a);
                 return hipGetLastError();
             };
             const bool whole = a.width % 8 == 0;
@@ -397,6 +414,7 @@ hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
         if (a.width <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
         if (a.width <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
         if (a.width <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+        if (a.width <= 6144) return go(integral_constant<int, 768>{}, integral_constant<int, 1>{});
         if (a.width <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
         return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
     });
