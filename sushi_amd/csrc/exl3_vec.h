@@ -120,31 +120,40 @@ __device__ __forceinline__ void load8_any(const void *p, int dt, uint32_t c, uin
     else load8<DT_F32, WHOLE>(p, c, width, v);
 }
 
-// Eight values of a type known to the wave alone, as they lie in memory: loads in flight need no conversion in a branch, which
-// would wait for them.
+// Eight values of a type known to the wave alone, as they lie in memory: the conversions, which wait for the loads, come when
+// they are asked for, and the loads need no branch by the type.
 struct RawAny {
     Words4 lo, hi;
     template <bool WHOLE>
     __device__ __forceinline__ void load(const void *p, int dt, uint32_t c, uint32_t width) {
+        const bool f32 = dt == DT_F32;
+        const char *at = static_cast<const char *>(p) + c * (f32 ? 4u : 2u);
         lo = hi = Words4{0, 0, 0, 0};
-        if (dt == DT_F32) {
-            Raw8<DT_F32> r;
-            load_raw<DT_F32, WHOLE>(p, c, width, r);
-            lo = Words4{r.w[0], r.w[1], r.w[2], r.w[3]};
-            hi = Words4{r.w[4], r.w[5], r.w[6], r.w[7]};
-        } else {
-            Raw8<DT_F16> r;
-            load_raw<DT_F16, WHOLE>(p, c, width, r);
-            lo = Words4{r.w[0], r.w[1], r.w[2], r.w[3]};
+        if (WHOLE ? c < width : c + 8 <= width) {
+            lo = *reinterpret_cast<const Words4At2 *>(at);
+            if (f32) hi = reinterpret_cast<const Words4At2 *>(at)[1];
+        } else if (!WHOLE) {
+            const int n = left_of(c, width);
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                if (q >= n) continue;
+                if (!f32) lo[q / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(at)[q] << (16 * (q & 1));
+                else if (q < 4) lo[q & 3] = reinterpret_cast<const uint32_t *>(at)[q];
+                else hi[q & 3] = reinterpret_cast<const uint32_t *>(at)[q];
+            }
         }
     }
     // Plus `add`.
     __device__ __forceinline__ void get(int dt, float add, float (&v)[8]) const {
+        if (dt == DT_F32) {
 #pragma unroll
-        for (int q = 0; q < 8; q++) {
-            const uint32_t half = q & 1 ? lo[q / 2] >> 16 : lo[q / 2] & 0xFFFFu;
-            const float x = __uint_as_float(q < 4 ? lo[q & 3] : hi[q & 3]);
-            v[q] = (dt == DT_F32 ? x : dt == DT_F16 ? h2f((uint16_t)half) : __uint_as_float(half << 16)) + add;
+            for (int q = 0; q < 8; q++) v[q] = __uint_as_float(q < 4 ? lo[q & 3] : hi[q & 3]) + add;
+        } else if (dt == DT_F16) {
+#pragma unroll
+            for (int q = 0; q < 8; q++) v[q] = h2f((uint16_t)(q & 1 ? lo[q / 2] >> 16 : lo[q / 2])) + add;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; q++) v[q] = __uint_as_float(q & 1 ? lo[q / 2] & 0xFFFF0000u : lo[q / 2] << 16) + add;
         }
     }
 };
