@@ -1895,7 +1895,7 @@ int32_t exl3_block_norm(const void *y, int32_t dtype, const void *h, int32_t h_d
 
 size_t exl3_block_norm_backward_workspace_size(int32_t rows, int32_t width) {
     if (rows < 0 || width <= 0 || width > kNormMaxWidth) return 0;
-    return kZeroBytes + align_up((size_t)norm_backward_parts(rows, width) * 3 * width * sizeof(float));
+    return kZeroBytes + align_up((size_t)norm_backward_most(rows, width) * 3 * width * sizeof(float));
 }
 
 int32_t exl3_block_norm_backward(const void *dh, const void *dx, const void *y, int32_t dtype, const void *h, int32_t h_dtype,

@@ -387,12 +387,19 @@ hipError_t run_norm(const NormArgs &a, hipStream_t s) {
 // A thread has one vector of the row up to 6144 values (12 waves: 168 registers), then two and four.
 static int backward_vectors(int width) { return width <= 6144 ? 1 : width <= 8192 ? 2 : 4; }
 
-// Workgroups of the gradient: what the CUs hold at once at a width, two workgroups of up to 8 waves each or one, and no more
-// than the rows.
-int norm_backward_parts(int rows, int width) {
+// Workgroups of the gradient.  More of them hide a row's latency (1.0 us a row of 512 values, 1.5 of 4096, its loads ahead) and
+// leave more parts to the join.  One a CU up to 2048 rows (narrow rows: two), then two where two fit (narrow rows: four), each
+// the same number of rows.  us in a graph at 256 / 512 / 1024 workgroups, bf16 with both norms: 333 rows of 4096 values 11.5 / 14.7
+// / -, 2048 rows 23.9 / 22.4 / 28.7, 8192 rows 65.8 / 62.2 / 66.1; rows of 512 values: 1024 of them 9.4 / 9.0 / 10.7, 8192
+// 39.6 / 25.7 / 20.0; 8192 rows of 6144 90.1 / 94.2 / 106.3.
+int norm_backward_most(int rows, int width) {
     const int waves = row_threads(width, backward_vectors(width)) / 64;
-    const int most = 256 * (waves <= 2 ? 8 : waves <= 4 ? 4 : waves <= 8 ? 2 : 1);
-    return rows < most ? rows : most;
+    const int a_cu = waves <= 2 ? (rows >= 4096 ? 4 : rows >= 512 ? 2 : 1) : waves <= 8 && rows >= 2048 ? 2 : 1;
+    return rows < 256 * a_cu ? rows : 256 * a_cu;
+}
+int norm_backward_parts(int rows, int width) {
+    const int most = norm_backward_most(rows, width), each = most ? (rows + most - 1) / most : 1;
+    return (rows + each - 1) / each;
 }
 
 hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
