@@ -425,7 +425,8 @@ int32_t exl3_router_backward(const void *logits, int32_t dtype, int32_t rows, in
  *   (1 or 2) largest c; of their experts the topk with the largest c,
  *   score_i = scale p_i / (renormalize ? sum over the picks of p : 1).
  * Picks are listed in falling c, equal ones (and equal groups) by their number; the order is that of the values in 64 bits
- * (without bias, and with one group or group_top 1, of the logits themselves), whatever the f32 roundings of another batch.
+ * (without bias or with one that is the same for every expert, the experts' is that of their logits, and with group_top 1 the
+ * groups' too), whatever the f32 roundings of another batch.
  * An expert is out of the choice by a logit of -inf or NaN (under softmax +inf too) or a bias of -inf or NaN; a row with a
  * NaN logit (under softmax +inf too) has NaN scores.  A slot that no expert is left for, and every slot of a row that mask
  * [rows] (bytes, or null) leaves out, holds id 0xFFFFFFFF and score 0, whatever the row's logits: a dropped slot for

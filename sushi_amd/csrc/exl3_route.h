@@ -3,8 +3,8 @@
 //   of G groups of E / G experts the `taken` with the largest value (the sum of a group's one or two largest c),
 //   of their experts the k with the largest c, listed in falling order, equal ones by their number,
 //   score_i = scale p_i / (renorm ? sum over the picks of p : 1).
-// Without bias, and with one group or a group's largest c as its value, the order of c is the order of x.  A logit of -inf
-// takes its expert out; so do a bias of -inf or NaN, a NaN logit and, under softmax, +inf, and the last two make the row's
+// Without bias, or with one that is the same for every expert, the experts' order is that of x, and the groups' too where their
+// value is one c.  A logit of -inf takes its expert out; so do a bias of -inf or NaN, a NaN logit and, under softmax, +inf, and the last two make the row's
 // scores NaN.  Slots that no expert is left for, and all slots of a row that `mask` leaves out, hold 0xFFFFFFFF and 0.
 #pragma once
 #include "exl3_router.h"
@@ -48,24 +48,40 @@ __device__ __forceinline__ void wave_best(double &c, int &i) {
     best_step<32>(c, i);
 }
 
+// exp(x) for x <= 0 to about an ulp: exp2 of the product with log2 e, times what its rounding left out.
+__device__ __forceinline__ float exp_near(float x) {
+    constexpr float HI = 1.44269504f, LO = 1.92596299e-8f, LN2 = 0.693147181f;
+    const float n = x * HI, rest = fmaf(x, HI, -n) + x * LO, e = __builtin_amdgcn_exp2f(n);
+    return x > -104.f ? fmaf(e, rest * LN2, e) : 0.f;  // (the rest of -inf is NaN)
+}
+// a / b for b of f32's middle range: a reciprocal and the quotient's remainder.
+__device__ __forceinline__ float quotient(float a, float b) {
+    const float r = rcp(b), q = a * r;
+    return fmaf(fmaf(-q, b, a), r, q);
+}
+
 // The score's part of pick x before the sum: p for a score that keeps its value, else p over a factor that the row's picks
 // share (`top`: their largest x or min(x, 0)), so that far negative logits keep their ratios.
 __device__ __forceinline__ float pick_weight(const RouteArgs &a, float x, float top, float row_max, float inv_den) {
-    if (!a.sigmoid) return a.renorm ? expf(x - top) : expf(x - row_max) * inv_den;
-    const float e = expf(-fabsf(x));
-    if (a.renorm) return expf(fminf(x, 0.f) - top) / (1.f + e);
-    return (x >= 0.f ? 1.f : e) / (1.f + e);
+    if (!a.sigmoid) return a.renorm ? exp_near(x - top) : exp_near(x - row_max) * inv_den;
+    const float e = exp_near(-fabsf(x));
+    if (a.renorm) return quotient(exp_near(fminf(x, 0.f) - top), 1.f + e);
+    return quotient(x >= 0.f ? 1.f : e, 1.f + e);
 }
 
-// A row by one wave, lane l taking experts l, l + 64, ...; everything that decides in 64 bits, held in `buf` (a value an expert,
-// the wave's).  Rolled loops: a wave that takes a row here has this code to fetch, and it is most of its time.
+// A row's values by one wave in 64 bits, lane l taking experts l, l + 64, ...: x or c, -inf for an expert that is out by its logit
+// or its bias.  In `buf`, the wave's.
+struct RowInfo {
+    float mx, inv;  // the softmax's
+    bool bad;
+};
 template <int DT>
-__device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int lane, double *buf) {
+__device__ __forceinline__ RowInfo row_values(const RouteArgs &a, size_t row, int lane, double *buf, bool by_logit) {
     const size_t at = row * a.experts;
-    const bool by_logit = !a.bias && (a.groups == 1 || a.group_top == 1);
     const bool whole = !a.sigmoid && !(by_logit && a.renorm);
     bool bad = false;
     float mx = -INFINITY;
+#pragma unroll 2
     for (int e = lane; e < a.experts; e += 64) {
         const float x = load_act<DT>(a.logits, at + e);
         const bool nan = x != x || (!a.sigmoid && x == INFINITY);
@@ -73,13 +89,13 @@ __device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int la
         mx = fmaxf(mx, nan ? -INFINITY : x);
         buf[e] = nan ? -INFINITY : (double)x;
     }
-    bad = __any(bad);
     mx = group_max<64>(mx);
+    mx = mx == -INFINITY ? 0.f : mx;
     double den = 0.;
     if (!by_logit || whole) {
-        const double from = a.sigmoid || mx == -INFINITY ? 0. : (double)mx;
+#pragma unroll 2
         for (int e = lane; e < a.experts; e += 64) {
-            const double x = buf[e], y = exp(a.sigmoid ? -x : x - from);
+            const double x = buf[e], y = exp(a.sigmoid ? -x : x - (double)mx);
             den += y;
             if (!by_logit) buf[e] = x == -INFINITY ? x : a.sigmoid ? 1. / (1. + y) : y;
         }
@@ -90,13 +106,47 @@ __device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int la
     }
     if (!by_logit) {
         for (int e = lane; e < a.experts; e += 64) {
-            double c = buf[e];
+            const double c = buf[e];
             const float b = a.bias ? a.bias[e] : 0.f;
             // (an expert that its bias takes out still has its share of the softmax)
             const bool off = c == -INFINITY || !(b > -INFINITY);
             buf[e] = off ? -INFINITY : (whole ? c / den : c) + (double)b;
         }
     }
+    return RowInfo{mx, whole ? (float)(1. / den) : 1.f, (bool)__any(bad)};
+}
+
+// Whether the bias is one finite value for every expert, or there is none.
+__device__ __forceinline__ bool same_bias(const RouteArgs &a, int lane) {
+    if (!a.bias) return true;
+    const float first = a.bias[0];
+    bool same = fabsf(first) < INFINITY;
+    for (int e = lane; e < a.experts; e += 64) same &= a.bias[e] == first;
+    return __all(same);
+}
+
+// A lane's pick of a row by one wave: its slot (past topk: none), its expert (NO_EXPERT: a slot without one).
+template <int DT>
+__device__ __forceinline__ void write_picks(const RouteArgs &a, size_t row, const RowInfo &info, int slot, int expert) {
+    const bool has = slot < a.topk && expert != NO_EXPERT;
+    const float px = has ? load_act<DT>(a.logits, row * a.experts + expert) : -INFINITY;
+    const float top = group_max<64>(a.sigmoid ? fminf(px, 0.f) : px);
+    float w = has ? pick_weight(a, px, top, info.mx, info.inv) : 0.f;
+    if (a.renorm) {
+        const float sum = group_sum<64>(w);
+        w = has ? quotient(w, sum) : 0.f;
+    }
+    if (slot < a.topk) {
+        a.inds[row * a.topk + slot] = has ? (uint32_t)expert : 0xFFFFFFFFu;
+        a.scores[row * a.topk + slot] = info.bad ? NAN : w * a.scale;
+    }
+}
+
+// A row by one wave, whatever it holds; by_logit: the experts' order is their logits'.
+template <int DT>
+__device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int lane, double *buf, bool by_logit) {
+    const bool groups_too = by_logit && a.group_top == 1;
+    RowInfo info = row_values<DT>(a, row, lane, buf, a.groups > 1 ? groups_too : by_logit);
     if (a.groups > 1) {
         // a lane a group
         const int size = a.experts / a.groups;
@@ -116,6 +166,7 @@ __device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int la
             ahead += better(w, g, worth, lane) ? 1 : 0;
         }
         const uint64_t open = __ballot(ahead < a.taken && worth > -INFINITY);
+        if (by_logit && !groups_too) info = row_values<DT>(a, row, lane, buf, true);
         for (int e = lane; e < a.experts; e += 64)
             if (!((open >> (e / size)) & 1)) buf[e] = -INFINITY;
     }
@@ -134,18 +185,41 @@ __device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int la
         if ((bi & 63) == lane) buf[bi] = -INFINITY;
         mine = lane == j ? bi : mine;
     }
-    const bool has = mine != NO_EXPERT;
-    const float px = has ? load_act<DT>(a.logits, at + mine) : -INFINITY;
-    const float top = group_max<64>(a.sigmoid ? fminf(px, 0.f) : px);
-    float w = has ? pick_weight(a, px, top, mx, 1.f / (float)den) : 0.f;
-    if (a.renorm) {
-        const float sum = group_sum<64>(w);
-        w = has ? w / sum : 0.f;
+    write_picks<DT>(a, row, info, lane, mine);
+}
+
+// A row whose groups are settled (bit g of `open`) and whose picks are all at least `least`, by one wave: the few values that are
+// stand in a list, a lane each, which counts those ahead of its own.  False with more than a wave of them.
+template <int DT>
+__device__ __forceinline__ bool settle_row(const RouteArgs &a, size_t row, int lane, double *buf, bool by_logit, uint64_t open,
+                                           double least) {
+    const RowInfo info = row_values<DT>(a, row, lane, buf, by_logit);
+    const int size = a.experts / a.groups;
+    wave_order();
+    // (a place of the list is behind every value that is still to be read)
+    int count = 0;
+    double mine = -INFINITY;
+    int expert = NO_EXPERT;
+    for (int e0 = 0; e0 < a.experts; e0 += 64) {
+        const int e = e0 + lane;
+        const double c = e < a.experts ? buf[e] : -INFINITY;
+        const bool is = c >= least && c > -INFINITY && ((open >> (a.groups > 1 ? min(e, a.experts - 1) / size : 0)) & 1);
+        uint64_t who = __ballot(is);
+        while (who) {
+            const int from = __ffsll((unsigned long long)who) - 1;
+            who &= who - 1;
+            if (count == 64) return false;
+            const double v = __shfl(c, from);
+            mine = lane == count ? v : mine;
+            expert = lane == count ? e0 + from : expert;
+            count++;
+        }
     }
-    if (lane < a.topk) {
-        a.inds[row * a.topk + lane] = has ? (uint32_t)mine : 0xFFFFFFFFu;
-        a.scores[row * a.topk + lane] = bad ? NAN : w * a.scale;
-    }
+    int ahead = 0;
+    for (int i = 0; i < count; i++) ahead += better(__shfl(mine, i), __shfl(expert, i), mine, expert) ? 1 : 0;
+    // lanes behind the list take the slots that no expert is left for
+    write_picks<DT>(a, row, info, lane < count ? ahead : lane, expert);
+    return true;
 }
 
 // More than eight picks (or more units than the lists hold): a wave a row.
@@ -162,7 +236,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_kernel(RouteArgs a) {
         }
         return;
     }
-    route_row<DT>(a, row, lane, row_buf + wave * a.experts);
+    route_row<DT>(a, row, lane, row_buf + wave * a.experts, same_bias(a, lane));
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -245,10 +319,16 @@ constexpr uint32_t kDistBase = 107u << 23, kDistOut = (1u << 28) - 1;
 __device__ __forceinline__ uint32_t dist_bits(float d) { return __builtin_elementwise_sub_sat(__float_as_uint(d), kDistBase); }
 __device__ __forceinline__ float bits_dist(uint32_t b) { return b == 0 ? 0.f : __uint_as_float(b + kDistBase); }
 
+// An integer of c's steps: 0 for what is not above it, NaN too (the conversion saturates, which C++ does not say).
+__device__ __forceinline__ uint32_t to_steps(float x) {
+    uint32_t r;
+    asm("v_cvt_u32_f32 %0, %1" : "=v"(r) : "v"(x));
+    return r;
+}
+
 template <int L, int T, int DT, bool BY_LOGIT, bool GROUPED>
 __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, int nu, int id_bits, int wave_lds) {
     constexpr int ROWS = 64 / L;
-    constexpr bool EXACT = BY_LOGIT && DT != DT_F32;
     constexpr float LOG2E = 1.4426950408889634f;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (L - 1), grp = lane / L;
     extern __shared__ __align__(16) double row_buf[];  // wave_lds bytes a wave
@@ -257,35 +337,48 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
     __shared__ float range[RT_WAVES][2];
     const int size = a.experts / a.groups, units = (size + 7) / 8;
     const uint32_t over = (65536 + units - 1) / units;  // u / units = u over >> 16 for the units here
-    auto first_of = [&](int u) { return GROUPED ? (int)(u * over >> 16) * (size - units * 8) + u * 8 : u * 8; };
+    auto group_of = [&](int u) { return GROUPED ? (int)(u * over >> 16) : 0; };
+    auto first_of = [&](int u) { return GROUPED ? group_of(u) * (size - units * 8) + u * 8 : u * 8; };
     auto count_of = [&](int u) {
-        const int g = GROUPED ? (int)(u * over >> 16) : 0;
+        const int g = group_of(u);
         return g < a.groups ? max(0, min(8, size - (u - g * units) * 8)) : 0;
     };
-    const int id_mask = EXACT ? 1023 : (1 << id_bits) - 1;  // a key's low bits: the complement of the expert's place, 8 u + q
-    float lo = 0.f, steps = 0.f, largest = 0.f;             // c's steps: (c - lo) steps + 1; no |c| is above `largest`
+    const int id_mask = (1 << id_bits) - 1;       // a key's low bits: the complement of the expert's place, 8 u + q
+    const int value_mask = 0x7FFFFFFF & ~id_mask;
+    float lo = 0.f, steps = 0.f, largest = 0.f;   // c's steps: (c - lo) steps + 1; no |c| is above `largest`
+    // A bias that is the same for every expert does not move the choice among experts: it goes by the logits, whose ties are ties.
+    bool by_logit = BY_LOGIT;
     if constexpr (!BY_LOGIT) {
         float least = INFINITY, most = -INFINITY;
+        bool out = false;
         for (int s = threadIdx.x; s < L * nu * 8; s += RT_THREADS) {
             const bool is = (s & 7) < count_of(s / 8);
-            float b = is ? a.bias ? a.bias[first_of(s / 8) + (s & 7)] : 0.f : -INFINITY;
+            const float b = is ? a.bias ? a.bias[first_of(s / 8) + (s & 7)] : 0.f : -INFINITY;
+            out |= is && !(b > -INFINITY);
             // (NaN is out of the choice; what passes 2^125 goes by 64 bits where it decides, and adds up in f32)
-            b = b > -INFINITY ? fminf(fmaxf(b, -0x1p125f), 0x1p125f) : -INFINITY;
-            bias_lds[s] = b;
+            bias_lds[s] = b > -INFINITY ? fminf(fmaxf(b, -0x1p125f), 0x1p125f) : -INFINITY;
             least = fminf(least, b > -INFINITY ? b : INFINITY);
             most = fmaxf(most, b);
         }
         least = -group_max<64>(-least);
         most = group_max<64>(most);
         range[wave][0] = least;
-        range[wave][1] = most;
+        range[wave][1] = __any(out) ? NAN : most;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < RT_WAVES; w++) least = fminf(least, range[w][0]), most = fmaxf(most, range[w][1]);
+        for (int w = 0; w < RT_WAVES; w++) {
+            out |= range[w][1] != range[w][1];
+            least = fminf(least, range[w][0]);
+            most = fmaxf(most, range[w][1]);
+        }
+        by_logit = !out && least == most && fabsf(most) < INFINITY;
+        least = fminf(fmaxf(least, -0x1p125f), 0x1p125f);
+        most = fminf(fmaxf(most, -0x1p125f), 0x1p125f);
         lo = least;
         largest = fmaxf(fabsf(least), fabsf(most) + 1.f);
         steps = most >= least ? (float)((1u << (31 - id_bits)) - 16) / (1.0625f + (most - least)) : 0.f;
     }
+    const bool exact = DT != DT_F32 && by_logit;      // keys that order as the choice does
     const int bad_class = a.sigmoid ? 0x003 : 0x203;  // NaN; under softmax +inf too
     const size_t rows = (size_t)a.rows, step = (size_t)gridDim.x * RT_WAVES * ROWS;
     for (size_t r0 = ((size_t)blockIdx.x * RT_WAVES + wave) * ROWS; r0 < rows; r0 += step) {
@@ -293,24 +386,32 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         const bool in = r < rows, live = in && (!a.mask || a.mask[in ? r : 0] != 0);
         const char *row = static_cast<const char *>(a.logits) + (in ? r : r0) * a.experts * (DT == DT_F32 ? 4 : 2);
         bool bad = false;
-        // A unit's logits, -inf for experts that are out by them and past the unit's own.
+        // A unit's logits, -inf for experts that are out by them and past the unit's own; whether the wave has any of those.
         auto load = [&](int u, float (&v)[8]) {
             Raw8<DT> raw;
             const int first = first_of(u), n = count_of(u);
             if (n > 0 && first + 8 <= a.experts) raw.load(elem<DT>(row, first));
             else raw.load_some(elem<DT>(row, first), n);
             if (n < 8) raw.keep(n);
+            bool odd = false;
 #pragma unroll
             for (int q = 0; q < 8; q++) {
-                const float x = raw.get(q);
-                const bool nan = __builtin_amdgcn_classf(x, bad_class);
-                bad |= nan;
-                v[q] = nan ? -INFINITY : x;
+                v[q] = raw.get(q);
+                odd |= __builtin_amdgcn_classf(v[q], bad_class | 0x004);
             }
+            odd = __any(odd);
+            if (odd)
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const bool nan = __builtin_amdgcn_classf(v[q], bad_class);
+                    bad |= nan;
+                    v[q] = nan ? -INFINITY : v[q];
+                }
+            return odd;
         };
         const bool whole = !a.sigmoid && !(BY_LOGIT && a.renorm);  // the softmax over the row
         float mx = -INFINITY, inv = 1.f;
-        if (whole || (BY_LOGIT && !EXACT)) {
+        if (whole || (by_logit && !exact)) {
 #pragma unroll 1
             for (int i = 0; i < nu; i++) {
                 float v[8];
@@ -334,27 +435,36 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         }
         // The values that the choice goes by, -inf for an expert that is out of it.
         auto values = [&](int u, float (&v)[8]) {
-            load(u, v);
-            if constexpr (!BY_LOGIT) {
+            float x[8];
+            const bool odd = load(u, x);
+            if constexpr (BY_LOGIT) {
+#pragma unroll
+                for (int q = 0; q < 8; q++) v[q] = x[q];
+            } else {
                 const float4 *b = reinterpret_cast<const float4 *>(bias_lds + u * 8);
                 const float4 b0 = b[0], b1 = b[1];
                 const float bias[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+                if (a.sigmoid) {
 #pragma unroll
-                for (int q = 0; q < 8; q++) {
-                    const float x = v[q];
-                    const float e = __builtin_amdgcn_exp2f(a.sigmoid ? -LOG2E * x : LOG2E * (x - mx));
-                    const float p = a.sigmoid ? rcp(1.f + e) : e * inv;
-                    v[q] = x == -INFINITY ? x : p + bias[q];
+                    for (int q = 0; q < 8; q++) v[q] = rcp(1.f + __builtin_amdgcn_exp2f(-LOG2E * x[q])) + bias[q];
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; q++) v[q] = fmaf(__builtin_amdgcn_exp2f(LOG2E * (x[q] - mx)), inv, bias[q]);
                 }
+                if (odd)
+#pragma unroll
+                    for (int q = 0; q < 8; q++) v[q] = x[q] == -INFINITY ? x[q] : v[q];
             }
         };
-        bool near = false;
+        bool near = false, near_group = false;
         uint64_t open = ~uint64_t(0);
         float *const vals = reinterpret_cast<float *>(mem) + grp * (L * nu * 8);
+        int *const list = reinterpret_cast<int *>(mem + 2560 * nu) + grp * a.groups;  // the open groups, in order
+        int opened = 0, units_left = nu;
         if constexpr (GROUPED) {
             // each unit's two largest, each group's, its place among the groups
             float2 *const unit_top = reinterpret_cast<float2 *>(mem + 2048 * nu) + grp * (L * nu);
-            float *const worth = reinterpret_cast<float *>(mem + 2560 * nu) + grp * a.groups;
+            float *const worth = reinterpret_cast<float *>(list);
 #pragma unroll 1
             for (int i = 0; i < nu; i++) {
                 float v[8];
@@ -366,9 +476,11 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
                     m2 = __builtin_amdgcn_fmed3f(m1, m2, v[q]);
                     m1 = fmaxf(m1, v[q]);
                 }
-                float4 *o = reinterpret_cast<float4 *>(vals + u * 8);
-                o[0] = float4{v[0], v[1], v[2], v[3]};
-                o[1] = float4{v[4], v[5], v[6], v[7]};
+                if (!by_logit) {
+                    float4 *o = reinterpret_cast<float4 *>(vals + u * 8);
+                    o[0] = float4{v[0], v[1], v[2], v[3]};
+                    o[1] = float4{v[4], v[5], v[6], v[7]};
+                }
                 unit_top[u] = float2{m1, m2};
             }
             wave_order();
@@ -383,10 +495,10 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
             }
             wave_order();
             open = 0;
+            const float tol = BY_LOGIT ? 0.f : near_of(a, inv, largest) * 2.f;
             for (int g0 = 0; g0 < a.groups; g0 += L) {
                 const int g = g0 + l;
                 const float w = g < a.groups ? worth[g] : -INFINITY;
-                const float tol = BY_LOGIT ? 0.f : near_of(a, inv, largest) * 2.f;
                 int ahead = 0, surely = 0, maybe = 0;
                 for (int o = 0; o < a.groups; o++) {
                     const float x = worth[o];
@@ -397,46 +509,66 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
                     }
                 }
                 const bool is = g < a.groups && w > -INFINITY;
-                if constexpr (!BY_LOGIT) near |= is && surely < a.taken && maybe >= a.taken;
+                if constexpr (!BY_LOGIT) near_group |= is && surely < a.taken && maybe >= a.taken;
                 const uint64_t b = __ballot(is && ahead < a.taken);
                 open |= ((b >> (lane & ~(L - 1))) & (L == 64 ? ~uint64_t(0) : (uint64_t(1) << (L & 63)) - 1)) << g0;
             }
             wave_order();
+            opened = __popcll(open);
+            for (int g = l; g < a.groups; g += L)
+                if ((open >> g) & 1) list[__popcll(open & ((uint64_t(1) << g) - 1))] = g;
+            wave_order();
+            units_left = (a.taken * units + L - 1) / L;
         }
         int best[T], next = INT32_MIN;
 #pragma unroll 1
-        for (int i = 0; i < nu; i++) {
-            const int u = i * L + l;
-            float v[8];
-            if constexpr (GROUPED) {
-                const float4 *o = reinterpret_cast<const float4 *>(vals + u * 8);
-                const float4 v0 = o[0], v1 = o[1];
-                const bool is = (open >> min((int)(u * over >> 16), 63)) & 1;
-                const float w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                for (int q = 0; q < 8; q++) v[q] = is ? w[q] : -INFINITY;
-            } else {
-                values(u, v);
+        for (int i = 0; i < units_left; i++) {
+            int u = i * L + l;
+            bool is = true;
+            if constexpr (GROUPED) {  // the u-th unit of the open groups
+                const int nth = group_of(u);
+                is = nth < opened;
+                u += is ? (list[nth] - nth) * units : -u;
             }
-            const int not_id = ~(u * 8) & id_mask;  // of the unit's first: q less for its q-th
+            float v[8];
+            int k8[8];
+            const int not_id = ~(u * 8 + 7) & id_mask;
+            if (by_logit) {
+                load(u, v);
+                if constexpr (GROUPED)
+                    if (!is)
+#pragma unroll
+                        for (int q = 0; q < 8; q++) v[q] = -INFINITY;
+                if (DT != DT_F32) {
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        const int b = __float_as_int(v[q] + 0.f);  // (-0 is 0)
+                        k8[q] = b ^ (((b >> 31) & value_mask) | not_id | (7 - q));
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {  // (what is out is at the end of the distances)
+                        const uint32_t d = min(dist_bits(mx - v[q]), kDistOut);
+                        k8[q] = (int)((~d << 3) & (uint32_t)value_mask) | not_id | (7 - q);
+                    }
+                }
+            } else {
+                if constexpr (GROUPED) {
+                    const float4 *o = reinterpret_cast<const float4 *>(vals + u * 8);
+                    const float4 v0 = o[0], v1 = o[1];
+                    v[0] = v0.x, v[1] = v0.y, v[2] = v0.z, v[3] = v0.w, v[4] = v1.x, v[5] = v1.y, v[6] = v1.z, v[7] = v1.w;
+                } else {
+                    values(u, v);
+                }
+                const float by = is ? steps : 0.f, one = is ? 1.f : 0.f;
+#pragma unroll
+                for (int q = 0; q < 8; q++) k8[q] = (int)(to_steps(fmaf(v[q] - lo, by, one)) << id_bits) | not_id | (7 - q);
+            }
 #pragma unroll
             for (int part = 0; part < 8 / T; part++) {
                 int k[T];
 #pragma unroll
-                for (int j = 0; j < T; j++) {
-                    const int q = part * T + j;
-                    const float x = v[q];
-                    if constexpr (EXACT) {
-                        const int b = __float_as_int(x + 0.f);  // (-0 is 0)
-                        k[j] = b ^ (((b >> 31) & (0x7FFFFFFF & ~1023)) | (not_id - q));
-                    } else if constexpr (BY_LOGIT) {
-                        const uint32_t d = x == -INFINITY ? kDistOut : min(dist_bits(mx - x), kDistOut - (1u << (id_bits - 3)));
-                        k[j] = (int)(((~d << 3) & (uint32_t)(0x7FFFFFFF & ~id_mask)) | (uint32_t)(not_id - q));
-                    } else {
-                        const uint32_t c = x == -INFINITY ? 0u : (uint32_t)((x - lo) * steps) + 1u;
-                        k[j] = (int)(c << id_bits | (uint32_t)(not_id - q));
-                    }
-                }
+                for (int j = 0; j < T; j++) k[j] = k8[part * T + j];
                 sort_keys(k);
                 if (part == 0 && i == 0) {
 #pragma unroll
@@ -453,44 +585,55 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         if constexpr (L > 16) merge_lanes<16>(best, next);
         if constexpr (L > 32) merge_lanes<32>(best, next);
         bad = group_any<L>(bad);
-        // keys of experts that are out: what -inf, kDistOut or no step makes
-        const int out = EXACT ? (int)(0xFF800000u ^ (0x7FFFFFFFu & ~1023u)) | 1023 : id_mask;
-        if constexpr (!EXACT) {
-            // Two values that decide and lie close: the row goes by 64 bits.
+        // keys of experts that are out: what -inf, the end of the distances or no step makes
+        const int out = exact ? (int)(0xFF800000u ^ (uint32_t)value_mask) | id_mask : id_mask;
+        // Two values that decide and lie close: the row goes by 64 bits.  `least`: no pick is below it.
+        double least = -INFINITY;
+        if (!exact) {
             int last = 0;
-            if constexpr (BY_LOGIT) {
-                const float tol = 0x1p-22f * fabsf(mx), part = 1.f - 2.f / (float)(1 << (26 - id_bits));  // two truncations
-                auto dist = [&](int key) { return bits_dist((~(uint32_t)key & (uint32_t)(0x7FFFFFFF & ~id_mask)) >> 3); };
+            if (by_logit) {
+                const float tol = 0x1p-22f * fabsf(mx), trunc = 2.f / (float)(1 << (26 - id_bits));  // two truncations
+                auto dist = [&](int key) { return bits_dist((~(uint32_t)key & (uint32_t)value_mask) >> 3); };
 #pragma unroll
                 for (int i = 0; i <= T; i++) {
                     const int key = i < T ? best[i < T ? i : 0] : next;
                     const float d = dist(key);
-                    // (at the end of the distances too)
-                    if (i <= a.topk && key > out)
-                        near |= (i > 0 && d * part - dist(last) <= tol + (d < 0x1p-19f ? 0x1p-20f : 0.f)) || (i < a.topk && d >= 0x1p11f);
+                    // (an expert that is out has a distance of its own only among the picks)
+                    if (i > 0 && i <= a.topk && key > out)
+                        near |= d * (1.f - trunc) - dist(last) <= tol + (d < 0x1p-19f ? 0x1p-20f : 0.f);
+                    if (i < a.topk) {
+                        near |= d >= 0x1p11f;  // at the end of the distances, or out
+                        least = d >= 0x1p11f ? -INFINITY : (double)mx - (double)d * (1. + trunc) - (double)tol - 0x1p-19;
+                    }
                     last = key;
                 }
             } else {
-                const int tol = (int)fminf(near_of(a, inv, largest) * steps, 0x1p30f) + 3;
+                const float err = near_of(a, inv, largest);
+                const int tol = (int)fminf(err * steps, 0x1p30f) + 3;
 #pragma unroll
                 for (int i = 0; i <= T; i++) {
                     const int key = (i < T ? best[i < T ? i : 0] : next) >> id_bits;
                     if (i > 0 && i <= a.topk && key > 0) near |= last - key <= tol;
+                    if (i == a.topk - 1 && key > 0) least = (double)lo + (double)(key - 5) / (double)steps - (double)err;
                     last = key;
                 }
             }
-            near = group_any<L>(near) && live;
+        }
+        if (!BY_LOGIT || DT == DT_F32) {
+            near = group_any<L>(near || near_group) && live;
+            near_group = group_any<L>(near_group);
         }
         // a lane a slot: its expert and its logit
-        int key = best[0];
+        int key = best[0], slot = l & (T - 1);
+        asm volatile("" : "+v"(slot));  // (its comparisons are not kept over the rows)
 #pragma unroll
-        for (int i = 1; i < T; i++) key = (l & (T - 1)) == i ? best[i] : key;
+        for (int i = 1; i < T; i++) key = slot == i ? best[i] : key;
         const bool has = l < T && l < a.topk && key > out;
         const int place = ~key & id_mask, e = GROUPED ? first_of(place >> 3) + (place & 7) : place;
         float px;
-        if constexpr (EXACT) {
-            const int b = key & ~1023;
-            px = __int_as_float(b ^ ((b >> 31) & (0x7FFFFFFF & ~1023)));
+        if (exact) {
+            const int b = key & ~id_mask;
+            px = __int_as_float(b ^ ((b >> 31) & value_mask));
         } else {
             px = load_act<DT>(elem<DT>(row, has ? e : 0), 0);
         }
@@ -499,22 +642,23 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         float w = has ? pick_weight(a, px, top, mx, inv) : 0.f;
         if (a.renorm) {
             const float sum = group_sum<T>(w);
-            w = has ? w / sum : 0.f;
+            w = has ? quotient(w, sum) : 0.f;
         }
         if (l < a.topk && in && !near) {
             a.inds[r * a.topk + l] = has && live ? (uint32_t)e : 0xFFFFFFFFu;
             a.scores[r * a.topk + l] = !live ? 0.f : bad ? NAN : w * a.scale;
         }
-        if constexpr (!EXACT) {
-            uint64_t again = __ballot(near && l == 0);
+        uint64_t again = __ballot(near && l == 0);
 #pragma unroll 1
-            while (again) {
-                const int at = __ffsll((unsigned long long)again) - 1;
-                again &= again - 1;
-                wave_order();
-                route_row<DT>(a, r0 + at / L, lane, reinterpret_cast<double *>(mem));
-                wave_order();
-            }
+        while (again) {
+            const int at = __ffsll((unsigned long long)again) - 1;
+            again &= again - 1;
+            wave_order();
+            double *const buf = reinterpret_cast<double *>(mem);
+            const uint64_t its_open = (uint64_t)__shfl((uint32_t)(open >> 32), at) << 32 | __shfl((uint32_t)open, at);
+            if (__shfl(near_group ? 1 : 0, at) || !settle_row<DT>(a, r0 + at / L, lane, buf, by_logit, its_open, __shfl(least, at)))
+                route_row<DT>(a, r0 + at / L, lane, buf, by_logit);
+            wave_order();
         }
     }
 }

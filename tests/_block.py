@@ -24,18 +24,17 @@ def route(logits, k, bias=None, score="softmax", groups=1, topk_groups=1, group_
     nan = x.isnan() | ((x == math.inf) if score == "softmax" else False)
     off = nan | (x == -math.inf)
     p = torch.where(nan, 0.0, probabilities(torch.where(nan, -math.inf, x), score))
-    c = x if bias is None and (groups == 1 or group_top == 1) else p
-    if bias is not None:
-        b = bias.double().cpu()
-        c, off = c + b, off | ~(b > -math.inf)
-    c = torch.where(off, -math.inf, c)
+    b = torch.zeros(E, dtype=torch.float64) if bias is None else bias.double().cpu()
+    off = off | ~(b > -math.inf)
+    by_logit = bool((b == b[0]).all()) and math.isfinite(b[0])  # the experts' order is their logits'
+    c = torch.where(off, -math.inf, x if by_logit else p + b)
     if groups > 1:
-        g = c.reshape(rows, groups, -1)
+        g = torch.where(off, -math.inf, x if by_logit and group_top == 1 else p + b).reshape(rows, groups, -1)
         best = g.sort(dim=-1, descending=True).values[..., :group_top]
         worth = torch.where(best > -math.inf, best, 0.0).sum(-1).where(best[..., 0] > -math.inf, torch.tensor(-math.inf, dtype=torch.float64))
         order = worth.sort(dim=-1, descending=True, stable=True).indices[:, :topk_groups]
         open_ = torch.zeros(rows, groups, dtype=torch.bool).scatter_(1, order, True)
-        c = torch.where(open_[..., None], g, -math.inf).reshape(rows, E)
+        c = torch.where(open_[..., None], c.reshape(rows, groups, -1), -math.inf).reshape(rows, E)
     val, inds = c.sort(dim=-1, descending=True, stable=True)
     has = val[:, :k] > -math.inf
     inds = inds[:, :k]
