@@ -333,7 +333,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (L - 1), grp = lane / L;
     extern __shared__ __align__(16) double row_buf[];  // wave_lds bytes a wave
     char *const mem = reinterpret_cast<char *>(row_buf) + wave * wave_lds;
-    __shared__ __align__(16) float bias_lds[BY_LOGIT ? 4 : 8 * kListUnits];
+    float *const bias_lds = reinterpret_cast<float *>(reinterpret_cast<char *>(row_buf) + RT_WAVES * wave_lds);  // behind the waves'
     __shared__ float range[RT_WAVES][2];
     const int size = a.experts / a.groups, units = (size + 7) / 8;
     const uint32_t over = (65536 + units - 1) / units;  // u / units = u over >> 16 for the units here
@@ -379,287 +379,288 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         steps = most >= least ? (float)((1u << (31 - id_bits)) - 16) / (1.0625f + (most - least)) : 0.f;
     }
     const bool exact = DT != DT_F32 && by_logit;      // keys that order as the choice does
+    const bool groups_by_logit = BY_LOGIT || (by_logit && a.group_top == 1);
     const int bad_class = a.sigmoid ? 0x003 : 0x203;  // NaN; under softmax +inf too
-    const size_t rows = (size_t)a.rows, step = (size_t)gridDim.x * RT_WAVES * ROWS;
-    for (size_t r0 = ((size_t)blockIdx.x * RT_WAVES + wave) * ROWS; r0 < rows; r0 += step) {
-        const size_t r = r0 + grp;
-        const bool in = r < rows, live = in && (!a.mask || a.mask[in ? r : 0] != 0);
-        const char *row = static_cast<const char *>(a.logits) + (in ? r : r0) * a.experts * (DT == DT_F32 ? 4 : 2);
-        bool bad = false;
-        // A unit's logits, -inf for experts that are out by them and past the unit's own; whether the wave has any of those.
-        auto load = [&](int u, float (&v)[8]) {
-            Raw8<DT> raw;
-            const int first = first_of(u), n = count_of(u);
-            if (n > 0 && first + 8 <= a.experts) raw.load(elem<DT>(row, first));
-            else raw.load_some(elem<DT>(row, first), n);
-            if (n < 8) raw.keep(n);
-            bool odd = false;
+    // (One set of rows a wave: in a loop over sets the compiler keeps the 64-bit path's constants in registers throughout.)
+    const size_t rows = (size_t)a.rows, r0 = ((size_t)blockIdx.x * RT_WAVES + wave) * ROWS;
+    if (r0 >= rows) return;
+    const size_t r = r0 + grp;
+    const bool in = r < rows, live = in && (!a.mask || a.mask[in ? r : 0] != 0);
+    const char *row = static_cast<const char *>(a.logits) + (in ? r : r0) * a.experts * (DT == DT_F32 ? 4 : 2);
+    bool bad = false;
+    // A unit's logits, -inf for experts that are out by them and past the unit's own; whether the wave has any of those.
+    auto load = [&](int u, float (&v)[8]) {
+        Raw8<DT> raw;
+        const int first = first_of(u), n = count_of(u);
+        if (n > 0 && first + 8 <= a.experts) raw.load(elem<DT>(row, first));
+        else raw.load_some(elem<DT>(row, first), n);
+        if (n < 8) raw.keep(n);
+        bool odd = false;
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            v[q] = raw.get(q);
+            odd |= __builtin_amdgcn_classf(v[q], bad_class | 0x004);
+        }
+        odd = __any(odd);
+        if (odd)
 #pragma unroll
             for (int q = 0; q < 8; q++) {
-                v[q] = raw.get(q);
-                odd |= __builtin_amdgcn_classf(v[q], bad_class | 0x004);
+                const bool nan = __builtin_amdgcn_classf(v[q], bad_class);
+                bad |= nan;
+                v[q] = nan ? -INFINITY : v[q];
             }
-            odd = __any(odd);
+        return odd;
+    };
+    const bool whole = !a.sigmoid && !(BY_LOGIT && a.renorm);  // the softmax over the row
+    float mx = -INFINITY, inv = 1.f;
+    if (whole || (by_logit && !exact)) {
+#pragma unroll 1
+        for (int i = 0; i < nu; i++) {
+            float v[8];
+            load(i * L + l, v);
+#pragma unroll
+            for (int q = 0; q < 8; q++) mx = fmaxf(mx, v[q]);
+        }
+        mx = group_max<L>(mx);
+        mx = mx == -INFINITY ? 0.f : mx;
+    }
+    if (whole) {
+        float den = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < nu; i++) {
+            float v[8];
+            load(i * L + l, v);
+#pragma unroll
+            for (int q = 0; q < 8; q++) den += __builtin_amdgcn_exp2f(LOG2E * (v[q] - mx));
+        }
+        inv = rcp(group_sum<L>(den));
+    }
+    // The values that the choice goes by, -inf for an expert that is out of it.
+    auto values = [&](int u, float (&v)[8]) {
+        float x[8];
+        const bool odd = load(u, x);
+        if constexpr (BY_LOGIT) {
+#pragma unroll
+            for (int q = 0; q < 8; q++) v[q] = x[q];
+        } else {
+            const float4 *b = reinterpret_cast<const float4 *>(bias_lds + u * 8);
+            const float4 b0 = b[0], b1 = b[1];
+            const float bias[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+            if (a.sigmoid) {
+#pragma unroll
+                for (int q = 0; q < 8; q++) v[q] = rcp(1.f + __builtin_amdgcn_exp2f(-LOG2E * x[q])) + bias[q];
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; q++) v[q] = fmaf(__builtin_amdgcn_exp2f(LOG2E * (x[q] - mx)), inv, bias[q]);
+            }
             if (odd)
 #pragma unroll
+                for (int q = 0; q < 8; q++) v[q] = x[q] == -INFINITY ? x[q] : v[q];
+        }
+    };
+    bool near = false, near_group = false;
+    uint64_t open = ~uint64_t(0);
+    float *const vals = reinterpret_cast<float *>(mem) + grp * (L * nu * 8 + 8);  // (rows at different banks)
+    int *const list = reinterpret_cast<int *>(mem + 2048 * nu + 32 * ROWS) + grp * a.groups;  // the open groups, in order
+    int opened = 0, units_left = nu;
+    if constexpr (GROUPED) {
+        // each group's two largest, its place among the groups
+        float *const worth = reinterpret_cast<float *>(list);
+#pragma unroll 1
+        for (int i = 0; i < nu; i++) {
+            float v[8];
+            const int u = i * L + l;
+            if (groups_by_logit) load(u, v);
+            else values(u, v);
+            float4 *o = reinterpret_cast<float4 *>(vals + u * 8);
+            o[0] = float4{v[0], v[1], v[2], v[3]};
+            o[1] = float4{v[4], v[5], v[6], v[7]};
+        }
+        wave_order();
+        for (int g = l; g < a.groups; g += L) {
+            float m1 = -INFINITY, m2 = -INFINITY;
+            int u = g % units;  // (lanes begin at different units, so at different banks)
+#pragma unroll 1
+            for (int j = 0; j < units; j++) {
+                const float4 *o = reinterpret_cast<const float4 *>(vals + (g * units + u) * 8);
+                const float4 v0 = o[0], v1 = o[1];
+                const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
                 for (int q = 0; q < 8; q++) {
-                    const bool nan = __builtin_amdgcn_classf(v[q], bad_class);
-                    bad |= nan;
-                    v[q] = nan ? -INFINITY : v[q];
-                }
-            return odd;
-        };
-        const bool whole = !a.sigmoid && !(BY_LOGIT && a.renorm);  // the softmax over the row
-        float mx = -INFINITY, inv = 1.f;
-        if (whole || (by_logit && !exact)) {
-#pragma unroll 1
-            for (int i = 0; i < nu; i++) {
-                float v[8];
-                load(i * L + l, v);
-#pragma unroll
-                for (int q = 0; q < 8; q++) mx = fmaxf(mx, v[q]);
-            }
-            mx = group_max<L>(mx);
-            mx = mx == -INFINITY ? 0.f : mx;
-        }
-        if (whole) {
-            float den = 0.f;
-#pragma unroll 1
-            for (int i = 0; i < nu; i++) {
-                float v[8];
-                load(i * L + l, v);
-#pragma unroll
-                for (int q = 0; q < 8; q++) den += __builtin_amdgcn_exp2f(LOG2E * (v[q] - mx));
-            }
-            inv = rcp(group_sum<L>(den));
-        }
-        // The values that the choice goes by, -inf for an expert that is out of it.
-        auto values = [&](int u, float (&v)[8]) {
-            float x[8];
-            const bool odd = load(u, x);
-            if constexpr (BY_LOGIT) {
-#pragma unroll
-                for (int q = 0; q < 8; q++) v[q] = x[q];
-            } else {
-                const float4 *b = reinterpret_cast<const float4 *>(bias_lds + u * 8);
-                const float4 b0 = b[0], b1 = b[1];
-                const float bias[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
-                if (a.sigmoid) {
-#pragma unroll
-                    for (int q = 0; q < 8; q++) v[q] = rcp(1.f + __builtin_amdgcn_exp2f(-LOG2E * x[q])) + bias[q];
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 8; q++) v[q] = fmaf(__builtin_amdgcn_exp2f(LOG2E * (x[q] - mx)), inv, bias[q]);
-                }
-                if (odd)
-#pragma unroll
-                    for (int q = 0; q < 8; q++) v[q] = x[q] == -INFINITY ? x[q] : v[q];
-            }
-        };
-        bool near = false, near_group = false;
-        uint64_t open = ~uint64_t(0);
-        float *const vals = reinterpret_cast<float *>(mem) + grp * (L * nu * 8);
-        int *const list = reinterpret_cast<int *>(mem + 2560 * nu) + grp * a.groups;  // the open groups, in order
-        int opened = 0, units_left = nu;
-        if constexpr (GROUPED) {
-            // each unit's two largest, each group's, its place among the groups
-            float2 *const unit_top = reinterpret_cast<float2 *>(mem + 2048 * nu) + grp * (L * nu);
-            float *const worth = reinterpret_cast<float *>(list);
-#pragma unroll 1
-            for (int i = 0; i < nu; i++) {
-                float v[8];
-                const int u = i * L + l;
-                values(u, v);
-                float m1 = v[0], m2 = -INFINITY;
-#pragma unroll
-                for (int q = 1; q < 8; q++) {
                     m2 = __builtin_amdgcn_fmed3f(m1, m2, v[q]);
                     m1 = fmaxf(m1, v[q]);
                 }
-                if (!by_logit) {
-                    float4 *o = reinterpret_cast<float4 *>(vals + u * 8);
-                    o[0] = float4{v[0], v[1], v[2], v[3]};
-                    o[1] = float4{v[4], v[5], v[6], v[7]};
-                }
-                unit_top[u] = float2{m1, m2};
+                u = u + 1 == units ? 0 : u + 1;
             }
-            wave_order();
-            for (int g = l; g < a.groups; g += L) {
-                float m1 = -INFINITY, m2 = -INFINITY;
-                for (int u = g * units; u < (g + 1) * units; u++) {
-                    const float2 o = unit_top[u];
-                    m2 = fmaxf(fmaxf(m2, o.y), fminf(m1, o.x));
-                    m1 = fmaxf(m1, o.x);
-                }
-                worth[g] = a.group_top == 2 && m2 > -INFINITY ? m1 + m2 : m1;
-            }
-            wave_order();
-            open = 0;
-            const float tol = BY_LOGIT ? 0.f : near_of(a, inv, largest) * 2.f;
-            for (int g0 = 0; g0 < a.groups; g0 += L) {
-                const int g = g0 + l;
-                const float w = g < a.groups ? worth[g] : -INFINITY;
-                int ahead = 0, surely = 0, maybe = 0;
-                for (int o = 0; o < a.groups; o++) {
-                    const float x = worth[o];
-                    ahead += x > w || (x == w && o < g) ? 1 : 0;
-                    if constexpr (!BY_LOGIT) {
-                        surely += x > w + tol ? 1 : 0;
-                        maybe += x >= w - tol && o != g ? 1 : 0;
-                    }
-                }
-                const bool is = g < a.groups && w > -INFINITY;
-                if constexpr (!BY_LOGIT) near_group |= is && surely < a.taken && maybe >= a.taken;
-                const uint64_t b = __ballot(is && ahead < a.taken);
-                open |= ((b >> (lane & ~(L - 1))) & (L == 64 ? ~uint64_t(0) : (uint64_t(1) << (L & 63)) - 1)) << g0;
-            }
-            wave_order();
-            opened = __popcll(open);
-            for (int g = l; g < a.groups; g += L)
-                if ((open >> g) & 1) list[__popcll(open & ((uint64_t(1) << g) - 1))] = g;
-            wave_order();
-            units_left = (a.taken * units + L - 1) / L;
+            worth[g] = a.group_top == 2 && m2 > -INFINITY ? m1 + m2 : m1;
         }
-        int best[T], next = INT32_MIN;
+        wave_order();
+        open = 0;
+        const float tol = near_of(a, inv, largest) * 2.f;
+        for (int g0 = 0; g0 < a.groups; g0 += L) {
+            const int g = g0 + l;
+            const float w = g < a.groups ? worth[g] : -INFINITY;
+            int ahead = 0, surely = 0, maybe = 0;
+            for (int o = 0; o < a.groups; o++) {
+                const float x = worth[o];
+                ahead += x > w || (x == w && o < g) ? 1 : 0;
+                if (!groups_by_logit) {
+                    surely += x > w + tol ? 1 : 0;
+                    maybe += x >= w - tol && o != g ? 1 : 0;
+                }
+            }
+            const bool is = g < a.groups && w > -INFINITY;
+            if (!groups_by_logit) near_group |= is && surely < a.taken && maybe >= a.taken;
+            const uint64_t b = __ballot(is && ahead < a.taken);
+            open |= ((b >> (lane & ~(L - 1))) & (L == 64 ? ~uint64_t(0) : (uint64_t(1) << (L & 63)) - 1)) << g0;
+        }
+        wave_order();
+        opened = __popcll(open);
+        for (int g = l; g < a.groups; g += L)
+            if ((open >> g) & 1) list[__popcll(open & ((uint64_t(1) << g) - 1))] = g;
+        wave_order();
+        units_left = (a.taken * units + L - 1) / L;
+    }
+    int best[T], next = INT32_MIN;
 #pragma unroll 1
-        for (int i = 0; i < units_left; i++) {
-            int u = i * L + l;
-            bool is = true;
-            if constexpr (GROUPED) {  // the u-th unit of the open groups
-                const int nth = group_of(u);
-                is = nth < opened;
-                u += is ? (list[nth] - nth) * units : -u;
-            }
-            float v[8];
-            int k8[8];
-            const int not_id = ~(u * 8 + 7) & id_mask;
-            if (by_logit) {
-                load(u, v);
-                if constexpr (GROUPED)
-                    if (!is)
+    for (int i = 0; i < units_left; i++) {
+        int u = i * L + l;
+        bool is = true;
+        if constexpr (GROUPED) {  // the u-th unit of the open groups
+            const int nth = group_of(u);
+            is = nth < opened;
+            u += is ? (list[nth] - nth) * units : -u;
+        }
+        float v[8];
+        int k8[8];
+        const int not_id = ~(u * 8 + 7) & id_mask;
+        auto kept = [&]() {
+            const float4 *o = reinterpret_cast<const float4 *>(vals + u * 8);
+            const float4 v0 = o[0], v1 = o[1];
+            v[0] = v0.x, v[1] = v0.y, v[2] = v0.z, v[3] = v0.w, v[4] = v1.x, v[5] = v1.y, v[6] = v1.z, v[7] = v1.w;
+        };
+        if (by_logit) {
+            if (GROUPED && groups_by_logit) kept();
+            else load(u, v);
+            if constexpr (GROUPED)
+                if (!is)
 #pragma unroll
-                        for (int q = 0; q < 8; q++) v[q] = -INFINITY;
-                if (DT != DT_F32) {
+                    for (int q = 0; q < 8; q++) v[q] = -INFINITY;
+            if (DT != DT_F32) {
 #pragma unroll
-                    for (int q = 0; q < 8; q++) {
-                        const int b = __float_as_int(v[q] + 0.f);  // (-0 is 0)
-                        k8[q] = b ^ (((b >> 31) & value_mask) | not_id | (7 - q));
-                    }
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 8; q++) {  // (what is out is at the end of the distances)
-                        const uint32_t d = min(dist_bits(mx - v[q]), kDistOut);
-                        k8[q] = (int)((~d << 3) & (uint32_t)value_mask) | not_id | (7 - q);
-                    }
+                for (int q = 0; q < 8; q++) {
+                    const int b = __float_as_int(v[q] + 0.f);  // (-0 is 0)
+                    k8[q] = b ^ (((b >> 31) & value_mask) | not_id | (7 - q));
                 }
             } else {
-                if constexpr (GROUPED) {
-                    const float4 *o = reinterpret_cast<const float4 *>(vals + u * 8);
-                    const float4 v0 = o[0], v1 = o[1];
-                    v[0] = v0.x, v[1] = v0.y, v[2] = v0.z, v[3] = v0.w, v[4] = v1.x, v[5] = v1.y, v[6] = v1.z, v[7] = v1.w;
-                } else {
-                    values(u, v);
-                }
-                const float by = is ? steps : 0.f, one = is ? 1.f : 0.f;
 #pragma unroll
-                for (int q = 0; q < 8; q++) k8[q] = (int)(to_steps(fmaf(v[q] - lo, by, one)) << id_bits) | not_id | (7 - q);
-            }
-#pragma unroll
-            for (int part = 0; part < 8 / T; part++) {
-                int k[T];
-#pragma unroll
-                for (int j = 0; j < T; j++) k[j] = k8[part * T + j];
-                sort_keys(k);
-                if (part == 0 && i == 0) {
-#pragma unroll
-                    for (int q = 0; q < T; q++) best[q] = k[q];
-                } else {
-                    merge_keys(best, k, next);
+                for (int q = 0; q < 8; q++) {  // (what is out is at the end of the distances)
+                    const uint32_t d = min(dist_bits(mx - v[q]), kDistOut);
+                    k8[q] = (int)((~d << 3) & (uint32_t)value_mask) | not_id | (7 - q);
                 }
             }
-        }
-        merge_lanes<1>(best, next);
-        merge_lanes<2>(best, next);
-        merge_lanes<4>(best, next);
-        if constexpr (L > 8) merge_lanes<8>(best, next);
-        if constexpr (L > 16) merge_lanes<16>(best, next);
-        if constexpr (L > 32) merge_lanes<32>(best, next);
-        bad = group_any<L>(bad);
-        // keys of experts that are out: what -inf, the end of the distances or no step makes
-        const int out = exact ? (int)(0xFF800000u ^ (uint32_t)value_mask) | id_mask : id_mask;
-        // Two values that decide and lie close: the row goes by 64 bits.  `least`: no pick is below it.
-        double least = -INFINITY;
-        if (!exact) {
-            int last = 0;
-            if (by_logit) {
-                const float tol = 0x1p-22f * fabsf(mx), trunc = 2.f / (float)(1 << (26 - id_bits));  // two truncations
-                auto dist = [&](int key) { return bits_dist((~(uint32_t)key & (uint32_t)value_mask) >> 3); };
-#pragma unroll
-                for (int i = 0; i <= T; i++) {
-                    const int key = i < T ? best[i < T ? i : 0] : next;
-                    const float d = dist(key);
-                    // (an expert that is out has a distance of its own only among the picks)
-                    if (i > 0 && i <= a.topk && key > out)
-                        near |= d * (1.f - trunc) - dist(last) <= tol + (d < 0x1p-19f ? 0x1p-20f : 0.f);
-                    if (i < a.topk) {
-                        near |= d >= 0x1p11f;  // at the end of the distances, or out
-                        least = d >= 0x1p11f ? -INFINITY : (double)mx - (double)d * (1. + trunc) - (double)tol - 0x1p-19;
-                    }
-                    last = key;
-                }
-            } else {
-                const float err = near_of(a, inv, largest);
-                const int tol = (int)fminf(err * steps, 0x1p30f) + 3;
-#pragma unroll
-                for (int i = 0; i <= T; i++) {
-                    const int key = (i < T ? best[i < T ? i : 0] : next) >> id_bits;
-                    if (i > 0 && i <= a.topk && key > 0) near |= last - key <= tol;
-                    if (i == a.topk - 1 && key > 0) least = (double)lo + (double)(key - 5) / (double)steps - (double)err;
-                    last = key;
-                }
-            }
-        }
-        if (!BY_LOGIT || DT == DT_F32) {
-            near = group_any<L>(near || near_group) && live;
-            near_group = group_any<L>(near_group);
-        }
-        // a lane a slot: its expert and its logit
-        int key = best[0], slot = l & (T - 1);
-        asm volatile("" : "+v"(slot));  // (its comparisons are not kept over the rows)
-#pragma unroll
-        for (int i = 1; i < T; i++) key = slot == i ? best[i] : key;
-        const bool has = l < T && l < a.topk && key > out;
-        const int place = ~key & id_mask, e = GROUPED ? first_of(place >> 3) + (place & 7) : place;
-        float px;
-        if (exact) {
-            const int b = key & ~id_mask;
-            px = __int_as_float(b ^ ((b >> 31) & value_mask));
         } else {
-            px = load_act<DT>(elem<DT>(row, has ? e : 0), 0);
+            if constexpr (GROUPED) kept();
+            else values(u, v);
+            const float by = is ? steps : 0.f, one = is ? 1.f : 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; q++) k8[q] = (int)(to_steps(fmaf(v[q] - lo, by, one)) << id_bits) | not_id | (7 - q);
         }
-        px = has ? px : -INFINITY;
-        const float top = group_max<T>(a.sigmoid ? fminf(px, 0.f) : px);
-        float w = has ? pick_weight(a, px, top, mx, inv) : 0.f;
-        if (a.renorm) {
-            const float sum = group_sum<T>(w);
-            w = has ? quotient(w, sum) : 0.f;
+#pragma unroll
+        for (int part = 0; part < 8 / T; part++) {
+            int k[T];
+#pragma unroll
+            for (int j = 0; j < T; j++) k[j] = k8[part * T + j];
+            sort_keys(k);
+            if (part == 0 && i == 0) {
+#pragma unroll
+                for (int q = 0; q < T; q++) best[q] = k[q];
+            } else {
+                merge_keys(best, k, next);
+            }
         }
-        if (l < a.topk && in && !near) {
-            a.inds[r * a.topk + l] = has && live ? (uint32_t)e : 0xFFFFFFFFu;
-            a.scores[r * a.topk + l] = !live ? 0.f : bad ? NAN : w * a.scale;
+    }
+    merge_lanes<1>(best, next);
+    merge_lanes<2>(best, next);
+    merge_lanes<4>(best, next);
+    if constexpr (L > 8) merge_lanes<8>(best, next);
+    if constexpr (L > 16) merge_lanes<16>(best, next);
+    if constexpr (L > 32) merge_lanes<32>(best, next);
+    bad = group_any<L>(bad);
+    // keys of experts that are out: what -inf, the end of the distances or no step makes
+    const int out = exact ? (int)(0xFF800000u ^ (uint32_t)value_mask) | id_mask : id_mask;
+    // Two values that decide and lie close: the row goes by 64 bits.  `least`: no pick is below it.
+    double least = -INFINITY;
+    if (!exact) {
+        int last = 0;
+        if (by_logit) {
+            const float tol = 0x1p-22f * fabsf(mx), trunc = 2.f / (float)(1 << (26 - id_bits));  // two truncations
+            auto dist = [&](int key) { return bits_dist((~(uint32_t)key & (uint32_t)value_mask) >> 3); };
+#pragma unroll
+            for (int i = 0; i <= T; i++) {
+                const int key = i < T ? best[i < T ? i : 0] : next;
+                const float d = dist(key);
+                // (an expert that is out has a distance of its own only among the picks)
+                if (i > 0 && i <= a.topk && key > out)
+                    near |= d * (1.f - trunc) - dist(last) <= tol + (d < 0x1p-19f ? 0x1p-20f : 0.f);
+                if (i < a.topk) {
+                    near |= d >= 0x1p11f;  // at the end of the distances, or out
+                    least = d >= 0x1p11f ? -INFINITY : (double)mx - (double)d * (1. + trunc) - (double)tol - 0x1p-19;
+                }
+                last = key;
+            }
+        } else {
+            const float err = near_of(a, inv, largest);
+            const int tol = (int)fminf(err * steps, 0x1p30f) + 3;
+#pragma unroll
+            for (int i = 0; i <= T; i++) {
+                const int key = (i < T ? best[i < T ? i : 0] : next) >> id_bits;
+                if (i > 0 && i <= a.topk && key > 0) near |= last - key <= tol;
+                if (i == a.topk - 1 && key > 0) least = (double)lo + (double)(key - 5) / (double)steps - (double)err;
+                last = key;
+            }
         }
-        uint64_t again = __ballot(near && l == 0);
+    }
+    if (!BY_LOGIT || DT == DT_F32) {
+        near = group_any<L>(near || near_group) && live;
+        near_group = group_any<L>(near_group);
+    }
+    // a lane a slot: its expert and its logit
+    int key = best[0], slot = l & (T - 1);
+    asm volatile("" : "+v"(slot));  // (its comparisons are not kept over the rows)
+#pragma unroll
+    for (int i = 1; i < T; i++) key = slot == i ? best[i] : key;
+    const bool has = l < T && l < a.topk && key > out;
+    const int place = ~key & id_mask, e = GROUPED ? first_of(place >> 3) + (place & 7) : place;
+    float px;
+    if (exact) {
+        const int b = key & ~id_mask;
+        px = __int_as_float(b ^ ((b >> 31) & value_mask));
+    } else {
+        px = load_act<DT>(elem<DT>(row, has ? e : 0), 0);
+    }
+    px = has ? px : -INFINITY;
+    const float top = group_max<T>(a.sigmoid ? fminf(px, 0.f) : px);
+    float w = has ? pick_weight(a, px, top, mx, inv) : 0.f;
+    if (a.renorm) {
+        const float sum = group_sum<T>(w);
+        w = has ? quotient(w, sum) : 0.f;
+    }
+    if (l < a.topk && in && !near) {
+        a.inds[r * a.topk + l] = has && live ? (uint32_t)e : 0xFFFFFFFFu;
+        a.scores[r * a.topk + l] = !live ? 0.f : bad ? NAN : w * a.scale;
+    }
+    uint64_t again = __ballot(near && l == 0);
 #pragma unroll 1
-        while (again) {
-            const int at = __ffsll((unsigned long long)again) - 1;
-            again &= again - 1;
-            wave_order();
-            double *const buf = reinterpret_cast<double *>(mem);
-            const uint64_t its_open = (uint64_t)__shfl((uint32_t)(open >> 32), at) << 32 | __shfl((uint32_t)open, at);
-            if (__shfl(near_group ? 1 : 0, at) || !settle_row<DT>(a, r0 + at / L, lane, buf, by_logit, its_open, __shfl(least, at)))
-                route_row<DT>(a, r0 + at / L, lane, buf, by_logit);
-            wave_order();
-        }
+    while (again) {
+        const int at = __ffsll((unsigned long long)again) - 1;
+        again &= again - 1;
+        wave_order();
+        double *const buf = reinterpret_cast<double *>(mem);
+        const uint64_t its_open = (uint64_t)__shfl((uint32_t)(open >> 32), at) << 32 | __shfl((uint32_t)open, at);
+        if (__shfl(near_group ? 1 : 0, at) || !settle_row<DT>(a, r0 + at / L, lane, buf, by_logit, its_open, __shfl(least, at)))
+            route_row<DT>(a, r0 + at / L, lane, buf, by_logit);
+        wave_order();
     }
 }
 
@@ -668,15 +669,15 @@ template <int L, int T, int DT>
 static hipError_t launch_lists(const RouteArgs &a, int units, hipStream_t s) {
     constexpr int at_once = RT_THREADS / L;
     const long wgs = ((long)a.rows + at_once - 1) / at_once;
-    const dim3 grid((unsigned)(wgs < 2048 ? wgs : 2048));
+    const dim3 grid((unsigned)wgs);
     const bool grouped = a.groups > 1, by_logit = !a.bias && (!grouped || a.group_top == 1);
     const int nu = (units + L - 1) / L;
     int id_bits = 6;
     while ((1 << id_bits) < L * nu * 8) id_bits++;
-    // the values, the units' two largest and the groups' worths of a wave's rows; a row's values in 64 bits
-    const int lists = grouped ? nu * 2560 + (64 / L * a.groups * 4 + 15) / 16 * 16 : 0, row = (a.experts * 8 + 15) / 16 * 16;
+    // the values and the groups' worths of a wave's rows; a row's values in 64 bits
+    const int lists = grouped ? nu * 2048 + 64 / L * 32 + (64 / L * a.groups * 4 + 15) / 16 * 16 : 0, row = (a.experts * 8 + 15) / 16 * 16;
     const int lds = lists > row ? lists : row;
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(RT_THREADS), RT_WAVES * lds, s, a, nu, id_bits, lds); };
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(RT_THREADS), RT_WAVES * lds + (by_logit ? 0 : L * nu * 32), s, a, nu, id_bits, lds); };
     if (by_logit) grouped ? go(route_lists_kernel<L, T, DT, true, true>) : go(route_lists_kernel<L, T, DT, true, false>);
     else grouped ? go(route_lists_kernel<L, T, DT, false, true>) : go(route_lists_kernel<L, T, DT, false, false>);
     return hipGetLastError();

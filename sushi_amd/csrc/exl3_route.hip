@@ -2,9 +2,20 @@
 
 namespace exl3 {
 
-// The choice of experts: exl3_route.h.
+// The choice of experts: exl3_route.h.  A launch takes up to 2^24 rows (its threads are numbered in 32 bits).
 hipError_t run_route(const RouteArgs &a, hipStream_t s) {
-    return a.dtype == DT_F16 ? run_route_f16(a, s) : a.dtype == DT_BF16 ? run_route_bf16(a, s) : run_route_f32(a, s);
+    constexpr int most = 1 << 24;
+    for (int r = 0; r < a.rows; r += min(most, a.rows - r)) {
+        RouteArgs c = a;
+        c.rows = min(most, a.rows - r);
+        c.logits = static_cast<const char *>(a.logits) + (size_t)r * a.experts * (a.dtype == DT_F32 ? 4 : 2);
+        c.mask = a.mask ? a.mask + r : nullptr;
+        c.inds = a.inds + (size_t)r * a.topk;
+        c.scores = a.scores + (size_t)r * a.topk;
+        const hipError_t e = a.dtype == DT_F16 ? run_route_f16(c, s) : a.dtype == DT_BF16 ? run_route_bf16(c, s) : run_route_f32(c, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
