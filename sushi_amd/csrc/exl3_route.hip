@@ -1,6 +1,11 @@
 #include "exl3_router.h"
+#include "exl3_vec.h"
+
+#include <algorithm>
 
 namespace exl3 {
+
+constexpr int RT_THREADS = 256;
 
 // The choice of experts: exl3_route.h.  A launch takes up to 2^24 rows (its threads are numbered in 32 bits).
 hipError_t run_route(const RouteArgs &a, hipStream_t s) {
@@ -25,14 +30,12 @@ hipError_t run_route(const RouteArgs &a, hipStream_t s) {
 //   sigmoid, renorm:  the same times 1 - p_i
 //   sigmoid:          dx_e = sum over slots i on e of p_i (1 - p_i) ds_i
 //   softmax:          dx_e = sum over slots i on e of p_i ds_i - p_e sum_j p_j ds_j
-// A slot whose id is past the experts has no score.  All but the last (DENSE) read the picked logits alone, and write a row
-// of zeros with the slots' terms in it.
-//
-// A row is held by L lanes as in the balance loss's kernel, lane l holding PER experts and SPL slots.
-constexpr int RT_THREADS = 256;
+// A slot whose id is past the experts has no score.
 
-template <int L, int PER, int SPL, int DT, bool VEC, bool DENSE>
-__global__ __launch_bounds__(RT_THREADS) void route_backward_kernel(RouteGradArgs a) {
+// The last form reads the whole row.  A row is held by L lanes as in the balance loss's kernel, lane l holding PER experts and
+// SPL slots; its row of LDS takes the slots' terms to the lanes that hold their experts (a wave's own rows: no barrier).
+template <int L, int PER, int SPL, int DT, bool VEC>
+__global__ __launch_bounds__(RT_THREADS) void route_backward_row_kernel(RouteGradArgs a) {
     constexpr int G = RT_THREADS / L;
     const int l = threadIdx.x & (L - 1), grp = threadIdx.x / L, e0 = l * PER;
     __shared__ __align__(16) float rows_lds[G][L * PER];
@@ -41,7 +44,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_backward_kernel(RouteGradArg
     for (size_t r0 = (size_t)blockIdx.x * G; r0 < rows; r0 += step) {
         const size_t r = r0 + grp;
         const bool in = r < rows, live = in && (!a.mask || a.mask[r] != 0);
-        float d[PER], ds[SPL], x[SPL];
+        float d[PER], t[SPL], x[SPL];
         int ind[SPL];
 #pragma unroll
         for (int i = 0; i < SPL; i++) {
@@ -49,80 +52,36 @@ __global__ __launch_bounds__(RT_THREADS) void route_backward_kernel(RouteGradArg
             const size_t slot = r * a.topk + j;
             const bool has = live && j < a.topk;
             ind[i] = has && a.inds[has ? slot : 0] < (uint32_t)a.experts ? (int)a.inds[slot] : -1;
-            ds[i] = ind[i] >= 0 ? a.dscores[slot] * a.scale : 0.f;
+            t[i] = ind[i] >= 0 ? a.dscores[slot] * a.scale : 0.f;
             x[i] = ind[i] >= 0 ? load_act<DT>(a.logits, r * a.experts + ind[i]) : -INFINITY;
         }
-        float mx = -INFINITY, inv = 0.f;
-        if constexpr (DENSE) {
-            Logits<PER, DT, VEC> row = {};
-            if (live) row.load(a.logits, r * a.experts, a.experts, e0);
-            row.unpack(a.experts, e0, live, d);
-            mx = d[0];
+        Logits<PER, DT, VEC> row = {};
+        if (live) row.load(a.logits, r * a.experts, a.experts, e0);
+        row.unpack(a.experts, e0, live, d);
+        float mx = d[0];
 #pragma unroll
-            for (int q = 1; q < PER; q++) mx = fmaxf(mx, d[q]);
-            mx = group_max<L>(mx);
-            const float base = mx == -INFINITY ? 0.f : mx;
-            float den = 0.f;
+        for (int q = 1; q < PER; q++) mx = fmaxf(mx, d[q]);
+        mx = group_max<L>(mx);
+        mx = mx == -INFINITY ? 0.f : mx;
+        float den = 0.f;
 #pragma unroll
-            for (int q = 0; q < PER; q++) {
-                d[q] = __expf(d[q] - base);
-                den += d[q];
-            }
-            den = group_sum<L>(den);
-            inv = den == 0.f ? 0.f : 1.f / den;
-            mx = base;
-        } else {
-            if (a.renorm) {
-#pragma unroll
-                for (int i = 0; i < SPL; i++) mx = fmaxf(mx, a.sigmoid ? fminf(x[i], 0.f) : x[i]);
-                mx = group_max<L>(mx);
-                mx = mx == -INFINITY ? 0.f : mx;
-            }
-#pragma unroll
-            for (int q = 0; q < PER; q++) d[q] = 0.f;
+        for (int q = 0; q < PER; q++) {
+            d[q] = __expf(d[q] - mx);
+            den += d[q];
         }
-        // the slots' terms
-        float t[SPL], dot = 0.f, sum = 0.f;
+        den = group_sum<L>(den);
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        float dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < SPL; i++) {
-            float w;
-            if constexpr (DENSE) w = expf(x[i] - mx) * inv;
-            else if (!a.sigmoid) w = expf(x[i] - mx);
-            else {
-                const float e = expf(-fabsf(x[i]));
-                w = a.renorm ? expf(fminf(x[i], 0.f) - mx) / (1.f + e) : (x[i] >= 0.f ? 1.f : e) / (1.f + e);
-            }
-            w = ind[i] >= 0 ? w : 0.f;
-            t[i] = w;
-            sum += w;
-            dot += w * ds[i];
+        for (int i = 0; i < SPL; i++) {  // the slots' terms
+            t[i] = ind[i] >= 0 ? expf(x[i] - mx) * inv * t[i] : 0.f;
+            dot += t[i];
         }
-        if (DENSE || a.renorm) dot = group_sum<L>(dot);
-        if constexpr (!DENSE) {
-            if (a.renorm) {
-                sum = group_sum<L>(sum);
-                inv = sum == 0.f ? 0.f : 1.f / sum;
-                dot *= inv;
-            }
-        }
+        dot = group_sum<L>(dot) * inv;
 #pragma unroll
-        for (int i = 0; i < SPL; i++) {
-            if constexpr (DENSE) t[i] *= ds[i];
-            else {
-                t[i] = a.renorm ? t[i] * inv * (ds[i] - dot) : t[i] * ds[i];
-                if (a.sigmoid) {
-                    const float e = expf(-fabsf(x[i]));
-                    t[i] *= (x[i] >= 0.f ? e : 1.f) / (1.f + e);
-                }
-            }
-        }
-        if constexpr (DENSE) {
-            const float c = dot * inv;
-#pragma unroll
-            for (int q = 0; q < PER; q++) d[q] *= -c;
-        }
-        // Into the row by way of LDS (a wave's own rows: no barrier).  Every slot leaves its number at its expert: where two
-        // of a row's slots name one expert, some slot does not find its own again.
+        for (int q = 0; q < PER; q++) d[q] *= -dot;
+        // Every slot leaves its number at its expert: where two of a row's slots name one expert, some slot does not find its
+        // own again.
         wave_order();
 #pragma unroll
         for (int i = 0; i < SPL; i++)
@@ -159,19 +118,106 @@ __global__ __launch_bounds__(RT_THREADS) void route_backward_kernel(RouteGradArg
     }
 }
 
+// The other forms read the picked logits alone and write rows of zeros with the slots' terms in them.  A wave has 64 / LS rows, a
+// lane a slot; the rows lie one after another in its LDS as they do in memory, so they leave in whole vectors whatever the
+// row's length.
+template <int LS, int DT>
+__global__ __launch_bounds__(RT_THREADS) void route_backward_picked_kernel(RouteGradArgs a, int wave_lds) {
+    constexpr int ROWS = 64 / LS, SIZE = DT == DT_F32 ? 4 : 2, N = 16 / SIZE;
+    using Word = std::conditional_t<DT == DT_F32, uint32_t, uint16_t>;
+    extern __shared__ __align__(16) char rows_mem[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & (LS - 1);
+    char *const mem = rows_mem + wave * wave_lds;
+    const size_t rows = (size_t)a.rows, r0 = ((size_t)blockIdx.x * (RT_THREADS / 64) + wave) * ROWS, r = r0 + lane / LS;
+    if (r0 >= rows) return;
+    const bool has = r < rows && j < a.topk && (!a.mask || a.mask[r] != 0);
+    const size_t slot = has ? r * a.topk + j : 0;
+    const uint32_t id = has ? a.inds[slot] : 0xFFFFFFFFu;
+    const bool is = id < (uint32_t)a.experts;
+    const float ds = is ? a.dscores[slot] * a.scale : 0.f;
+    const float x = is ? load_act<DT>(a.logits, r * a.experts + id) : -INFINITY;
+    for (int i = lane * 16; i < wave_lds; i += 1024) *reinterpret_cast<uint4 *>(mem + i) = uint4{0, 0, 0, 0};
+    float t = ds;
+    const float e = a.sigmoid ? expf(-fabsf(x)) : 0.f;  // sigmoid(x) = (x < 0 ? e : 1) / (1 + e), 1 - sigmoid(x) the other way round
+    if (a.renorm) {
+        float mx = group_max<LS>(a.sigmoid ? fminf(x, 0.f) : x);
+        mx = mx == -INFINITY ? 0.f : mx;
+        float w = is ? (a.sigmoid ? expf(fminf(x, 0.f) - mx) / (1.f + e) : expf(x - mx)) : 0.f;
+        const float sum = group_sum<LS>(w);
+        w = sum == 0.f ? 0.f : w / sum;
+        t = w * (ds - group_sum<LS>(w * ds));
+    } else {
+        t = ds * ((x >= 0.f ? 1.f : e) / (1.f + e));
+    }
+    if (a.sigmoid) t *= (x >= 0.f ? e : 1.f) / (1.f + e);
+    // A slot leaves its number at its expert: where two of a row's slots name one expert, some slot does not find its own again.
+    Word *const at = reinterpret_cast<Word *>(mem) + (lane / LS) * a.experts + (is ? id : 0);
+    wave_order();
+    if (is) *at = (Word)(j + 1);
+    wave_order();
+    if (__any(is && *at != (Word)(j + 1))) {  // equal experts' terms add in slot order, and each of their slots has the sum
+        float sum = 0.f;
+        for (int i = 0; i < LS; i++) sum += (uint32_t)__shfl((int)id, i, LS) == id ? __shfl(t, i, LS) : 0.f;
+        t = sum;
+    }
+    wave_order();
+    if (is) {
+        if constexpr (DT == DT_F32) *at = __float_as_uint(t);
+        else if constexpr (DT == DT_F16) *at = __half_as_ushort(__float2half_rn(t));
+        else *at = __bfloat16_as_ushort(__float2bfloat16(t));
+    }
+    wave_order();
+    const int count = (int)min((size_t)ROWS, rows - r0) * a.experts;
+    char *const out = static_cast<char *>(a.dlogits) + r0 * a.experts * SIZE;
+    for (int i = lane * N; i < count; i += 64 * N) {
+        if (i + N <= count) {
+            *reinterpret_cast<Words4At2 *>(out + i * SIZE) = *reinterpret_cast<const Words4 *>(mem + i * SIZE);
+        } else {
+            for (int q = i; q < count; q++) reinterpret_cast<Word *>(out)[q] = reinterpret_cast<const Word *>(mem)[q];
+        }
+    }
+}
+
+template <int LS, int DT>
+static hipError_t launch_picked(const RouteGradArgs &a, hipStream_t s) {
+    const int size = DT == DT_F32 ? 4 : 2, lds = (64 / LS * a.experts * size + 15) / 16 * 16;
+    constexpr int at_once = RT_THREADS / LS, most = 1 << 24;  // rows a launch
+    for (int r = 0; r < a.rows; r += std::min(most, a.rows - r)) {
+        RouteGradArgs c = a;
+        c.rows = std::min(most, a.rows - r);
+        c.logits = static_cast<const char *>(a.logits) + (size_t)r * a.experts * size;
+        c.inds = a.inds + (size_t)r * a.topk;
+        c.dscores = a.dscores + (size_t)r * a.topk;
+        c.mask = a.mask ? a.mask + r : nullptr;
+        c.dlogits = static_cast<char *>(a.dlogits) + (size_t)r * a.experts * size;
+        hipLaunchKernelGGL((route_backward_picked_kernel<LS, DT>), dim3((unsigned)((c.rows + at_once - 1) / at_once)), dim3(RT_THREADS),
+                           RT_THREADS / 64 * lds, s, c, lds);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
 hipError_t run_route_backward(const RouteGradArgs &a, hipStream_t s) {
-    const bool dense = !a.sigmoid && !a.renorm;
+    if (a.sigmoid || a.renorm)
+        return with_dtype(a.dtype, [&](auto DT) {
+            constexpr int dt = decltype(DT)::value;
+            // lanes a row: its slots, and so many that a wave's rows take 8 KiB at most
+            const int row = a.experts * (dt == DT_F32 ? 4 : 2);
+            if (a.topk <= 8 && row <= 1024) return launch_picked<8, dt>(a, s);
+            if (a.topk <= 16 && row <= 2048) return launch_picked<16, dt>(a, s);
+            return launch_picked<32, dt>(a, s);
+        });
     return with_shape(a.experts, [&](auto L, auto PER) {
         return with_dtype(a.dtype, [&](auto DT) {
             constexpr int l = decltype(L)::value, per = decltype(PER)::value, dt = decltype(DT)::value;
             const long groups = ((long)a.rows + RT_THREADS / l - 1) / (RT_THREADS / l);
-            const dim3 grid((unsigned)(groups < 2048 ? groups : 2048));
+            const dim3 grid((unsigned)(groups < 8192 ? groups : 8192));
             const bool vec = whole_vectors<per, dt>(a.logits, a.experts) && whole_vectors<per, dt>(a.dlogits, a.experts);
             auto launch = [&](auto SPL) {
                 constexpr int spl = decltype(SPL)::value;
                 auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(RT_THREADS), 0, s, a); };
-                if (dense) vec ? go(route_backward_kernel<l, per, spl, dt, true, true>) : go(route_backward_kernel<l, per, spl, dt, false, true>);
-                else vec ? go(route_backward_kernel<l, per, spl, dt, true, false>) : go(route_backward_kernel<l, per, spl, dt, false, false>);
+                vec ? go(route_backward_row_kernel<l, per, spl, dt, true>) : go(route_backward_row_kernel<l, per, spl, dt, false>);
                 return hipGetLastError();
             };
             if constexpr (l < 32)
