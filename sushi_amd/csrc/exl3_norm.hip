@@ -9,7 +9,7 @@
 #include "exl3_vec.h"
 #include "exl3_epilogue.h"
 
-#include <initializer_list>
+#include <algorithm>
 #include <type_traits>
 
 namespace exl3 {
@@ -47,10 +47,10 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[N]) {
     }
 }
 
-__device__ __forceinline__ const void *row_at(const void *p, size_t row, int width, int dt) {
+__host__ __device__ __forceinline__ const void *row_at(const void *p, size_t row, int width, int dt) {
     return p ? static_cast<const char *>(p) + row * width * (dt == DT_F32 ? 4 : 2) : nullptr;
 }
-__device__ __forceinline__ void *row_at(void *p, size_t row, int width, int dt) {
+__host__ __device__ __forceinline__ void *row_at(void *p, size_t row, int width, int dt) {
     return p ? static_cast<char *>(p) + row * width * (dt == DT_F32 ? 4 : 2) : nullptr;
 }
 
@@ -366,7 +366,7 @@ static hipError_t with_types(int dt, int ht, F f) {
 // The threads of a row of `width` values at nv vectors each, in whole waves.
 static int row_threads(int width, int nv) { return (width + 512 * nv - 1) / (512 * nv) * 64; }
 
-hipError_t run_norm(const NormArgs &a, hipStream_t s) {
+static hipError_t launch_norm(const NormArgs &a, hipStream_t s) {
     return with_types(a.dtype, a.hdtype, [&](auto DT, auto HT) {
         constexpr int dt = decltype(DT)::value, ht = decltype(HT)::value;
         auto go = [&](auto MAXT, auto NV) {
@@ -382,6 +382,24 @@ hipError_t run_norm(const NormArgs &a, hipStream_t s) {
         if (a.width <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
         return go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
     });
+}
+
+// A launch takes up to 2^21 rows (its threads are numbered in 32 bits).
+hipError_t run_norm(const NormArgs &a, hipStream_t s) {
+    constexpr int most = 1 << 21;
+    for (int r = 0; r < a.rows; r += std::min(most, a.rows - r)) {
+        NormArgs c = a;
+        c.rows = std::min(most, a.rows - r);
+        c.y = row_at(a.y, r, a.width, a.dtype);
+        c.h = row_at(a.h, r, a.width, a.hdtype);
+        c.h_out = row_at(a.h_out, r, a.width, a.hdtype);
+        c.x_out = row_at(a.x_out, r, a.width, a.dtype);
+        if (a.gate_kind == GATE_ROW || a.gate_kind == GATE_FULL)
+            c.gate = row_at(a.gate, r, a.gate_kind == GATE_ROW ? 1 : a.width, a.gate_dtype);
+        const hipError_t e = launch_norm(c, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // A thread has one vector of the row up to 6144 values (12 waves: 168 registers), then two and four.

@@ -1241,8 +1241,8 @@ def moe_route(router_logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] 
     dev, guard = _on_one_device("moe_route", lg, bias, mask)
     with guard:
         shape = (*lg.shape[:-1], max(k, 0))
-        inds = torch.empty(shape, dtype=torch.int32, device=dev)
-        scores = torch.empty(shape, dtype=torch.float32, device=dev)
+        inds = lg.new_empty(shape, dtype=torch.int32)
+        scores = lg.new_empty(shape, dtype=torch.float32)
         _check(_lib.load().exl3_route(lg.data_ptr(), dt, rows, experts, k, _ptr(bias), code, groups, topk_groups, group_top,
                                       bool(renormalize), float(scale), _ptr(mask), inds.data_ptr(), scores.data_ptr(),
                                       _raw_stream(dev.index)))
@@ -1367,11 +1367,9 @@ def block_norm_backward(dh: Optional[torch.Tensor], dx: Optional[torch.Tensor], 
     with guard:
         dy = torch.empty_like(y)
         dres = torch.empty_like(stream_like) if with_dresidual else None
-        dpost = None if post_weight is None else torch.empty(width, dtype=torch.float32, device=dev)
-        dpre = None if pre_weight is None else torch.empty(width, dtype=torch.float32, device=dev)
-        dgate = None
-        if gate is not None:
-            dgate = torch.empty(gate.shape, dtype=gate.dtype if kind == _GATE_FULL else torch.float32, device=dev)
+        dpost = None if post_weight is None else y.new_empty(width, dtype=torch.float32)
+        dpre = None if pre_weight is None else y.new_empty(width, dtype=torch.float32)
+        dgate = None if gate is None else y.new_empty(gate.shape, dtype=gate.dtype if kind == _GATE_FULL else torch.float32)
         L = _lib.load()
         stream = _raw_stream(dev.index)
         ws = workspace.get(dev, L.exl3_block_norm_backward_workspace_size(rows, width), stream)
@@ -1399,12 +1397,12 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional
     if not grads:
         raise BadExl3Shape("clip_grad_norm: no gradients")
     outs = None if out is None else list(out)
-    if outs is not None and [t.shape for t in outs] != [t.shape for t in grads]:
+    if outs is not None and (len(outs) != len(grads) or any(o.shape != g.shape for o, g in zip(outs, grads))):
         raise BadExl3Shape("clip_grad_norm: out must hold a tensor of each gradient's shape")
     n = len(grads)
     dev, guard = _on_one_device("clip_grad_norm", *grads, *(outs or ()))
     with guard:
-        result = torch.empty(2, dtype=torch.float32, device=dev)
+        result = grads[0].new_empty(2, dtype=torch.float32)
         L = _lib.load()
         stream = _raw_stream(dev.index)
         ws = workspace.get(dev, L.exl3_clip_grad_norm_workspace_size(n), stream)
