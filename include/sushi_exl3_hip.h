@@ -454,7 +454,8 @@ int32_t exl3_route_backward(const void *logits, int32_t dtype, int32_t rows, int
  * y and x_out [rows][width] in dtype, h (or null: 0) and h_out in h_dtype, which is dtype or f32; post and pre [width] in
  * f16, bf16 or f32 each, or null (without pre there is no x_out); gate by gate_kind: none, [width] or [rows] in gate_dtype, or
  * [rows][width] in dtype.  x_out comes of the h_out that is not rounded yet; each output is rounded once.  h_out may be h and
- * x_out may be y; other overlaps of an output are refused.  eps > 0, width <= 16384.
+ * x_out may be y; other overlaps of an output are refused.  2^-126 <= eps < inf, width <= 16384.  Sums are f32: a row whose
+ * squares pass f32's range norms to zeros (an infinity among its values to NaN).
  *
  * Backward, from dh (like h_out, or null: 0), dx (like x_out, with pre), y and h (h_out as the forward wrote it, with pre):
  * dy (like y), dresidual (like h, or null: not wanted), dpost and dpre f32 [width] (with post, pre), dgate as gate was broadcast:

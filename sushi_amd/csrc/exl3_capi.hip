@@ -1838,7 +1838,7 @@ int32_t block_norm_checks(const char *what, int32_t dtype, int32_t h_dtype, int3
     if (gate_kind < GATE_NONE || gate_kind > GATE_FULL || (rows > 0 && (gate_kind != GATE_NONE) != (gate != nullptr)))
         return fail(EXL3_ERR_BAD_SHAPE, "%s: gate kind %d and its operand do not agree", what, gate_kind);
     if (gate_kind == GATE_FULL && gate_dtype != dtype) return fail(EXL3_ERR_BAD_DTYPE, "%s: a full gate is in y's type", what);
-    if (!(eps > 0.f)) return fail(EXL3_ERR_BAD_SHAPE, "%s: eps must be positive", what);
+    if (!(eps >= 0x1p-126f) || eps == INFINITY) return fail(EXL3_ERR_BAD_SHAPE, "%s: eps must be positive and normal", what);
     *gate_bytes = gate_kind == GATE_NONE ? 0
                                          : (gate_kind == GATE_CHANNEL ? 1 : (size_t)rows) * (gate_kind == GATE_ROW ? 1 : (size_t)width) *
                                                elem_size(gate_dtype);

@@ -1329,6 +1329,7 @@ def block_norm(y: torch.Tensor, h: Optional[torch.Tensor] = None, post_weight: O
 
     y and x share a dtype (f16, bf16 or f32); h and h_new are in that or f32 (without h, h_new is in y's).  post_weight and
     pre_weight [D] f16, bf16 or f32 each; gate [D] or [.., 1] in any of them, or like y.  x comes of h_new before its rounding.
+    D up to 16384.
     Not recorded by autograd."""
     rows, width, kind = _block_norm_operands("block_norm", y, (h,), post_weight, pre_weight, gate)
     dt = _dt(y, "y")

@@ -72,7 +72,7 @@ NORM_CASES = [
     (-1, dict(rows=-1)), (-1, dict(width=0)), (-1, dict(width=16385)), (-2, dict(dt=3)), (-2, dict(hdt=0)), (-2, dict(dt=2)),
     (-2, dict(pdt=5)), (-2, dict(qdt=3)), (-2, dict(gate=13 * B, kind=1, gdt=4)), (-2, dict(gate=13 * B, kind=3, gdt=2)),
     (-1, dict(gate=13 * B)), (-1, dict(kind=1)), (-1, dict(gate=13 * B, kind=4)), (-1, dict(kind=-1)),
-    (-1, dict(eps=0.0)), (-1, dict(eps=-1e-6)), (-1, dict(eps=math.nan)), (-1, dict(y=None)), (-1, dict(y=B + 1)), (-1, dict(h=2 * B + 1)),
+    (-1, dict(eps=0.0)), (-1, dict(eps=-1e-6)), (-1, dict(eps=math.nan)), (-1, dict(eps=1e-40)), (-1, dict(eps=math.inf)), (-1, dict(y=None)), (-1, dict(y=B + 1)), (-1, dict(h=2 * B + 1)),
     (-1, dict(post=5 * B + 1)), (-1, dict(gate=13 * B + 2, kind=2, gdt=2)),
 ]
 
