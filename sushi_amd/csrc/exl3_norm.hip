@@ -135,6 +135,7 @@ __global__ __launch_bounds__(MAXT == 64 ? 256 : MAXT) void norm_kernel(NormArgs 
 template <int DT, int HT, int MAXT, int NV, bool WHOLE, bool CHANNEL>
 __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CHANNEL ? 4 : 2) void norm_backward_kernel(NormGradArgs a) {
     constexpr bool REGS = NV <= 2, AHEAD = NV == 1;
+    constexpr bool GATE_AHEAD = AHEAD && !CHANNEL && (WHOLE || MAXT != 512);  // (there 128 registers do not hold it)
     const int t = threadIdx.x, TPR = blockDim.x;
     __shared__ float red[2][MAXT / 64][3], red2[2][MAXT / 64][1];
     if (MAXT > 64) {
@@ -186,12 +187,15 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
     struct Row {
         Raw8<DT> y[NV], dx[REGS ? NV : 1];
         Raw8<HT> dh[1], h[REGS ? NV : 1];
+        Raw8<DT> gate[1];  // like y
     };
     auto fetch = [&](size_t row, Row &r) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             load_raw<DT, WHOLE>(row_at(a.y, row, a.width, DT), col(i), a.width, r.y[i]);
             if (AHEAD && a.dh) load_raw<HT, WHOLE>(row_at(a.dh, row, a.width, HT), col(i), a.width, r.dh[0]);
+            if (GATE_AHEAD && gate_kind == GATE_FULL)
+                load_raw<DT, WHOLE>(row_at(a.gate, row, a.width, DT), col(i), a.width, r.gate[0]);
             if (REGS && a.pre) {
                 load_raw<HT, WHOLE>(row_at(a.h, row, a.width, HT), col(i), a.width, r.h[i % (REGS ? NV : 1)]);
                 load_raw<DT, WHOLE>(row_at(a.dx, row, a.width, DT), col(i), a.width, r.dx[i % (REGS ? NV : 1)]);
@@ -202,24 +206,36 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
     if constexpr (AHEAD) {
         fetch(blockIdx.x, now);
         RawAny pre, post, gate;
-        if (a.pre) pre.load<WHOLE>(a.pre, a.pre_dtype, col(0), a.width);
-        if (a.post) post.load<WHOLE>(a.post, a.post_dtype, col(0), a.width);
-        if (CHANNEL) gate.load<WHOLE>(a.gate, a.gate_dtype, col(0), a.width);
-        if (a.pre) pre.get(a.pre_dtype, a.offset, wpre);
-        if (a.post) post.get(a.post_dtype, a.offset, wpost);
+        if (a.pre) pre.load_row<WHOLE>(a.pre, a.pre_dtype, col(0), a.width);
+        if (a.post) post.load_row<WHOLE>(a.post, a.post_dtype, col(0), a.width);
+        if (CHANNEL) gate.load_row<WHOLE>(a.gate, a.gate_dtype, col(0), a.width);
+        if (a.pre) pre.settle<WHOLE>(a.pre_dtype, col(0), a.width), pre.get(a.pre_dtype, a.offset, wpre);
+        if (a.post) post.settle<WHOLE>(a.post_dtype, col(0), a.width), post.get(a.post_dtype, a.offset, wpost);
         else
 #pragma unroll
             for (int q = 0; q < 8; q++) wpost[q] = 1.f;
-        if (CHANNEL) gate.get(a.gate_dtype, 0.f, wgate);
+        if (CHANNEL) gate.settle<WHOLE>(a.gate_dtype, col(0), a.width), gate.get(a.gate_dtype, 0.f, wgate);
     }
     for (size_t row = blockIdx.x; row < (size_t)a.rows; row += gridDim.x, first = false, flip ^= 1) {
         auto again = [&](int i) -> int {  // where vector i of h and dx is
             if constexpr (REGS) return i;
             load_raw<HT, WHOLE>(row_at(a.h, row, a.width, HT), col(i), a.width, now.h[0]);
             load_raw<DT, WHOLE>(row_at(a.dx, row, a.width, DT), col(i), a.width, now.dx[0]);
+            settle<HT, WHOLE>(col(i), a.width, now.h[0]);
+            settle<DT, WHOLE>(col(i), a.width, now.dx[0]);
             return 0;
         };
         if constexpr (!AHEAD) fetch(row, now);
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            settle<DT, WHOLE>(col(i), a.width, now.y[i]);
+            if (AHEAD && a.dh) settle<HT, WHOLE>(col(i), a.width, now.dh[0]);
+            if (GATE_AHEAD && gate_kind == GATE_FULL) settle<DT, WHOLE>(col(i), a.width, now.gate[0]);
+            if (REGS && a.pre) {
+                settle<HT, WHOLE>(col(i), a.width, now.h[i % (REGS ? NV : 1)]);
+                settle<DT, WHOLE>(col(i), a.width, now.dx[i % (REGS ? NV : 1)]);
+            }
+        }
         const float row_gate = gate_kind == GATE_ROW ? load_any(a.gate, a.gate_dtype, row) : 1.f;
         Raw8<DT> y[NV];
         float H[NV][8];
@@ -247,7 +263,7 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
         }
         // (a row's h and dx leave for good below where they are kept, so that the next row's may come)
         Raw8<HT> h1 = now.h[0];
-        Raw8<DT> dx1 = now.dx[0];
+        Raw8<DT> dx1 = now.dx[0], gate1 = now.gate[0];
         if constexpr (AHEAD) {
             if (row + gridDim.x < (size_t)a.rows) fetch(row + gridDim.x, now);
         }
@@ -283,6 +299,9 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
                 if constexpr (CHANNEL && AHEAD) {
 #pragma unroll
                     for (int q = 0; q < 8; q++) g[q] = wgate[q];
+                } else if constexpr (GATE_AHEAD) {
+#pragma unroll
+                    for (int q = 0; q < 8; q++) g[q] = gate1.get(q);
                 } else {
                     gate8<DT, WHOLE>(a.gate, gate_kind, a.gate_dtype, row, col(i), a.width, g);
                 }
@@ -423,6 +442,7 @@ int norm_backward_parts(int rows, int width) {
 hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
     hipError_t e = with_types(a.dtype, a.hdtype, [&](auto DT, auto HT) {
         constexpr int dt = decltype(DT)::value, ht = decltype(HT)::value;
+        const bool whole = a.width % 8 == 0;
         auto go = [&](auto MAXT, auto NV) {
             constexpr int maxt = decltype(MAXT)::value, nv = decltype(NV)::value;
             auto kernel = [&](auto WHOLE, auto CHANNEL) {
@@ -430,16 +450,17 @@ hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
                                    dim3(row_threads(a.width, nv)), 0, s, a);
                 return hipGetLastError();
             };
-            const bool whole = a.width % 8 == 0;
             using std::true_type, std::false_type;
-            if (a.gate_kind == GATE_CHANNEL) return whole ? kernel(true_type{}, true_type{}) : kernel(false_type{}, true_type{});
-            return whole ? kernel(true_type{}, false_type{}) : kernel(false_type{}, false_type{});
+            if constexpr (!(maxt == 768 && ht == DT_F32))
+                if (!whole) return a.gate_kind == GATE_CHANNEL ? kernel(false_type{}, true_type{}) : kernel(false_type{}, false_type{});
+            return a.gate_kind == GATE_CHANNEL ? kernel(true_type{}, true_type{}) : kernel(true_type{}, false_type{});
         };
         using std::integral_constant;
         if (a.width <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
         if (a.width <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
         if (a.width <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
-        if (a.width <= 6144) return go(integral_constant<int, 768>{}, integral_constant<int, 1>{});
+        // (rows with an f32 stream that end inside a vector want more than the 168 registers of 12 waves)
+        if (a.width <= 6144 && (whole || ht != DT_F32)) return go(integral_constant<int, 768>{}, integral_constant<int, 1>{});
         if (a.width <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
         return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
     });
