@@ -1965,7 +1965,7 @@ int32_t exl3_block_norm_backward(const void *dh, const void *dx, const void *y, 
     a.dpost = dpost;
     a.dpre = dpre;
     a.dgate = dgate;
-    a.parts = norm_backward_parts(rows, width);
+    a.parts = norm_backward_parts(a);
     a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kZeroBytes);
     return launched(run_norm_backward(a, stream), "exl3_block_norm_backward");
 }

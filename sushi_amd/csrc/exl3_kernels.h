@@ -474,7 +474,7 @@ struct NormGradArgs {
     int parts;       // workgroups
     float *part;     // [parts][sums][width]: dpre, dpost and dgate [width], those that there are
 };
-int norm_backward_parts(int rows, int width);  // of the gradient, and the most for up to that many rows
+int norm_backward_parts(const NormGradArgs &a);  // of the gradient, and the most of up to that many rows
 int norm_backward_most(int rows, int width);
 hipError_t run_norm(const NormArgs &a, hipStream_t s);
 hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s);

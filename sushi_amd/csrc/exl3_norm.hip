@@ -32,7 +32,7 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[N]) {
 #pragma unroll
     for (int k = 0; k < N; k++) v[k] = wave_total(v[k]);
     if constexpr (MAXT > 64) {
-        const int wave = threadIdx.x >> 6;
+        const int wave = (MAXT <= 256 ? threadIdx.x % MAXT : threadIdx.x) >> 6;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int k = 0; k < N; k++) red[wave][k] = v[k];
@@ -132,13 +132,17 @@ __global__ __launch_bounds__(MAXT == 64 ? 256 : MAXT) void norm_kernel(NormArgs 
 
 // The gradient.  A workgroup takes rows blockIdx.x, + gridDim.x, ..., with the next row's values in flight, and keeps its columns'
 // sums (dpre, dpost, a channel gate's) in registers, up to 16 a thread, or in its part, and leaves them there for the join.
-template <int DT, int HT, int MAXT, int NV, bool WHOLE, bool CHANNEL>
-__global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CHANNEL ? 4 : 2) void norm_backward_kernel(NormGradArgs a) {
+// TEAMS rows at a time where rows are narrow, MAXT threads each: as many rows in flight in fewer parts.
+template <int DT, int HT, int MAXT, int NV, bool WHOLE, bool CHANNEL, int TEAMS>
+__global__ __launch_bounds__(MAXT *TEAMS, NV == 1 && MAXT * TEAMS <= 512 && HT != DT_F32 && !CHANNEL ? 4 : 2) void norm_backward_kernel(NormGradArgs a) {
     constexpr bool REGS = NV <= 2, AHEAD = NV == 1;
     constexpr bool GATE_AHEAD = AHEAD && !CHANNEL && (WHOLE || MAXT != 512);  // (there 128 registers do not hold it)
-    const int t = threadIdx.x, TPR = blockDim.x;
-    __shared__ float red[2][MAXT / 64][3], red2[2][MAXT / 64][1];
-    if (MAXT > 64) {
+    const int TPR = TEAMS > 1 ? MAXT : blockDim.x, t = TEAMS > 1 ? threadIdx.x % MAXT : threadIdx.x;
+    const int team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / MAXT) : 0;
+    __shared__ float reds[TEAMS][2][MAXT / 64][3], reds2[TEAMS][2][MAXT / 64][1];
+    auto &red = reds[team];
+    auto &red2 = reds2[team];
+    if (MAXT > 64 && TEAMS == 1) {
         for (int i = t; i < 6 * MAXT / 64; i += TPR) (&red[0][0][0])[i] = 0.f;
         if (t < 2 * MAXT / 64) (&red2[0][0][0])[t] = 0.f;
         __syncthreads();
@@ -151,11 +155,14 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
     float *part_post = part + (a.pre ? a.width : 0), *part_gate = part_post + (a.post ? a.width : 0);
     using Acc = float[REGS ? NV : 1][8];
     Acc acc_pre = {}, acc_post = {}, acc_gate = {};
-    bool first = true;
+    bool first = true, live = true;  // (a team past the last row takes that row and leaves nothing of it)
     int flip = 0;
+    const size_t rows = (size_t)a.rows, step = (size_t)gridDim.x * TEAMS;
+    auto row_of = [&](size_t row0) { return TEAMS > 1 ? min(row0 + team, rows - 1) : row0; };
     auto col = [&](int i) { return (uint32_t)(i * TPR + t) * 8; };
     auto add = [&](Acc &acc, float *at, int i, const float (&v)[8]) {
         if constexpr (REGS) {
+            if (TEAMS > 1 && !live) return;
 #pragma unroll
             for (int q = 0; q < 8; q++) acc[i][q] += v[q];
         } else {
@@ -204,7 +211,7 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
     };
     Row now;
     if constexpr (AHEAD) {
-        fetch(blockIdx.x, now);
+        fetch(row_of((size_t)blockIdx.x * TEAMS), now);
         RawAny pre, post, gate;
         if (a.pre) pre.load_row<WHOLE>(a.pre, a.pre_dtype, col(0), a.width);
         if (a.post) post.load_row<WHOLE>(a.post, a.post_dtype, col(0), a.width);
@@ -216,7 +223,9 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
             for (int q = 0; q < 8; q++) wpost[q] = 1.f;
         if (CHANNEL) gate.settle<WHOLE>(a.gate_dtype, col(0), a.width), gate.get(a.gate_dtype, 0.f, wgate);
     }
-    for (size_t row = blockIdx.x; row < (size_t)a.rows; row += gridDim.x, first = false, flip ^= 1) {
+    for (size_t row0 = (size_t)blockIdx.x * TEAMS; row0 < rows; row0 += step, first = false, flip ^= 1) {
+        const size_t row = row_of(row0);
+        live = TEAMS == 1 || row0 + team < rows;
         auto again = [&](int i) -> int {  // where vector i of h and dx is
             if constexpr (REGS) return i;
             load_raw<HT, WHOLE>(row_at(a.h, row, a.width, HT), col(i), a.width, now.h[0]);
@@ -265,7 +274,7 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
         Raw8<HT> h1 = now.h[0];
         Raw8<DT> dx1 = now.dx[0], gate1 = now.gate[0];
         if constexpr (AHEAD) {
-            if (row + gridDim.x < (size_t)a.rows) fetch(row + gridDim.x, now);
+            if (row0 + step < rows) fetch(row_of(row0 + step), now);
         }
         if (a.pre || a.post) row_sum<MAXT, 3>(s, red[flip]);
         const float r = a.pre ? __builtin_amdgcn_rsqf(s[0] * inv_width + a.eps) : 0.f;
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
                 }
                 add(acc_pre, part, i, d);
             }
-            if (a.dres) {
+            if (a.dres && live) {
 #pragma unroll
                 for (int q = 0; q < 8; q++) d[q] = a.residual_scale * H[i][q];
                 store8<HT, WHOLE>(row_at(a.dres, row, a.width, HT), col(i), a.width, d);
@@ -311,7 +320,7 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
                     H[i][q] *= g[q];
                 }
                 if (CHANNEL) add(acc_gate, part_gate, i, d);
-                else store8<DT, WHOLE>(row_at(a.dgate, row, a.width, DT), col(i), a.width, d);
+                else if (live) store8<DT, WHOLE>(row_at(a.dgate, row, a.width, DT), col(i), a.width, d);
             }
             if (a.post) {
 #pragma unroll
@@ -328,16 +337,32 @@ __global__ __launch_bounds__(MAXT, NV == 1 && MAXT <= 512 && HT != DT_F32 && !CH
         }
         if (a.post || gate_kind == GATE_ROW) row_sum<MAXT, 1>(s2, red2[flip]);
         // (a row's gate is a factor of the whole row: its gradient and the mean come of one sum)
-        if (gate_kind == GATE_ROW && t == 0) static_cast<float *>(a.dgate)[row] = s2[0] * qf;
+        if (gate_kind == GATE_ROW && t == 0 && live) static_cast<float *>(a.dgate)[row] = s2[0] * qf;
         const float along_y = qf * qf * (s2[0] * inv_width), out = qf * row_gate;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
 #pragma unroll
             for (int q = 0; q < 8; q++) H[i][q] = out * (a.post ? H[i][q] - now_y(i, q) * along_y : H[i][q]);
-            store8<DT, WHOLE>(row_at(a.dy, row, a.width, DT), col(i), a.width, H[i]);
+            if (live) store8<DT, WHOLE>(row_at(a.dy, row, a.width, DT), col(i), a.width, H[i]);
         }
     }
-    if constexpr (REGS) {
+    if constexpr (TEAMS > 1) {  // the teams' sums, in order
+        __shared__ __align__(16) float fold[TEAMS][MAXT * 8];
+        auto join = [&](const float (&acc)[8], float *to) {
+            store8<DT_F32, WHOLE>(fold[team], col(0), a.width, acc);
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.width; c += MAXT * TEAMS) {
+                float s = fold[0][c];
+#pragma unroll
+                for (int k = 1; k < TEAMS; k++) s += fold[k][c];
+                to[c] = s;
+            }
+            __syncthreads();
+        };
+        if (a.pre) join(acc_pre[0], part);
+        if (a.post) join(acc_post[0], part_post);
+        if (CHANNEL) join(acc_gate[0], part_gate);
+    } else if constexpr (REGS) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             if (a.pre) store8<DT_F32, WHOLE>(part, col(i), a.width, acc_pre[i]);
@@ -421,22 +446,27 @@ hipError_t run_norm(const NormArgs &a, hipStream_t s) {
     return hipSuccess;
 }
 
-// A thread has one vector of the row up to 6144 values (12 waves: 168 registers), then two and four.
-static int backward_vectors(int width) { return width <= 6144 ? 1 : width <= 8192 ? 2 : 4; }
+// Rows of up to 2048 values go by teams of one, two or four waves, eight waves a workgroup: with a workgroup a row there would be
+// four times the parts for as many rows in flight (8192 bf16 rows of 512 / 680 values: 20.0 / 24.4 us, by teams 13.7 / 19.6).
+constexpr int backward_teams(int width) { return width <= 512 ? 8 : width <= 1024 ? 4 : width <= 2048 ? 2 : 1; }
 
 // Workgroups of the gradient.  More of them hide a row's latency (1.0 us a row of 512 values, 1.5 of 4096, its loads ahead) and
-// leave more parts to the join.  One a CU up to 2048 rows (narrow rows: two), then two where two fit (narrow rows: four), each
-// the same number of rows.  us in a graph at 256 / 512 / 1024 workgroups, bf16 with both norms: 333 rows of 4096 values 11.5 / 14.7
-// / -, 2048 rows 23.9 / 22.4 / 28.7, 8192 rows 65.8 / 62.2 / 66.1; rows of 512 values: 1024 of them 9.4 / 9.0 / 10.7, 8192
-// 39.6 / 25.7 / 20.0; 8192 rows of 6144 90.1 / 94.2 / 106.3.
-int norm_backward_most(int rows, int width) {
-    const int waves = row_threads(width, backward_vectors(width)) / 64;
-    const int a_cu = waves <= 2 ? (rows >= 4096 ? 4 : rows >= 512 ? 2 : 1) : waves <= 8 && rows >= 2048 ? 2 : 1;
-    return rows < 256 * a_cu ? rows : 256 * a_cu;
+// leave more parts to the join.  One a CU; two where both fit on it by their registers (without an f32 stream and a channel gate)
+// and there are rows enough, each the same number of rows.  us in a graph at 256 / 512 / 1024 workgroups, bf16 with both norms:
+// 8192 rows of 200 values 12.2 / 12.3 / 14.9, 16384 of 512 20.0 / 19.2 / 22.7; 2048 of 680 10.3 / 11.0 / 11.0, 8192 of 680
+// 22.2 / 19.6 / 23.0; 333 rows of 4096 11.5 / 14.7 / -, 2048 rows 23.9 / 22.4 / 28.7, 8192 rows 65.8 / 62.2 / 66.1; 8192 rows of
+// 6144 90.1 / 94.2 / 106.3; f32, 8192 rows of 1024 29.4 / 32.4 / 38.6.
+static int backward_workgroups(int rows, int width, bool two) {
+    const int teams = backward_teams(width), sets = (int)(((long)rows + teams - 1) / teams);
+    const bool many = rows >= (width <= 512 ? 16384 : width <= 2048 ? 4096 : 2048) && width <= 4096;
+    return std::min(sets, two && many ? 512 : 256);
 }
-int norm_backward_parts(int rows, int width) {
-    const int most = norm_backward_most(rows, width), each = most ? (rows + most - 1) / most : 1;
-    return (rows + each - 1) / each;
+int norm_backward_most(int rows, int width) { return backward_workgroups(rows, width, true); }
+int norm_backward_parts(const NormGradArgs &a) {
+    const int teams = backward_teams(a.width), sets = (int)(((long)a.rows + teams - 1) / teams);
+    const int most = backward_workgroups(a.rows, a.width, a.hdtype != DT_F32 && a.gate_kind != GATE_CHANNEL);
+    const int each = most ? (sets + most - 1) / most : 1;
+    return (sets + each - 1) / each;
 }
 
 hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
@@ -444,10 +474,10 @@ hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
         constexpr int dt = decltype(DT)::value, ht = decltype(HT)::value;
         const bool whole = a.width % 8 == 0;
         auto go = [&](auto MAXT, auto NV) {
-            constexpr int maxt = decltype(MAXT)::value, nv = decltype(NV)::value;
+            constexpr int maxt = decltype(MAXT)::value, nv = decltype(NV)::value, teams = maxt <= 256 ? 512 / maxt : 1;
             auto kernel = [&](auto WHOLE, auto CHANNEL) {
-                hipLaunchKernelGGL((norm_backward_kernel<dt, ht, maxt, nv, decltype(WHOLE)::value, decltype(CHANNEL)::value>), dim3(a.parts),
-                                   dim3(row_threads(a.width, nv)), 0, s, a);
+                hipLaunchKernelGGL((norm_backward_kernel<dt, ht, maxt, nv, decltype(WHOLE)::value, decltype(CHANNEL)::value, teams>),
+                                   dim3(a.parts), dim3(teams > 1 ? maxt * teams : row_threads(a.width, nv)), 0, s, a);
                 return hipGetLastError();
             };
             using std::true_type, std::false_type;
@@ -457,6 +487,7 @@ hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
         };
         using std::integral_constant;
         if (a.width <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+        if (a.width <= 1024) return go(integral_constant<int, 128>{}, integral_constant<int, 1>{});
         if (a.width <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
         if (a.width <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
         // (rows with an f32 stream that end inside a vector want more than the 168 registers of 12 waves)
