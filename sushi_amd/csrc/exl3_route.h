@@ -387,12 +387,14 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
     const size_t r = r0 + grp;
     const bool in = r < rows, live = in && (!a.mask || a.mask[in ? r : 0] != 0);
     const char *row = static_cast<const char *>(a.logits) + (in ? r : r0) * a.experts * (DT == DT_F32 ? 4 : 2);
+    // A vector may pass the row's end into the next rows, and its values there go; past the last row it goes by elements.
+    const int reach = (int)min(rows - (in ? r : r0), (size_t)8) * a.experts;
     bool bad = false;
     // A unit's logits, -inf for experts that are out by them and past the unit's own; whether the wave has any of those.
     auto load = [&](int u, float (&v)[8]) {
         Raw8<DT> raw;
         const int first = first_of(u), n = count_of(u);
-        if (n > 0 && first + 8 <= a.experts) raw.load(elem<DT>(row, first));
+        if (n > 0 && first + 8 <= reach) raw.load(elem<DT>(row, first));
         else raw.load_some(elem<DT>(row, first), n);
         if (n < 8) raw.keep(n);
         bool odd = false;
