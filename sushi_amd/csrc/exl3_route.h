@@ -247,11 +247,11 @@ __global__ __launch_bounds__(RT_THREADS) void route_kernel(RouteArgs a) {
 // A key is 32 bits: a value and, in the low bits, the complement of its expert's place, so a comparator of a sorting network
 // is one maximum and one minimum of integers.  (A whole f32 above a number, as an f64, costs four times as much a comparator:
 // 65521 rows of 256 bf16 logits 23.6 us.)  The value is
-//   a 16-bit logit, whose f32 bits leave the low ones free (EXACT: the keys' order is the choice's),
-//   an f32 logit's distance from the row's largest, as a float of 5 exponent bits (2^-20 .. 2^12) and what mantissa is left,
+//   a 16-bit logit, whose f32 bits leave the low ones free (the keys' order is the choice's),
+//   an f32 logit without its low bits (6 to 10 of them): those that share a key are put in order by the logits themselves,
 //   or c in steps of the range that p and the bias span.
-// Where two values of the last two kinds decide and lie closer than their key or c's own f32 error tells, the wave takes the
-// row again in 64 bits.
+// Where two values of c decide and lie closer than c's steps or its f32 error tell, and where f32 logits at the edge of the picks
+// share a key and differ, the wave takes the row again in 64 bits.
 //
 // The loops over a lane's units stay rolled: the kernel is short, so a call of few rows fetches less of it, and few registers
 // leave room for more waves.
@@ -313,11 +313,6 @@ __device__ __forceinline__ bool group_any(bool v) {
 __device__ __forceinline__ float near_of(const RouteArgs &a, float inv_den, float c) {
     return (a.sigmoid ? 0x1p-21f : 0x1p-17f * inv_den) + 0x1p-22f * c;
 }
-
-// M - v as 31 bits, and back (to its truncation): 0 below 2^-20, 0x7FFFFFFF for an expert that is out.
-constexpr uint32_t kDistBase = 107u << 23, kDistOut = (1u << 28) - 1;
-__device__ __forceinline__ uint32_t dist_bits(float d) { return __builtin_elementwise_sub_sat(__float_as_uint(d), kDistBase); }
-__device__ __forceinline__ float bits_dist(uint32_t b) { return b == 0 ? 0.f : __uint_as_float(b + kDistBase); }
 
 // An integer of c's steps: 0 for what is not above it, NaN too (the conversion saturates, which C++ does not say).
 __device__ __forceinline__ uint32_t to_steps(float x) {
@@ -415,7 +410,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
     };
     const bool whole = !a.sigmoid && !(BY_LOGIT && a.renorm);  // the softmax over the row
     float mx = -INFINITY, inv = 1.f;
-    if (whole || (by_logit && !exact)) {
+    if (whole) {
 #pragma unroll 1
         for (int i = 0; i < nu; i++) {
             float v[8];
@@ -523,46 +518,49 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         wave_order();
         units_left = (a.taken * units + L - 1) / L;
     }
-    int best[T], next = INT32_MIN;
-#pragma unroll 1
-    for (int i = 0; i < units_left; i++) {
-        int u = i * L + l;
+    // The lane's i-th unit of those left, and whether there is one; its kept values; its logits, -inf for what is out.
+    auto unit_of = [&](int i, int &u) {
+        u = i * L + l;
         bool is = true;
         if constexpr (GROUPED) {  // the u-th unit of the open groups
             const int nth = group_of(u);
             is = nth < opened;
             u += is ? (list[nth] - nth) * units : -u;
         }
+        return is;
+    };
+    auto kept = [&](int u, float (&v)[8]) {
+        const float4 *o = reinterpret_cast<const float4 *>(vals + u * 8);
+        const float4 v0 = o[0], v1 = o[1];
+        v[0] = v0.x, v[1] = v0.y, v[2] = v0.z, v[3] = v0.w, v[4] = v1.x, v[5] = v1.y, v[6] = v1.z, v[7] = v1.w;
+    };
+    auto logits_of = [&](int u, bool is, float (&v)[8]) {
+        if (GROUPED && groups_by_logit) kept(u, v);
+        else load(u, v);
+        if constexpr (GROUPED)
+            if (!is)
+#pragma unroll
+                for (int q = 0; q < 8; q++) v[q] = -INFINITY;
+    };
+    // A logit's part of its key: its bits in the order of integers (-0 is 0), an f32's without the low ones.
+    auto logit_key = [&](float v) {
+        const int b = __float_as_int(v + 0.f);
+        return (b ^ ((b >> 31) & value_mask)) & ~id_mask;
+    };
+    int best[T], next = INT32_MIN;
+#pragma unroll 1
+    for (int i = 0; i < units_left; i++) {
+        int u;
+        const bool is = unit_of(i, u);
         float v[8];
         int k8[8];
         const int not_id = ~(u * 8 + 7) & id_mask;
-        auto kept = [&]() {
-            const float4 *o = reinterpret_cast<const float4 *>(vals + u * 8);
-            const float4 v0 = o[0], v1 = o[1];
-            v[0] = v0.x, v[1] = v0.y, v[2] = v0.z, v[3] = v0.w, v[4] = v1.x, v[5] = v1.y, v[6] = v1.z, v[7] = v1.w;
-        };
         if (by_logit) {
-            if (GROUPED && groups_by_logit) kept();
-            else load(u, v);
-            if constexpr (GROUPED)
-                if (!is)
+            logits_of(u, is, v);
 #pragma unroll
-                    for (int q = 0; q < 8; q++) v[q] = -INFINITY;
-            if (DT != DT_F32) {
-#pragma unroll
-                for (int q = 0; q < 8; q++) {
-                    const int b = __float_as_int(v[q] + 0.f);  // (-0 is 0)
-                    k8[q] = b ^ (((b >> 31) & value_mask) | not_id | (7 - q));
-                }
-            } else {
-#pragma unroll
-                for (int q = 0; q < 8; q++) {  // (what is out is at the end of the distances)
-                    const uint32_t d = min(dist_bits(mx - v[q]), kDistOut);
-                    k8[q] = (int)((~d << 3) & (uint32_t)value_mask) | not_id | (7 - q);
-                }
-            }
+            for (int q = 0; q < 8; q++) k8[q] = logit_key(v[q]) | not_id | (7 - q);
         } else {
-            if constexpr (GROUPED) kept();
+            if constexpr (GROUPED) kept(u, v);
             else values(u, v);
             const float by = is ? steps : 0.f, one = is ? 1.f : 0.f;
 #pragma unroll
@@ -589,26 +587,21 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
     if constexpr (L > 16) merge_lanes<16>(best, next);
     if constexpr (L > 32) merge_lanes<32>(best, next);
     bad = group_any<L>(bad);
-    // keys of experts that are out: what -inf, the end of the distances or no step makes
-    const int out = exact ? (int)(0xFF800000u ^ (uint32_t)value_mask) | id_mask : id_mask;
-    // Two values that decide and lie close: the row goes by 64 bits.  `least`: no pick is below it.
+    // keys of experts that are out: what -inf or no step makes
+    const int out = by_logit ? (int)(0xFF800000u ^ (uint32_t)value_mask) | id_mask : id_mask;
+    // Two values of c that decide and lie close: the row goes by 64 bits.  `least`: no pick is below it.  f32 logits are out of
+    // order only among those that share a key: `tied` picks, or the last pick and the next at the `edge`.
     double least = -INFINITY;
+    bool tied = false, edge = false;
     if (!exact) {
         int last = 0;
         if (by_logit) {
-            const float tol = 0x1p-22f * fabsf(mx), trunc = 2.f / (float)(1 << (26 - id_bits));  // two truncations
-            auto dist = [&](int key) { return bits_dist((~(uint32_t)key & (uint32_t)value_mask) >> 3); };
 #pragma unroll
             for (int i = 0; i <= T; i++) {
                 const int key = i < T ? best[i < T ? i : 0] : next;
-                const float d = dist(key);
-                // (an expert that is out has a distance of its own only among the picks)
-                if (i > 0 && i <= a.topk && key > out)
-                    near |= d * (1.f - trunc) - dist(last) <= tol + (d < 0x1p-19f ? 0x1p-20f : 0.f);
-                if (i < a.topk) {
-                    near |= d >= 0x1p11f;  // at the end of the distances, or out
-                    least = d >= 0x1p11f ? -INFINITY : (double)mx - (double)d * (1. + trunc) - (double)tol - 0x1p-19;
-                }
+                const bool same = i > 0 && key > out && !((key ^ last) & ~id_mask);
+                tied |= same && i < a.topk;
+                edge |= same && i == a.topk;
                 last = key;
             }
         } else {
@@ -622,10 +615,6 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
                 last = key;
             }
         }
-    }
-    if (!BY_LOGIT || DT == DT_F32) {
-        near = group_any<L>(near || near_group) && live;
-        near_group = group_any<L>(near_group);
     }
     // a lane a slot: its expert and its logit
     int key = best[0], slot = l & (T - 1);
@@ -642,6 +631,40 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         px = load_act<DT>(elem<DT>(row, has ? e : 0), 0);
     }
     px = has ? px : -INFINITY;
+    int to = l;
+    if constexpr (DT == DT_F32) {
+        if (__any(edge)) {  // in order all the same if what shares the last pick's key is equal to it
+            const float x = __shfl(px, a.topk - 1, L);
+            const int shared = __shfl(key, a.topk - 1, L) & ~id_mask;
+            bool other = false;
+#pragma unroll 1
+            for (int i = 0; i < units_left; i++) {
+                int u;
+                const bool is = unit_of(i, u);
+                float v[8];
+                logits_of(u, is, v);
+#pragma unroll
+                for (int q = 0; q < 8; q++) other |= logit_key(v[q]) == shared && v[q] != x;
+            }
+            if (edge && group_any<L>(other)) {
+                near = true;
+                least = __int_as_float(shared < 0 ? (shared ^ value_mask) | id_mask : shared);
+            }
+        }
+        if (__any(tied)) {
+            int ahead = 0;
+            for (int j = 0; j < a.topk; j++) {
+                const float x = __shfl(px, j, L);
+                const int o = __shfl(e, j, L);
+                ahead += x > px || (x == px && o < e) ? 1 : 0;
+            }
+            to = has ? ahead : l;
+        }
+    }
+    if (!BY_LOGIT || DT == DT_F32) {
+        near = group_any<L>(near || near_group) && live;
+        near_group = group_any<L>(near_group);
+    }
     const float top = group_max<T>(a.sigmoid ? fminf(px, 0.f) : px);
     float w = has ? pick_weight(a, px, top, mx, inv) : 0.f;
     if (a.renorm) {
@@ -649,8 +672,8 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         w = has ? quotient(w, sum) : 0.f;
     }
     if (l < a.topk && in && !near) {
-        a.inds[r * a.topk + l] = has && live ? (uint32_t)e : 0xFFFFFFFFu;
-        a.scores[r * a.topk + l] = !live ? 0.f : bad ? NAN : w * a.scale;
+        a.inds[r * a.topk + to] = has && live ? (uint32_t)e : 0xFFFFFFFFu;
+        a.scores[r * a.topk + to] = !live ? 0.f : bad ? NAN : w * a.scale;
     }
     uint64_t again = __ballot(near && l == 0);
 #pragma unroll 1
