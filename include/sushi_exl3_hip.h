@@ -87,7 +87,7 @@ typedef enum {
     EXL3_ERR_WINDOW_TOO_NARROW = -14,        /* encoder: WindowTooNarrow */
     EXL3_ERR_HESSIAN = -15,                  /* quantizer: HessianNotPositiveDefinite (src/encoder/quantize.zig:351) */
     EXL3_ERR_GROUP_MISSING = -16,            /* Exl3GroupMissing (src/exl3/root.zig:647) */
-    EXL3_ERR_ACTIVATION = -17                /* an activation outside exl3_act (an extension's) */
+    EXL3_ERR_ACTIVATION = -17                /* an activation outside exl3_act, a score outside exl3_score (extensions') */
 } exl3_status;
 
 /* One projection's bank (`Proj`, src/exl3/root.zig:28-30). */
