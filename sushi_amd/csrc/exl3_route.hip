@@ -121,7 +121,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_backward_row_kernel(RouteGra
 
 // The other forms read the picked logits alone and write rows of zeros with the slots' terms in them.  A wave has 64 / LS rows, a
 // lane a slot; the rows lie one after another in its LDS as they do in memory, so they leave in whole vectors whatever the
-// row's length.  Bound by the rows' writes: 65521 rows of 256 bf16, sigmoid over eight slots, 10.9 us (4.0 TB/s with the slots'
+// row's length.  Bound by the rows' writes: 65521 rows of 256 bf16, sigmoid over eight slots, 10.9 us (3.6 TB/s with the slots'
 // reads; as the kernel above does it, a row's lanes holding its experts, 16.5).
 template <int LS, int DT>
 __global__ __launch_bounds__(RT_THREADS) void route_backward_picked_kernel(RouteGradArgs a, int wave_lds) {
