@@ -189,35 +189,58 @@ __device__ __forceinline__ void route_row(const RouteArgs &a, size_t row, int la
     write_picks<DT>(a, row, info, lane, mine);
 }
 
-// A row whose groups are settled (bit g of `open`) and whose picks are all at least `least`, by one wave: the few values that are
-// stand in a list, a lane each, which counts those ahead of its own.  False with more than a wave of them.
+// A row whose groups are settled (bit g of `open`) and whose picks are all at least `least`, by one wave: the few experts that may
+// be stand in a list, a lane each, which counts those ahead of its own.  False with more than a wave of them.  A sigmoid is a
+// logit's own, so only those of the list are taken in 64 bits.
+constexpr int kSettleLds = 64 * 4;  // the list, behind a row's values
 template <int DT>
 __device__ __forceinline__ bool settle_row(const RouteArgs &a, size_t row, int lane, double *buf, bool by_logit, uint64_t open,
                                            double least) {
-    const RowInfo info = row_values<DT>(a, row, lane, buf, by_logit);
+    const bool own = a.sigmoid && !by_logit;
+    RowInfo info = {0.f, 1.f, false};
+    if (!own) info = row_values<DT>(a, row, lane, buf, by_logit);
+    int *const list = reinterpret_cast<int *>(buf + a.experts);
     const int size = a.experts / a.groups;
     wave_order();
-    // (a place of the list is behind every value that is still to be read)
     int count = 0;
-    double mine = -INFINITY;
-    int expert = NO_EXPERT;
+    bool bad = false;
     for (int e0 = 0; e0 < a.experts; e0 += 64) {
-        const int e = e0 + lane;
-        const double c = e < a.experts ? buf[e] : -INFINITY;
-        const bool is = c >= least && c > -INFINITY && ((open >> (a.groups > 1 ? min(e, a.experts - 1) / size : 0)) & 1);
-        uint64_t who = __ballot(is);
-        while (who) {
-            const int from = __ffsll((unsigned long long)who) - 1;
-            who &= who - 1;
-            if (count == 64) return false;
-            const double v = __shfl(c, from);
-            mine = lane == count ? v : mine;
-            expert = lane == count ? e0 + from : expert;
-            count++;
+        const int e = e0 + lane, at = min(e, a.experts - 1);
+        bool is = e < a.experts && ((open >> (a.groups > 1 ? at / size : 0)) & 1);
+        double c = -INFINITY;
+        if (own) {
+            const float x = load_act<DT>(a.logits, row * a.experts + at), b = a.bias ? a.bias[at] : 0.f;
+            bad |= x != x;
+            // (to twice what near_of allows)
+            const float near = rcp(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)) + b;
+            is = is && x > -INFINITY && b > -INFINITY && (double)near + (double)(0x1p-20f + 0x1p-21f * fabsf(near)) >= least;
+        } else {
+            c = buf[at];
+            is = is && c >= least && c > -INFINITY;
         }
+        const uint64_t who = __ballot(is);
+        const int place = count + (int)__popcll(who & ((uint64_t(1) << lane) - 1));
+        count += (int)__popcll(who);
+        if (count > 64) return false;
+        if (is) {  // (a value's place is never past its expert's)
+            list[place] = e;
+            if (!own) buf[place] = c;
+        }
+        wave_order();
+    }
+    const int expert = lane < count ? list[lane] : NO_EXPERT;
+    double mine = -INFINITY;
+    if (own) {
+        info.bad = (bool)__any(bad);
+        if (lane < count) mine = 1. / (1. + exp(-(double)load_act<DT>(a.logits, row * a.experts + expert))) + (double)(a.bias ? a.bias[expert] : 0.f);
+    } else if (lane < count) {
+        mine = buf[lane];
     }
     int ahead = 0;
-    for (int i = 0; i < count; i++) ahead += better(__shfl(mine, i), __shfl(expert, i), mine, expert) ? 1 : 0;
+    for (int i = 0; i < count; i++) {
+        const double c = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(mine), i), __builtin_amdgcn_readlane(__double2loint(mine), i));
+        ahead += better(c, __builtin_amdgcn_readlane(expert, i), mine, expert) ? 1 : 0;
+    }
     // lanes behind the list take the slots that no expert is left for
     write_picks<DT>(a, row, info, lane < count ? ahead : lane, expert);
     return true;
@@ -707,8 +730,8 @@ static hipError_t launch_lists(const RouteArgs &a, int units, hipStream_t s) {
     const int nu = (units + L - 1) / L;
     int id_bits = 6;
     while ((1 << id_bits) < L * nu * 8) id_bits++;
-    // the values and the groups' worths of a wave's rows; a row's values in 64 bits
-    const int lists = grouped ? nu * 2048 + 64 / L * 32 + (64 / L * a.groups * 4 + 15) / 16 * 16 : 0, row = (a.experts * 8 + 15) / 16 * 16;
+    // the values and the groups' worths of a wave's rows; a row's values in 64 bits and the list that settles it
+    const int lists = grouped ? nu * 2048 + 64 / L * 32 + (64 / L * a.groups * 4 + 15) / 16 * 16 : 0, row = (a.experts * 8 + kSettleLds + 15) / 16 * 16;
     const int lds = lists > row ? lists : row;
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(RT_THREADS), RT_WAVES * lds + (by_logit ? 0 : L * nu * 32), s, a, nu, id_bits, lds); };
     if (by_logit) grouped ? go(route_lists_kernel<L, T, DT, true, true>) : go(route_lists_kernel<L, T, DT, true, false>);
