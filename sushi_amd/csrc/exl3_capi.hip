@@ -2020,9 +2020,11 @@ int32_t exl3_clip_grad_norm(int32_t count, const void *const *grads, const int64
         for (; next < count && t.count < kClipTensors; next++) {
             if (!numel[next]) continue;
             const int k = t.count++;
-            t.e[k] = {grads[next], out ? out[next] : const_cast<void *>(grads[next]), numel[next], t.chunks, (uint8_t)dtypes[next],
+            const int32_t chunks = (int32_t)((numel[next] + kClipChunk - 1) / kClipChunk);
+            t.e[k] = {grads[next], out ? out[next] : const_cast<void *>(grads[next]), t.chunks,
+                      (uint16_t)(numel[next] - (int64_t)(chunks - 1) * kClipChunk), (uint8_t)dtypes[next],
                       (uint8_t)(out ? out_dtypes[next] : dtypes[next])};
-            t.chunks += (int32_t)((numel[next] + kClipChunk - 1) / kClipChunk);
+            t.chunks += chunks;
         }
     };
     ClipTensors t{};

@@ -1,7 +1,7 @@
 // The clip of many gradients by their global norm: norm = sqrt(sum of all g^2), scale = norm <= max_norm ? 1 : max_norm / norm,
 // out = g scale.  Two passes over the gradients, as the scale needs every one of them; each is bound by its bytes: 193 tensors of
 // 573 MB (bf16 and f32) in place take 347 us, 5.0 TB/s over two reads and a write.  Small ones are launches, one a pass for every
-// 120 tensors (what a launch's arguments hold): 6 tensors of 0.5 MB take 7.1 us, 144 of 2.6 MB 15.
+// 160 tensors (what a launch's arguments hold): 6 tensors of 0.5 MB take 7.1 us.
 //
 // The tensors of a launch come as arguments.  They are cut into chunks of kClipChunk elements, numbered over the launch, and a
 // workgroup takes a run of them, so that it looks for its tensor once for each that it touches.  Squares are summed in 64 bits
@@ -31,9 +31,11 @@ __device__ __forceinline__ void for_run(const ClipTensors &t, F f) {
     const int per = (t.chunks + (int)gridDim.x - 1) / (int)gridDim.x;
     int first = min(t.chunks, (int)blockIdx.x * per), last = min(t.chunks, first + per);
     while (first < last) {
-        const ClipEntry e = t.e[tensor_of(t, BACK ? last - 1 : first)];
+        const int k = tensor_of(t, BACK ? last - 1 : first), past = k + 1 < t.count ? t.e[min(k + 1, kClipTensors - 1)].first : t.chunks;
+        const ClipEntry e = t.e[k];
         const int c = BACK ? max(first, e.first) : first;
-        const int64_t from = (int64_t)(c - e.first) * kClipChunk, end = min(from + (int64_t)(last - c) * kClipChunk, e.n);
+        const int64_t from = (int64_t)(c - e.first) * kClipChunk, n = (int64_t)(past - 1 - e.first) * kClipChunk + e.last;
+        const int64_t end = min(from + (int64_t)(last - c) * kClipChunk, n);
         f(e, from, end);
         if (BACK) last = c;
         else first += (int)((end - from + kClipChunk - 1) / kClipChunk);

@@ -480,15 +480,15 @@ hipError_t run_norm(const NormArgs &a, hipStream_t s);
 hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s);
 
 // The clip of many gradients by their global norm (exl3_clip.hip): the tensors of one launch as arguments.
-constexpr int kClipTensors = 120;    // a launch's (its arguments stay within 4 KiB)
+constexpr int kClipTensors = 160;    // a launch's (its arguments stay within 4 KiB)
 constexpr int kClipChunk = 8192;     // elements: what a workgroup takes, or a run of
 constexpr int kClipParts = 1024;     // workgroups a launch
 constexpr int64_t kClipMaxElements = int64_t(1) << 36;  // of a tensor: a launch's chunks are numbered in 32 bits
 struct ClipEntry {
     const void *g;
     void *out;
-    int64_t n;
     int32_t first;                   // its first chunk in the launch
+    uint16_t last;                   // elements of its last chunk
     uint8_t dtype, out_dtype;
 };
 struct ClipTensors {

@@ -280,9 +280,9 @@ __global__ __launch_bounds__(RT_THREADS) void route_kernel(RouteArgs a) {
 // The loops over a lane's units stay rolled: the kernel is short, so a call of few rows fetches less of it, and few registers
 // leave room for more waves.
 //
-// Long calls are bound by the issue of vector instructions: 65521 bf16 rows of 256 experts with bias and groups take 34 us, 177
-// instructions a row (22 of a wave's eight rows' each), 19 us of issue, and 4 to 5 us for the rows that go by 64 bits after the
-// others; by the logits alone 12.6 us (f32 21.6), against 7.3 for the bytes.  Short ones are a launch and one row's latency:
+// Long calls are bound by the issue of vector instructions: 65521 bf16 rows of 256 experts with bias and groups take 32 us, about
+// 175 instructions a row, 19 us of issue, and some us for the rows that go by 64 bits after the others; by the logits alone
+// 12.6 us (f32 20), against 7.3 (13) for the bytes.  Short ones are a launch and one row's latency:
 // 6.1 us for 32 rows with bias and groups, 2.6 to 4 by the logits.
 __device__ __forceinline__ void comparator(int &a, int &b) {
     const int hi = max(a, b), lo = min(a, b);
