@@ -1,6 +1,6 @@
 // Eight neighbouring values of an array at any alignment of its elements, as a vector load or store: global memory takes
 // 16 bytes at any address, so rows of odd widths and operands that begin anywhere need no path of their own.  What passes
-// the array's end goes by elements.
+// the array's end goes by elements, or as the last eight values before it.
 #pragma once
 #include "exl3_kernels.h"
 
@@ -114,14 +114,6 @@ struct Raw8 {
     }
 };
 
-// How many of the eight values from c on lie before `width`, counted where it is asked for: in a loop over rows the masks of
-// a row's last vector would otherwise be kept in scalar registers that the loop needs.
-__device__ __forceinline__ int left_of(uint32_t c, uint32_t width) {
-    int n = max(0, (int)(width - c));
-    asm volatile("" : "+v"(n));
-    return n;
-}
-
 // A number counted where it is asked for: in a loop over rows the masks of a row's last vector would otherwise be kept in scalar
 // registers that the loop needs.
 __device__ __forceinline__ int opaque(int n) {
@@ -132,7 +124,7 @@ __device__ __forceinline__ int opaque(int n) {
 // A thread's eight values of a row, from column c on.  A row whose width is no multiple of eight ends inside a vector: that
 // thread takes the row's last eight values instead and leaves out the first `skip`, which are another's: one vector load as
 // everywhere, where elements one by one would each wait for the one before (gradient of 4096 rows of 3079 bf16 values with a
-// channel gate: 83 us by elements, 58 so, 42 at 3080).  Past the row's end all eight are left out.  WHOLE: the width is a multiple
+// channel gate: 83 us by elements, 58 so; 53 and, at 3080, 37 with the workgroups there are now).  Past the row's end all eight are left out.  WHOLE: the width is a multiple
 // of eight, so a vector lies inside or outside.
 struct Place {
     int c, skip;
@@ -143,6 +135,7 @@ __device__ __forceinline__ Place place_of(uint32_t c, uint32_t width) {
     const int at = opaque(min((int)c, (int)width - 8));
     return {at, min(8, (int)c - at)};
 }
+
 // The values as they lie in memory, those to be left out among them (a row of fewer than eight: its elements).
 template <int DT, bool WHOLE>
 __device__ __forceinline__ void load_raw(const void *p, uint32_t c, uint32_t width, Raw8<DT> &r) {
@@ -181,33 +174,12 @@ __device__ __forceinline__ void load8_any(const void *p, int dt, uint32_t c, uin
 // they are asked for, and the loads need no branch by the type.
 struct RawAny {
     Words4 lo, hi;
-    template <bool WHOLE>
-    __device__ __forceinline__ void load(const void *p, int dt, uint32_t c, uint32_t width) {
-        const bool f32 = dt == DT_F32;
-        const char *at = static_cast<const char *>(p) + c * (f32 ? 4u : 2u);
-        lo = hi = Words4{0, 0, 0, 0};
-        if (WHOLE ? c < width : c + 8 <= width) {
-            lo = *reinterpret_cast<const Words4At2 *>(at);
-            if (f32) hi = reinterpret_cast<const Words4At2 *>(at)[1];
-        } else if (!WHOLE) {
-            const int n = left_of(c, width);
-#pragma unroll
-            for (int q = 0; q < 8; q++) {
-                if (q >= n) continue;
-                if (!f32) lo[q / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(at)[q] << (16 * (q & 1));
-                else if (q < 4) lo[q & 3] = reinterpret_cast<const uint32_t *>(at)[q];
-                else hi[q & 3] = reinterpret_cast<const uint32_t *>(at)[q];
-            }
-        }
-    }
     // As load_raw and settle.
     template <bool WHOLE>
     __device__ __forceinline__ void load_row(const void *p, int dt, uint32_t c, uint32_t width) {
-        if (WHOLE) {
-            load<WHOLE>(p, dt, c, width);
-            return;
-        }
-        if (width < 8) {
+        lo = hi = Words4{0, 0, 0, 0};
+        if (WHOLE && c >= width) return;
+        if (!WHOLE && width < 8) {
             Raw8<DT_F32> wide;
             Raw8<DT_F16> half;
             wide.clear(), half.clear();
@@ -217,15 +189,13 @@ struct RawAny {
             for (int q = 0; q < 4; q++) lo[q] = dt == DT_F32 ? wide.w[q] : half.w[q], hi[q] = wide.w[4 + q];
             return;
         }
-        const uint32_t at = (uint32_t)place_of<WHOLE>(c, width).c;
-        const char *s = static_cast<const char *>(p) + at * (dt == DT_F32 ? 4u : 2u);
-        lo = *reinterpret_cast<const Words4At2 *>(s);
-        hi = Words4{0, 0, 0, 0};
-        if (dt == DT_F32) hi = reinterpret_cast<const Words4At2 *>(s)[1];
+        const char *at = static_cast<const char *>(p) + (uint32_t)place_of<WHOLE>(c, width).c * (dt == DT_F32 ? 4u : 2u);
+        lo = *reinterpret_cast<const Words4At2 *>(at);
+        if (dt == DT_F32) hi = reinterpret_cast<const Words4At2 *>(at)[1];
     }
     template <bool WHOLE>
     __device__ __forceinline__ void settle(int dt, uint32_t c, uint32_t width) {
-        if (WHOLE || width < 8) return;
+        if (WHOLE || width < 8) return;  // (a row of fewer than eight came so)
         const int skip = opaque(place_of<WHOLE>(c, width).skip);
         if (skip <= 0) return;
 #pragma unroll
