@@ -124,8 +124,8 @@ __device__ __forceinline__ int opaque(int n) {
 // A thread's eight values of a row, from column c on.  A row whose width is no multiple of eight ends inside a vector: that
 // thread takes the row's last eight values instead and leaves out the first `skip`, which are another's: one vector load as
 // everywhere, where elements one by one would each wait for the one before (gradient of 4096 rows of 3079 bf16 values with a
-// channel gate: 83 us by elements, 58 so; 53 and, at 3080, 37 with the workgroups there are now).  Past the row's end all eight are left out.  WHOLE: the width is a multiple
-// of eight, so a vector lies inside or outside.
+// channel gate: 83 us by elements, 58 so; 53 and, at 3080, 37 with the workgroups there are now).  Past the row's end all eight
+// are left out.  WHOLE: the width is a multiple of eight, so a vector lies inside or outside.
 struct Place {
     int c, skip;
 };
