@@ -358,7 +358,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
     extern __shared__ __align__(16) double row_buf[];  // wave_lds bytes a wave
     char *const mem = reinterpret_cast<char *>(row_buf) + wave * wave_lds;
     float *const bias_lds = reinterpret_cast<float *>(reinterpret_cast<char *>(row_buf) + RT_WAVES * wave_lds);  // behind the waves'
-    __shared__ float range[RT_WAVES][2];
+    __shared__ float range[RT_WAVES][3];
     const int size = a.experts / a.groups, units = (size + 7) / 8;
     const uint32_t over = (65536 + units - 1) / units;  // u / units = u over >> 16 for the units here
     auto group_of = [&](int u) { return GROUPED ? (int)(u * over >> 16) : 0; };
@@ -387,11 +387,12 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
         least = -group_max<64>(-least);
         most = group_max<64>(most);
         range[wave][0] = least;
-        range[wave][1] = __any(out) ? NAN : most;
+        range[wave][1] = most;
+        range[wave][2] = __any(out) ? 1.f : 0.f;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < RT_WAVES; w++) {
-            out |= range[w][1] != range[w][1];
+            out |= range[w][2] != 0.f;
             least = fminf(least, range[w][0]);
             most = fmaxf(most, range[w][1]);
         }
