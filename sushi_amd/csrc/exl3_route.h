@@ -372,6 +372,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
     float lo = 0.f, steps = 0.f, largest = 0.f;   // c's steps: (c - lo) steps + 1; no |c| is above `largest`
     // A bias that is the same for every expert does not move the choice among experts: it goes by the logits, whose ties are ties.
     bool by_logit = BY_LOGIT;
+    bool far = false;  // a bias past 2^125: keys and groups' values do not tell it from others, so every row goes by 64 bits
     if constexpr (!BY_LOGIT) {
         float least = INFINITY, most = -INFINITY;
         bool out = false;
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
             const bool is = (s & 7) < count_of(s / 8);
             const float b = is ? a.bias ? a.bias[first_of(s / 8) + (s & 7)] : 0.f : -INFINITY;
             out |= is && !(b > -INFINITY);
-            // (NaN is out of the choice; what passes 2^125 goes by 64 bits where it decides, and adds up in f32)
+            // (NaN is out of the choice; what passes 2^125 ends there, so that sums stay in f32: see `far`)
             bias_lds[s] = b > -INFINITY ? fminf(fmaxf(b, -0x1p125f), 0x1p125f) : -INFINITY;
             least = fminf(least, b > -INFINITY ? b : INFINITY);
             most = fmaxf(most, b);
@@ -397,6 +398,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
             most = fmaxf(most, range[w][1]);
         }
         by_logit = !out && least == most && fabsf(most) < INFINITY;
+        far = least < -0x1p125f || most > 0x1p125f;
         least = fminf(fmaxf(least, -0x1p125f), 0x1p125f);
         most = fminf(fmaxf(most, -0x1p125f), 0x1p125f);
         lo = least;
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(RT_THREADS) void route_lists_kernel(RouteArgs a, in
                 for (int q = 0; q < 8; q++) v[q] = x[q] == -INFINITY ? x[q] : v[q];
         }
     };
-    bool near = false, near_group = false;
+    bool near = false, near_group = far;
     uint64_t open = ~uint64_t(0);
     float *const vals = reinterpret_cast<float *>(mem) + grp * (L * nu * 8 + 8);  // (rows at different banks)
     int *const list = reinterpret_cast<int *>(mem + 2048 * nu + 32 * ROWS) + grp * a.groups;  // the open groups, in order
