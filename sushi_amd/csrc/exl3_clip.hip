@@ -122,10 +122,11 @@ __global__ __launch_bounds__(CL_THREADS) void clip_norm_kernel(ClipTensors t, Cl
             a.result[0] = (float)norm;
             const double scale = norm <= (double)a.max_norm ? 1. : (double)a.max_norm / norm;  // NaN stays NaN
             a.result[1] = (float)scale;
-            // Below f32's normal range (a norm past 1e38) a factor has lost bits: it then comes in two.
-            const bool tiny = scale > 0. && scale < 0x1p-100;
-            a.factors[0] = tiny ? (float)(scale * 0x1p64) : (float)scale;
-            a.factors[1] = tiny ? 0x1p-64f : 1.f;
+            // Towards the end of f32's range a factor loses bits, where its products with a far norm's gradients need not: it
+            // then comes as a mantissa and a power of two (down to 2^-300, past any one factor).
+            int power = 0;
+            a.factors[0] = (float)(scale > 0. && scale < 0x1p-100 ? frexp(scale, &power) : scale);
+            a.factors[1] = (float)power;
         }
     }
 }
@@ -133,12 +134,12 @@ __global__ __launch_bounds__(CL_THREADS) void clip_norm_kernel(ClipTensors t, Cl
 // Each vector is read by the thread that writes it, in place too.  From the end to the beginning, as the first pass read the end
 // last: what of it the memory-side cache still holds is not read from memory again.
 template <int DT, int OT>
-__device__ __forceinline__ void scaled(const char *g, char *out, int64_t count, float scale, float rest) {
+__device__ __forceinline__ void scaled(const char *g, char *out, int64_t count, float scale, int power) {
     constexpr int SIZE = DT == DT_F32 ? 4 : 2, OSIZE = OT == DT_F32 ? 4 : 2;
     auto times = [&](const Raw8<DT> &r, Raw8<OT> &o) {
         float v[8];
 #pragma unroll
-        for (int q = 0; q < 8; q++) v[q] = r.get(q) * scale * rest;
+        for (int q = 0; q < 8; q++) v[q] = __builtin_amdgcn_ldexpf(r.get(q) * scale, power);
         o.set(v);
     };
     const int64_t whole = count / CL_STEP * CL_STEP;
@@ -150,7 +151,7 @@ __device__ __forceinline__ void scaled(const char *g, char *out, int64_t count, 
             times(r, o);
             o.store(out + i * OSIZE);
         } else {
-            for (int64_t j = i; j < count; j++) store_act<OT>(out, j, load_act<DT>(g, j) * scale * rest);
+            for (int64_t j = i; j < count; j++) store_act<OT>(out, j, __builtin_amdgcn_ldexpf(load_act<DT>(g, j) * scale, power));
         }
     }
     for (int64_t i = whole - CL_STEP + (int64_t)threadIdx.x * 8; i >= 0; i -= CL_STEP) {
@@ -167,21 +168,22 @@ __device__ __forceinline__ void scaled(const char *g, char *out, int64_t count, 
 }
 
 template <int DT>
-__device__ __forceinline__ void scaled_to(const char *g, char *out, int ot, int64_t count, float scale, float rest) {
-    if (ot == DT_F16) scaled<DT, DT_F16>(g, out, count, scale, rest);
-    else if (ot == DT_BF16) scaled<DT, DT_BF16>(g, out, count, scale, rest);
-    else scaled<DT, DT_F32>(g, out, count, scale, rest);
+__device__ __forceinline__ void scaled_to(const char *g, char *out, int ot, int64_t count, float scale, int power) {
+    if (ot == DT_F16) scaled<DT, DT_F16>(g, out, count, scale, power);
+    else if (ot == DT_BF16) scaled<DT, DT_BF16>(g, out, count, scale, power);
+    else scaled<DT, DT_F32>(g, out, count, scale, power);
 }
 
 __global__ __launch_bounds__(CL_THREADS) void clip_scale_kernel(ClipTensors t, const float *factors) {
-    const float scale = factors[0], rest = factors[1];
+    const float scale = factors[0];
+    const int power = (int)factors[1];
     for_run<true>(t, [&](const ClipEntry &e, int64_t from, int64_t end) {
-        if (scale == 1.f && e.g == e.out) return;  // in place there is nothing to do
+        if (scale == 1.f && !power && e.g == e.out) return;  // in place there is nothing to do
         const char *g = static_cast<const char *>(e.g) + from * (e.dtype == DT_F32 ? 4 : 2);
         char *out = static_cast<char *>(e.out) + from * (e.out_dtype == DT_F32 ? 4 : 2);
-        if (e.dtype == DT_F16) scaled_to<DT_F16>(g, out, e.out_dtype, end - from, scale, rest);
-        else if (e.dtype == DT_BF16) scaled_to<DT_BF16>(g, out, e.out_dtype, end - from, scale, rest);
-        else scaled_to<DT_F32>(g, out, e.out_dtype, end - from, scale, rest);
+        if (e.dtype == DT_F16) scaled_to<DT_F16>(g, out, e.out_dtype, end - from, scale, power);
+        else if (e.dtype == DT_BF16) scaled_to<DT_BF16>(g, out, e.out_dtype, end - from, scale, power);
+        else scaled_to<DT_F32>(g, out, e.out_dtype, end - from, scale, power);
     });
 }
 

@@ -502,7 +502,7 @@ struct ClipArgs {
     uint32_t *counter;  // zero between calls
     float max_norm;
     float *result;      // [2]: norm, scale
-    float *factors;     // [2]: whose product is the scale that the second pass multiplies by
+    float *factors;     // [2]: a factor and the power of two beside it that the second pass multiplies by
 };
 inline int clip_parts(int chunks) { return chunks < kClipParts ? chunks : kClipParts; }
 hipError_t run_clip_norm(const ClipTensors &t, const ClipArgs &a, bool last, hipStream_t s);
