@@ -1144,6 +1144,14 @@ class BalanceLoss(NamedTuple):
     weight: torch.Tensor
 
 
+def _rows_of(what: str, t: torch.Tensor) -> int:
+    """The rows of [.., width], which the library counts in 32 bits."""
+    rows = t.numel() // t.shape[-1] if t.shape[-1] else 0
+    if rows > 0x7FFFFFFF:
+        raise BadExl3Shape(f"{what}: {rows} rows (up to 2^31 - 1)")
+    return rows
+
+
 def _router_operands(router_logits, inds, mask, what: str):
     lg = router_logits
     if lg.dim() < 1 or inds.dim() != lg.dim() or inds.shape[:-1] != lg.shape[:-1] or \
@@ -1154,8 +1162,7 @@ def _router_operands(router_logits, inds, mask, what: str):
         raise BadExl3Dtype(f"{what}: inds dtype {inds.dtype} (u32/i32)")
     if mask is not None and mask.dtype not in (torch.bool, torch.uint8):
         raise BadExl3Dtype(f"{what}: mask dtype {mask.dtype} (bool or u8)")
-    experts = lg.shape[-1]
-    return (lg.numel() // experts if experts else 0), experts, inds.shape[-1]
+    return _rows_of(what, lg), lg.shape[-1], inds.shape[-1]
 
 
 def moe_balance_loss(router_logits: torch.Tensor, inds: torch.Tensor, mask: Optional[torch.Tensor] = None,
@@ -1237,7 +1244,7 @@ def moe_route(router_logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] 
     if bias is not None and (bias.shape != (experts,) or bias.dtype != torch.float32):
         raise BadExl3Shape(f"moe_route: bias {tuple(bias.shape)} {bias.dtype}, expected {(experts,)} in float32")
     code, dt = _score(score), _dt(lg, "logits")
-    rows = lg.numel() // experts if experts else 0
+    rows = _rows_of("moe_route", lg)
     dev, guard = _on_one_device("moe_route", lg, bias, mask)
     with guard:
         shape = (*lg.shape[:-1], max(k, 0))
@@ -1312,7 +1319,7 @@ def _block_norm_operands(what: str, y, hs, post_weight, pre_weight, gate):
             kind = _GATE_FULL
         else:
             raise BadExl3Shape(f"{what}: gate {tuple(gate.shape)} for y {tuple(shape)}: one value a channel, a row or each")
-    return (y.numel() // width if width else 0), width, kind
+    return _rows_of(what, y), width, kind
 
 
 def _dt_or(t: Optional[torch.Tensor], what: str, default: int = 0) -> int:
