@@ -479,7 +479,9 @@ int32_t exl3_block_norm_backward(const void *dh, const void *dx, const void *y, 
  * dtypes, out and out_dtypes are host arrays, read before the call returns (a captured graph keeps the addresses that they held).  A
  * tensor of numel values lies contiguous in f16, bf16 or f32; out null: in place, with nothing written where scale is 1;
  * else each out[i] holds numel[i] values of its type and overlaps no other tensor (it may be grads[i] in the same type).
- * Squares add in 64 bits.  A norm of inf makes scale 0 (and inf * 0 NaN), of NaN NaN.  max_norm >= 0, inf for the norm alone.
+ * Squares add in 64 bits, and scale is of the norm in 64 bits: one past f32's range is inf in result and clips all the same.
+ * An infinity among the values makes norm inf and, by a finite max_norm, scale 0 (and inf * 0 NaN); NaN makes both NaN.
+ * max_norm >= 0; by inf scale is 1 unless NaN: without out that is the norm alone, with it a copy.
  * Equal calls give equal bits. */
 size_t exl3_clip_grad_norm_workspace_size(int32_t count);
 int32_t exl3_clip_grad_norm(int32_t count, const void *const *grads, const int64_t *numel, const int32_t *dtypes,

@@ -1399,8 +1399,9 @@ class GradNorm(NamedTuple):
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None) -> GradNorm:
     """Clips gradients (f16, bf16 or f32 each, of any shapes) by their global norm, on the device: norm = sqrt(sum of all g^2),
     scale = min(1, max_norm / norm), g *= scale in place, or g scale into ``out`` (a tensor for each gradient, of any of these
-    dtypes and the same shape).  ``max_norm`` inf with no ``out`` only measures.  A norm of inf or NaN comes out as that, with a
-    scale of 0 or NaN.  Squares add in 64 bits and in a fixed order: equal calls give equal bits."""
+    dtypes and the same shape).  ``max_norm`` inf with no ``out`` only measures (with ``out`` it copies).  An infinity or NaN
+    among the values is the norm's, with a scale of 0 (1 by a ``max_norm`` of inf) or NaN; a norm past f32's range comes out as
+    inf, its scale as it is.  Squares add in 64 bits and in a fixed order: equal calls give equal bits."""
     grads = list(grads)
     if not grads:
         raise BadExl3Shape("clip_grad_norm: no gradients")
