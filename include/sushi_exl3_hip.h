@@ -427,12 +427,12 @@ int32_t exl3_router_backward(const void *logits, int32_t dtype, int32_t rows, in
  * Picks are listed in falling c, equal ones (and equal groups) by their number; the order is that of the values in 64 bits
  * (without bias or with one that is the same for every expert, the experts' is that of their logits, and with group_top 1 the
  * groups' too), whatever the f32 roundings of another batch.
- * An expert is out of the choice by a logit of -inf or NaN (under softmax +inf too) or a bias of -inf or NaN; a row with a
- * NaN logit (under softmax +inf too) has NaN scores.  A slot that no expert is left for, and every slot of a row that mask
- * [rows] (bytes, or null) leaves out, holds id 0xFFFFFFFF and score 0, whatever the row's logits: a dropped slot for
- * exl3_balance_loss and the gradients (exl3_moe clamps it to the last expert, times 0).  inds [rows][topk], scores f32
- * [rows][topk]; they overlap no input and not each other (refused).  experts <= 1024, topk <= 32, groups <= 64 and a divisor of
- * experts, topk_groups groups hold at least topk experts.
+ * An expert is out of the choice by a logit of -inf or NaN (under softmax +inf too) or a bias of -inf or NaN (a finite bias
+ * keeps it in, and one far from the others slows every row down); a row with a NaN logit (under softmax +inf too) has NaN
+ * scores.  A slot that no expert is left for, and every slot of a row that mask [rows] (bytes, or null) leaves out, holds id
+ * 0xFFFFFFFF and score 0, whatever the row's logits: a dropped slot for exl3_balance_loss and the gradients (exl3_moe clamps
+ * it to the last expert, times 0).  inds [rows][topk], scores f32 [rows][topk]; they overlap no input and not each other
+ * (refused).  experts <= 1024, topk <= 32, groups <= 64 and a divisor of experts, topk_groups groups hold at least topk experts.
  *
  * exl3_route_backward: dlogits (like logits; it overlaps no input) from dscores f32 [rows][topk], the choice held fixed.  With
  * r the scores over scale and ds = scale dscores, the row's slots i on expert e add up (a dropped slot has none):

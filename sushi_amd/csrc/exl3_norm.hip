@@ -8,10 +8,10 @@
 // the h' that was kept.
 //
 // Both passes are bound by the rows' bytes: a row stays in registers between its loads and its stores, whatever its norms need
-// over it.  Forward, bf16 with both norms: 16384 rows of 4096 values 99 us (5.4 TB/s; a large copy reaches 5.2), 2047 rows of 5120
-// with an f32 stream and a gate 24; one row of 4096 3.5 us, a launch and two row sums.  Gradient: 16384 rows of 4096 155 us
-// (5.2 TB/s); 333 rows of 2560, f16 with an f32 stream and a channel gate, 10.2: the latency of two rows (7.5) and the join's
-// launch.
+// over it.  Forward, bf16 with both norms: 16384 rows of 4096 values 98 us (5.5 TB/s; a large copy reaches 5.2), 8192 rows of
+// 8192 / 16384 96 / 191, 2047 rows of 5120 with an f32 stream and a gate 25; one row of 4096 3.5 us, a launch and two row sums.  Gradient:
+// 16384 rows of 4096 155 us (5.2 TB/s); 333 rows of 2560, f16 with an f32 stream and a channel gate, 10.2: the latency of two rows
+// (7.5) and the join's launch.
 #include "exl3_vec.h"
 #include "exl3_epilogue.h"
 
@@ -498,6 +498,8 @@ hipError_t run_norm_backward(const NormGradArgs &a, hipStream_t s) {
         if (a.width <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
         // (rows with an f32 stream that end inside a vector want more than the 168 registers of 12 waves)
         if (a.width <= 6144 && (whole || ht != DT_F32)) return go(integral_constant<int, 768>{}, integral_constant<int, 1>{});
+        // (without the next row's loads ahead; past 8192 values the sums are kept in the part, and h and dx read twice: 8192 bf16
+        // rows of 8192 / 16384 values take 198 / 654 us, 156 and 312 for the bytes)
         if (a.width <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
         return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
     });

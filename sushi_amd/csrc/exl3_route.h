@@ -49,13 +49,14 @@ __device__ __forceinline__ void wave_best(double &c, int &i) {
     best_step<32>(c, i);
 }
 
-// exp(x) for x <= 0 to about an ulp: exp2 of the product with log2 e, times what its rounding left out.
+// exp(x) for x <= 0 to about an ulp: exp2 of the product with log2 e in two f32, as Cody and Waite split a constant, times what
+// the product's rounding left out.
 __device__ __forceinline__ float exp_near(float x) {
     constexpr float HI = 1.44269504f, LO = 1.92596299e-8f, LN2 = 0.693147181f;
     const float n = x * HI, rest = fmaf(x, HI, -n) + x * LO, e = __builtin_amdgcn_exp2f(n);
     return x > -104.f ? fmaf(e, rest * LN2, e) : 0.f;  // (the rest of -inf is NaN)
 }
-// a / b for b of f32's middle range: a reciprocal and the quotient's remainder.
+// a / b for b of f32's middle range: a reciprocal and one Newton step, by the quotient's remainder.
 __device__ __forceinline__ float quotient(float a, float b) {
     const float r = rcp(b), q = a * r;
     return fmaf(fmaf(-q, b, a), r, q);
@@ -246,7 +247,8 @@ __device__ __forceinline__ bool settle_row(const RouteArgs &a, size_t row, int l
     return true;
 }
 
-// More than eight picks (or more units than the lists hold): a wave a row.
+// More than eight picks (or more units than the lists hold): a wave a row, each pick a pass over the row's values.  Bound by the
+// issue of those: 65521 bf16 rows of 256 with 12 picks take 125 us by the logits, 160 with a bias, 202 with groups too.
 template <int DT>
 __global__ __launch_bounds__(RT_THREADS) void route_kernel(RouteArgs a) {
     extern __shared__ double row_buf[];
@@ -280,10 +282,14 @@ __global__ __launch_bounds__(RT_THREADS) void route_kernel(RouteArgs a) {
 // The loops over a lane's units stay rolled: the kernel is short, so a call of few rows fetches less of it, and few registers
 // leave room for more waves.
 //
-// Long calls are bound by the issue of vector instructions: 65521 bf16 rows of 256 experts with bias and groups take 32 us, about
-// 175 instructions a row, 19 us of issue, and some us for the rows that go by 64 bits after the others; by the logits alone
-// 12.6 us (f32 20), against 7.3 (13) for the bytes.  Short ones are a launch and one row's latency:
-// 6.1 us for 32 rows with bias and groups, 2.6 to 4 by the logits.
+// Long calls are bound by the issue of vector instructions more than by their bytes: 65521 bf16 rows of 256 experts by the logits
+// alone take 12.7 us, 97 instructions a row and 10.4 us of issue (7.3 for the bytes); of f32 logits 20 to 22, 111 a row, 11.8 of
+// issue and 13 for the bytes; with bias and groups 32, 180 a row, 20 of issue, the rest of it the rows that go by 64 bits after the
+// others and a second generation of workgroups (36 KB of LDS each).  A masked row is computed as any other.  Short calls are a
+// launch and one row's latency: 6.1 us for 32 rows with bias and groups, 2.6 to 4 by the logits.
+//
+// The steps of c span the whole bias, so one expert far from the others leaves them few: with one at -100 / -1e4 / -1e9 the 32 us
+// become 47 / 145 / 248, as more and more rows go by 64 bits.  An expert at -inf is out and costs nothing.
 __device__ __forceinline__ void comparator(int &a, int &b) {
     const int hi = max(a, b), lo = min(a, b);
     a = hi;

@@ -1233,8 +1233,9 @@ def moe_route(router_logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] 
     (inds [.., k] i32, scores [.., k] f32).  With p the logits' softmax or sigmoid (``score``) and c = p + bias ([E] f32, for the
     choice alone): of ``groups`` groups of neighbouring experts the ``topk_groups`` with the largest sum of their ``group_top`` (1
     or 2) largest c, of their experts the k largest c in falling order, equal ones by their number; the scores are scale p, over
-    the sum of the picks' p with ``renormalize``.  A logit or bias of -inf takes its expert out.  Slots that no expert is left for
-    and rows that mask [..] leaves out hold -1 and 0.  The choice is that of 64-bit values: it does not change with the batch."""
+    the sum of the picks' p with ``renormalize``.  A logit or bias of -inf takes its expert out (a far finite bias does not, and slows
+    every row down: masks are -inf).  Slots that no expert is left for and rows that mask [..] leaves out hold -1 and 0.  The choice
+    is that of 64-bit values: it does not change with the batch."""
     lg = router_logits
     if lg.dim() < 1 or (mask is not None and mask.shape != lg.shape[:-1]):
         raise BadExl3Shape(f"moe_route: logits {tuple(lg.shape)}" + ("" if mask is None else f", mask {tuple(mask.shape)}"))
